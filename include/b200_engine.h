@@ -130,6 +130,134 @@ B200_API int b200_copy_async(b200_engine_t *e, uint64_t dst, uint64_t src, uint6
  * calls share the array: calls that overlap on the GPU race. */
 B200_API int b200_argmax_f32_noalloc(uint64_t y, int n, int index_base, uint64_t out, void *stream);
 
+/* ------------------------------------------------------------ serving ops
+ * What a server of several sequences needs around the GEMVs: a key-value
+ * cache in pages, attention of one new token per sequence over it, eviction
+ * from it by accumulated attention weight, and a sampler. No counterpart in
+ * the reference, which has one sequence, a cache [layer][head][position] and
+ * a host sampler (tp_llama.cpp:643-705, 809-815, 894-936).
+ *
+ * All calls queue on the engine's stream, allocate nothing and can be
+ * recorded into a graph. Lengths, page tables and sampler settings are read
+ * on the device, so the host need not know them; what a call finds there
+ * that it cannot use is handled as each call says, never read out of range. */
+#define B200_F32 0
+#define B200_F16 1
+#define B200_BF16 2
+
+/* A paged cache. Slot i of sequence b lies in page table[b][i / page_size] at
+ * row i % page_size of each head; a row is head_dim contiguous elements. The
+ * strides (in elements) order pages, heads and rows freely, so a pool
+ * [page][head][row][head_dim] and one [page][row][head][head_dim] both do. k
+ * and v share strides; both addresses and all strides are multiples of 16
+ * bytes. lengths[b] (< 0: 0; beyond table_cols * page_size: that) slots are in
+ * use. A page number outside [0, n_pages) stands for rows that are not there:
+ * they take no part in attention and nothing is written to them. */
+typedef struct {
+    uint64_t k, v;
+    int dtype;           /* B200_F32, B200_F16 or B200_BF16 */
+    int n_pages, page_size, n_head_kv;
+    int head_dim;        /* a multiple of 8, at most 256 */
+    int64_t page_stride, head_stride, row_stride;
+    uint64_t table;      /* int32 [batch][table_stride] */
+    int64_t table_stride;
+    int table_cols;      /* table_cols * page_size <= 1048576 slots a sequence */
+    uint64_t lengths;    /* int32 [batch] */
+    int batch;
+} b200_kv_t;
+
+/* Append: row i of a sequence's new rows goes to slot lengths[b] + i, rounded
+ * to the cache's type (to nearest even); its position seen[b] + i and a weight
+ * of 0 go beside it. Rows past the last slot, or in a page that is not there,
+ * are dropped. */
+typedef struct {
+    uint64_t k_new, v_new;             /* [n_tokens][n_head_kv][head_dim], strides in elements */
+    int dtype;                         /* B200_F32 or the cache's type */
+    int n_tokens;
+    int64_t token_stride, head_stride; /* both and the addresses multiples of 16 bytes */
+    uint64_t offsets;                  /* int32 [batch + 1]: sequence b has rows offsets[b] up to offsets[b + 1],
+                                          from 0 to n_tokens in all, not falling; 0: row b is sequence b's */
+    uint64_t seen;                     /* int32 [batch]: tokens each sequence has had; 0: as lengths */
+    uint64_t positions;                /* int32 [batch][n_head_kv][aux_stride], or 0 */
+    uint64_t weights;                  /* float [batch][n_head_kv][aux_stride], or 0 */
+    int64_t aux_stride;                /* >= table_cols * page_size */
+    uint64_t lengths_out, seen_out;    /* int32 [batch], or 0; may be lengths and seen themselves */
+} b200_kv_append_t;
+B200_API int b200_kv_append(b200_engine_t *e, const b200_kv_t *kv, const b200_kv_append_t *a);
+
+/* Attention of one new token per sequence over its slots in use:
+ * s = scale * q . k, out = sum exp(s) v / sum exp(s), lse = log sum exp(s);
+ * with no slot left, out = 0 and lse = -infinity. n_head / n_head_kv query
+ * heads read each cache head. Dot products, the running maximum and sum and
+ * the output are held in float32; the rounding to the output's type is the
+ * last step. With weights_out the weights of the softmax, summed over the
+ * query heads of a cache head, are added up: weights_out = decay * weights +
+ * sum, for slots in use (others are not written). */
+typedef struct {
+    uint64_t q, out;                   /* [batch][n_head][head_dim], strides in elements, rows contiguous */
+    int dtype;                         /* of both: the cache's type, or B200_F32 with a B200_F16 cache */
+    int n_head;                        /* a multiple of n_head_kv */
+    int64_t q_batch_stride, q_head_stride, out_batch_stride, out_head_stride;
+    float scale;
+    uint64_t lse;                      /* float [batch][n_head], or 0 */
+    uint64_t weights;                  /* float [batch][n_head_kv][aux_stride]; 0: as zeros */
+    uint64_t weights_out;              /* the same shape, may be `weights` itself; 0: not wanted */
+    int64_t aux_stride;
+    float decay;
+    uint64_t workspace;                /* with weights_out: b200_kv_attend_workspace() bytes, 16-byte aligned */
+    uint64_t workspace_bytes;
+} b200_kv_attend_t;
+B200_API uint64_t b200_kv_attend_workspace(const b200_kv_t *kv, int n_head);
+B200_API int b200_kv_attend(b200_engine_t *e, const b200_kv_t *kv, const b200_kv_attend_t *a);
+
+/* Eviction: each head of a sequence with more than `budget` slots in use keeps
+ * the tokens at positions >= seen[b] - recent or < sinks, then those of the
+ * largest weights (the lower slot where equal; NaN is the smallest), budget in
+ * all (of tokens kept by position, too, the lower slots if they are more).
+ * The i-th kept slot >= budget moves into the i-th slot < budget that was
+ * given up -- key and value rows, weight and position -- and nothing else
+ * moves, so slots are not in the order of their positions afterwards
+ * (attention does not mind). Slots < the new length of weights_out and
+ * positions_out are written, no others. Sequences within budget are left as
+ * they are. Pages must not be shared between sequences that are cut. */
+typedef struct {
+    uint64_t weights, weights_out;     /* float [batch][n_head_kv][aux_stride]; may be the same */
+    uint64_t positions, positions_out; /* int32, the same shape; may be the same */
+    int64_t aux_stride;
+    uint64_t seen;                     /* int32 [batch] */
+    uint64_t lengths_out;              /* int32 [batch], or 0; may be the cache's lengths */
+    int budget, recent, sinks;         /* budget >= 1, recent + sinks <= budget */
+} b200_kv_evict_t;
+B200_API int b200_kv_evict(b200_engine_t *e, const b200_kv_t *kv, const b200_kv_evict_t *a);
+
+/* Sampling. With x a row's logits (NaN counts as -infinity), M the largest and
+ * T the temperature, token i weighs w_i = floor(2^40 * 2^((x_i - M) * c)),
+ * c = log2(e) / T, whole numbers whose sums do not depend on an order. Filters
+ * keep a prefix of the tokens in falling order of x (the lower index where
+ * equal): top_k its first k; top_p the fewest of those whose weight reaches
+ * p of theirs together, at least one; min_p those with
+ * 2^((x_i - M) * c) >= min_p. The token is the first whose weight, added to
+ * that of all kept tokens of lower index, passes u of the whole; u and p count
+ * in units of 2^-24. So the same logits and u give the same token on every
+ * run. A temperature of 0 (or less, or NaN) takes the lowest index of the
+ * largest logit. Where M is +infinity, the tokens at it weigh the same and all
+ * others nothing; a row with no logit above -infinity gives token -1. */
+typedef struct {
+    uint64_t logits;                   /* [batch][row_stride] */
+    int dtype;                         /* B200_F32, B200_F16 or B200_BF16 */
+    int batch;
+    int n_vocab;                       /* at most 4194304 */
+    int64_t row_stride;
+    uint64_t temperature;              /* float [batch]; 0: all 1 */
+    uint64_t top_k;                    /* int32 [batch], <= 0 in a row: off; 0: off */
+    uint64_t top_p;                    /* float [batch], >= 1 or NaN in a row: off; 0: off */
+    uint64_t min_p;                    /* float [batch], <= 0 or NaN in a row: off; 0: off */
+    uint64_t u;                        /* float [batch] in [0, 1) (clamped to it; NaN: 0) */
+    uint64_t token;                    /* int32 [batch] */
+    uint64_t logprob;                  /* float [batch]: log of the token's share of the kept weight, or 0 */
+} b200_sample_t;
+B200_API int b200_sample(b200_engine_t *e, const b200_sample_t *s);
+
 /* Block until the engine's queued work is done (bounded; -ETIMEDOUT). */
 B200_API int b200_engine_sync(b200_engine_t *e, int timeout_ms);
 /* Device status word (see gemv_dev_status); reading clears it. */

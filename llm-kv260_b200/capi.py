@@ -54,6 +54,46 @@ class b200_decoder_config_t(ctypes.Structure):
                [(n, c_int) for n in ("ctx_max", "kv_f16", "round_mode", "exact_norm", "persistent")]
 
 
+c_i64 = ctypes.c_int64
+
+
+class b200_kv_t(ctypes.Structure):
+    """include/b200_engine.h"""
+    _fields_ = [("k", c_u64), ("v", c_u64), ("dtype", c_int), ("n_pages", c_int), ("page_size", c_int),
+                ("n_head_kv", c_int), ("head_dim", c_int), ("page_stride", c_i64), ("head_stride", c_i64),
+                ("row_stride", c_i64), ("table", c_u64), ("table_stride", c_i64), ("table_cols", c_int),
+                ("lengths", c_u64), ("batch", c_int)]
+
+
+class b200_kv_append_t(ctypes.Structure):
+    """include/b200_engine.h"""
+    _fields_ = [("k_new", c_u64), ("v_new", c_u64), ("dtype", c_int), ("n_tokens", c_int), ("token_stride", c_i64),
+                ("head_stride", c_i64), ("offsets", c_u64), ("seen", c_u64), ("positions", c_u64), ("weights", c_u64),
+                ("aux_stride", c_i64), ("lengths_out", c_u64), ("seen_out", c_u64)]
+
+
+class b200_kv_attend_t(ctypes.Structure):
+    """include/b200_engine.h"""
+    _fields_ = [("q", c_u64), ("out", c_u64), ("dtype", c_int), ("n_head", c_int), ("q_batch_stride", c_i64),
+                ("q_head_stride", c_i64), ("out_batch_stride", c_i64), ("out_head_stride", c_i64),
+                ("scale", ctypes.c_float), ("lse", c_u64), ("weights", c_u64), ("weights_out", c_u64),
+                ("aux_stride", c_i64), ("decay", ctypes.c_float), ("workspace", c_u64), ("workspace_bytes", c_u64)]
+
+
+class b200_kv_evict_t(ctypes.Structure):
+    """include/b200_engine.h"""
+    _fields_ = [("weights", c_u64), ("weights_out", c_u64), ("positions", c_u64), ("positions_out", c_u64),
+                ("aux_stride", c_i64), ("seen", c_u64), ("lengths_out", c_u64), ("budget", c_int), ("recent", c_int),
+                ("sinks", c_int)]
+
+
+class b200_sample_t(ctypes.Structure):
+    """include/b200_engine.h"""
+    _fields_ = [("logits", c_u64), ("dtype", c_int), ("batch", c_int), ("n_vocab", c_int), ("row_stride", c_i64),
+                ("temperature", c_u64), ("top_k", c_u64), ("top_p", c_u64), ("min_p", c_u64), ("u", c_u64),
+                ("token", c_u64), ("logprob", c_u64)]
+
+
 SIGNATURES: dict[str, tuple] = {
     # gemv_dev.h
     "gemv_dev_open": (c_int, [P(gemv_dev_t)]),
@@ -107,6 +147,11 @@ SIGNATURES: dict[str, tuple] = {
     "b200_copy_async": (c_int, [c_vp, c_u64, c_u64, c_u64]),
     "b200_repack_q4_0": (c_int, [c_vp, c_u64, c_int, c_int, c_u64]),
     "b200_device_count": (c_int, []),
+    "b200_kv_append": (c_int, [c_vp, P(b200_kv_t), P(b200_kv_append_t)]),
+    "b200_kv_attend_workspace": (c_u64, [P(b200_kv_t), c_int]),
+    "b200_kv_attend": (c_int, [c_vp, P(b200_kv_t), P(b200_kv_attend_t)]),
+    "b200_kv_evict": (c_int, [c_vp, P(b200_kv_t), P(b200_kv_evict_t)]),
+    "b200_sample": (c_int, [c_vp, P(b200_sample_t)]),
     # b200_comm.h
     "b200_comm_create": (c_int, [P(c_vp), c_int, c_int, c_int, c_int]),
     "b200_comm_handle_bytes": (c_int, []),

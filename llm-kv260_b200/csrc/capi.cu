@@ -17,6 +17,7 @@
 #include "../../include/gemv_dev.h"
 #include "../../include/udmabuf.h"
 #include "q4gemv.h"
+#include "serve.h"
 
 using namespace b200;
 
@@ -477,6 +478,7 @@ struct b200_engine {
     uint8_t *xscratch;  // quantised x for the two-kernel f32 path
     void *sel_scratch;  // argmax candidates
     void *fsel_scratch; // fused greedy pick: per-CTA candidates + ticket
+    void *serve_scratch; // serving ops: tickets and the parts of split sequences
     b200_engine_config_t cfg;
 };
 
@@ -587,6 +589,8 @@ extern "C" int b200_engine_open(b200_engine_t **out, int device) {
     if (err == cudaSuccess) err = cudaMalloc(&e->sel_scratch, static_cast<size_t>(argmax_scratch_bytes()));
     if (err == cudaSuccess) err = cudaMalloc(&e->fsel_scratch, static_cast<size_t>(tile_select_scratch_bytes()));
     if (err == cudaSuccess) err = cudaMemset(e->fsel_scratch, 0, static_cast<size_t>(tile_select_scratch_bytes()));
+    if (err == cudaSuccess) err = cudaMalloc(&e->serve_scratch, serve_scratch_bytes());
+    if (err == cudaSuccess) err = cudaMemset(e->serve_scratch, 0, serve_scratch_bytes());
     if (err != cudaSuccess) {
         b200_engine_close(e);
         return cuda_fail(err, "engine set-up");
@@ -614,6 +618,7 @@ extern "C" int b200_engine_close(b200_engine_t *e) {
     if (e->xscratch) cudaFree(e->xscratch);
     if (e->sel_scratch) cudaFree(e->sel_scratch);
     if (e->fsel_scratch) cudaFree(e->fsel_scratch);
+    if (e->serve_scratch) cudaFree(e->serve_scratch);
     if (e->fork) cudaEventDestroy(e->fork);
     if (e->done) cudaEventDestroy(e->done);
     if (e->side) cudaStreamDestroy(e->side);
@@ -835,4 +840,42 @@ extern "C" int b200_copy_async(b200_engine_t *e, uint64_t dst, uint64_t src, uin
     const cudaError_t err = cudaMemcpyAsync(reinterpret_cast<void *>(dst), reinterpret_cast<const void *>(src),
                                             static_cast<size_t>(bytes), cudaMemcpyDefault, e->stream);
     return err == cudaSuccess ? 0 : cuda_fail(err, "cudaMemcpyAsync");
+}
+
+// ============================================================== serving ops
+
+extern "C" int b200_kv_append(b200_engine_t *e, const b200_kv_t *kv, const b200_kv_append_t *a) {
+    if (!e) return fail(kErrInval, "engine not open");
+    const char *why = nullptr;
+    if (kv_append_validate(kv, a, &why)) return fail(kErrInval, "kv_append: %s", why);
+    if (int rc = use_device(e->device)) return rc;
+    const cudaError_t err = kv_append_launch(kv, a, e->serve_scratch, e->stream);
+    return err == cudaSuccess ? 0 : cuda_fail(err, "kv_append launch");
+}
+
+extern "C" int b200_kv_attend(b200_engine_t *e, const b200_kv_t *kv, const b200_kv_attend_t *a) {
+    if (!e) return fail(kErrInval, "engine not open");
+    const char *why = nullptr;
+    if (kv_attend_validate(kv, a, &why)) return fail(kErrInval, "kv_attend: %s", why);
+    if (int rc = use_device(e->device)) return rc;
+    const cudaError_t err = kv_attend_launch(kv, a, e->serve_scratch, e->stream);
+    return err == cudaSuccess ? 0 : cuda_fail(err, "kv_attend launch");
+}
+
+extern "C" int b200_kv_evict(b200_engine_t *e, const b200_kv_t *kv, const b200_kv_evict_t *a) {
+    if (!e) return fail(kErrInval, "engine not open");
+    const char *why = nullptr;
+    if (kv_evict_validate(kv, a, &why)) return fail(kErrInval, "kv_evict: %s", why);
+    if (int rc = use_device(e->device)) return rc;
+    const cudaError_t err = kv_evict_launch(kv, a, e->serve_scratch, e->stream);
+    return err == cudaSuccess ? 0 : cuda_fail(err, "kv_evict launch");
+}
+
+extern "C" int b200_sample(b200_engine_t *e, const b200_sample_t *s) {
+    if (!e) return fail(kErrInval, "engine not open");
+    const char *why = nullptr;
+    if (sample_validate(s, &why)) return fail(kErrInval, "sample: %s", why);
+    if (int rc = use_device(e->device)) return rc;
+    const cudaError_t err = sample_launch(s, e->stream);
+    return err == cudaSuccess ? 0 : cuda_fail(err, "sample launch");
 }

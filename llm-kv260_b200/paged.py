@@ -1,0 +1,77 @@
+"""A paged key-value cache as the serving calls take it (b200_kv_t,
+include/b200_engine.h): Engine.kv_append, kv_attend and kv_evict."""
+
+from __future__ import annotations
+
+from . import capi
+
+DTYPES = {"torch.float32": 0, "torch.float16": 1, "torch.bfloat16": 2}   # B200_F32, B200_F16, B200_BF16
+
+
+def dtype_code(t, name: str) -> int:
+    code = DTYPES.get(str(t.dtype))
+    if code is None:
+        raise ValueError(f"{name} must be float32, float16 or bfloat16, not {t.dtype}")
+    return code
+
+
+def typed(t, dtype: str, name: str, shape=None):
+    """t, if it is a CUDA tensor of that type (and shape); else ValueError."""
+    if not t.is_cuda or str(t.dtype) != "torch." + dtype:
+        raise ValueError(f"{name} must be a CUDA {dtype} tensor")
+    if shape is not None and tuple(t.shape) != tuple(shape):
+        raise ValueError(f"{name} must have shape {tuple(shape)}, not {tuple(t.shape)}")
+    return t
+
+
+def rows(t, name: str, shape) -> tuple[int, int]:
+    """Strides of a tensor's first two dimensions, its last one contiguous."""
+    if not t.is_cuda:
+        raise ValueError(f"{name} must be a CUDA tensor")
+    if tuple(t.shape) != tuple(shape):
+        raise ValueError(f"{name} must have shape {tuple(shape)}, not {tuple(t.shape)}")
+    s = t.stride()
+    if s[2] != 1 and shape[2] != 1:
+        raise ValueError(f"{name}: a row must be contiguous")
+    return s[0], s[1]
+
+
+class PagedKV:
+    """Pools k and v, [n_pages, n_head_kv, page_size, head_dim] views of one
+    type and the same strides, rows contiguous; table int32 [batch, columns],
+    the pages of each sequence; lengths int32 [batch], its slots in use.
+
+    The object holds the tensors, and reads nothing of them itself: a caller
+    fills the table as it hands pages out, and the calls advance or cut the
+    lengths."""
+
+    def __init__(self, k, v, table, lengths):
+        if k.dim() != 4 or k.shape != v.shape or k.dtype != v.dtype or k.stride() != v.stride():
+            raise ValueError("k and v must be [n_pages, n_head_kv, page_size, head_dim] alike in type and strides")
+        if not (k.is_cuda and v.is_cuda):
+            raise ValueError("k and v must be CUDA tensors")
+        if k.stride(3) != 1:
+            raise ValueError("a cache row must be contiguous")
+        typed(table, "int32", "table")
+        if table.dim() != 2 or (table.shape[1] > 1 and table.stride(1) != 1):
+            raise ValueError("table must be [batch, columns] with contiguous rows")
+        typed(lengths, "int32", "lengths", (table.shape[0],))
+        if not lengths.is_contiguous():
+            raise ValueError("lengths must be contiguous")
+        self.k, self.v, self.table, self.lengths = k, v, table, lengths
+        self.n_pages, self.n_head_kv, self.page_size, self.head_dim = k.shape
+        self.batch, cols = table.shape
+        self.capacity = cols * self.page_size
+        st = k.stride()
+        self.c = capi.b200_kv_t(k.data_ptr(), v.data_ptr(), dtype_code(k, "k"), self.n_pages, self.page_size,
+                                self.n_head_kv, self.head_dim, st[0], st[1], st[2], table.data_ptr(),
+                                max(table.stride(0), cols), cols, lengths.data_ptr(), self.batch)
+
+    def aux(self, t, dtype: str, name: str) -> tuple[int, int]:
+        """Address and head stride of a [batch, n_head_kv, >= capacity] tensor beside the cache (weights, positions)."""
+        typed(t, dtype, name)
+        if t.dim() != 3 or tuple(t.shape[:2]) != (self.batch, self.n_head_kv) or t.shape[2] < self.capacity:
+            raise ValueError(f"{name} must be [{self.batch}, {self.n_head_kv}, >= {self.capacity}]")
+        if not t.is_contiguous():
+            raise ValueError(f"{name} must be contiguous")
+        return t.data_ptr(), t.shape[2]
