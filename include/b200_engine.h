@@ -204,10 +204,11 @@ typedef struct {
     uint64_t weights_out;              /* the same shape, may be `weights` itself; 0: not wanted */
     int64_t aux_stride;
     float decay;
-    uint64_t workspace;                /* with weights_out: b200_kv_attend_workspace() bytes, 16-byte aligned */
+    uint64_t workspace;                /* b200_kv_attend_workspace() bytes, 16-byte aligned; holds nothing between calls */
     uint64_t workspace_bytes;
 } b200_kv_attend_t;
-B200_API uint64_t b200_kv_attend_workspace(const b200_kv_t *kv, int n_head);
+/* Bytes a call with these sizes needs, the more of them with weights_out (0 for unusable sizes). */
+B200_API uint64_t b200_kv_attend_workspace(const b200_kv_t *kv, int n_head, int with_weights);
 B200_API int b200_kv_attend(b200_engine_t *e, const b200_kv_t *kv, const b200_kv_attend_t *a);
 
 /* Eviction: each head of a sequence with more than `budget` slots in use keeps

@@ -148,7 +148,7 @@ SIGNATURES: dict[str, tuple] = {
     "b200_repack_q4_0": (c_int, [c_vp, c_u64, c_int, c_int, c_u64]),
     "b200_device_count": (c_int, []),
     "b200_kv_append": (c_int, [c_vp, P(b200_kv_t), P(b200_kv_append_t)]),
-    "b200_kv_attend_workspace": (c_u64, [P(b200_kv_t), c_int]),
+    "b200_kv_attend_workspace": (c_u64, [P(b200_kv_t), c_int, c_int]),
     "b200_kv_attend": (c_int, [c_vp, P(b200_kv_t), P(b200_kv_attend_t)]),
     "b200_kv_evict": (c_int, [c_vp, P(b200_kv_t), P(b200_kv_evict_t)]),
     "b200_sample": (c_int, [c_vp, P(b200_sample_t)]),

@@ -202,10 +202,8 @@ class Engine:
         shape = (kv.batch, q.shape[1], kv.head_dim)
         qs, os_ = rows(q, "q", shape), rows(out, "out", shape)
         (w, wo), aux = self._aux(kv, weights=weights, weights_out=weights_out)
-        ws, ws_bytes = 0, 0
-        if wo:
-            ws_bytes = int(lib().b200_kv_attend_workspace(ctypes.byref(kv.c), shape[1]))
-            ws = self._workspace(ws_bytes)
+        ws_bytes = int(lib().b200_kv_attend_workspace(ctypes.byref(kv.c), shape[1], int(wo != 0)))
+        ws = self._workspace(ws_bytes)
         a = capi.b200_kv_attend_t(
             q.data_ptr(), out.data_ptr(), dtype_code(q, "q"), shape[1], qs[0], qs[1], os_[0], os_[1],
             kv.head_dim ** -0.5 if scale is None else scale,

@@ -732,7 +732,9 @@ def test_refusals(torch_mod, pkg, eng):
     seen = torch.zeros(2, dtype=torch.int32, device="cuda")
     new = torch.zeros(2, 2, 64, device="cuda")
     ap = capi.b200_kv_append_t(new.data_ptr(), new.data_ptr(), 0, 2, 128, 64, 0, 0, 0, 0, 0, 0, 0)
-    at = capi.b200_kv_attend_t(q.data_ptr(), q.data_ptr(), 0, 4, 256, 64, 256, 64, 0.125, lse.data_ptr(), 0, 0, 0, 1.0, 0, 0)
+    ws = torch.zeros(64 << 20, dtype=torch.uint8, device="cuda")
+    at = capi.b200_kv_attend_t(q.data_ptr(), q.data_ptr(), 0, 4, 256, 64, 256, 64, 0.125, lse.data_ptr(), 0, 0, 0, 1.0,
+                               ws.data_ptr(), ws.numel())
     ev = capi.b200_kv_evict_t(aux.data_ptr(), aux.data_ptr(), pos.data_ptr(), pos.data_ptr(), cache.capacity,
                               seen.data_ptr(), 0, 8, 2, 1)
     sm = capi.b200_sample_t(q.data_ptr(), 0, 2, 256, 256, 0, 0, 0, 0, lse.data_ptr(), seen.data_ptr(), 0)
@@ -748,6 +750,11 @@ def test_refusals(torch_mod, pkg, eng):
         assert rc == -22, (change, rc)
         assert lib.b200_last_error()
 
+    # as they are, the calls are taken: each refusal below is of its one change
+    for call, arg in ((lib.b200_kv_append, ap), (lib.b200_kv_attend, at), (lib.b200_kv_evict, ev)):
+        assert call(eng.h, ctypes.byref(cache.c), ctypes.byref(arg)) == 0
+    assert lib.b200_sample(eng.h, ctypes.byref(sm)) == 0
+    eng.sync()
     kvs = [dict(kv_dtype=3), dict(kv_dtype=-1), dict(kv_batch=0), dict(kv_n_pages=0), dict(kv_page_size=0),
            dict(kv_head_dim=60), dict(kv_head_dim=0), dict(kv_head_dim=264), dict(kv_n_head_kv=0), dict(kv_table_cols=0),
            dict(kv_table_cols=1 << 20), dict(kv_table_stride=1), dict(kv_k=0), dict(kv_v=0), dict(kv_table=0),
@@ -764,10 +771,11 @@ def test_refusals(torch_mod, pkg, eng):
         refused(lib.b200_kv_append, cache.c, ap, **change)
     for change in (dict(dtype=2), dict(n_head=3), dict(n_head=0), dict(q=0), dict(out=0), dict(q=q.data_ptr() + 2),
                    dict(scale=float("nan")), dict(scale=float("inf")), dict(q_head_stride=-1),
-                   dict(weights=aux.data_ptr()), dict(weights_out=aux.data_ptr(), aux_stride=cache.capacity),
-                   dict(weights_out=aux.data_ptr(), aux_stride=1, workspace=aux.data_ptr(), workspace_bytes=1 << 30),
-                   dict(weights_out=aux.data_ptr(), aux_stride=cache.capacity, workspace=aux.data_ptr(),
-                        workspace_bytes=3),
+                   dict(weights=aux.data_ptr()),
+                   dict(weights_out=aux.data_ptr(), aux_stride=1), dict(workspace=0), dict(workspace_bytes=3),
+                   dict(workspace=ws.data_ptr() + 8),
+                   dict(weights_out=aux.data_ptr(), aux_stride=cache.capacity,
+                        workspace_bytes=lib.b200_kv_attend_workspace(ctypes.byref(cache.c), 4, 0)),
                    dict(n_head=2 * 257), dict(kv_dtype=2), dict(kv_dtype=0, dtype=1)):
         refused(lib.b200_kv_attend, cache.c, at, **change)
     for change in (dict(weights=0), dict(weights_out=0), dict(positions=0), dict(positions_out=0), dict(seen=0),
