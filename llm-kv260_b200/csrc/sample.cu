@@ -1,4 +1,17 @@
 // b200_sample: the next token of each row of logits.
+//
+// A row lies in the shared memory of a cluster of CTAs, so its logits are read
+// from memory once; where even eight CTAs have no room for it, the later passes
+// read it again through the L2. Weights are whole numbers, so every sum is the
+// same in any order, and atomics do no harm.
+//
+// The cut that the filters make is found among few candidates. For top-k, the
+// k-th largest of the threads' own maxima bounds the k-th largest logit from
+// below; for top-p, sums over the tokens within 2^-8 and 2^-14 of the largest
+// show whether those hold enough weight. The candidates go to one CTA, which
+// selects by 8-bit digits. A row whose candidates are too many for the list
+// (equal logits, a flat distribution) is cut by the same digits over the whole
+// row.
 #include <cuda_runtime.h>
 
 #include "common.cuh"
@@ -8,10 +21,14 @@ namespace b200 {
 
 namespace {
 
-constexpr int kThreads = 1024;
+constexpr int kThreads = 512;
 constexpr int kWarps = kThreads / 32;
+constexpr int kMaxCluster = 8;
 constexpr int kUnitBits = 40;                  // a token's largest weight is 2^40
 constexpr int kShareBits = 24;                 // u and top_p count in 2^-24
+constexpr int kList = 4096;                    // candidates
+constexpr int kBins = 1024;                    // of the threads' maxima
+constexpr int kMaxListK = 2048;                // top_k beyond this goes by the whole row
 
 using u64 = unsigned long long;
 
@@ -19,6 +36,7 @@ struct SampleArgs {
     const char *logits;
     long long row_stride;   // elements
     int n;
+    int slice;              // 16-byte pieces of a row that a CTA takes
     const float *temperature;
     const int *top_k;
     const float *top_p, *min_p, *u;
@@ -33,10 +51,16 @@ __device__ __forceinline__ uint32_t order_key(float x) {
     return u ^ (u >> 31 ? 0xffffffffu : 0x80000000u);
 }
 
-// 2^((x - top) c), 1 at the top itself (where x - top or c may not be finite).
-// No fused multiply-add: the weight is the same wherever it is computed.
+// log2 of a token's weight, 0 at the top itself (where x - top or c may not be
+// finite). No fused multiply-add: it is the same wherever it is computed.
 __device__ __forceinline__ float exponent(float x, float top, float c) {
     return x == top ? 0.0f : x == -INFINITY ? -INFINITY : __fmul_rn(__fsub_rn(x, top), c);
+}
+// 2^y, to 2 units in its last place; below 2^-41, where a weight is 0, as 0.
+__device__ __forceinline__ float power(float y) {
+    float e;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(y));
+    return y >= -41.0f ? e : 0.0f;
 }
 __device__ __forceinline__ u64 units(float e) { return static_cast<u64>(e * static_cast<float>(1ull << kUnitBits)); }
 
@@ -48,33 +72,72 @@ __device__ __forceinline__ u64 part_up(u64 share, u64 total) {
     return part(share, total) + (((total & 0xffffff) * share & 0xffffff) != 0);
 }
 
-__device__ __forceinline__ u64 block_sum(u64 v, u64 *s) {
-    for (int k = 16; k; k >>= 1) v += __shfl_xor_sync(kFullMask, v, k);
-    __syncthreads();
-    if ((threadIdx.x & 31) == 0) s[threadIdx.x >> 5] = v;
-    __syncthreads();
-    v = s[threadIdx.x & 31];
-    for (int k = 16; k; k >>= 1) v += __shfl_xor_sync(kFullMask, v, k);
+// Another CTA's shared memory (cluster_map addresses).
+__device__ __forceinline__ unsigned cluster_add(uint32_t a, unsigned v) {
+    unsigned old;
+    asm volatile("atom.shared::cluster.add.u32 %0, [%1], %2;" : "=r"(old) : "r"(a), "r"(v) : "memory");
+    return old;
+}
+__device__ __forceinline__ void cluster_store(uint32_t a, u64 v) {
+    asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(a), "l"(v) : "memory");
+}
+__device__ __forceinline__ unsigned cluster_load(uint32_t a) {
+    unsigned v;
+    asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(a) : "memory");
+    return v;
+}
+__device__ __forceinline__ u64 cluster_load64(uint32_t a) {
+    u64 v;
+    asm volatile("ld.shared::cluster.u64 %0, [%1];" : "=l"(v) : "r"(a) : "memory");
     return v;
 }
 
 struct Shared {
-    u64 mass[256];
-    unsigned count[256];
-    u64 warp[32];
-    u64 before, left;
+    u64 mass[2][256];                   // sums by digit, of this call's pass and the one before
+    unsigned count[2][256];
+    unsigned bins[kBins];               // rank 0: the threads' maxima by their distance from the top
+    u64 gather[kMaxCluster][7];         // what every CTA of the cluster tells the others, each thing in a place of its own
+    u64 warp[kWarps];
+    u64 left;
+    u64 weight;
     uint32_t prefix;
-    int index;
+    unsigned listed;                    // rank 0
+    int bin;
 };
 
-// The 8-bit digit at which the sum over bins, taken from the highest, first
-// reaches s.left (as counts or as masses); narrows s.prefix to it.
-template <typename V>
+// Inclusive prefix of one value per thread, and the total.
+__device__ __forceinline__ u64 block_scan(u64 v, u64 *s, u64 *total) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    for (int k = 1; k < 32; k <<= 1) {
+        const u64 y = __shfl_up_sync(kFullMask, v, k);
+        if (lane >= k) v += y;
+    }
+    __syncthreads();
+    if (lane == 31) s[warp] = v;
+    __syncthreads();
+    u64 all = 0;
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) {
+        if (w < warp) v += s[w];
+        all += s[w];
+    }
+    *total = all;
+    return v;
+}
+__device__ __forceinline__ u64 warp_sum(u64 v) {
+    for (int k = 16; k; k >>= 1) v += __shfl_xor_sync(kFullMask, v, k);
+    return v;
+}
+
+// The digit at which the sum over 256 bins (from the highest, or the lowest)
+// first reaches s.left; narrows s.prefix to it. The first warp's work.
+template <bool kFromTop, typename V>
 __device__ __forceinline__ void pick_bin(Shared &s, const V *bins, int shift) {
     if (threadIdx.x >= 32) return;
     const int lane = threadIdx.x;
     u64 c[8], mine = 0;
-    for (int j = 0; j < 8; ++j) mine += c[j] = bins[255 - (lane * 8 + j)];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) mine += c[j] = bins[kFromTop ? 255 - (lane * 8 + j) : lane * 8 + j];
     u64 x = mine;
     for (int k = 1; k < 32; k <<= 1) {
         const u64 y = __shfl_up_sync(kFullMask, x, k);
@@ -86,194 +149,570 @@ __device__ __forceinline__ void pick_bin(Shared &s, const V *bins, int shift) {
     if (lane == __ffs(there) - 1) {
         int j = 0;
         while (before + c[j] < left) before += c[j++];
-        s.prefix |= static_cast<uint32_t>(255 - (lane * 8 + j)) << shift;
+        const int bin = lane * 8 + j;
+        s.prefix |= static_cast<uint32_t>(kFromTop ? 255 - bin : bin) << shift;
         s.left = left - before;
     }
 }
 
-// One CTA per row.
-template <typename T>
-__global__ void __launch_bounds__(kThreads) sample_kernel(const SampleArgs a) {
-    __shared__ Shared s;
-    const int row = blockIdx.x, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, n = a.n;
-    const T *logits = reinterpret_cast<const T *>(a.logits) + row * a.row_stride;
-    const auto at = [&](int i) { return clean(to_float(logits[i])); };
+// Add w to a 64-bit sum in this CTA's shared memory: its halves are summed by
+// 32-bit atomics, which the hardware has, with the low half's carry.
+__device__ __forceinline__ void add_mass(u64 *sum, u64 w) {
+    unsigned *half = reinterpret_cast<unsigned *>(sum);
+    const unsigned lo = static_cast<unsigned>(w), old = atomicAdd(half, lo);
+    const unsigned hi = static_cast<unsigned>(w >> 32) + (old + lo < old);
+    if (hi) atomicAdd(half + 1, hi);
+}
 
-    float top = -INFINITY;
-    for (int i = tid; i < n; i += kThreads) top = fmaxf(top, at(i));
-    for (int k = 16; k; k >>= 1) top = fmaxf(top, __shfl_xor_sync(kFullMask, top, k));
-    if (lane == 0) s.count[warp] = __float_as_uint(top);
-    if (tid == 0) s.index = n;
+// Selection among the N candidates of the list: value(key, idx, &digits) says
+// whether a candidate takes part, what it adds, and by which number it is
+// ordered; `from` is that number's highest digit's shift.
+template <bool kFromTop, typename F>
+__device__ __forceinline__ void select_listed(Shared &s, const u64 *list, int n, int from, u64 left, F value) {
+    const int tid = threadIdx.x;
+    if (tid == 0) s.prefix = 0, s.left = left;
+    for (int shift = from; shift >= 0; shift -= 8) {
+        if (tid < 256) s.mass[0][tid] = 0;
+        __syncthreads();
+        const uint32_t prefix = s.prefix, mask = shift == from ? 0 : kFullMask << (shift + 8);
+        for (int i = tid; i < n; i += kThreads) {
+            uint32_t digits;
+            const u64 w = value(list[i], &digits);
+            if (w && (digits & mask) == prefix) add_mass(&s.mass[0][digits >> shift & 255], w);
+        }
+        __syncthreads();
+        pick_bin<kFromTop>(s, s.mass[0], shift);
+        __syncthreads();
+    }
+}
+
+template <typename T, bool kCached>
+__global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleArgs a) {
+    constexpr int kVe = 16 / sizeof(T);         // elements of a piece
+    extern __shared__ __align__(16) char dyn[];
+    __shared__ Shared s;
+    u64 *list = reinterpret_cast<u64 *>(dyn);   // rank 0: kList candidates, key << 32 | index
+    uint4 *kept_row = reinterpret_cast<uint4 *>(dyn + kList * 8);
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, n = a.n;
+    const unsigned rank = cluster_ctarank();
+    unsigned ctas;
+    asm("mov.u32 %0, %%cluster_nctarank;" : "=r"(ctas));
+    const int row = blockIdx.x / ctas;
+    const T *logits = reinterpret_cast<const T *>(a.logits) + row * a.row_stride;
+    // Pieces are counted from the 16-byte boundary at or before the row's first element: element i of the row is
+    // element i + skew of the pieces.
+    const int skew = static_cast<int>((reinterpret_cast<uintptr_t>(logits) & 15) / sizeof(T));
+    const int pieces = (n + skew + kVe - 1) / kVe;
+    const int p0 = min(static_cast<int>(rank) * a.slice, pieces), p1 = min(p0 + a.slice, pieces);
+    const uint4 *aligned = reinterpret_cast<const uint4 *>(logits - skew);
+    // A warp's pieces lie side by side, so that its tokens do: [w0, w1).
+    const int per_warp = (a.slice / kWarps + 31) / 32 * 32;
+    const int w0 = min(p0 + warp * per_warp, p1), w1 = min(w0 + per_warp, p1);
+
+    const auto fetch = [&](int p) {             // from memory; what is not of the row is -infinity
+        if (p * kVe >= skew && (p + 1) * kVe - skew <= n) return __ldg(aligned + p);
+        union { uint4 v; T t[kVe]; } u;
+#pragma unroll
+        for (int j = 0; j < kVe; ++j) {
+            const int i = p * kVe + j - skew;
+            u.t[j] = i >= 0 && i < n ? logits[i] : from_float<T>(-INFINITY);
+        }
+        return u.v;
+    };
+    const auto piece = [&](int p, float x[kVe]) {
+        union { uint4 v; T t[kVe]; } u;
+        u.v = kCached ? kept_row[p - p0] : fetch(p);
+#pragma unroll
+        for (int j = 0; j < kVe; ++j) x[j] = to_float(u.t[j]);
+    };
+
+    // The largest logit, and the smallest of the threads' maxima that are above -infinity.
+    for (int i = tid; i < kBins; i += kThreads) s.bins[i] = 0;
+    if (tid == 0) s.listed = 0;
+    float own = -INFINITY;                      // the thread's maximum (fmaxf passes NaN over)
+#pragma unroll 4
+    for (int p = w0 + lane; p < w1; p += 32) {
+        union { uint4 v; T t[kVe]; } u;
+        u.v = fetch(p);
+        if (kCached) kept_row[p - p0] = u.v;
+#pragma unroll
+        for (int j = 0; j < kVe; ++j) own = fmaxf(own, to_float(u.t[j]));
+    }
+    float top = own, low = own == -INFINITY ? INFINITY : own;
+    for (int k = 16; k; k >>= 1) {
+        top = fmaxf(top, __shfl_xor_sync(kFullMask, top, k));
+        low = fminf(low, __shfl_xor_sync(kFullMask, low, k));
+    }
+    if (lane == 0) s.warp[warp] = static_cast<u64>(__float_as_uint(top)) << 32 | __float_as_uint(low);
     __syncthreads();
-    top = __uint_as_float(s.count[lane]);
-    for (int k = 16; k; k >>= 1) top = fmaxf(top, __shfl_xor_sync(kFullMask, top, k));
-    __syncthreads();
+    // What each CTA has to say goes to all: gather[rank][slot], and the barrier of the cluster.
+    const auto tell = [&](int slot, u64 v) {
+        if (tid < static_cast<int>(ctas)) cluster_store(cluster_map(&s.gather[rank][slot], tid), v);
+    };
+    {
+        u64 v = s.warp[lane % kWarps];
+        top = __uint_as_float(static_cast<unsigned>(v >> 32));
+        low = __uint_as_float(static_cast<unsigned>(v));
+        for (int k = 16; k; k >>= 1) {
+            top = fmaxf(top, __shfl_xor_sync(kFullMask, top, k));
+            low = fminf(low, __shfl_xor_sync(kFullMask, low, k));
+        }
+        tell(0, static_cast<u64>(__float_as_uint(top)) << 32 | __float_as_uint(low));
+    }
+    cluster_sync_all();
+    for (unsigned q = 0; q < ctas; ++q) {
+        top = fmaxf(top, __uint_as_float(static_cast<unsigned>(s.gather[q][0] >> 32)));
+        low = fminf(low, __uint_as_float(static_cast<unsigned>(s.gather[q][0])));
+    }
+    top += 0.0f;                                // -0 as 0, as the keys have it
+
     const float temp = a.temperature ? a.temperature[row] : 1.0f;
     if (top == -INFINITY) {
-        if (tid == 0) {
+        if (rank == 0 && tid == 0) {
             a.token[row] = -1;
             if (a.logprob) a.logprob[row] = -INFINITY;
         }
         return;
     }
-    if (!(temp > 0.0f)) {
-        for (int i = tid; i < n; i += kThreads)
-            if (at(i) == top) {
-                atomicMin(&s.index, i);
-                break;
-            }
+    if (!(temp > 0.0f)) {                       // the first of the largest
+        int first = 0x7fffffff;
+        for (int p = w0 + lane; p < w1 && first == 0x7fffffff; p += 32) {
+            float x[kVe];
+            piece(p, x);
+#pragma unroll
+            for (int j = kVe - 1; j >= 0; --j)
+                if (x[j] == top) first = p * kVe + j - skew;
+        }
+        for (int k = 16; k; k >>= 1) first = min(first, __shfl_xor_sync(kFullMask, first, k));
+        if (lane == 0) s.warp[warp] = first;
         __syncthreads();
-        if (tid == 0) {
-            a.token[row] = s.index;
+        for (int w = 0; w < kWarps; ++w) first = min(first, static_cast<int>(s.warp[w]));
+        tell(1, first);
+        cluster_sync_all();
+        if (rank == 0 && tid == 0) {
+            for (unsigned q = 0; q < ctas; ++q) first = min(first, static_cast<int>(s.gather[q][1]));
+            a.token[row] = first;
             if (a.logprob) a.logprob[row] = 0.0f;
         }
         return;
     }
     const float c = __fdiv_rn(1.44269504088896340736f, temp);
     const float min_p = a.min_p && a.min_p[row] > 0.0f ? a.min_p[row] : 0.0f;
-    const auto weight = [&](float x) { return units(exp2f(exponent(x, top, c))); };
-
-    // What the filters keep: keys above `edge`, and the first `ties` at it.
-    uint32_t edge = 0;
-    u64 ties = 0;
-    const int k = a.top_k ? a.top_k[row] : 0;
-    if (k > 0 && k < n) {
-        if (tid == 0) s.prefix = 0, s.left = static_cast<u64>(k);
-        for (int shift = 24; shift >= 0; shift -= 8) {
-            if (tid < 256) s.count[tid] = 0;
-            __syncthreads();
-            const uint32_t prefix = s.prefix, mask = shift == 24 ? 0 : kFullMask << (shift + 8);
-            for (int i = tid; i < n; i += kThreads) {
-                const uint32_t key = order_key(at(i));
-                if ((key & mask) == prefix) atomicAdd(&s.count[(key >> shift) & 255], 1u);
-            }
-            __syncthreads();
-            pick_bin(s, s.count, shift);
-            __syncthreads();
-        }
-        edge = s.prefix;
-        ties = s.left;
-        __syncthreads();
-    }
+    const auto weight = [&](float x) { return units(power(exponent(x, top, c))); };
+    const int k = a.top_k && a.top_k[row] > 0 && a.top_k[row] < n ? a.top_k[row] : 0;
     const float share_p = a.top_p ? a.top_p[row] : 1.0f;
     const long long p24 = share_p < 1.0f ? __float2ll_rn(fmaxf(share_p, 0.0f) * 16777216.0f) : 1ll << kShareBits;
-    if (p24 < 1ll << kShareBits) {
-        u64 sum = 0, at_edge = 0;
-        for (int i = tid; i < n; i += kThreads) {
-            const float x = at(i);
-            const uint32_t key = order_key(x);
-            if (key > edge) sum += weight(x);
-            else if (key == edge) at_edge = weight(x);
+    const bool by_p = p24 < 1ll << kShareBits;
+    const float u = a.u[row];
+    const u64 share = u > 0.0f ? static_cast<u64>(fminf(u, 1.0f - 0x1p-24f) * 16777216.0f) : 0;
+    const auto finish = [&](int token, float x, u64 total) {
+        a.token[row] = token;
+        if (a.logprob)
+            a.logprob[row] = exponent(x, top, c) * 0.693147180559945309417f -
+                             logf(static_cast<float>(total) * (1.0f / static_cast<float>(1ull << kUnitBits)));
+    };
+
+    // The smallest logit that can be kept, where few enough can be.
+    bool listed = false;
+    float floor_x = -INFINITY;
+    if (k > 0 && k <= kMaxListK) {
+        listed = true;
+        const float scale = top > low ? (kBins - 1) / (top - low) : 0.0f;   // 0 where top - low overflows, too
+        if (own != -INFINITY) {
+            const int bin = own == top ? 0 : min(static_cast<int>((top - own) * scale), kBins - 1);
+            cluster_add(cluster_map(&s.bins[bin], 0), 1);
         }
-        sum = block_sum(sum, s.warp);
-        // every tie weighs the same: one thread's is all that is needed
-        if (tid == 0) s.before = 0;
+        cluster_sync_all();
+        // the bin with the k-th largest maximum: its far edge, and a little for the rounding of the bins
+        const uint32_t bins = cluster_map(s.bins, 0);
+        constexpr int kPer = kBins / kThreads;
+        u64 mine[kPer], sum = 0, total;
+        for (int j = 0; j < kPer; ++j) sum += mine[j] = cluster_load(bins + (tid * kPer + j) * 4);
+        u64 before = block_scan(sum, s.warp, &total) - sum;
+        if (tid == 0) s.bin = kBins;
         __syncthreads();
-        if (at_edge) s.before = at_edge;
+        if (before < static_cast<u64>(k) && static_cast<u64>(k) <= before + sum) {
+            int j = 0;
+            while (before + mine[j] < static_cast<u64>(k)) before += mine[j++];
+            s.bin = tid * kPer + j;
+        }
         __syncthreads();
-        at_edge = s.before * ties;
-        u64 need = part_up(static_cast<u64>(p24), sum + at_edge);
-        if (need < 1) need = 1;
+        if (s.bin < kBins - 1 && scale > 0.0f) floor_x = top - (s.bin + 1.01f) / scale;
+    } else if (k == 0 && by_p) {
+        // the weight of all tokens, and of those within 2^-8 and 2^-14 of the largest
+        u64 all = 0, near = 0, mid = 0;
+        for (int p = w0 + lane; p < w1; p += 32) {
+            float x[kVe];
+            piece(p, x);
+#pragma unroll
+            for (int j = 0; j < kVe; ++j) {
+                const float y = exponent(x[j], top, c);
+                const u64 w = units(power(y));
+                all += w;
+                if (y >= -14.0f) mid += w;
+                if (y >= -8.0f) near += w;
+            }
+        }
+        all = warp_sum(all), near = warp_sum(near), mid = warp_sum(mid);
+        if (lane == 0) s.mass[0][warp] = all, s.mass[0][32 + warp] = near, s.mass[0][64 + warp] = mid;
         __syncthreads();
-        if (tid == 0) s.prefix = 0, s.left = need;
-        for (int shift = 24; shift >= 0; shift -= 8) {
-            if (tid < 256) s.mass[tid] = 0;
-            __syncthreads();
-            const uint32_t prefix = s.prefix, mask = shift == 24 ? 0 : kFullMask << (shift + 8);
-            for (int i = tid; i < n; i += kThreads) {
-                const float x = at(i);
-                const uint32_t key = order_key(x);
-                if (key > edge && (key & mask) == prefix) {
-                    const u64 w = weight(x);
-                    if (w) atomicAdd(&s.mass[(key >> shift) & 255], w);
+        all = near = mid = 0;
+        for (int w = 0; w < kWarps; ++w) all += s.mass[0][w], near += s.mass[0][32 + w], mid += s.mass[0][64 + w];
+        tell(1, all), tell(2, near), tell(3, mid);
+        cluster_sync_all();
+        all = near = mid = 0;
+        for (unsigned q = 0; q < ctas; ++q) all += s.gather[q][1], near += s.gather[q][2], mid += s.gather[q][3];
+        const u64 need = part_up(static_cast<u64>(p24), all);
+        s.weight = all;                         // every thread writes the same
+        listed = need <= mid;
+        floor_x = need <= near ? -8.0f : -14.0f;   // in exponents here
+    }
+    if (listed) {
+        const uint32_t where = cluster_map(&s.listed, 0), there = cluster_map(list, 0);
+        for (int base = w0; base < w1; base += 32) {
+            const int p = base + lane;
+            float x[kVe];
+            unsigned take = 0;
+            if (p < w1) {
+                piece(p, x);
+#pragma unroll
+                for (int j = 0; j < kVe; ++j) {
+                    x[j] = clean(x[j]);
+                    if (k > 0 ? x[j] >= floor_x && x[j] != -INFINITY : exponent(x[j], top, c) >= floor_x) take |= 1u << j;
                 }
             }
-            if (tid == 0 && at_edge && (edge & mask) == prefix) atomicAdd(&s.mass[(edge >> shift) & 255], at_edge);
+            if (!__any_sync(kFullMask, take)) continue;
+            int at = __popc(take), sum = at;
+            for (int j = 1; j < 32; j <<= 1) {
+                const int y = __shfl_up_sync(kFullMask, at, j);
+                if (lane >= j) at += y;
+            }
+            sum = __shfl_sync(kFullMask, at, 31);
+            unsigned first = 0;
+            if (lane == 31) first = cluster_add(where, sum);
+            at += static_cast<int>(__shfl_sync(kFullMask, first, 31)) - __popc(take);
+#pragma unroll
+            for (int j = 0; j < kVe; ++j)
+                if (take >> j & 1) {
+                    if (at < kList)
+                        cluster_store(there + at * 8, static_cast<u64>(order_key(x[j])) << 32 | static_cast<unsigned>(p * kVe + j - skew));
+                    ++at;
+                }
+        }
+        cluster_sync_all();
+        listed = cluster_load(where) <= static_cast<unsigned>(kList);
+        cluster_sync_all();                     // all have read it: rank 0 may end
+        if (listed && rank != 0) return;        // and does the rest, in its own memory
+    }
+    if (listed) {
+        const int m = static_cast<int>(s.listed);
+        const auto value_of = [](u64 e) {
+            const uint32_t key = static_cast<uint32_t>(e >> 32);
+            return __uint_as_float(key ^ (key >> 31 ? 0x80000000u : 0xffffffffu));
+        };
+        uint32_t edge = 0;
+        u64 ties = 0, total;
+        if (k > 0 && k < m) {
+            select_listed<true>(s, list, m, 24, k, [](u64 e, uint32_t *d) {
+                *d = static_cast<uint32_t>(e >> 32);
+                return 1ull;
+            });
+            edge = s.prefix;
+            ties = s.left;
+        }
+        if (by_p) {
+            u64 sum = 0;
+            if (k > 0) {                        // of the k, the ties at the edge by their number
+                for (int i = tid; i < m; i += kThreads)
+                    if (static_cast<uint32_t>(list[i] >> 32) > edge) sum += weight(value_of(list[i]));
+                block_scan(sum, s.warp, &sum);
+            } else {
+                sum = s.weight;
+            }
+            u64 w_edge = 0;
+            if (edge) {
+                const uint32_t bits = edge ^ (edge >> 31 ? 0x80000000u : 0xffffffffu);
+                w_edge = weight(__uint_as_float(bits)) * ties;
+            }
+            u64 need = part_up(static_cast<u64>(p24), sum + w_edge);
+            if (need < 1) need = 1;
             __syncthreads();
-            pick_bin(s, s.mass, shift);
+            if (tid == 0) s.prefix = 0, s.left = need;
+            for (int shift = 24; shift >= 0; shift -= 8) {
+                if (tid < 256) s.mass[0][tid] = 0;
+                __syncthreads();
+                const uint32_t prefix = s.prefix, mask = shift == 24 ? 0 : kFullMask << (shift + 8);
+                for (int i = tid; i < m; i += kThreads) {
+                    const uint32_t key = static_cast<uint32_t>(list[i] >> 32);
+                    if (key > edge && (key & mask) == prefix) {
+                        const u64 w = weight(value_of(list[i]));
+                        if (w) add_mass(&s.mass[0][key >> shift & 255], w);
+                    }
+                }
+                if (tid == 0 && w_edge && (edge & mask) == prefix) add_mass(&s.mass[0][edge >> shift & 255], w_edge);
+                __syncthreads();
+                pick_bin<true>(s, s.mass[0], shift);
+                __syncthreads();
+            }
+            edge = s.prefix;
+            const uint32_t bits = edge ^ (edge >> 31 ? 0x80000000u : 0xffffffffu);
+            const u64 w = weight(__uint_as_float(bits));
+            ties = (s.left + w - 1) / w;
+            __syncthreads();
+        }
+        if (min_p > 1.0f) edge = order_key(top), ties = 1;
+        // the ties' lowest indexes: up to `last`
+        u64 equal = 0;
+        for (int i = tid; i < m; i += kThreads) equal += static_cast<uint32_t>(list[i] >> 32) == edge;
+        block_scan(equal, s.warp, &equal);
+        uint32_t last = kFullMask;
+        if (ties < equal) {
+            select_listed<false>(s, list, m, 16, ties, [edge](u64 e, uint32_t *d) {
+                *d = static_cast<uint32_t>(e);
+                return static_cast<u64>(static_cast<uint32_t>(e >> 32) == edge);
+            });
+            last = s.prefix;
+        }
+        const auto kept = [&](u64 e, uint32_t *d) -> u64 {
+            const uint32_t key = static_cast<uint32_t>(e >> 32);
+            *d = static_cast<uint32_t>(e);
+            if (key < edge || (key == edge && *d > last)) return 0;
+            const float x = value_of(e), v = power(exponent(x, top, c));
+            return v < min_p && x != top ? 0 : units(v);
+        };
+        u64 sum = 0;
+        for (int i = tid; i < m; i += kThreads) {
+            uint32_t d;
+            sum += kept(list[i], &d);
+        }
+        block_scan(sum, s.warp, &total);
+        __syncthreads();
+        select_listed<false>(s, list, m, 16, part(share, total) + 1, kept);
+        const uint32_t token = s.prefix;
+        for (int i = tid; i < m; i += kThreads)
+            if (static_cast<uint32_t>(list[i]) == token) finish(static_cast<int>(token), value_of(list[i]), total);
+        return;
+    }
+
+    // The whole row, cut by 8-bit digits of its keys where it is cut at all: above `edge`, and the first `ties` at it.
+    uint32_t edge = 0;
+    u64 ties = 0;
+    int turn = 0;
+    const auto select_row = [&](u64 left, bool by_mass, u64 edge_mass) {
+        if (tid == 0) s.prefix = 0, s.left = left;
+        for (int shift = 24; shift >= 0; shift -= 8, turn ^= 1) {
+            if (tid < 256) s.mass[turn][tid] = 0, s.count[turn][tid] = 0;
+            __syncthreads();
+            const uint32_t prefix = s.prefix, mask = shift == 24 ? 0 : kFullMask << (shift + 8);
+            for (int p = w0 + lane; p < w1; p += 32) {
+                float x[kVe];
+                piece(p, x);
+#pragma unroll
+                for (int j = 0; j < kVe; ++j) {
+                    const float v = clean(x[j]);
+                    const uint32_t key = order_key(v);
+                    const int i = p * kVe + j - skew;
+                    if (i < 0 || i >= n || (key & mask) != prefix) continue;
+                    if (!by_mass) {
+                        atomicAdd(&s.count[turn][key >> shift & 255], 1u);
+                    } else if (key > edge) {
+                        const u64 w = weight(v);
+                        if (w) add_mass(&s.mass[turn][key >> shift & 255], w);
+                    }
+                }
+            }
+            if (rank == 0 && tid == 0 && edge_mass && (edge & mask) == prefix) add_mass(&s.mass[turn][edge >> shift & 255], edge_mass);
+            // every CTA adds up all CTAs' sums; the next pass uses the other set, so one barrier a pass is enough
+            cluster_sync_all();
+            u64 sum = 0;
+            if (tid < 256)
+                for (unsigned q = 0; q < ctas; ++q)
+                    sum += by_mass ? cluster_load64(cluster_map(&s.mass[turn][tid], q)) : cluster_load(cluster_map(&s.count[turn][tid], q));
+            __syncthreads();
+            u64 *all = reinterpret_cast<u64 *>(s.bins);
+            if (tid < 256) all[tid] = sum;
+            __syncthreads();
+            pick_bin<true>(s, all, shift);
             __syncthreads();
         }
         edge = s.prefix;
-        const u64 left = s.left;
-        const uint32_t u = edge ^ (edge >> 31 ? 0x80000000u : 0xffffffffu);
-        const u64 w = weight(__uint_as_float(u));
-        ties = (left + w - 1) / w;
+        left = s.left;
         __syncthreads();
+        return left;
+    };
+    if (k > 0) ties = select_row(k, false, 0);
+    if (by_p) {
+        u64 sum = 0;
+        for (int p = w0 + lane; p < w1; p += 32) {
+            float x[kVe];
+            piece(p, x);
+#pragma unroll
+            for (int j = 0; j < kVe; ++j) {
+                const float v = clean(x[j]);
+                if (order_key(v) > edge) sum += weight(v);
+            }
+        }
+        block_scan(sum, s.warp, &sum);
+        tell(4, sum);
+        cluster_sync_all();
+        sum = 0;
+        for (unsigned q = 0; q < ctas; ++q) sum += s.gather[q][4];
+        u64 at_edge = 0;
+        if (edge) {
+            const uint32_t bits = edge ^ (edge >> 31 ? 0x80000000u : 0xffffffffu);
+            at_edge = weight(__uint_as_float(bits)) * ties;
+        }
+        u64 need = part_up(static_cast<u64>(p24), sum + at_edge);
+        if (need < 1) need = 1;
+        const u64 left = select_row(need, true, at_edge);
+        const uint32_t bits = edge ^ (edge >> 31 ? 0x80000000u : 0xffffffffu);
+        const u64 w = weight(__uint_as_float(bits));
+        ties = (left + w - 1) / w;
     }
     if (min_p > 1.0f) edge = order_key(top), ties = 1;
 
-    // The kept weight of each warp's stretch of the row, and where u falls.
-    const int per_warp = ((n + kWarps - 1) / kWarps + 31) / 32 * 32;
-    const int i0 = min(warp * per_warp, n), i1 = min(i0 + per_warp, n);
-    u64 sum = 0, equal = 0, w_edge = 0;
-    const auto kept = [&](float x, u64 *w, bool *tie) {
-        const uint32_t key = order_key(x);
-        *w = 0;
+    // The kept weight of each warp's tokens, and where u falls among them.
+    const auto kept = [&](float x, bool *tie) -> u64 {
         *tie = false;
-        if (key < edge) return;
-        const float e = exp2f(exponent(x, top, c));
-        if (e < min_p && x != top) return;
-        *w = units(e);
-        *tie = key == edge;
+        if (edge) {
+            const uint32_t key = order_key(x);
+            if (key < edge) return 0;
+            *tie = key == edge;
+        }
+        const float e = power(exponent(x, top, c));
+        return e < min_p && x != top ? 0 : units(e);
     };
-    for (int i = i0 + lane; i < i1; i += 32) {
-        u64 w;
-        bool tie;
-        kept(at(i), &w, &tie);
-        if (tie) ++equal, w_edge = w;
-        else sum += w;
+    u64 sum = 0, equal = 0, w_edge = 0;
+    for (int p = w0 + lane; p < w1; p += 32) {
+        float x[kVe];
+        piece(p, x);
+#pragma unroll
+        for (int j = 0; j < kVe; ++j) {
+            bool tie;
+            const u64 w = kept(clean(x[j]), &tie);
+            if (tie) ++equal, w_edge = w; else sum += w;
+        }
     }
-    for (int x = 16; x; x >>= 1) {
-        sum += __shfl_xor_sync(kFullMask, sum, x);
-        equal += __shfl_xor_sync(kFullMask, equal, x);
-        w_edge = max(w_edge, __shfl_xor_sync(kFullMask, w_edge, x));
-    }
-    if (lane == 0) s.warp[warp] = equal;
-    __syncthreads();
+    sum = warp_sum(sum);
     u64 ties_before = 0;
-    for (int j = 0; j < warp; ++j) ties_before += s.warp[j];
-    const u64 mine = ties > ties_before ? min(equal, ties - ties_before) : 0;
-    sum += mine * w_edge;
+    if (edge) {
+        equal = warp_sum(equal);
+        for (int j = 16; j; j >>= 1) w_edge = max(w_edge, __shfl_xor_sync(kFullMask, w_edge, j));
+        __syncthreads();
+        if (lane == 0) s.warp[warp] = equal;
+        __syncthreads();
+        u64 here = 0;
+        for (int w = 0; w < kWarps; ++w) {
+            if (w < warp) ties_before += s.warp[w];
+            here += s.warp[w];
+        }
+        tell(5, here);
+        cluster_sync_all();
+        for (unsigned q = 0; q < rank; ++q) ties_before += s.gather[q][5];
+        sum += (ties > ties_before ? min(equal, ties - ties_before) : 0) * w_edge;
+    }
     __syncthreads();
     if (lane == 0) s.warp[warp] = sum;
     __syncthreads();
     u64 before = 0, total = 0;
-    for (int j = 0; j < kWarps; ++j) {
-        if (j < warp) before += s.warp[j];
-        total += s.warp[j];
+    for (int w = 0; w < kWarps; ++w) {
+        if (w < warp) before += s.warp[w];
+        total += s.warp[w];
     }
-    const float u = a.u[row];
-    const u64 share = u > 0.0f ? static_cast<u64>(fminf(u, 1.0f - 0x1p-24f) * 16777216.0f) : 0;
+    tell(6, total);
+    cluster_sync_all();
+    total = 0;
+    for (unsigned q = 0; q < ctas; ++q) {
+        if (q < rank) before += s.gather[q][6];
+        total += s.gather[q][6];
+    }
     const u64 target = part(share, total);
-    if (before <= target && target < before + sum) {
-        u64 run = before, seen = ties_before;
-        for (int base = i0; base < i1; base += 32) {
-            const int i = base + lane;
-            u64 w = 0;
-            bool tie = false;
-            float x = -INFINITY;
-            if (i < i1) kept(x = at(i), &w, &tie);
-            const unsigned eq = __ballot_sync(kFullMask, tie);
-            if (tie && seen + __popc(eq & ((1u << lane) - 1)) >= ties) w = 0;
-            u64 upto = w;
+    if (target < before || target >= before + sum) return;
+    u64 run = before, seen = ties_before;
+    for (int base = w0; base < w1; base += 32) {
+        const int p = base + lane;
+        u64 w[kVe], mine = 0;
+        float x[kVe];
+        unsigned eq = 0;
+        if (p < w1) {
+            piece(p, x);
+#pragma unroll
+            for (int j = 0; j < kVe; ++j) {
+                bool tie;
+                x[j] = clean(x[j]);
+                w[j] = kept(x[j], &tie);
+                if (tie) eq |= 1u << j;
+            }
+        }
+        if (edge) {                             // ties past the last one that is kept weigh nothing
+            int upto = __popc(eq);
             for (int j = 1; j < 32; j <<= 1) {
-                const u64 y = __shfl_up_sync(kFullMask, upto, j);
+                const int y = __shfl_up_sync(kFullMask, upto, j);
                 if (lane >= j) upto += y;
             }
-            const unsigned hit = __ballot_sync(kFullMask, run + upto > target);
-            if (hit) {
-                if (lane == __ffs(hit) - 1) {
-                    a.token[row] = i;
-                    if (a.logprob)
-                        a.logprob[row] = exponent(x, top, c) * 0.693147180559945309417f -
-                                         logf(static_cast<float>(total) * (1.0f / static_cast<float>(1ull << kUnitBits)));
-                }
-                break;
-            }
-            run += __shfl_sync(kFullMask, upto, 31);
-            seen += __popc(eq);
+            u64 t = seen + upto - __popc(eq);
+#pragma unroll
+            for (int j = 0; j < kVe; ++j)
+                if (eq >> j & 1 && t++ >= ties) w[j] = 0;
+            seen += __shfl_sync(kFullMask, upto, 31);
         }
+        if (p < w1)
+#pragma unroll
+            for (int j = 0; j < kVe; ++j) mine += w[j];
+        u64 upto = mine;
+        for (int j = 1; j < 32; j <<= 1) {
+            const u64 y = __shfl_up_sync(kFullMask, upto, j);
+            if (lane >= j) upto += y;
+        }
+        const unsigned hit = __ballot_sync(kFullMask, run + upto > target);
+        if (hit) {
+            if (lane == __ffs(hit) - 1) {
+                u64 at = run + upto - mine;
+                bool done = false;
+#pragma unroll
+                for (int j = 0; j < kVe; ++j) {
+                    at += w[j];
+                    if (!done && at > target) {
+                        done = true;
+                        finish(p * kVe + j - skew, x[j], total);
+                    }
+                }
+            }
+            return;
+        }
+        run += __shfl_sync(kFullMask, upto, 31);
     }
+}
+
+template <typename T, bool kCached>
+cudaError_t launch(const SampleArgs &a, int batch, int ctas, cudaStream_t stream) {
+    const int smem = kList * 8 + (kCached ? a.slice * 16 : 0);
+    if (!ensure_smem(reinterpret_cast<const void *>(sample_kernel<T, kCached>), smem)) return cudaErrorInvalidValue;
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(batch * ctas);
+    cfg.blockDim = dim3(kThreads);
+    cfg.dynamicSmemBytes = static_cast<size_t>(smem);
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = static_cast<unsigned>(ctas);
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, sample_kernel<T, kCached>, a);
+}
+
+// CTAs to a row: as many as give each at least 16 KB of it and the GPU work
+// (a few rows alone), or as its share must have to fit beside another CTA's.
+template <typename T>
+cudaError_t launch_rows(SampleArgs a, int batch, cudaStream_t stream) {
+    constexpr int kVe = 16 / sizeof(T);
+    constexpr int kFit = 68 * 1024, kMost = 180 * 1024;
+    const int pieces = (a.n + 2 * kVe - 2) / kVe;          // wherever the row begins
+    int ctas = 1;
+    while (ctas < kMaxCluster && (pieces * 16 / ctas > kFit || (batch * ctas < sm_count() && pieces * 16 / ctas >= 2 * 16384))) ctas *= 2;
+    a.slice = ((pieces + ctas - 1) / ctas + kWarps * 32 - 1) / (kWarps * 32) * (kWarps * 32);
+    return a.slice * 16 <= kMost ? launch<T, true>(a, batch, ctas, stream) : launch<T, false>(a, batch, ctas, stream);
 }
 
 }  // namespace
@@ -304,10 +743,9 @@ cudaError_t sample_launch(const b200_sample_t *p, cudaStream_t stream) {
     a.u = reinterpret_cast<const float *>(p->u);
     a.token = reinterpret_cast<int *>(p->token);
     a.logprob = reinterpret_cast<float *>(p->logprob);
-    if (p->dtype == B200_F32) sample_kernel<float><<<p->batch, kThreads, 0, stream>>>(a);
-    else if (p->dtype == B200_F16) sample_kernel<__half><<<p->batch, kThreads, 0, stream>>>(a);
-    else sample_kernel<__nv_bfloat16><<<p->batch, kThreads, 0, stream>>>(a);
-    return cudaGetLastError();
+    if (p->dtype == B200_F32) return launch_rows<float>(a, p->batch, stream);
+    if (p->dtype == B200_F16) return launch_rows<__half>(a, p->batch, stream);
+    return launch_rows<__nv_bfloat16>(a, p->batch, stream);
 }
 
 }  // namespace b200
