@@ -7,11 +7,12 @@
 //
 // The cut that the filters make is found among few candidates. For top-k, the
 // k-th largest of the threads' own maxima bounds the k-th largest logit from
-// below; for top-p, sums over the tokens within 2^-8 and 2^-14 of the largest
-// show whether those hold enough weight. The candidates go to one CTA, which
-// selects by 8-bit digits. A row whose candidates are too many for the list
-// (equal logits, a flat distribution) is cut by the same digits over the whole
-// row.
+// below; for top-p, a sum over the tokens within 2^-10 of the largest shows
+// whether those hold enough weight. The candidates go to one CTA, which
+// orders a few each against each, and selects among more by 8-bit digits. A row that they do not settle (a flat distribution,
+// a large k) is summed by distance from the top over all its tokens first, and
+// the bin that the cut falls in goes to the list; one with too many equal logits
+// for that is cut by digits of all its keys.
 #include <cuda_runtime.h>
 
 #include "common.cuh"
@@ -29,6 +30,8 @@ constexpr int kShareBits = 24;                 // u and top_p count in 2^-24
 constexpr int kList = 4096;                    // candidates
 constexpr int kBins = 1024;                    // of the threads' maxima
 constexpr int kMaxListK = 2048;                // top_k beyond this goes by the whole row
+constexpr float kNear = -10.0f;                // exponents near the top, tried first for top-p
+constexpr int kFew = 256;                      // candidates that are ordered each against each
 
 using u64 = unsigned long long;
 
@@ -37,6 +40,7 @@ struct SampleArgs {
     long long row_stride;   // elements
     int n;
     int slice;              // 16-byte pieces of a row that a CTA takes
+    unsigned *status;       // the device's status word
     const float *temperature;
     const int *top_k;
     const float *top_p, *min_p, *u;
@@ -62,7 +66,24 @@ __device__ __forceinline__ float power(float y) {
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(y));
     return y >= -41.0f ? e : 0.0f;
 }
-__device__ __forceinline__ u64 units(float e) { return static_cast<u64>(e * static_cast<float>(1ull << kUnitBits)); }
+// floor(2^40 e), e <= 1, as (hi - kBase) * 2^23 + (lo - kBase): adding 2^23 with
+// rounding down leaves a whole number in the low bits, on the ordinary float
+// pipe (a conversion to 64 bits has a small part of its rate). Sums of hi and
+// of lo stay apart, in 32 bits, as long as they are short.
+constexpr uint32_t kBase = 0x4b000000u;        // bits of 2^23
+__device__ __forceinline__ void split_units(float e, uint32_t *hi, uint32_t *lo) {
+    const float t = e * 131072.0f, h = __fadd_rd(t, 8388608.0f);
+    *hi = __float_as_uint(h);
+    *lo = __float_as_uint(__fmaf_rd(t - (h - 8388608.0f), 8388608.0f, 8388608.0f));
+}
+__device__ __forceinline__ u64 join_units(uint32_t hi, uint32_t lo, uint32_t count) {
+    return (static_cast<u64>(hi - count * kBase) << 23) + (lo - count * kBase);
+}
+__device__ __forceinline__ u64 units(float e) {
+    uint32_t hi, lo;
+    split_units(e, &hi, &lo);
+    return join_units(hi, lo, 1);
+}
 
 // floor(share * total / 2^24), total < 2^62, and the same rounded up.
 __device__ __forceinline__ u64 part(u64 share, u64 total) {
@@ -93,10 +114,10 @@ __device__ __forceinline__ u64 cluster_load64(uint32_t a) {
 }
 
 struct Shared {
-    u64 mass[2][256];                   // sums by digit, of this call's pass and the one before
-    unsigned count[2][256];
+    u64 mass[2][256];                   // sums by digit, of this pass and the one before
+    u64 sums[kBins];                    // sums by distance from the top
     unsigned bins[kBins];               // rank 0: the threads' maxima by their distance from the top
-    u64 gather[kMaxCluster][7];         // what every CTA of the cluster tells the others, each thing in a place of its own
+    u64 gather[kMaxCluster][9];         // what every CTA of the cluster tells the others, each thing in a place of its own
     u64 warp[kWarps];
     u64 left;
     u64 weight;
@@ -186,11 +207,16 @@ __device__ __forceinline__ void select_listed(Shared &s, const u64 *list, int n,
     }
 }
 
+__device__ __forceinline__ float value_of(uint32_t key) {
+    return __uint_as_float(key ^ (key >> 31 ? 0x80000000u : 0xffffffffu));
+}
+
 template <typename T, bool kCached>
 __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleArgs a) {
     constexpr int kVe = 16 / sizeof(T);         // elements of a piece
     extern __shared__ __align__(16) char dyn[];
     __shared__ Shared s;
+    __shared__ uint64_t s_bar[kWarps];
     u64 *list = reinterpret_cast<u64 *>(dyn);   // rank 0: kList candidates, key << 32 | index
     uint4 *kept_row = reinterpret_cast<uint4 *>(dyn + kList * 8);
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, n = a.n;
@@ -226,17 +252,32 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleArgs a)
         for (int j = 0; j < kVe; ++j) x[j] = to_float(u.t[j]);
     };
 
+    if (kCached) {                              // a warp's whole pieces by one bulk copy, those at the row's ends apart
+        const int whole = (n + skew) / kVe, b0 = max(w0, skew ? 1 : 0), b1 = min(w1, whole);
+        if (lane == 0) {
+            mbar_init(&s_bar[warp], 1);
+            fence_mbar_init();
+            if (b0 < b1) {
+                mbar_arrive_expect_tx(&s_bar[warp], (b1 - b0) * 16);
+                bulk_g2s(kept_row + (b0 - p0), aligned + b0, (b1 - b0) * 16, &s_bar[warp], l2_policy_evict_first());
+            }
+        }
+        if (lane == 1 && w0 == 0 && skew && w1 > 0) kept_row[0] = fetch(0);
+        if (lane == 2 && w0 <= whole && whole < w1 && !(whole == 0 && skew)) kept_row[whole - p0] = fetch(whole);
+        __syncwarp();
+        if (b0 < b1) wait_stage(&s_bar[warp], 0, a.status);
+    }
+
     // The largest logit, and the smallest of the threads' maxima that are above -infinity.
     for (int i = tid; i < kBins; i += kThreads) s.bins[i] = 0;
     if (tid == 0) s.listed = 0;
     float own = -INFINITY;                      // the thread's maximum (fmaxf passes NaN over)
 #pragma unroll 4
     for (int p = w0 + lane; p < w1; p += 32) {
-        union { uint4 v; T t[kVe]; } u;
-        u.v = fetch(p);
-        if (kCached) kept_row[p - p0] = u.v;
+        float x[kVe];
+        piece(p, x);
 #pragma unroll
-        for (int j = 0; j < kVe; ++j) own = fmaxf(own, to_float(u.t[j]));
+        for (int j = 0; j < kVe; ++j) own = fmaxf(own, x[j]);
     }
     float top = own, low = own == -INFINITY ? INFINITY : own;
     for (int k = 16; k; k >>= 1) {
@@ -299,6 +340,14 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleArgs a)
     const float c = __fdiv_rn(1.44269504088896340736f, temp);
     const float min_p = a.min_p && a.min_p[row] > 0.0f ? a.min_p[row] : 0.0f;
     const auto weight = [&](float x) { return units(power(exponent(x, top, c))); };
+    // where x - top and c are finite numbers, the exponent is their product, whatever x (-infinity, NaN: far below 0)
+    const bool plain = top < INFINITY && c < INFINITY;
+    const auto plain_power = [&](float x, float *y) {
+        *y = fmaxf(__fmul_rn(__fsub_rn(x, top), c), -64.0f);
+        float e;
+        asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(*y));
+        return e;
+    };
     const int k = a.top_k && a.top_k[row] > 0 && a.top_k[row] < n ? a.top_k[row] : 0;
     const float share_p = a.top_p ? a.top_p[row] : 1.0f;
     const long long p24 = share_p < 1.0f ? __float2ll_rn(fmaxf(share_p, 0.0f) * 16777216.0f) : 1ll << kShareBits;
@@ -339,36 +388,40 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleArgs a)
         __syncthreads();
         if (s.bin < kBins - 1 && scale > 0.0f) floor_x = top - (s.bin + 1.01f) / scale;
     } else if (k == 0 && by_p) {
-        // the weight of all tokens, and of those within 2^-8 and 2^-14 of the largest
-        u64 all = 0, near = 0, mid = 0;
+        // the weight of all tokens, and of those within 2^-10 of the largest
+        u64 all = 0, near = 0;
         for (int p = w0 + lane; p < w1; p += 32) {
             float x[kVe];
             piece(p, x);
+            uint32_t hi = 0, lo = 0, near_hi = 0, near_lo = 0, near_count = 0;
 #pragma unroll
             for (int j = 0; j < kVe; ++j) {
-                const float y = exponent(x[j], top, c);
-                const u64 w = units(power(y));
-                all += w;
-                if (y >= -14.0f) mid += w;
-                if (y >= -8.0f) near += w;
+                float y, e;
+                if (plain) e = plain_power(x[j], &y);
+                else e = power(y = exponent(x[j], top, c));
+                uint32_t h, l;
+                split_units(e, &h, &l);
+                hi += h, lo += l;
+                if (y >= kNear) near_hi += h, near_lo += l, ++near_count;
             }
+            all += join_units(hi, lo, kVe);
+            near += join_units(near_hi, near_lo, near_count);
         }
-        all = warp_sum(all), near = warp_sum(near), mid = warp_sum(mid);
-        if (lane == 0) s.mass[0][warp] = all, s.mass[0][32 + warp] = near, s.mass[0][64 + warp] = mid;
+        all = warp_sum(all), near = warp_sum(near);
+        if (lane == 0) s.mass[0][warp] = all, s.mass[0][32 + warp] = near;
         __syncthreads();
-        all = near = mid = 0;
-        for (int w = 0; w < kWarps; ++w) all += s.mass[0][w], near += s.mass[0][32 + w], mid += s.mass[0][64 + w];
-        tell(1, all), tell(2, near), tell(3, mid);
+        all = near = 0;
+        for (int w = 0; w < kWarps; ++w) all += s.mass[0][w], near += s.mass[0][32 + w];
+        tell(1, all), tell(2, near);
         cluster_sync_all();
-        all = near = mid = 0;
-        for (unsigned q = 0; q < ctas; ++q) all += s.gather[q][1], near += s.gather[q][2], mid += s.gather[q][3];
-        const u64 need = part_up(static_cast<u64>(p24), all);
+        all = near = 0;
+        for (unsigned q = 0; q < ctas; ++q) all += s.gather[q][1], near += s.gather[q][2];
         s.weight = all;                         // every thread writes the same
-        listed = need <= mid;
-        floor_x = need <= near ? -8.0f : -14.0f;   // in exponents here
+        listed = part_up(static_cast<u64>(p24), all) <= near;
     }
-    if (listed) {
-        const uint32_t where = cluster_map(&s.listed, 0), there = cluster_map(list, 0);
+    // Tokens that `wanted` names go to rank 0's list; true where it holds all of them. Between two cluster barriers.
+    const uint32_t where = cluster_map(&s.listed, 0), there = cluster_map(list, 0);
+    const auto collect = [&](auto wanted) {
         for (int base = w0; base < w1; base += 32) {
             const int p = base + lane;
             float x[kVe];
@@ -376,18 +429,16 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleArgs a)
             if (p < w1) {
                 piece(p, x);
 #pragma unroll
-                for (int j = 0; j < kVe; ++j) {
-                    x[j] = clean(x[j]);
-                    if (k > 0 ? x[j] >= floor_x && x[j] != -INFINITY : exponent(x[j], top, c) >= floor_x) take |= 1u << j;
-                }
+                for (int j = 0; j < kVe; ++j)
+                    if (wanted(x[j] = clean(x[j]))) take |= 1u << j;
             }
             if (!__any_sync(kFullMask, take)) continue;
-            int at = __popc(take), sum = at;
+            int at = __popc(take);
             for (int j = 1; j < 32; j <<= 1) {
                 const int y = __shfl_up_sync(kFullMask, at, j);
                 if (lane >= j) at += y;
             }
-            sum = __shfl_sync(kFullMask, at, 31);
+            const int sum = __shfl_sync(kFullMask, at, 31);
             unsigned first = 0;
             if (lane == 31) first = cluster_add(where, sum);
             at += static_cast<int>(__shfl_sync(kFullMask, first, 31)) - __popc(take);
@@ -400,16 +451,65 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleArgs a)
                 }
         }
         cluster_sync_all();
-        listed = cluster_load(where) <= static_cast<unsigned>(kList);
-        cluster_sync_all();                     // all have read it: rank 0 may end
-        if (listed && rank != 0) return;        // and does the rest, in its own memory
+        const bool all = cluster_load(where) <= static_cast<unsigned>(kList);
+        cluster_sync_all();                     // all have read it: rank 0 may go on, or end
+        return all;
+    };
+    if (listed) {
+        if (k > 0) listed = collect([&](float x) { return x >= floor_x && x != -INFINITY; });
+        else listed = collect([&](float x) { return exponent(x, top, c) >= kNear; });
+        if (listed && rank != 0) return;        // rank 0 does the rest, in its own memory
     }
     if (listed) {
         const int m = static_cast<int>(s.listed);
-        const auto value_of = [](u64 e) {
-            const uint32_t key = static_cast<uint32_t>(e >> 32);
-            return __uint_as_float(key ^ (key >> 31 ? 0x80000000u : 0xffffffffu));
-        };
+        if (m <= kFew) {
+            // Each candidate against each, kThreads / wide threads to one: its rank and the weight before it, both in
+            // falling order; then, of what is kept, the weight of lower indexes.
+            int wide = 32;
+            while (wide < m) wide *= 2;
+            const int i = tid & (wide - 1), part0 = tid / wide, parts = kThreads / wide;
+            const u64 e = i < m ? list[i] ^ 0xffffffffull : 0;     // the lower index is the larger number
+            const float x = value_of(static_cast<uint32_t>(e >> 32)), v = power(exponent(x, top, c));
+            const u64 w = i < m ? units(v) : 0;
+            u64 *weights = s.mass[0], *kept = s.mass[1];
+            if (tid < wide) weights[i] = w;
+            __syncthreads();
+            u64 before = 0, sum;
+            unsigned ahead = 0;
+            for (int j = part0; j < m; j += parts)
+                if ((list[j] ^ 0xffffffffull) > e) ++ahead, before += weights[j];
+            s.sums[tid] = before;
+            s.bins[tid] = ahead;
+            __syncthreads();
+            before = ahead = 0;
+            for (int j = 0; j < parts; ++j) before += s.sums[j * wide + i], ahead += s.bins[j * wide + i];
+            bool keep = i < m && (k == 0 || ahead < static_cast<unsigned>(k));
+            if (by_p) {
+                u64 all = s.weight;
+                if (k > 0) block_scan(tid < wide && keep ? w : 0, s.warp, &all);
+                u64 need = part_up(static_cast<u64>(p24), all);
+                if (need < 1) need = 1;
+                keep = keep && before < need;
+            }
+            keep = keep && (v >= min_p || ahead == 0);
+            const u64 mine = keep ? w : 0;
+            block_scan(tid < wide ? mine : 0, s.warp, &sum);
+            if (tid < wide) kept[i] = mine;
+            const u64 target = part(share, sum);
+            const uint32_t index = static_cast<uint32_t>(list[i < m ? i : 0]);
+            __syncthreads();
+            before = 0;
+            for (int j = part0; j < m; j += parts)
+                if (static_cast<uint32_t>(list[j]) < index) before += kept[j];
+            s.sums[tid] = before;
+            __syncthreads();
+            if (tid < wide && mine) {
+                before = 0;
+                for (int j = 0; j < parts; ++j) before += s.sums[j * wide + i];
+                if (before <= target && target < before + mine) finish(static_cast<int>(index), x, sum);
+            }
+            return;
+        }
         uint32_t edge = 0;
         u64 ties = 0, total;
         if (k > 0 && k < m) {
@@ -424,16 +524,13 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleArgs a)
             u64 sum = 0;
             if (k > 0) {                        // of the k, the ties at the edge by their number
                 for (int i = tid; i < m; i += kThreads)
-                    if (static_cast<uint32_t>(list[i] >> 32) > edge) sum += weight(value_of(list[i]));
+                    if (static_cast<uint32_t>(list[i] >> 32) > edge) sum += weight(value_of(static_cast<uint32_t>(list[i] >> 32)));
                 block_scan(sum, s.warp, &sum);
             } else {
                 sum = s.weight;
             }
             u64 w_edge = 0;
-            if (edge) {
-                const uint32_t bits = edge ^ (edge >> 31 ? 0x80000000u : 0xffffffffu);
-                w_edge = weight(__uint_as_float(bits)) * ties;
-            }
+            if (edge) w_edge = weight(value_of(edge)) * ties;
             u64 need = part_up(static_cast<u64>(p24), sum + w_edge);
             if (need < 1) need = 1;
             __syncthreads();
@@ -445,7 +542,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleArgs a)
                 for (int i = tid; i < m; i += kThreads) {
                     const uint32_t key = static_cast<uint32_t>(list[i] >> 32);
                     if (key > edge && (key & mask) == prefix) {
-                        const u64 w = weight(value_of(list[i]));
+                        const u64 w = weight(value_of(static_cast<uint32_t>(list[i] >> 32)));
                         if (w) add_mass(&s.mass[0][key >> shift & 255], w);
                     }
                 }
@@ -455,8 +552,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleArgs a)
                 __syncthreads();
             }
             edge = s.prefix;
-            const uint32_t bits = edge ^ (edge >> 31 ? 0x80000000u : 0xffffffffu);
-            const u64 w = weight(__uint_as_float(bits));
+            const u64 w = weight(value_of(edge));
             ties = (s.left + w - 1) / w;
             __syncthreads();
         }
@@ -477,7 +573,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleArgs a)
             const uint32_t key = static_cast<uint32_t>(e >> 32);
             *d = static_cast<uint32_t>(e);
             if (key < edge || (key == edge && *d > last)) return 0;
-            const float x = value_of(e), v = power(exponent(x, top, c));
+            const float x = value_of(key), v = power(exponent(x, top, c));
             return v < min_p && x != top ? 0 : units(v);
         };
         u64 sum = 0;
@@ -490,18 +586,99 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleArgs a)
         select_listed<false>(s, list, m, 16, part(share, total) + 1, kept);
         const uint32_t token = s.prefix;
         for (int i = tid; i < m; i += kThreads)
-            if (static_cast<uint32_t>(list[i]) == token) finish(static_cast<int>(token), value_of(list[i]), total);
+            if (static_cast<uint32_t>(list[i]) == token) finish(static_cast<int>(token), value_of(static_cast<uint32_t>(list[i] >> 32)), total);
         return;
     }
 
-    // The whole row, cut by 8-bit digits of its keys where it is cut at all: above `edge`, and the first `ties` at it.
+    // The whole row. What the filters keep of it: keys above `edge`, and the first `ties` at it. First by the
+    // distance from the top, in kBins bins up to where a weight is 0; then among the tokens of the bin it falls in;
+    // where those are too many for the list, by 8-bit digits of all keys.
     uint32_t edge = 0;
     u64 ties = 0;
-    int turn = 0;
-    const auto select_row = [&](u64 left, bool by_mass, u64 edge_mass) {
+    constexpr float kBinsPerOctave = kBins / 41.0f;
+    const auto bin_of = [&](float x) {
+        const float y = exponent(x, top, c);
+        return y > -41.0f ? min(static_cast<int>(-y * kBinsPerOctave), kBins - 1) : kBins - 1;
+    };
+    // `left` tokens (or weight, `total` in all) are kept, of those above the present edge and edge_mass at it
+    const auto cut_row = [&](u64 left, bool by_mass, u64 total, u64 edge_mass) {
+        for (int i = tid; i < kBins; i += kThreads) s.sums[i] = 0;
+        if (tid == 0) s.listed = 0;
+        __syncthreads();
+        // tokens so light that all of them together are less than what is given up: the sums from the top do not
+        // come to them
+        const u64 least = by_mass ? (total - left) / static_cast<u64>(n) : 0;
+        for (int p = w0 + lane; p < w1; p += 32) {
+            float x[kVe];
+            piece(p, x);
+#pragma unroll
+            for (int j = 0; j < kVe; ++j) {
+                const float v = clean(x[j]);
+                const int i = p * kVe + j - skew;
+                if (!by_mass) {
+                    if (i >= 0 && i < n) add_mass(&s.sums[bin_of(v)], 1);
+                } else if (order_key(v) > edge) {
+                    const u64 w = weight(v);
+                    if (w > least) add_mass(&s.sums[bin_of(v)], w);
+                }
+            }
+        }
+        if (rank == 0 && tid == 0 && edge_mass) add_mass(&s.sums[bin_of(value_of(edge))], edge_mass);
+        cluster_sync_all();
+        constexpr int kPer = kBins / kThreads;
+        u64 mine[kPer], sum = 0, all;
+        for (int j = 0; j < kPer; ++j) {
+            mine[j] = 0;
+            for (unsigned q = 0; q < ctas; ++q) mine[j] += cluster_load64(cluster_map(&s.sums[tid * kPer + j], q));
+            sum += mine[j];
+        }
+        u64 before = block_scan(sum, s.warp, &all) - sum;
+        if (before < left && left <= before + sum) {
+            int j = 0;
+            while (before + mine[j] < left) before += mine[j++];
+            s.bin = tid * kPer + j;
+            s.weight = left - before;
+        }
+        __syncthreads();
+        const int bin = s.bin;
+        const u64 inside = s.weight;
+        if (bin == kBins - 1) {                 // (of the counts) what follows weighs nothing
+            cluster_sync_all();
+            return;
+        }
+        u64 w = 1;
+        if (collect([&](float x) { return bin_of(x) == bin && (!by_mass || order_key(x) > edge); })) {
+            if (rank == 0) {
+                const int m = static_cast<int>(s.listed);
+                const uint32_t old = edge;
+                if (tid == 0) s.prefix = 0, s.left = inside;
+                for (int shift = 24; shift >= 0; shift -= 8) {
+                    if (tid < 256) s.mass[0][tid] = 0;
+                    __syncthreads();
+                    const uint32_t prefix = s.prefix, mask = shift == 24 ? 0 : kFullMask << (shift + 8);
+                    for (int i = tid; i < m; i += kThreads) {
+                        const uint32_t key = static_cast<uint32_t>(list[i] >> 32);
+                        if ((key & mask) == prefix) add_mass(&s.mass[0][key >> shift & 255], by_mass ? weight(value_of(key)) : 1);
+                    }
+                    if (tid == 0 && edge_mass && bin_of(value_of(old)) == bin && (old & mask) == prefix)
+                        add_mass(&s.mass[0][old >> shift & 255], edge_mass);
+                    __syncthreads();
+                    pick_bin<true>(s, s.mass[0], shift);
+                    __syncthreads();
+                }
+                if (by_mass) w = weight(value_of(s.prefix));
+                tell(by_mass ? 8 : 7, static_cast<u64>(s.prefix) << 32 | ((s.left + w - 1) / w));
+            }
+            cluster_sync_all();
+            edge = static_cast<uint32_t>(s.gather[0][by_mass ? 8 : 7] >> 32);
+            ties = static_cast<uint32_t>(s.gather[0][by_mass ? 8 : 7]);
+            return;
+        }
+        const uint32_t old = edge;
+        int turn = 0;
         if (tid == 0) s.prefix = 0, s.left = left;
         for (int shift = 24; shift >= 0; shift -= 8, turn ^= 1) {
-            if (tid < 256) s.mass[turn][tid] = 0, s.count[turn][tid] = 0;
+            if (tid < 256) s.mass[turn][tid] = 0;
             __syncthreads();
             const uint32_t prefix = s.prefix, mask = shift == 24 ? 0 : kFullMask << (shift + 8);
             for (int p = w0 + lane; p < w1; p += 32) {
@@ -512,35 +689,30 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleArgs a)
                     const float v = clean(x[j]);
                     const uint32_t key = order_key(v);
                     const int i = p * kVe + j - skew;
-                    if (i < 0 || i >= n || (key & mask) != prefix) continue;
-                    if (!by_mass) {
-                        atomicAdd(&s.count[turn][key >> shift & 255], 1u);
-                    } else if (key > edge) {
-                        const u64 w = weight(v);
-                        if (w) add_mass(&s.mass[turn][key >> shift & 255], w);
-                    }
+                    if (i < 0 || i >= n || (key & mask) != prefix || (by_mass && key <= old)) continue;
+                    const u64 add = by_mass ? weight(v) : 1;
+                    if (add) add_mass(&s.mass[turn][key >> shift & 255], add);
                 }
             }
-            if (rank == 0 && tid == 0 && edge_mass && (edge & mask) == prefix) add_mass(&s.mass[turn][edge >> shift & 255], edge_mass);
+            if (rank == 0 && tid == 0 && edge_mass && (old & mask) == prefix) add_mass(&s.mass[turn][old >> shift & 255], edge_mass);
             // every CTA adds up all CTAs' sums; the next pass uses the other set, so one barrier a pass is enough
             cluster_sync_all();
             u64 sum = 0;
             if (tid < 256)
-                for (unsigned q = 0; q < ctas; ++q)
-                    sum += by_mass ? cluster_load64(cluster_map(&s.mass[turn][tid], q)) : cluster_load(cluster_map(&s.count[turn][tid], q));
+                for (unsigned q = 0; q < ctas; ++q) sum += cluster_load64(cluster_map(&s.mass[turn][tid], q));
             __syncthreads();
-            u64 *all = reinterpret_cast<u64 *>(s.bins);
-            if (tid < 256) all[tid] = sum;
+            u64 *sums = s.sums;
+            if (tid < 256) sums[tid] = sum;
             __syncthreads();
-            pick_bin<true>(s, all, shift);
+            pick_bin<true>(s, sums, shift);
             __syncthreads();
         }
         edge = s.prefix;
-        left = s.left;
-        __syncthreads();
-        return left;
+        if (by_mass) w = weight(value_of(edge));
+        ties = (s.left + w - 1) / w;
+        cluster_sync_all();
     };
-    if (k > 0) ties = select_row(k, false, 0);
+    if (k > 0) cut_row(k, false, 0, 0);
     if (by_p) {
         u64 sum = 0;
         for (int p = w0 + lane; p < w1; p += 32) {
@@ -557,40 +729,47 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleArgs a)
         cluster_sync_all();
         sum = 0;
         for (unsigned q = 0; q < ctas; ++q) sum += s.gather[q][4];
-        u64 at_edge = 0;
-        if (edge) {
-            const uint32_t bits = edge ^ (edge >> 31 ? 0x80000000u : 0xffffffffu);
-            at_edge = weight(__uint_as_float(bits)) * ties;
-        }
+        const u64 at_edge = edge ? weight(value_of(edge)) * ties : 0;
         u64 need = part_up(static_cast<u64>(p24), sum + at_edge);
         if (need < 1) need = 1;
-        const u64 left = select_row(need, true, at_edge);
-        const uint32_t bits = edge ^ (edge >> 31 ? 0x80000000u : 0xffffffffu);
-        const u64 w = weight(__uint_as_float(bits));
-        ties = (left + w - 1) / w;
+        cut_row(need, true, sum + at_edge, at_edge);
     }
     if (min_p > 1.0f) edge = order_key(top), ties = 1;
 
     // The kept weight of each warp's tokens, and where u falls among them.
+    const float edge_x = value_of(edge);        // (not a number where there is none)
     const auto kept = [&](float x, bool *tie) -> u64 {
-        *tie = false;
-        if (edge) {
-            const uint32_t key = order_key(x);
-            if (key < edge) return 0;
-            *tie = key == edge;
-        }
+        *tie = edge && x == edge_x;
+        if (edge && !(x >= edge_x)) return 0;
         const float e = power(exponent(x, top, c));
         return e < min_p && x != top ? 0 : units(e);
     };
     u64 sum = 0, equal = 0, w_edge = 0;
-    for (int p = w0 + lane; p < w1; p += 32) {
-        float x[kVe];
-        piece(p, x);
+    if (plain && edge == 0 && min_p == 0.0f) {
+#pragma unroll 2
+        for (int p = w0 + lane; p < w1; p += 32) {
+            float x[kVe];
+            piece(p, x);
+            uint32_t hi = 0, lo = 0;
 #pragma unroll
-        for (int j = 0; j < kVe; ++j) {
-            bool tie;
-            const u64 w = kept(clean(x[j]), &tie);
-            if (tie) ++equal, w_edge = w; else sum += w;
+            for (int j = 0; j < kVe; ++j) {
+                float y;
+                uint32_t h, l;
+                split_units(plain_power(x[j], &y), &h, &l);
+                hi += h, lo += l;
+            }
+            sum += join_units(hi, lo, kVe);
+        }
+    } else {
+        for (int p = w0 + lane; p < w1; p += 32) {
+            float x[kVe];
+            piece(p, x);
+#pragma unroll
+            for (int j = 0; j < kVe; ++j) {
+                bool tie;
+                const u64 w = kept(clean(x[j]), &tie);
+                if (tie) ++equal, w_edge = w; else sum += w;
+            }
         }
     }
     sum = warp_sum(sum);
@@ -707,7 +886,7 @@ cudaError_t launch(const SampleArgs &a, int batch, int ctas, cudaStream_t stream
 template <typename T>
 cudaError_t launch_rows(SampleArgs a, int batch, cudaStream_t stream) {
     constexpr int kVe = 16 / sizeof(T);
-    constexpr int kFit = 68 * 1024, kMost = 180 * 1024;
+    constexpr int kFit = 64 * 1024, kMost = 180 * 1024;
     const int pieces = (a.n + 2 * kVe - 2) / kVe;          // wherever the row begins
     int ctas = 1;
     while (ctas < kMaxCluster && (pieces * 16 / ctas > kFit || (batch * ctas < sm_count() && pieces * 16 / ctas >= 2 * 16384))) ctas *= 2;
@@ -743,6 +922,8 @@ cudaError_t sample_launch(const b200_sample_t *p, cudaStream_t stream) {
     a.u = reinterpret_cast<const float *>(p->u);
     a.token = reinterpret_cast<int *>(p->token);
     a.logprob = reinterpret_cast<float *>(p->logprob);
+    a.status = status_word();
+    if (!a.status) return cudaErrorInvalidDevice;
     if (p->dtype == B200_F32) return launch_rows<float>(a, p->batch, stream);
     if (p->dtype == B200_F16) return launch_rows<__half>(a, p->batch, stream);
     return launch_rows<__nv_bfloat16>(a, p->batch, stream);

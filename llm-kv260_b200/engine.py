@@ -11,7 +11,7 @@ import ctypes
 
 from . import capi
 from .capi import check, lib
-from .paged import PagedKV, dtype_code, rows, typed
+from .paged import PagedKV, address, dtype_code, rows
 
 QK = 32
 BLOCK_BYTES = 18
@@ -79,6 +79,7 @@ class Engine:
         h = ctypes.c_void_p()
         check(lib().b200_engine_open(ctypes.byref(h), device), "b200_engine_open")
         self.h = h
+        self._structs, self._ws = {}, None
         self.set_stream(current_stream_handle(device) if stream is None else stream)
 
     def close(self) -> None:
@@ -159,16 +160,19 @@ class Engine:
     def prefetch(self, W: QMat) -> None:
         check(lib().b200_prefetch(self.h, ctypes.byref(W.c)), "b200_prefetch")
 
-    def _aux(self, kv: PagedKV, **tensors) -> tuple[list[int], int]:
-        """Addresses (0 for None) of weights and positions beside a cache, and the stride they must share."""
-        addr, stride = [], 0
-        for name, t in tensors.items():
-            a, n = (0, 0) if t is None else kv.aux(t, "int32" if name.startswith("positions") else "float32", name)
-            if n and stride and n != stride:
-                raise ValueError("weights and positions must have one shape")
-            stride = stride or n
-            addr.append(a)
-        return addr, stride
+    def _call(self, name: str, struct, values, kv: PagedKV | None = None) -> None:
+        """The C call of that name, its argument struct (one per engine, filled anew each time) set to `values`."""
+        L = lib()
+        kept = self._structs.get(name)
+        if kept is None:
+            c = struct()
+            kept = self._structs[name] = (getattr(L, name), c, ctypes.byref(c), [f for f, _ in struct._fields_])
+        fn, c, ref, fields = kept
+        for f, v in zip(fields, values):
+            setattr(c, f, v)
+        rc = fn(self.h, ref) if kv is None else fn(self.h, kv.ref, ref)
+        if rc < 0:
+            check(rc, name)
 
     def kv_append(self, kv: PagedKV, k_new, v_new, offsets=None, seen=None, positions=None, weights=None,
                   lengths_out=None, seen_out=None) -> None:
@@ -179,43 +183,45 @@ class Engine:
         n = k_new.shape[0]
         shape = (n, kv.n_head_kv, kv.head_dim)
         st = rows(k_new, "k_new", shape)
-        if rows(v_new, "v_new", shape) != st or v_new.dtype != k_new.dtype:
+        if rows(v_new, "v_new", shape) != st or v_new.dtype is not k_new.dtype:
             raise ValueError("k_new and v_new must be alike in type and strides")
-        (pos, w), aux = self._aux(kv, positions=positions, weights=weights)
+        pos, stride = (0, 0) if positions is None else kv.aux(positions, "int32", "positions")
+        w, stride2 = (0, stride) if weights is None else kv.aux(weights, "float32", "weights")
+        if pos and stride != stride2:
+            raise ValueError("weights and positions must have one shape")
         b = (kv.batch,)
-        lengths_out = kv.lengths if lengths_out is None else typed(lengths_out, "int32", "lengths_out", b)
-        seen_out = seen if seen_out is None else typed(seen_out, "int32", "seen_out", b)
-        a = capi.b200_kv_append_t(
+        self._call("b200_kv_append", capi.b200_kv_append_t, (
             k_new.data_ptr(), v_new.data_ptr(), dtype_code(k_new, "k_new"), n, st[0], st[1],
-            0 if offsets is None else dev_ptr(typed(offsets, "int32", "offsets", (kv.batch + 1,))),
-            0 if seen is None else dev_ptr(typed(seen, "int32", "seen", b)), pos, w, aux, dev_ptr(lengths_out),
-            0 if seen_out is None else dev_ptr(seen_out))
-        check(lib().b200_kv_append(self.h, ctypes.byref(kv.c), ctypes.byref(a)), "b200_kv_append")
+            address(offsets, "int32", "offsets", (kv.batch + 1,)), address(seen, "int32", "seen", b), pos, w, stride2,
+            address(kv.lengths if lengths_out is None else lengths_out, "int32", "lengths_out", b),
+            address(seen if seen_out is None else seen_out, "int32", "seen_out", b)), kv)
 
     def kv_attend(self, kv: PagedKV, q, out, lse=None, scale: float | None = None, weights=None, weights_out=None,
                   decay: float = 1.0) -> None:
         """out = softmax(scale q K^T) V for one token per sequence: q and out [batch, n_head, head_dim], lse float32
         [batch, n_head]; scale 1 / sqrt(head_dim) by default. With weights_out, the softmax's weights summed over
         the query heads of a cache head are added to decay * weights (None: zeros)."""
-        if q.dim() != 3 or q.dtype != out.dtype:
+        if q.dim() != 3 or q.dtype is not out.dtype:
             raise ValueError("q and out must be [batch, n_head, head_dim] of one type")
-        shape = (kv.batch, q.shape[1], kv.head_dim)
+        n_head = q.shape[1]
+        shape = (kv.batch, n_head, kv.head_dim)
         qs, os_ = rows(q, "q", shape), rows(out, "out", shape)
-        (w, wo), aux = self._aux(kv, weights=weights, weights_out=weights_out)
-        ws_bytes = int(lib().b200_kv_attend_workspace(ctypes.byref(kv.c), shape[1], int(wo != 0)))
-        ws = self._workspace(ws_bytes)
-        a = capi.b200_kv_attend_t(
-            q.data_ptr(), out.data_ptr(), dtype_code(q, "q"), shape[1], qs[0], qs[1], os_[0], os_[1],
-            kv.head_dim ** -0.5 if scale is None else scale,
-            0 if lse is None else dev_ptr(typed(lse, "float32", "lse", shape[:2])), w, wo, aux, decay, ws, ws_bytes)
-        check(lib().b200_kv_attend(self.h, ctypes.byref(kv.c), ctypes.byref(a)), "b200_kv_attend")
+        wo, stride = (0, 0) if weights_out is None else kv.aux(weights_out, "float32", "weights_out")
+        w, stride2 = (0, stride) if weights is None else kv.aux(weights, "float32", "weights")
+        if wo and stride != stride2:
+            raise ValueError("weights and weights_out must have one shape")
+        ws_bytes = lib().b200_kv_attend_workspace(kv.ref, n_head, 1 if wo else 0)
+        self._call("b200_kv_attend", capi.b200_kv_attend_t, (
+            q.data_ptr(), out.data_ptr(), dtype_code(q, "q"), n_head, qs[0], qs[1], os_[0], os_[1],
+            kv.head_dim ** -0.5 if scale is None else scale, address(lse, "float32", "lse", (kv.batch, n_head)), w, wo,
+            stride2, decay, self._workspace(ws_bytes), ws_bytes), kv)
 
     def _workspace(self, nbytes: int) -> int:
         """Device memory of this engine's own for calls on its stream, kept and grown; one that is given back stays
         reserved until the work queued on that stream is done."""
-        torch = _torch()
-        have = getattr(self, "_ws", None)
+        have = self._ws
         if have is None or have.numel() < nbytes:
+            torch = _torch()
             if have is not None and self.stream:
                 have.record_stream(torch.cuda.ExternalStream(self.stream, device=self.device))
             self._ws = have = torch.empty(nbytes, dtype=torch.uint8, device=f"cuda:{self.device}")
@@ -226,30 +232,30 @@ class Engine:
         """Cut every sequence and head to `budget` slots: the `recent` newest of `seen` tokens, the first `sinks` and
         the largest weights stay. Rows move inside the cache; weights, positions and lengths go to the outputs, by
         default in place."""
-        weights_out = weights if weights_out is None else weights_out
-        positions_out = positions if positions_out is None else positions_out
-        (w, wo, p, po), aux = self._aux(kv, weights=weights, weights_out=weights_out, positions=positions,
-                                        positions_out=positions_out)
+        w, stride = kv.aux(weights, "float32", "weights")
+        wo, s1 = (w, stride) if weights_out is None else kv.aux(weights_out, "float32", "weights_out")
+        p, s2 = kv.aux(positions, "int32", "positions")
+        po, s3 = (p, s2) if positions_out is None else kv.aux(positions_out, "int32", "positions_out")
+        if not stride == s1 == s2 == s3:
+            raise ValueError("weights and positions must have one shape")
         b = (kv.batch,)
-        lengths_out = kv.lengths if lengths_out is None else typed(lengths_out, "int32", "lengths_out", b)
-        a = capi.b200_kv_evict_t(w, wo, p, po, aux, dev_ptr(typed(seen, "int32", "seen", b)), dev_ptr(lengths_out),
-                                 budget, recent, sinks)
-        check(lib().b200_kv_evict(self.h, ctypes.byref(kv.c), ctypes.byref(a)), "b200_kv_evict")
+        self._call("b200_kv_evict", capi.b200_kv_evict_t, (
+            w, wo, p, po, stride, address(seen, "int32", "seen", b),
+            address(kv.lengths if lengths_out is None else lengths_out, "int32", "lengths_out", b), budget, recent,
+            sinks), kv)
 
     def sample(self, logits, u, token, logprob=None, temperature=None, top_k=None, top_p=None, min_p=None) -> None:
         """token int32 [batch] (and the log of its probability) drawn from logits [batch, n_vocab] with the uniform
         numbers u float32 [batch]; temperature, top_p and min_p float32 [batch], top_k int32 [batch], None: off."""
         if logits.dim() != 2 or not logits.is_cuda or (logits.shape[1] > 1 and logits.stride(1) != 1):
             raise ValueError("logits must be a CUDA tensor [batch, n_vocab] with contiguous rows")
-        b = (logits.shape[0],)
-
-        def opt(t, name, dtype="float32"):
-            return 0 if t is None else dev_ptr(typed(t, dtype, name, b))
-
-        s = capi.b200_sample_t(logits.data_ptr(), dtype_code(logits, "logits"), b[0], logits.shape[1], logits.stride(0),
-                               opt(temperature, "temperature"), opt(top_k, "top_k", "int32"), opt(top_p, "top_p"),
-                               opt(min_p, "min_p"), opt(u, "u"), opt(token, "token", "int32"), opt(logprob, "logprob"))
-        check(lib().b200_sample(self.h, ctypes.byref(s)), "b200_sample")
+        n, vocab = logits.shape
+        b = (n,)
+        self._call("b200_sample", capi.b200_sample_t, (
+            logits.data_ptr(), dtype_code(logits, "logits"), n, vocab, logits.stride(0),
+            address(temperature, "float32", "temperature", b), address(top_k, "int32", "top_k", b),
+            address(top_p, "float32", "top_p", b), address(min_p, "float32", "min_p", b), address(u, "float32", "u", b),
+            address(token, "int32", "token", b), address(logprob, "float32", "logprob", b)))
 
     def sync(self, timeout_ms: int = 10000) -> None:
         check(lib().b200_engine_sync(self.h, timeout_ms), "b200_engine_sync")

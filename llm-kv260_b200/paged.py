@@ -3,37 +3,51 @@ include/b200_engine.h): Engine.kv_append, kv_attend and kv_evict."""
 
 from __future__ import annotations
 
+import ctypes
+
 from . import capi
 
-DTYPES = {"torch.float32": 0, "torch.float16": 1, "torch.bfloat16": 2}   # B200_F32, B200_F16, B200_BF16
+_CODES: dict = {}          # torch dtype -> B200_F32, B200_F16, B200_BF16
+
+
+def codes() -> dict:
+    if not _CODES:
+        import torch
+        _CODES.update({torch.float32: 0, torch.float16: 1, torch.bfloat16: 2})
+        _CODES["int32"], _CODES["float32"] = torch.int32, torch.float32
+    return _CODES
 
 
 def dtype_code(t, name: str) -> int:
-    code = DTYPES.get(str(t.dtype))
+    code = (_CODES or codes()).get(t.dtype)
     if code is None:
         raise ValueError(f"{name} must be float32, float16 or bfloat16, not {t.dtype}")
     return code
 
 
-def typed(t, dtype: str, name: str, shape=None):
-    """t, if it is a CUDA tensor of that type (and shape); else ValueError."""
-    if not t.is_cuda or str(t.dtype) != "torch." + dtype:
+def address(t, dtype: str, name: str, shape) -> int:
+    """Device address of a contiguous CUDA tensor of that type ("int32" or "float32") and shape; 0 for None."""
+    if t is None:
+        return 0
+    if not t.is_cuda or t.dtype is not (_CODES or codes())[dtype]:
         raise ValueError(f"{name} must be a CUDA {dtype} tensor")
-    if shape is not None and tuple(t.shape) != tuple(shape):
-        raise ValueError(f"{name} must have shape {tuple(shape)}, not {tuple(t.shape)}")
-    return t
+    if t.shape != shape:
+        raise ValueError(f"{name} must have shape {shape}, not {tuple(t.shape)}")
+    if not t.is_contiguous():
+        raise ValueError(f"{name} must be contiguous")
+    return t.data_ptr()
 
 
 def rows(t, name: str, shape) -> tuple[int, int]:
     """Strides of a tensor's first two dimensions, its last one contiguous."""
     if not t.is_cuda:
         raise ValueError(f"{name} must be a CUDA tensor")
-    if tuple(t.shape) != tuple(shape):
-        raise ValueError(f"{name} must have shape {tuple(shape)}, not {tuple(t.shape)}")
-    s = t.stride()
-    if s[2] != 1 and shape[2] != 1:
+    if t.shape != shape:
+        raise ValueError(f"{name} must have shape {shape}, not {tuple(t.shape)}")
+    s0, s1, s2 = t.stride()
+    if s2 != 1 and shape[2] != 1:
         raise ValueError(f"{name}: a row must be contiguous")
-    return s[0], s[1]
+    return s0, s1
 
 
 class PagedKV:
@@ -52,12 +66,11 @@ class PagedKV:
             raise ValueError("k and v must be CUDA tensors")
         if k.stride(3) != 1:
             raise ValueError("a cache row must be contiguous")
-        typed(table, "int32", "table")
+        if not table.is_cuda or table.dtype is not codes()["int32"]:
+            raise ValueError("table must be a CUDA int32 tensor")
         if table.dim() != 2 or (table.shape[1] > 1 and table.stride(1) != 1):
             raise ValueError("table must be [batch, columns] with contiguous rows")
-        typed(lengths, "int32", "lengths", (table.shape[0],))
-        if not lengths.is_contiguous():
-            raise ValueError("lengths must be contiguous")
+        at = address(lengths, "int32", "lengths", (table.shape[0],))
         self.k, self.v, self.table, self.lengths = k, v, table, lengths
         self.n_pages, self.n_head_kv, self.page_size, self.head_dim = k.shape
         self.batch, cols = table.shape
@@ -65,13 +78,12 @@ class PagedKV:
         st = k.stride()
         self.c = capi.b200_kv_t(k.data_ptr(), v.data_ptr(), dtype_code(k, "k"), self.n_pages, self.page_size,
                                 self.n_head_kv, self.head_dim, st[0], st[1], st[2], table.data_ptr(),
-                                max(table.stride(0), cols), cols, lengths.data_ptr(), self.batch)
+                                max(table.stride(0), cols), cols, at, self.batch)
+        self.ref = ctypes.byref(self.c)
 
     def aux(self, t, dtype: str, name: str) -> tuple[int, int]:
         """Address and head stride of a [batch, n_head_kv, >= capacity] tensor beside the cache (weights, positions)."""
-        typed(t, dtype, name)
-        if t.dim() != 3 or tuple(t.shape[:2]) != (self.batch, self.n_head_kv) or t.shape[2] < self.capacity:
+        if t.dim() != 3 or t.shape[2] < self.capacity:
             raise ValueError(f"{name} must be [{self.batch}, {self.n_head_kv}, >= {self.capacity}]")
-        if not t.is_contiguous():
-            raise ValueError(f"{name} must be contiguous")
-        return t.data_ptr(), t.shape[2]
+        n = t.shape[2]
+        return address(t, dtype, name, (self.batch, self.n_head_kv, n)), n
