@@ -31,6 +31,7 @@ constexpr int kList = 4096;                    // candidates
 constexpr int kBins = 1024;                    // of the threads' maxima
 constexpr int kMaxListK = 2048;                // top_k beyond this goes by the whole row
 constexpr float kNear = -10.0f;                // exponents near the top, tried first for top-p
+enum : int { kTellTop, kTellFirst, kTellAll, kTellNear, kTellSum, kTellTies, kTellKept, kTellCut, kTellList = kTellCut + 2, kTold = kTellList + 3 };
 constexpr int kFew = 256;                      // candidates that are ordered each against each
 
 using u64 = unsigned long long;
@@ -94,36 +95,56 @@ __device__ __forceinline__ u64 part_up(u64 share, u64 total) {
 }
 
 // Another CTA's shared memory (cluster_map addresses).
-__device__ __forceinline__ unsigned cluster_add(uint32_t a, unsigned v) {
-    unsigned old;
-    asm volatile("atom.shared::cluster.add.u32 %0, [%1], %2;" : "=r"(old) : "r"(a), "r"(v) : "memory");
-    return old;
-}
 __device__ __forceinline__ void cluster_store(uint32_t a, u64 v) {
     asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(a), "l"(v) : "memory");
 }
-__device__ __forceinline__ unsigned cluster_load(uint32_t a) {
-    unsigned v;
-    asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(a) : "memory");
-    return v;
+// The sums over the cluster of two neighbouring values in every CTA, all loads
+// on their way at once.
+__device__ __forceinline__ void cluster_sum2(const u64 *mine, unsigned ctas, u64 sum[2]) {
+    u64 v[kMaxCluster][2];
+#pragma unroll
+    for (unsigned q = 0; q < kMaxCluster; ++q) {
+        v[q][0] = v[q][1] = 0;
+        if (q < ctas)
+            asm volatile("ld.shared::cluster.v2.u64 {%0, %1}, [%2];" : "=l"(v[q][0]), "=l"(v[q][1]) : "r"(cluster_map(mine, q)) : "memory");
+    }
+    sum[0] = sum[1] = 0;
+#pragma unroll
+    for (unsigned q = 0; q < kMaxCluster; ++q) sum[0] += v[q][0], sum[1] += v[q][1];
 }
-__device__ __forceinline__ u64 cluster_load64(uint32_t a) {
-    u64 v;
-    asm volatile("ld.shared::cluster.u64 %0, [%1];" : "=l"(v) : "r"(a) : "memory");
-    return v;
+__device__ __forceinline__ void cluster_sum2(const unsigned *mine, unsigned ctas, u64 sum[2]) {
+    unsigned v[kMaxCluster][2];
+#pragma unroll
+    for (unsigned q = 0; q < kMaxCluster; ++q) {
+        v[q][0] = v[q][1] = 0;
+        if (q < ctas)
+            asm volatile("ld.shared::cluster.v2.u32 {%0, %1}, [%2];" : "=r"(v[q][0]), "=r"(v[q][1]) : "r"(cluster_map(mine, q)) : "memory");
+    }
+    sum[0] = sum[1] = 0;
+#pragma unroll
+    for (unsigned q = 0; q < kMaxCluster; ++q) sum[0] += v[q][0], sum[1] += v[q][1];
 }
 
+struct Yes {
+    static constexpr bool value = true;
+};
+struct No {
+    static constexpr bool value = false;
+};
+
 struct Shared {
-    u64 mass[2][256];                   // sums by digit, of this pass and the one before
-    u64 sums[kBins];                    // sums by distance from the top
-    unsigned bins[kBins];               // rank 0: the threads' maxima by their distance from the top
-    u64 gather[kMaxCluster][9];         // what every CTA of the cluster tells the others, each thing in a place of its own
-    u64 warp[kWarps];
+    alignas(16) u64 mass[2][256];       // sums by digit, of this pass and the one before
+    alignas(16) u64 sums[kBins];        // sums by distance from the top
+    u64 gather[kMaxCluster][kTold];     // what every CTA of the cluster tells the others, each thing in a place of its own
+    u64 warp[kWarps], warp_ties[kWarps];
     u64 left;
     u64 weight;
     uint32_t prefix;
-    unsigned listed;                    // rank 0
+    unsigned listed;                    // candidates of this CTA
     int bin;
+
+    // the threads' maxima by their distance from the top: in the upper half of the sums, which come later
+    __device__ __forceinline__ unsigned *bins() { return reinterpret_cast<unsigned *>(sums + kBins / 2); }
 };
 
 // Inclusive prefix of one value per thread, and the total.
@@ -176,13 +197,29 @@ __device__ __forceinline__ void pick_bin(Shared &s, const V *bins, int shift) {
     }
 }
 
+__device__ __forceinline__ unsigned shared_add(uint32_t a, unsigned v) {
+    unsigned old;
+    asm volatile("atom.shared.add.u32 %0, [%1], %2;" : "=r"(old) : "r"(a), "r"(v) : "memory");
+    return old;
+}
+
+// The same where `on`, as one predicated instruction: no branch, so that several are on their way at once.
+__device__ __forceinline__ unsigned shared_add_if(uint32_t a, unsigned v, bool on) {
+    unsigned old;
+    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %3, 0;\n\tmov.u32 %0, 0;\n\t@p atom.shared.add.u32 %0, [%1], %2;\n\t}"
+                 : "=&r"(old)
+                 : "r"(a), "r"(v), "r"(static_cast<unsigned>(on))
+                 : "memory");
+    return old;
+}
+
 // Add w to a 64-bit sum in this CTA's shared memory: its halves are summed by
 // 32-bit atomics, which the hardware has, with the low half's carry.
 __device__ __forceinline__ void add_mass(u64 *sum, u64 w) {
-    unsigned *half = reinterpret_cast<unsigned *>(sum);
-    const unsigned lo = static_cast<unsigned>(w), old = atomicAdd(half, lo);
+    const uint32_t a = smem_addr(sum);
+    const unsigned lo = static_cast<unsigned>(w), old = shared_add(a, lo);
     const unsigned hi = static_cast<unsigned>(w >> 32) + (old + lo < old);
-    if (hi) atomicAdd(half + 1, hi);
+    if (hi) shared_add(a + 4, hi);
 }
 
 // Selection among the N candidates of the list: value(key, idx, &digits) says
@@ -269,7 +306,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleArgs a)
     }
 
     // The largest logit, and the smallest of the threads' maxima that are above -infinity.
-    for (int i = tid; i < kBins; i += kThreads) s.bins[i] = 0;
+    for (int i = tid; i < kBins; i += kThreads) s.bins()[i] = 0;
     if (tid == 0) s.listed = 0;
     float own = -INFINITY;                      // the thread's maximum (fmaxf passes NaN over)
 #pragma unroll 4
@@ -298,12 +335,12 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleArgs a)
             top = fmaxf(top, __shfl_xor_sync(kFullMask, top, k));
             low = fminf(low, __shfl_xor_sync(kFullMask, low, k));
         }
-        tell(0, static_cast<u64>(__float_as_uint(top)) << 32 | __float_as_uint(low));
+        tell(kTellTop, static_cast<u64>(__float_as_uint(top)) << 32 | __float_as_uint(low));
     }
     cluster_sync_all();
     for (unsigned q = 0; q < ctas; ++q) {
-        top = fmaxf(top, __uint_as_float(static_cast<unsigned>(s.gather[q][0] >> 32)));
-        low = fminf(low, __uint_as_float(static_cast<unsigned>(s.gather[q][0])));
+        top = fmaxf(top, __uint_as_float(static_cast<unsigned>(s.gather[q][kTellTop] >> 32)));
+        low = fminf(low, __uint_as_float(static_cast<unsigned>(s.gather[q][kTellTop])));
     }
     top += 0.0f;                                // -0 as 0, as the keys have it
 
@@ -328,10 +365,10 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleArgs a)
         if (lane == 0) s.warp[warp] = first;
         __syncthreads();
         for (int w = 0; w < kWarps; ++w) first = min(first, static_cast<int>(s.warp[w]));
-        tell(1, first);
+        tell(kTellFirst, first);
         cluster_sync_all();
         if (rank == 0 && tid == 0) {
-            for (unsigned q = 0; q < ctas; ++q) first = min(first, static_cast<int>(s.gather[q][1]));
+            for (unsigned q = 0; q < ctas; ++q) first = min(first, static_cast<int>(s.gather[q][kTellFirst]));
             a.token[row] = first;
             if (a.logprob) a.logprob[row] = 0.0f;
         }
@@ -369,95 +406,97 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleArgs a)
         const float scale = top > low ? (kBins - 1) / (top - low) : 0.0f;   // 0 where top - low overflows, too
         if (own != -INFINITY) {
             const int bin = own == top ? 0 : min(static_cast<int>((top - own) * scale), kBins - 1);
-            cluster_add(cluster_map(&s.bins[bin], 0), 1);
+            atomicAdd(&s.bins()[bin], 1u);
         }
         cluster_sync_all();
         // the bin with the k-th largest maximum: its far edge, and a little for the rounding of the bins
-        const uint32_t bins = cluster_map(s.bins, 0);
-        constexpr int kPer = kBins / kThreads;
-        u64 mine[kPer], sum = 0, total;
-        for (int j = 0; j < kPer; ++j) sum += mine[j] = cluster_load(bins + (tid * kPer + j) * 4);
+        u64 mine[2], total;
+        cluster_sum2(&s.bins()[2 * tid], ctas, mine);
+        const u64 sum = mine[0] + mine[1];
         u64 before = block_scan(sum, s.warp, &total) - sum;
         if (tid == 0) s.bin = kBins;
         __syncthreads();
         if (before < static_cast<u64>(k) && static_cast<u64>(k) <= before + sum) {
-            int j = 0;
-            while (before + mine[j] < static_cast<u64>(k)) before += mine[j++];
-            s.bin = tid * kPer + j;
+            s.bin = 2 * tid + (before + mine[0] < static_cast<u64>(k));
         }
         __syncthreads();
         if (s.bin < kBins - 1 && scale > 0.0f) floor_x = top - (s.bin + 1.01f) / scale;
     } else if (k == 0 && by_p) {
         // the weight of all tokens, and of those within 2^-10 of the largest
         u64 all = 0, near = 0;
-        for (int p = w0 + lane; p < w1; p += 32) {
-            float x[kVe];
-            piece(p, x);
-            uint32_t hi = 0, lo = 0, near_hi = 0, near_lo = 0, near_count = 0;
+        const auto weigh_all = [&](auto is_plain) {
+#pragma unroll 2
+            for (int p = w0 + lane; p < w1; p += 32) {
+                float x[kVe];
+                piece(p, x);
+                uint32_t hi = 0, lo = 0, near_hi = 0, near_lo = 0;
 #pragma unroll
-            for (int j = 0; j < kVe; ++j) {
-                float y, e;
-                if (plain) e = plain_power(x[j], &y);
-                else e = power(y = exponent(x[j], top, c));
-                uint32_t h, l;
-                split_units(e, &h, &l);
-                hi += h, lo += l;
-                if (y >= kNear) near_hi += h, near_lo += l, ++near_count;
+                for (int j = 0; j < kVe; ++j) {
+                    float y, e;
+                    if constexpr (decltype(is_plain)::value) e = plain_power(x[j], &y);
+                    else e = power(y = exponent(x[j], top, c));
+                    uint32_t h, l;
+                    split_units(e, &h, &l);
+                    hi += h, lo += l;
+                    const uint32_t is_near = y >= kNear ? kFullMask : 0;
+                    near_hi += (h - kBase) & is_near, near_lo += (l - kBase) & is_near;
+                }
+                all += join_units(hi, lo, kVe);
+                near += join_units(near_hi, near_lo, 0);
             }
-            all += join_units(hi, lo, kVe);
-            near += join_units(near_hi, near_lo, near_count);
-        }
+        };
+        if (plain) weigh_all(Yes()); else weigh_all(No());
         all = warp_sum(all), near = warp_sum(near);
         if (lane == 0) s.mass[0][warp] = all, s.mass[0][32 + warp] = near;
         __syncthreads();
         all = near = 0;
         for (int w = 0; w < kWarps; ++w) all += s.mass[0][w], near += s.mass[0][32 + w];
-        tell(1, all), tell(2, near);
+        tell(kTellAll, all), tell(kTellNear, near);
         cluster_sync_all();
         all = near = 0;
-        for (unsigned q = 0; q < ctas; ++q) all += s.gather[q][1], near += s.gather[q][2];
+        for (unsigned q = 0; q < ctas; ++q) all += s.gather[q][kTellAll], near += s.gather[q][kTellNear];
         s.weight = all;                         // every thread writes the same
         listed = part_up(static_cast<u64>(p24), all) <= near;
     }
-    // Tokens that `wanted` names go to rank 0's list; true where it holds all of them. Between two cluster barriers.
-    const uint32_t where = cluster_map(&s.listed, 0), there = cluster_map(list, 0);
-    const auto collect = [&](auto wanted) {
-        for (int base = w0; base < w1; base += 32) {
-            const int p = base + lane;
+    // Tokens that `wanted` names go to this CTA's list, and from there to rank 0's; true where that holds all of them.
+    // Call `turn` of a row; s.listed is 0 before it, and rank 0 has the number after it.
+    const auto collect = [&](int turn, auto wanted) {
+        for (int p = w0 + lane; p < w1; p += 32) {
             float x[kVe];
+            piece(p, x);
             unsigned take = 0;
-            if (p < w1) {
-                piece(p, x);
 #pragma unroll
-                for (int j = 0; j < kVe; ++j)
-                    if (wanted(x[j] = clean(x[j]))) take |= 1u << j;
-            }
-            if (!__any_sync(kFullMask, take)) continue;
-            int at = __popc(take);
-            for (int j = 1; j < 32; j <<= 1) {
-                const int y = __shfl_up_sync(kFullMask, at, j);
-                if (lane >= j) at += y;
-            }
-            const int sum = __shfl_sync(kFullMask, at, 31);
-            unsigned first = 0;
-            if (lane == 31) first = cluster_add(where, sum);
-            at += static_cast<int>(__shfl_sync(kFullMask, first, 31)) - __popc(take);
+            for (int j = 0; j < kVe; ++j)
+                if (wanted(x[j] = clean(x[j]))) take |= 1u << j;
+            if (!take) continue;
+            unsigned at = atomicAdd(&s.listed, static_cast<unsigned>(__popc(take)));
 #pragma unroll
             for (int j = 0; j < kVe; ++j)
                 if (take >> j & 1) {
-                    if (at < kList)
-                        cluster_store(there + at * 8, static_cast<u64>(order_key(x[j])) << 32 | static_cast<unsigned>(p * kVe + j - skew));
+                    if (at < kList) list[at] = static_cast<u64>(order_key(x[j])) << 32 | static_cast<unsigned>(p * kVe + j - skew);
                     ++at;
                 }
         }
+        __syncthreads();
+        const unsigned mine = s.listed;
+        tell(kTellList + turn, mine);
         cluster_sync_all();
-        const bool all = cluster_load(where) <= static_cast<unsigned>(kList);
-        cluster_sync_all();                     // all have read it: rank 0 may go on, or end
-        return all;
+        u64 before = 0, all = 0;
+        for (unsigned q = 0; q < ctas; ++q) {
+            if (q < rank) before += s.gather[q][kTellList + turn];
+            all += s.gather[q][kTellList + turn];
+        }
+        if (all <= kList && rank > 0) {
+            const uint32_t there = cluster_map(list, 0) + static_cast<uint32_t>(before) * 8;
+            for (unsigned i = tid; i < mine; i += kThreads) cluster_store(there + i * 8, list[i]);
+        }
+        if (rank == 0 && tid == 0) s.listed = static_cast<unsigned>(all);
+        cluster_sync_all();
+        return all <= kList;
     };
     if (listed) {
-        if (k > 0) listed = collect([&](float x) { return x >= floor_x && x != -INFINITY; });
-        else listed = collect([&](float x) { return exponent(x, top, c) >= kNear; });
+        if (k > 0) listed = collect(0, [&](float x) { return x >= floor_x && x != -INFINITY; });
+        else listed = collect(0, [&](float x) { return exponent(x, top, c) >= kNear; });
         if (listed && rank != 0) return;        // rank 0 does the rest, in its own memory
     }
     if (listed) {
@@ -479,10 +518,10 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleArgs a)
             for (int j = part0; j < m; j += parts)
                 if ((list[j] ^ 0xffffffffull) > e) ++ahead, before += weights[j];
             s.sums[tid] = before;
-            s.bins[tid] = ahead;
+            s.bins()[tid] = ahead;
             __syncthreads();
             before = ahead = 0;
-            for (int j = 0; j < parts; ++j) before += s.sums[j * wide + i], ahead += s.bins[j * wide + i];
+            for (int j = 0; j < parts; ++j) before += s.sums[j * wide + i], ahead += s.bins()[j * wide + i];
             bool keep = i < m && (k == 0 || ahead < static_cast<unsigned>(k));
             if (by_p) {
                 u64 all = s.weight;
@@ -596,10 +635,8 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleArgs a)
     uint32_t edge = 0;
     u64 ties = 0;
     constexpr float kBinsPerOctave = kBins / 41.0f;
-    const auto bin_of = [&](float x) {
-        const float y = exponent(x, top, c);
-        return y > -41.0f ? min(static_cast<int>(-y * kBinsPerOctave), kBins - 1) : kBins - 1;
-    };
+    const auto bin_of_y = [](float y) { return y > -41.0f ? min(static_cast<int>(-y * kBinsPerOctave), kBins - 1) : kBins - 1; };
+    const auto bin_of = [&](float x) { return bin_of_y(exponent(x, top, c)); };
     // `left` tokens (or weight, `total` in all) are kept, of those above the present edge and edge_mass at it
     const auto cut_row = [&](u64 left, bool by_mass, u64 total, u64 edge_mass) {
         for (int i = tid; i < kBins; i += kThreads) s.sums[i] = 0;
@@ -607,37 +644,45 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleArgs a)
         __syncthreads();
         // tokens so light that all of them together are less than what is given up: the sums from the top do not
         // come to them
+        const float old_x = edge ? value_of(edge) : -INFINITY;
         const u64 least = by_mass ? (total - left) / static_cast<u64>(n) : 0;
         for (int p = w0 + lane; p < w1; p += 32) {
             float x[kVe];
             piece(p, x);
+            if (!by_mass) {
 #pragma unroll
-            for (int j = 0; j < kVe; ++j) {
-                const float v = clean(x[j]);
-                const int i = p * kVe + j - skew;
-                if (!by_mass) {
-                    if (i >= 0 && i < n) add_mass(&s.sums[bin_of(v)], 1);
-                } else if (order_key(v) > edge) {
-                    const u64 w = weight(v);
-                    if (w > least) add_mass(&s.sums[bin_of(v)], w);
+                for (int j = 0; j < kVe; ++j) {
+                    const int i = p * kVe + j - skew;
+                    if (i >= 0 && i < n) atomicAdd(reinterpret_cast<unsigned *>(&s.sums[bin_of(clean(x[j]))]), 1u);
+                }
+            } else {                            // as add_mass, the atomics of a piece one behind the other
+                unsigned old[kVe];
+                uint32_t at[kVe];
+                u64 w[kVe];
+#pragma unroll
+                for (int j = 0; j < kVe; ++j) {
+                    const float y = exponent(x[j], top, c);
+                    w[j] = units(x[j] > old_x ? power(y) : 0.0f);
+                    if (w[j] <= least) w[j] = 0;
+                    at[j] = smem_addr(&s.sums[bin_of_y(y)]);
+                    old[j] = shared_add_if(at[j], static_cast<unsigned>(w[j]), w[j] != 0);
+                }
+#pragma unroll
+                for (int j = 0; j < kVe; ++j) {
+                    const unsigned lo = static_cast<unsigned>(w[j]), hi = static_cast<unsigned>(w[j] >> 32) + (old[j] + lo < old[j]);
+                    shared_add_if(at[j] + 4, hi, hi != 0);
                 }
             }
         }
         if (rank == 0 && tid == 0 && edge_mass) add_mass(&s.sums[bin_of(value_of(edge))], edge_mass);
         cluster_sync_all();
-        constexpr int kPer = kBins / kThreads;
-        u64 mine[kPer], sum = 0, all;
-        for (int j = 0; j < kPer; ++j) {
-            mine[j] = 0;
-            for (unsigned q = 0; q < ctas; ++q) mine[j] += cluster_load64(cluster_map(&s.sums[tid * kPer + j], q));
-            sum += mine[j];
-        }
-        u64 before = block_scan(sum, s.warp, &all) - sum;
+        u64 mine[2], all;
+        cluster_sum2(&s.sums[2 * tid], ctas, mine);
+        const u64 sum = mine[0] + mine[1], before = block_scan(sum, s.warp, &all) - sum;
         if (before < left && left <= before + sum) {
-            int j = 0;
-            while (before + mine[j] < left) before += mine[j++];
-            s.bin = tid * kPer + j;
-            s.weight = left - before;
+            const bool second = before + mine[0] < left;
+            s.bin = 2 * tid + second;
+            s.weight = left - before - (second ? mine[0] : 0);
         }
         __syncthreads();
         const int bin = s.bin;
@@ -647,12 +692,22 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleArgs a)
             return;
         }
         u64 w = 1;
-        if (collect([&](float x) { return bin_of(x) == bin && (!by_mass || order_key(x) > edge); })) {
+        if (collect(1 + by_mass, [&](float x) { return bin_of(x) == bin && (!by_mass || order_key(x) > edge); })) {
             if (rank == 0) {
                 const int m = static_cast<int>(s.listed);
                 const uint32_t old = edge;
-                if (tid == 0) s.prefix = 0, s.left = inside;
-                for (int shift = 24; shift >= 0; shift -= 8) {
+                const bool edge_here = edge_mass && bin_of(value_of(old)) == bin;
+                // the keys of a bin are near each other: from the first digit in which any differs from the first
+                uint32_t differ = edge_here ? old ^ static_cast<uint32_t>(list[0] >> 32) : 0;
+                for (int i = tid; i < m; i += kThreads) differ |= static_cast<uint32_t>(list[i] >> 32) ^ static_cast<uint32_t>(list[0] >> 32);
+                differ = __reduce_or_sync(kFullMask, differ);
+                if (lane == 0) s.warp[warp] = differ;
+                __syncthreads();
+                for (int q = 0; q < kWarps; ++q) differ |= static_cast<uint32_t>(s.warp[q]);
+                const int from = differ >> 24 ? 24 : differ >> 16 ? 16 : differ >> 8 ? 8 : 0;
+                const uint32_t above = from == 24 ? 0 : kFullMask << (from + 8);
+                if (tid == 0) s.prefix = static_cast<uint32_t>(list[0] >> 32) & above, s.left = inside;
+                for (int shift = from; shift >= 0; shift -= 8) {
                     if (tid < 256) s.mass[0][tid] = 0;
                     __syncthreads();
                     const uint32_t prefix = s.prefix, mask = shift == 24 ? 0 : kFullMask << (shift + 8);
@@ -660,18 +715,18 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleArgs a)
                         const uint32_t key = static_cast<uint32_t>(list[i] >> 32);
                         if ((key & mask) == prefix) add_mass(&s.mass[0][key >> shift & 255], by_mass ? weight(value_of(key)) : 1);
                     }
-                    if (tid == 0 && edge_mass && bin_of(value_of(old)) == bin && (old & mask) == prefix)
+                    if (tid == 0 && edge_here && (old & mask) == prefix)
                         add_mass(&s.mass[0][old >> shift & 255], edge_mass);
                     __syncthreads();
                     pick_bin<true>(s, s.mass[0], shift);
                     __syncthreads();
                 }
                 if (by_mass) w = weight(value_of(s.prefix));
-                tell(by_mass ? 8 : 7, static_cast<u64>(s.prefix) << 32 | ((s.left + w - 1) / w));
+                tell(kTellCut + by_mass, static_cast<u64>(s.prefix) << 32 | ((s.left + w - 1) / w));
             }
             cluster_sync_all();
-            edge = static_cast<uint32_t>(s.gather[0][by_mass ? 8 : 7] >> 32);
-            ties = static_cast<uint32_t>(s.gather[0][by_mass ? 8 : 7]);
+            edge = static_cast<uint32_t>(s.gather[0][kTellCut + by_mass] >> 32);
+            ties = static_cast<uint32_t>(s.gather[0][kTellCut + by_mass]);
             return;
         }
         const uint32_t old = edge;
@@ -697,14 +752,9 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleArgs a)
             if (rank == 0 && tid == 0 && edge_mass && (old & mask) == prefix) add_mass(&s.mass[turn][old >> shift & 255], edge_mass);
             // every CTA adds up all CTAs' sums; the next pass uses the other set, so one barrier a pass is enough
             cluster_sync_all();
-            u64 sum = 0;
-            if (tid < 256)
-                for (unsigned q = 0; q < ctas; ++q) sum += cluster_load64(cluster_map(&s.mass[turn][tid], q));
+            if (tid < 128) cluster_sum2(&s.mass[turn][2 * tid], ctas, &s.sums[2 * tid]);
             __syncthreads();
-            u64 *sums = s.sums;
-            if (tid < 256) sums[tid] = sum;
-            __syncthreads();
-            pick_bin<true>(s, sums, shift);
+            pick_bin<true>(s, s.sums, shift);
             __syncthreads();
         }
         edge = s.prefix;
@@ -725,10 +775,10 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleArgs a)
             }
         }
         block_scan(sum, s.warp, &sum);
-        tell(4, sum);
+        tell(kTellSum, sum);
         cluster_sync_all();
         sum = 0;
-        for (unsigned q = 0; q < ctas; ++q) sum += s.gather[q][4];
+        for (unsigned q = 0; q < ctas; ++q) sum += s.gather[q][kTellSum];
         const u64 at_edge = edge ? weight(value_of(edge)) * ties : 0;
         u64 need = part_up(static_cast<u64>(p24), sum + at_edge);
         if (need < 1) need = 1;
@@ -737,129 +787,105 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleArgs a)
     if (min_p > 1.0f) edge = order_key(top), ties = 1;
 
     // The kept weight of each warp's tokens, and where u falls among them.
-    const float edge_x = value_of(edge);        // (not a number where there is none)
-    const auto kept = [&](float x, bool *tie) -> u64 {
-        *tie = edge && x == edge_x;
-        if (edge && !(x >= edge_x)) return 0;
-        const float e = power(exponent(x, top, c));
-        return e < min_p && x != top ? 0 : units(e);
-    };
-    u64 sum = 0, equal = 0, w_edge = 0;
-    if (plain && edge == 0 && min_p == 0.0f) {
+    const float edge_x = edge ? value_of(edge) : -INFINITY;
+    // ties that weigh something: all of them are summed, and those too many taken off again
+    const bool tied = edge && !(power(exponent(edge_x, top, c)) < min_p && edge_x != top);
+    const u64 w_edge = tied ? weight(edge_x) : 0;
+    u64 sum = 0, equal = 0;
+    const auto weigh_kept = [&](auto is_plain, auto is_cut) {
 #pragma unroll 2
         for (int p = w0 + lane; p < w1; p += 32) {
             float x[kVe];
             piece(p, x);
             uint32_t hi = 0, lo = 0;
+            int ties_here = 0;
 #pragma unroll
             for (int j = 0; j < kVe; ++j) {
-                float y;
+                float y, e;
                 uint32_t h, l;
-                split_units(plain_power(x[j], &y), &h, &l);
+                if constexpr (decltype(is_plain)::value) e = plain_power(x[j], &y);
+                else e = power(exponent(x[j], top, c));
+                if constexpr (decltype(is_cut)::value) {
+                    e = (x[j] < edge_x) | ((e < min_p) & (x[j] != top)) ? 0.0f : e;
+                    ties_here += x[j] == edge_x;
+                }
+                split_units(e, &h, &l);
                 hi += h, lo += l;
             }
             sum += join_units(hi, lo, kVe);
+            equal += ties_here;
         }
-    } else {
-        for (int p = w0 + lane; p < w1; p += 32) {
-            float x[kVe];
-            piece(p, x);
-#pragma unroll
-            for (int j = 0; j < kVe; ++j) {
-                bool tie;
-                const u64 w = kept(clean(x[j]), &tie);
-                if (tie) ++equal, w_edge = w; else sum += w;
-            }
-        }
-    }
+    };
+    const bool cut = edge || min_p > 0.0f;
+    if (plain && !cut) weigh_kept(Yes(), No());
+    else if (plain) weigh_kept(Yes(), Yes());
+    else weigh_kept(No(), Yes());
     sum = warp_sum(sum);
-    u64 ties_before = 0;
-    if (edge) {
-        equal = warp_sum(equal);
-        for (int j = 16; j; j >>= 1) w_edge = max(w_edge, __shfl_xor_sync(kFullMask, w_edge, j));
-        __syncthreads();
-        if (lane == 0) s.warp[warp] = equal;
-        __syncthreads();
-        u64 here = 0;
-        for (int w = 0; w < kWarps; ++w) {
-            if (w < warp) ties_before += s.warp[w];
-            here += s.warp[w];
-        }
-        tell(5, here);
-        cluster_sync_all();
-        for (unsigned q = 0; q < rank; ++q) ties_before += s.gather[q][5];
-        sum += (ties > ties_before ? min(equal, ties - ties_before) : 0) * w_edge;
-    }
+    if (cut) equal = warp_sum(equal);
     __syncthreads();
-    if (lane == 0) s.warp[warp] = sum;
+    if (lane == 0) s.warp[warp] = sum, s.warp_ties[warp] = equal;
     __syncthreads();
-    u64 before = 0, total = 0;
-    for (int w = 0; w < kWarps; ++w) {
-        if (w < warp) before += s.warp[w];
-        total += s.warp[w];
-    }
-    tell(6, total);
+    sum = equal = 0;
+    for (int w = 0; w < kWarps; ++w) sum += s.warp[w], equal += s.warp_ties[w];
+    tell(kTellKept, sum);
+    tell(kTellTies, equal);
     cluster_sync_all();
-    total = 0;
+    // of a stretch's `eq` ties, `seen` before it, those kept
+    const auto kept_ties = [&](u64 seen, u64 eq) { return tied ? seen >= ties ? 0 : min(eq, ties - seen) : eq; };
+    u64 total = 0, before = 0, seen = 0, mine = 0, seen_all = 0;
     for (unsigned q = 0; q < ctas; ++q) {
-        if (q < rank) before += s.gather[q][6];
-        total += s.gather[q][6];
+        const u64 eq = s.gather[q][kTellTies], part_sum = s.gather[q][kTellKept] - (eq - kept_ties(seen_all, eq)) * w_edge;
+        if (q == rank) before = total, seen = seen_all, mine = part_sum;
+        total += part_sum;
+        seen_all += eq;
     }
     const u64 target = part(share, total);
-    if (target < before || target >= before + sum) return;
-    u64 run = before, seen = ties_before;
-    for (int base = w0; base < w1; base += 32) {
-        const int p = base + lane;
-        u64 w[kVe], mine = 0;
+    if (target < before || target >= before + mine) return;
+    // this CTA's, then: the warp's stretch it falls in, which all threads go over, a piece each
+    int win = 0;
+    for (;; ++win) {
+        const u64 eq = s.warp_ties[win], part_sum = s.warp[win] - (eq - kept_ties(seen, eq)) * w_edge;
+        if (target < before + part_sum) break;
+        before += part_sum;
+        seen += eq;
+    }
+    const int f0 = min(p0 + win * per_warp, p1), f1 = min(f0 + per_warp, p1);
+    for (int base = f0; base < f1; base += kThreads) {
+        const int p = base + tid;
         float x[kVe];
-        unsigned eq = 0;
-        if (p < w1) {
-            piece(p, x);
+        u64 w[kVe], all = 0, weight_all;
+        if (p < f1) piece(p, x);
+        u64 skip = seen;
+        if (tied) {
+            u64 eq = 0, eq_all;
+            if (p < f1)
+#pragma unroll
+                for (int j = 0; j < kVe; ++j) eq += x[j] == edge_x;
+            skip = seen + block_scan(eq, s.mass[0], &eq_all) - eq;
+            seen += eq_all;
+        }
+#pragma unroll
+        for (int j = 0; j < kVe; ++j) {
+            w[j] = 0;
+            if (p >= f1) continue;
+            const float e = power(exponent(x[j], top, c));
+            if (!(x[j] < edge_x || (e < min_p && x[j] != top)) && !(tied && x[j] == edge_x && skip++ >= ties)) w[j] = units(e);
+            all += w[j];
+        }
+        u64 at = before + block_scan(all, s.mass[1], &weight_all) - all;
+        if (at <= target && target < at + all) {
+            bool done = false;
 #pragma unroll
             for (int j = 0; j < kVe; ++j) {
-                bool tie;
-                x[j] = clean(x[j]);
-                w[j] = kept(x[j], &tie);
-                if (tie) eq |= 1u << j;
-            }
-        }
-        if (edge) {                             // ties past the last one that is kept weigh nothing
-            int upto = __popc(eq);
-            for (int j = 1; j < 32; j <<= 1) {
-                const int y = __shfl_up_sync(kFullMask, upto, j);
-                if (lane >= j) upto += y;
-            }
-            u64 t = seen + upto - __popc(eq);
-#pragma unroll
-            for (int j = 0; j < kVe; ++j)
-                if (eq >> j & 1 && t++ >= ties) w[j] = 0;
-            seen += __shfl_sync(kFullMask, upto, 31);
-        }
-        if (p < w1)
-#pragma unroll
-            for (int j = 0; j < kVe; ++j) mine += w[j];
-        u64 upto = mine;
-        for (int j = 1; j < 32; j <<= 1) {
-            const u64 y = __shfl_up_sync(kFullMask, upto, j);
-            if (lane >= j) upto += y;
-        }
-        const unsigned hit = __ballot_sync(kFullMask, run + upto > target);
-        if (hit) {
-            if (lane == __ffs(hit) - 1) {
-                u64 at = run + upto - mine;
-                bool done = false;
-#pragma unroll
-                for (int j = 0; j < kVe; ++j) {
-                    at += w[j];
-                    if (!done && at > target) {
-                        done = true;
-                        finish(p * kVe + j - skew, x[j], total);
-                    }
+                at += w[j];
+                if (!done && at > target) {
+                    done = true;
+                    finish(p * kVe + j - skew, clean(x[j]), total);
                 }
             }
-            return;
         }
-        run += __shfl_sync(kFullMask, upto, 31);
+        before += weight_all;
+        if (target < before) return;
     }
 }
 
