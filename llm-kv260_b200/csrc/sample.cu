@@ -31,7 +31,7 @@ constexpr int kList = 4096;                    // candidates
 constexpr int kBins = 1024;                    // of the threads' maxima
 constexpr int kMaxListK = 2048;                // top_k beyond this goes by the whole row
 constexpr float kNear = -10.0f;                // exponents near the top, tried first for top-p
-enum : int { kTellTop, kTellFirst, kTellAll, kTellNear, kTellSum, kTellTies, kTellKept, kTellCut, kTellList = kTellCut + 2, kTold = kTellList + 3 };
+enum : int { kTellTop, kTellFirst, kTellAll, kTellNear, kTellSum, kTellTies, kTellKept, kTellCut, kTellAbove = kTellCut + 2, kTellList = kTellAbove + 2, kTold = kTellList + 3 };
 constexpr int kFew = 256;                      // candidates that are ordered each against each
 
 using u64 = unsigned long long;
@@ -141,34 +141,45 @@ struct Shared {
     u64 weight;
     uint32_t prefix;
     unsigned listed;                    // candidates of this CTA
-    int bin;
+    int bin, last_bin;
 
     // the threads' maxima by their distance from the top: in the upper half of the sums, which come later
     __device__ __forceinline__ unsigned *bins() { return reinterpret_cast<unsigned *>(sums + kBins / 2); }
 };
 
-// Inclusive prefix of one value per thread, and the total.
-__device__ __forceinline__ u64 block_scan(u64 v, u64 *s, u64 *total) {
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    for (int k = 1; k < 32; k <<= 1) {
+// Every warp does these sums for itself, from values that the warps (or CTAs)
+// left, a lane to each: a loop over them in every thread would cost as much as
+// a pass over the row.
+template <int kWidth>
+__device__ __forceinline__ u64 lanes_scan(u64 v) {   // inclusive, over the first kWidth lanes
+    const int lane = threadIdx.x & 31;
+#pragma unroll
+    for (int k = 1; k < kWidth; k <<= 1) {
         const u64 y = __shfl_up_sync(kFullMask, v, k);
         if (lane >= k) v += y;
     }
+    return v;
+}
+template <int kWidth>
+__device__ __forceinline__ u64 lanes_sum(u64 v) {    // over each kWidth lanes
+#pragma unroll
+    for (int k = kWidth / 2; k; k >>= 1) v += __shfl_xor_sync(kFullMask, v, k);
+    return v;
+}
+__device__ __forceinline__ u64 warp_sum(u64 v) { return lanes_sum<32>(v); }
+__device__ __forceinline__ u64 warps_total(const u64 *s) { return lanes_sum<kWarps>(s[threadIdx.x % kWarps]); }
+
+// Inclusive prefix of one value per thread, and the total.
+__device__ __forceinline__ u64 block_scan(u64 v, u64 *s, u64 *total) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    v = lanes_scan<32>(v);
     __syncthreads();
     if (lane == 31) s[warp] = v;
     __syncthreads();
-    u64 all = 0;
-#pragma unroll
-    for (int w = 0; w < kWarps; ++w) {
-        if (w < warp) v += s[w];
-        all += s[w];
-    }
-    *total = all;
-    return v;
-}
-__device__ __forceinline__ u64 warp_sum(u64 v) {
-    for (int k = 16; k; k >>= 1) v += __shfl_xor_sync(kFullMask, v, k);
-    return v;
+    const u64 upto = lanes_scan<kWarps>(s[lane % kWarps]);
+    *total = __shfl_sync(kFullMask, upto, kWarps - 1);
+    const u64 before = __shfl_sync(kFullMask, upto, warp > 0 ? warp - 1 : 0);
+    return warp > 0 ? v + before : v;
 }
 
 // The digit at which the sum over 256 bins (from the highest, or the lowest)
@@ -203,14 +214,10 @@ __device__ __forceinline__ unsigned shared_add(uint32_t a, unsigned v) {
     return old;
 }
 
-// The same where `on`, as one predicated instruction: no branch, so that several are on their way at once.
-__device__ __forceinline__ unsigned shared_add_if(uint32_t a, unsigned v, bool on) {
-    unsigned old;
-    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %3, 0;\n\tmov.u32 %0, 0;\n\t@p atom.shared.add.u32 %0, [%1], %2;\n\t}"
-                 : "=&r"(old)
-                 : "r"(a), "r"(v), "r"(static_cast<unsigned>(on))
+// Without the old value, and only where `on`: one predicated instruction, so that several are on their way at once.
+__device__ __forceinline__ void shared_add_if(uint32_t a, unsigned v, bool on) {
+    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %2, 0;\n\t@p red.shared.add.u32 [%0], %1;\n\t}" ::"r"(a), "r"(v), "r"(static_cast<unsigned>(on))
                  : "memory");
-    return old;
 }
 
 // Add w to a 64-bit sum in this CTA's shared memory: its halves are summed by
@@ -338,10 +345,17 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleArgs a)
         tell(kTellTop, static_cast<u64>(__float_as_uint(top)) << 32 | __float_as_uint(low));
     }
     cluster_sync_all();
-    for (unsigned q = 0; q < ctas; ++q) {
-        top = fmaxf(top, __uint_as_float(static_cast<unsigned>(s.gather[q][kTellTop] >> 32)));
-        low = fminf(low, __uint_as_float(static_cast<unsigned>(s.gather[q][kTellTop])));
+    {
+        const u64 v = s.gather[lane % ctas][kTellTop];
+        top = __uint_as_float(static_cast<unsigned>(v >> 32));
+        low = __uint_as_float(static_cast<unsigned>(v));
+        for (int k = kMaxCluster / 2; k; k >>= 1) {
+            top = fmaxf(top, __shfl_xor_sync(kFullMask, top, k));
+            low = fminf(low, __shfl_xor_sync(kFullMask, low, k));
+        }
     }
+    // a value that every CTA told, summed over the cluster
+    const auto told = [&](int slot) { return lanes_sum<kMaxCluster>(lane % kMaxCluster < ctas ? s.gather[lane % kMaxCluster][slot] : 0); };
     top += 0.0f;                                // -0 as 0, as the keys have it
 
     const float temp = a.temperature ? a.temperature[row] : 1.0f;
@@ -361,10 +375,10 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleArgs a)
             for (int j = kVe - 1; j >= 0; --j)
                 if (x[j] == top) first = p * kVe + j - skew;
         }
-        for (int k = 16; k; k >>= 1) first = min(first, __shfl_xor_sync(kFullMask, first, k));
+        first = __reduce_min_sync(kFullMask, first);
         if (lane == 0) s.warp[warp] = first;
         __syncthreads();
-        for (int w = 0; w < kWarps; ++w) first = min(first, static_cast<int>(s.warp[w]));
+        first = __reduce_min_sync(kFullMask, static_cast<int>(s.warp[lane % kWarps]));
         tell(kTellFirst, first);
         cluster_sync_all();
         if (rank == 0 && tid == 0) {
@@ -379,10 +393,15 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleArgs a)
     const auto weight = [&](float x) { return units(power(exponent(x, top, c))); };
     // where x - top and c are finite numbers, the exponent is their product, whatever x (-infinity, NaN: far below 0)
     const bool plain = top < INFINITY && c < INFINITY;
-    const auto plain_power = [&](float x, float *y) {
-        *y = fmaxf(__fmul_rn(__fsub_rn(x, top), c), -64.0f);
+    // The passes over a row are written without branches: exponents that are far below 0 at least, their powers, and
+    // masks. `is_plain` (Yes or No) says whether `plain` holds.
+    const auto y_of = [&](auto is_plain, float x) {
+        if constexpr (decltype(is_plain)::value) return fmaxf(__fmul_rn(__fsub_rn(x, top), c), -64.0f);
+        else return fmaxf(exponent(x, top, c), -64.0f);
+    };
+    const auto power_of = [](float y) {
         float e;
-        asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(*y));
+        asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(y));
         return e;
     };
     const int k = a.top_k && a.top_k[row] > 0 && a.top_k[row] < n ? a.top_k[row] : 0;
@@ -432,11 +451,9 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleArgs a)
                 uint32_t hi = 0, lo = 0, near_hi = 0, near_lo = 0;
 #pragma unroll
                 for (int j = 0; j < kVe; ++j) {
-                    float y, e;
-                    if constexpr (decltype(is_plain)::value) e = plain_power(x[j], &y);
-                    else e = power(y = exponent(x[j], top, c));
+                    const float y = y_of(is_plain, x[j]);
                     uint32_t h, l;
-                    split_units(e, &h, &l);
+                    split_units(power_of(y), &h, &l);
                     hi += h, lo += l;
                     const uint32_t is_near = y >= kNear ? kFullMask : 0;
                     near_hi += (h - kBase) & is_near, near_lo += (l - kBase) & is_near;
@@ -449,17 +466,16 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleArgs a)
         all = warp_sum(all), near = warp_sum(near);
         if (lane == 0) s.mass[0][warp] = all, s.mass[0][32 + warp] = near;
         __syncthreads();
-        all = near = 0;
-        for (int w = 0; w < kWarps; ++w) all += s.mass[0][w], near += s.mass[0][32 + w];
+        all = warps_total(s.mass[0]), near = warps_total(s.mass[0] + 32);
         tell(kTellAll, all), tell(kTellNear, near);
         cluster_sync_all();
-        all = near = 0;
-        for (unsigned q = 0; q < ctas; ++q) all += s.gather[q][kTellAll], near += s.gather[q][kTellNear];
+        all = told(kTellAll), near = told(kTellNear);
         s.weight = all;                         // every thread writes the same
         listed = part_up(static_cast<u64>(p24), all) <= near;
     }
     // Tokens that `wanted` names go to this CTA's list, and from there to rank 0's; true where that holds all of them.
     // Call `turn` of a row; s.listed is 0 before it, and rank 0 has the number after it.
+    u64 above = 0;                              // this thread's share of what lies above the list, from the second call on
     const auto collect = [&](int turn, auto wanted) {
         for (int p = w0 + lane; p < w1; p += 32) {
             float x[kVe];
@@ -467,25 +483,27 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleArgs a)
             unsigned take = 0;
 #pragma unroll
             for (int j = 0; j < kVe; ++j)
-                if (wanted(x[j] = clean(x[j]))) take |= 1u << j;
+                take |= static_cast<unsigned>(wanted(x[j])) << j;
             if (!take) continue;
             unsigned at = atomicAdd(&s.listed, static_cast<unsigned>(__popc(take)));
 #pragma unroll
             for (int j = 0; j < kVe; ++j)
                 if (take >> j & 1) {
-                    if (at < kList) list[at] = static_cast<u64>(order_key(x[j])) << 32 | static_cast<unsigned>(p * kVe + j - skew);
+                    if (at < kList) list[at] = static_cast<u64>(order_key(clean(x[j]))) << 32 | static_cast<unsigned>(p * kVe + j - skew);
                     ++at;
                 }
         }
+        if (turn > 0) {
+            above = warp_sum(above);
+            if (lane == 0) s.warp[warp] = above;
+        }
         __syncthreads();
         const unsigned mine = s.listed;
+        if (turn > 0) tell(kTellAbove + turn - 1, warps_total(s.warp));
         tell(kTellList + turn, mine);
         cluster_sync_all();
-        u64 before = 0, all = 0;
-        for (unsigned q = 0; q < ctas; ++q) {
-            if (q < rank) before += s.gather[q][kTellList + turn];
-            all += s.gather[q][kTellList + turn];
-        }
+        const u64 upto = lanes_scan<kMaxCluster>(lane < static_cast<int>(ctas) ? s.gather[lane % kMaxCluster][kTellList + turn] : 0);
+        const u64 all = __shfl_sync(kFullMask, upto, kMaxCluster - 1), before = __shfl_sync(kFullMask, upto, rank) - mine;
         if (all <= kList && rank > 0) {
             const uint32_t there = cluster_map(list, 0) + static_cast<uint32_t>(before) * 8;
             for (unsigned i = tid; i < mine; i += kThreads) cluster_store(there + i * 8, list[i]);
@@ -495,8 +513,9 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleArgs a)
         return all <= kList;
     };
     if (listed) {
-        if (k > 0) listed = collect(0, [&](float x) { return x >= floor_x && x != -INFINITY; });
-        else listed = collect(0, [&](float x) { return exponent(x, top, c) >= kNear; });
+        if (k > 0) listed = collect(0, [&](float x) { return (x >= floor_x) & (x != -INFINITY); });
+        else if (plain) listed = collect(0, [&](float x) { return y_of(Yes(), x) >= kNear; });
+        else listed = collect(0, [&](float x) { return y_of(No(), x) >= kNear; });
         if (listed && rank != 0) return;        // rank 0 does the rest, in its own memory
     }
     if (listed) {
@@ -635,68 +654,87 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleArgs a)
     uint32_t edge = 0;
     u64 ties = 0;
     constexpr float kBinsPerOctave = kBins / 41.0f;
-    const auto bin_of_y = [](float y) { return y > -41.0f ? min(static_cast<int>(-y * kBinsPerOctave), kBins - 1) : kBins - 1; };
+    const auto bin_of_y = [](float y) {         // 1023 for all that weighs nothing, NaN among it
+        return static_cast<int>(__float_as_uint(__fmaf_rd(-fmaxf(y, -40.97f), kBinsPerOctave, 8388608.0f)) - kBase);
+    };
     const auto bin_of = [&](float x) { return bin_of_y(exponent(x, top, c)); };
     // `left` tokens (or weight, `total` in all) are kept, of those above the present edge and edge_mass at it
     const auto cut_row = [&](u64 left, bool by_mass, u64 total, u64 edge_mass) {
-        for (int i = tid; i < kBins; i += kThreads) s.sums[i] = 0;
-        if (tid == 0) s.listed = 0;
+        unsigned *sums = reinterpret_cast<unsigned *>(s.sums);
+        for (int i = tid; i < kBins; i += kThreads) sums[i] = 0;
+        if (tid == 0) s.listed = 0, s.bin = 0, s.last_bin = kBins - 2;
         __syncthreads();
-        // tokens so light that all of them together are less than what is given up: the sums from the top do not
-        // come to them
+        // Weights are summed in units of 2^shift, in which all of them fit 32 bits: short by less than a unit each,
+        // so the cut lies in one of a few bins. Tokens so light that all of them together are less than what is given
+        // up need not be summed: the sums from the top do not come to them.
+        const int shift = by_mass ? max(0, 32 - __clzll(static_cast<long long>(total))) : 0;
+        const unsigned light = by_mass ? max(static_cast<unsigned>((total - left) / static_cast<u64>(n) >> shift), 1u) - 1 : 0;
         const float old_x = edge ? value_of(edge) : -INFINITY;
-        const u64 least = by_mass ? (total - left) / static_cast<u64>(n) : 0;
-        for (int p = w0 + lane; p < w1; p += 32) {
-            float x[kVe];
-            piece(p, x);
-            if (!by_mass) {
+        const uint32_t sums_at = smem_addr(sums);
+        const auto sum_up = [&](auto is_plain, auto mass) {
+            for (int p = w0 + lane; p < w1; p += 32) {
+                float x[kVe];
+                piece(p, x);
 #pragma unroll
                 for (int j = 0; j < kVe; ++j) {
-                    const int i = p * kVe + j - skew;
-                    if (i >= 0 && i < n) atomicAdd(reinterpret_cast<unsigned *>(&s.sums[bin_of(clean(x[j]))]), 1u);
-                }
-            } else {                            // as add_mass, the atomics of a piece one behind the other
-                unsigned old[kVe];
-                uint32_t at[kVe];
-                u64 w[kVe];
-#pragma unroll
-                for (int j = 0; j < kVe; ++j) {
-                    const float y = exponent(x[j], top, c);
-                    w[j] = units(x[j] > old_x ? power(y) : 0.0f);
-                    if (w[j] <= least) w[j] = 0;
-                    at[j] = smem_addr(&s.sums[bin_of_y(y)]);
-                    old[j] = shared_add_if(at[j], static_cast<unsigned>(w[j]), w[j] != 0);
-                }
-#pragma unroll
-                for (int j = 0; j < kVe; ++j) {
-                    const unsigned lo = static_cast<unsigned>(w[j]), hi = static_cast<unsigned>(w[j] >> 32) + (old[j] + lo < old[j]);
-                    shared_add_if(at[j] + 4, hi, hi != 0);
+                    const float y = y_of(is_plain, x[j]);
+                    unsigned add;
+                    if constexpr (decltype(mass)::value) {
+                        add = static_cast<unsigned>(units(power_of(y)) >> shift);
+                        add = (x[j] > old_x) & (add > light) ? add : 0;
+                    } else {
+                        const int i = p * kVe + j - skew;
+                        add = (i >= 0) & (i < n);
+                    }
+                    shared_add_if(sums_at + bin_of_y(y) * 4, add, add != 0);
                 }
             }
-        }
-        if (rank == 0 && tid == 0 && edge_mass) add_mass(&s.sums[bin_of(value_of(edge))], edge_mass);
+        };
+        if (!by_mass) sum_up(No(), No());
+        else if (plain) sum_up(Yes(), Yes());
+        else sum_up(No(), Yes());
+        if (rank == 0 && tid == 0 && edge_mass) atomicAdd(&sums[bin_of(value_of(edge))], static_cast<unsigned>(edge_mass >> shift));
         cluster_sync_all();
         u64 mine[2], all;
-        cluster_sum2(&s.sums[2 * tid], ctas, mine);
-        const u64 sum = mine[0] + mine[1], before = block_scan(sum, s.warp, &all) - sum;
-        if (before < left && left <= before + sum) {
-            const bool second = before + mine[0] < left;
-            s.bin = 2 * tid + second;
-            s.weight = left - before - (second ? mine[0] : 0);
+        cluster_sum2(&sums[2 * tid], ctas, mine);
+        const u64 before = block_scan(mine[0] + mine[1], s.warp, &all) - mine[0] - mine[1];
+        {
+            const u64 half = before + mine[0], upto = half + mine[1];
+            const u64 sure = left + ((1ull << shift) - 1) >> shift, slack = by_mass ? static_cast<u64>(n) + 1 : 0;
+            const u64 maybe = sure > slack ? sure - slack : 0;
+            if (before < maybe && maybe <= upto) s.bin = 2 * tid + (half < maybe);
+            if (before < sure && sure <= upto) s.last_bin = 2 * tid + (half < sure);
         }
         __syncthreads();
-        const int bin = s.bin;
-        const u64 inside = s.weight;
+        const int bin = s.bin, last_bin = s.last_bin;
         if (bin == kBins - 1) {                 // (of the counts) what follows weighs nothing
             cluster_sync_all();
             return;
         }
         u64 w = 1;
-        if (collect(1 + by_mass, [&](float x) { return bin_of(x) == bin && (!by_mass || order_key(x) > edge); })) {
+        above = edge_mass && rank == 0 && tid == 0 && bin_of(value_of(edge)) < bin ? edge_mass : 0;
+        const auto near_cut = [&](auto is_plain, auto mass) {
+            return collect(1 + by_mass, [&](float x) {
+                const float y = y_of(is_plain, x);
+                const int b = bin_of_y(y);
+                if constexpr (decltype(mass)::value) {
+                    const bool open = x > old_x;
+                    above += units(open & (b < bin) ? power_of(y) : 0.0f);
+                    return open & (b >= bin) & (b <= last_bin);
+                } else {
+                    above += b < bin;
+                    return (b >= bin) & (b <= last_bin);
+                }
+            });
+        };
+        const bool fits = !by_mass ? near_cut(No(), No()) : plain ? near_cut(Yes(), Yes()) : near_cut(No(), Yes());
+        if (fits) {
+            const u64 inside = left - told(kTellAbove + by_mass);
             if (rank == 0) {
                 const int m = static_cast<int>(s.listed);
                 const uint32_t old = edge;
-                const bool edge_here = edge_mass && bin_of(value_of(old)) == bin;
+                const int old_bin = bin_of(value_of(old));
+                const bool edge_here = edge_mass && old_bin >= bin && old_bin <= last_bin;
                 // the keys of a bin are near each other: from the first digit in which any differs from the first
                 uint32_t differ = edge_here ? old ^ static_cast<uint32_t>(list[0] >> 32) : 0;
                 for (int i = tid; i < m; i += kThreads) differ |= static_cast<uint32_t>(list[i] >> 32) ^ static_cast<uint32_t>(list[0] >> 32);
@@ -777,8 +815,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleArgs a)
         block_scan(sum, s.warp, &sum);
         tell(kTellSum, sum);
         cluster_sync_all();
-        sum = 0;
-        for (unsigned q = 0; q < ctas; ++q) sum += s.gather[q][kTellSum];
+        sum = told(kTellSum);
         const u64 at_edge = edge ? weight(value_of(edge)) * ties : 0;
         u64 need = part_up(static_cast<u64>(p24), sum + at_edge);
         if (need < 1) need = 1;
@@ -801,10 +838,8 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleArgs a)
             int ties_here = 0;
 #pragma unroll
             for (int j = 0; j < kVe; ++j) {
-                float y, e;
+                float e = power_of(y_of(is_plain, x[j]));
                 uint32_t h, l;
-                if constexpr (decltype(is_plain)::value) e = plain_power(x[j], &y);
-                else e = power(exponent(x[j], top, c));
                 if constexpr (decltype(is_cut)::value) {
                     e = (x[j] < edge_x) | ((e < min_p) & (x[j] != top)) ? 0.0f : e;
                     ties_here += x[j] == edge_x;
@@ -825,29 +860,30 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleArgs a)
     __syncthreads();
     if (lane == 0) s.warp[warp] = sum, s.warp_ties[warp] = equal;
     __syncthreads();
-    sum = equal = 0;
-    for (int w = 0; w < kWarps; ++w) sum += s.warp[w], equal += s.warp_ties[w];
-    tell(kTellKept, sum);
-    tell(kTellTies, equal);
+    tell(kTellKept, warps_total(s.warp));
+    tell(kTellTies, warps_total(s.warp_ties));
     cluster_sync_all();
-    // of a stretch's `eq` ties, `seen` before it, those kept
-    const auto kept_ties = [&](u64 seen, u64 eq) { return tied ? seen >= ties ? 0 : min(eq, ties - seen) : eq; };
-    u64 total = 0, before = 0, seen = 0, mine = 0, seen_all = 0;
-    for (unsigned q = 0; q < ctas; ++q) {
-        const u64 eq = s.gather[q][kTellTies], part_sum = s.gather[q][kTellKept] - (eq - kept_ties(seen_all, eq)) * w_edge;
-        if (q == rank) before = total, seen = seen_all, mine = part_sum;
-        total += part_sum;
-        seen_all += eq;
-    }
-    const u64 target = part(share, total);
-    if (target < before || target >= before + mine) return;
+    // Stretches of the row, a lane to each: their ties and sums, without the ties past the last one that is kept.
+    const auto stretches = [&](u64 seen, u64 eq, u64 part_sum, u64 *ties_upto) {
+        *ties_upto = lanes_scan<16>(eq);
+        const u64 first = seen + *ties_upto - eq;
+        return lanes_scan<16>(part_sum - (tied ? eq - (first >= ties ? 0 : min(eq, ties - first)) : 0) * w_edge);
+    };
+    static_assert(kMaxCluster <= 16 && kWarps <= 16, "a lane to each");
+    const bool here = lane < static_cast<int>(ctas);
+    u64 ties_upto;
+    const u64 upto = stretches(0, here ? s.gather[lane % kMaxCluster][kTellTies] : 0, here ? s.gather[lane % kMaxCluster][kTellKept] : 0, &ties_upto);
+    const u64 total = __shfl_sync(kFullMask, upto, 15), target = part(share, total);
+    const unsigned cta = __ffs(__ballot_sync(kFullMask, upto > target)) - 1;
+    if (rank != cta) return;
     // this CTA's, then: the warp's stretch it falls in, which all threads go over, a piece each
-    int win = 0;
-    for (;; ++win) {
-        const u64 eq = s.warp_ties[win], part_sum = s.warp[win] - (eq - kept_ties(seen, eq)) * w_edge;
-        if (target < before + part_sum) break;
-        before += part_sum;
-        seen += eq;
+    u64 before = __shfl_sync(kFullMask, upto, rank > 0 ? rank - 1 : 0), seen = __shfl_sync(kFullMask, ties_upto, rank > 0 ? rank - 1 : 0);
+    if (rank == 0) before = seen = 0;
+    const u64 warp_upto = before + stretches(seen, lane < kWarps ? s.warp_ties[lane % kWarps] : 0, lane < kWarps ? s.warp[lane % kWarps] : 0, &ties_upto);
+    const int win = __ffs(__ballot_sync(kFullMask, warp_upto > target)) - 1;
+    if (win > 0) {
+        before = __shfl_sync(kFullMask, warp_upto, win - 1);
+        seen += __shfl_sync(kFullMask, ties_upto, win - 1);
     }
     const int f0 = min(p0 + win * per_warp, p1), f1 = min(f0 + per_warp, p1);
     for (int base = f0; base < f1; base += kThreads) {
