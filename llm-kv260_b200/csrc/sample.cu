@@ -802,20 +802,24 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleArgs a)
     };
     if (k > 0) cut_row(k, false, 0, 0);
     if (by_p) {
-        u64 sum = 0;
-        for (int p = w0 + lane; p < w1; p += 32) {
-            float x[kVe];
-            piece(p, x);
+        u64 sum = s.weight;                     // of all tokens, where there is no top-k
+        if (k > 0) {
+            sum = 0;
+            const float old_x = edge ? value_of(edge) : -INFINITY;
+            const auto weigh_above = [&](auto is_plain) {
+                for (int p = w0 + lane; p < w1; p += 32) {
+                    float x[kVe];
+                    piece(p, x);
 #pragma unroll
-            for (int j = 0; j < kVe; ++j) {
-                const float v = clean(x[j]);
-                if (order_key(v) > edge) sum += weight(v);
-            }
+                    for (int j = 0; j < kVe; ++j) sum += units(x[j] > old_x ? power_of(y_of(is_plain, x[j])) : 0.0f);
+                }
+            };
+            if (plain) weigh_above(Yes()); else weigh_above(No());
+            block_scan(sum, s.warp, &sum);
+            tell(kTellSum, sum);
+            cluster_sync_all();
+            sum = told(kTellSum);
         }
-        block_scan(sum, s.warp, &sum);
-        tell(kTellSum, sum);
-        cluster_sync_all();
-        sum = told(kTellSum);
         const u64 at_edge = edge ? weight(value_of(edge)) * ties : 0;
         u64 need = part_up(static_cast<u64>(p24), sum + at_edge);
         if (need < 1) need = 1;
