@@ -27,58 +27,96 @@ struct AppendArgs {
 // Eight consecutive elements, as the copy's unit: 16 bytes of a 16-bit type,
 // 32 of float32.
 template <typename T>
-struct alignas(16) Eight {
-    T v[8];
+struct Eight {
+    uint4 v[sizeof(T) / 2];
 };
 
+template <typename T>
+__device__ __forceinline__ Eight<T> load8(const char *p) {
+    Eight<T> r;
+#pragma unroll
+    for (int i = 0; i < static_cast<int>(sizeof(T) / 2); ++i) r.v[i] = __ldcs(reinterpret_cast<const uint4 *>(p) + i);
+    return r;
+}
+template <typename T>
+__device__ __forceinline__ void store8(char *p, const Eight<T> &s) {
+#pragma unroll
+    for (int i = 0; i < static_cast<int>(sizeof(T) / 2); ++i) reinterpret_cast<uint4 *>(p)[i] = s.v[i];
+}
+// To nearest even, two to a word.
+__device__ __forceinline__ uint32_t pack2(float lo, float hi, __half) {
+    const __half2 h = __floats2half2_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t *>(&h);
+}
+__device__ __forceinline__ uint32_t pack2(float lo, float hi, __nv_bfloat16) {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t *>(&h);
+}
 template <typename Src, typename Dst>
 __device__ __forceinline__ Eight<Dst> convert(const Eight<Src> &s) {
-    Eight<Dst> d;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) d.v[i] = from_float<Dst>(to_float(s.v[i]));
-    return d;
+    if constexpr (sizeof(Src) == sizeof(Dst)) {
+        return s;
+    } else {
+        const auto f = [](uint32_t u) { return __uint_as_float(u); };
+        Eight<Dst> d;
+        d.v[0].x = pack2(f(s.v[0].x), f(s.v[0].y), Dst());
+        d.v[0].y = pack2(f(s.v[0].z), f(s.v[0].w), Dst());
+        d.v[0].z = pack2(f(s.v[1].x), f(s.v[1].y), Dst());
+        d.v[0].w = pack2(f(s.v[1].z), f(s.v[1].w), Dst());
+        return d;
+    }
 }
 
-// The copy is bound by memory: each thread takes eight elements of one row of
-// k and of v. A CTA takes whole tokens, so that a row's page is looked up once
-// per thread, and consecutive threads write consecutive bytes of a row.
+// The copy is bound by memory: a thread takes eight elements of a row of k and
+// of v, of kTokens tokens at a time, and has asked for all of them before it
+// looks up where they go (sequence, length, page: reads that wait for one
+// another). Consecutive threads write consecutive bytes of a row.
 template <typename Src, typename Dst>
 __global__ void __launch_bounds__(kThreads) kv_append_kernel(const AppendArgs a) {
+    constexpr int kTokens = sizeof(Src) == 4 ? 2 : 4;
     const int per_row = a.kv.head_dim / 8;
     const int units = a.kv.n_head_kv * per_row;      // of a token
     const int lane_units = min(units, kThreads);
-    const int tokens = kThreads / lane_units;        // a CTA's at a time
+    const int tokens = kThreads / lane_units;        // side by side in a CTA
     const int ty = threadIdx.x / lane_units, tx = threadIdx.x - ty * lane_units;
-    for (long long t = static_cast<long long>(blockIdx.x) * tokens + ty; ty < tokens && t < a.n_tokens;
-         t += static_cast<long long>(gridDim.x) * tokens) {
-        int b = static_cast<int>(t), i = 0;
-        if (a.offsets) {
-            int lo = 0, hi = a.kv.batch;             // offsets[lo] <= t < offsets[hi]
-            while (hi - lo > 1) {
-                const int mid = (lo + hi) >> 1;
-                if (a.offsets[mid] <= t) lo = mid; else hi = mid;
-            }
-            b = lo;
-            i = static_cast<int>(t) - a.offsets[lo];
+    const int slots = a.kv.cols * a.kv.page_size;
+    const long long t0 = static_cast<long long>(blockIdx.x) * tokens * kTokens + ty;
+    for (int u = tx; u < units && ty < tokens; u += lane_units) {
+        const int h = u / per_row, c = u - h * per_row;
+        Eight<Src> k[kTokens], v[kTokens];
+#pragma unroll
+        for (int x = 0; x < kTokens; ++x) {
+            const long long t = t0 + x * tokens;
+            if (t >= a.n_tokens) break;
+            const long long src = t * a.token_stride + h * a.head_stride + c * static_cast<int>(sizeof(Eight<Src>));
+            k[x] = load8<Src>(a.k_new + src);
+            v[x] = load8<Src>(a.v_new + src);
         }
-        const int at = min(max(a.kv.lengths[b], 0), a.kv.cols * a.kv.page_size);
-        const int slot = at + i;
-        if (i < 0 || slot >= a.kv.cols * a.kv.page_size) continue;
-        const int pos = (a.seen ? a.seen[b] : at) + i;
-        const long long row = kv_row(a.kv, b, 0, slot);
-        for (int u = tx; u < units; u += lane_units) {
-            const int h = u / per_row, c = u - h * per_row;
+#pragma unroll
+        for (int x = 0; x < kTokens; ++x) {
+            const long long t = t0 + x * tokens;
+            if (t >= a.n_tokens) break;
+            int b = static_cast<int>(t), i = 0;
+            if (a.offsets) {
+                int lo = 0, hi = a.kv.batch;         // offsets[lo] <= t < offsets[hi]
+                while (hi - lo > 1) {
+                    const int mid = (lo + hi) >> 1;
+                    if (a.offsets[mid] <= t) lo = mid; else hi = mid;
+                }
+                b = lo;
+                i = static_cast<int>(t) - a.offsets[lo];
+            }
+            const int at = kv_length(a.kv, b), slot = at + i;
+            if (i < 0 || slot >= slots) continue;
+            const long long row = kv_row(a.kv, b, h, slot);
             if (row >= 0) {
-                const long long src = t * a.token_stride + h * a.head_stride + c * static_cast<int>(sizeof(Eight<Src>));
-                const long long dst = row + h * a.kv.head_stride + c * static_cast<int>(sizeof(Eight<Dst>));
-                const Eight<Src> k = *reinterpret_cast<const Eight<Src> *>(a.k_new + src);
-                const Eight<Src> v = *reinterpret_cast<const Eight<Src> *>(a.v_new + src);
-                *reinterpret_cast<Eight<Dst> *>(a.kv.k + dst) = convert<Src, Dst>(k);
-                *reinterpret_cast<Eight<Dst> *>(a.kv.v + dst) = convert<Src, Dst>(v);
+                const long long dst = row + c * static_cast<int>(sizeof(Eight<Dst>));
+                store8<Dst>(a.kv.k + dst, convert<Src, Dst>(k[x]));
+                store8<Dst>(a.kv.v + dst, convert<Src, Dst>(v[x]));
             }
             if (c == 0) {
                 const long long aux = (static_cast<long long>(b) * a.kv.n_head_kv + h) * a.aux_stride + slot;
-                if (a.positions) a.positions[aux] = pos;
+                if (a.positions) a.positions[aux] = (a.seen ? a.seen[b] : at) + i;
                 if (a.weights) a.weights[aux] = 0.0f;
             }
         }
@@ -99,7 +137,7 @@ __global__ void __launch_bounds__(kThreads) kv_append_kernel(const AppendArgs a)
 template <typename Src, typename Dst>
 cudaError_t launch(const AppendArgs &a, cudaStream_t stream) {
     const int units = a.kv.n_head_kv * a.kv.head_dim / 8;
-    const int tokens = kThreads / (units < kThreads ? units : kThreads);
+    const int tokens = kThreads / (units < kThreads ? units : kThreads) * (sizeof(Src) == 4 ? 2 : 4);
     const int grid = a.n_tokens > 0 ? (a.n_tokens + tokens - 1) / tokens : 1;
     kv_append_kernel<Src, Dst><<<grid, kThreads, 0, stream>>>(a);
     return cudaGetLastError();
