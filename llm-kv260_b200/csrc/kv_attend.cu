@@ -37,7 +37,8 @@ namespace {
 constexpr int kWarps = 4;
 constexpr int kThreads = kWarps * 32;
 constexpr int kUnit = 16;              // slots
-constexpr int kJoin = 64;              // parts whose weights are at hand at a time
+constexpr int kJoin = 8;               // parts joined at a time
+constexpr int kShort = 40;             // units of a head that are not worth splitting
 constexpr int kMaxCtas = 1024;         // of the grid
 constexpr float kLog2e = 1.44269504088896340736f;
 // The reference m trails the maximum by 7 to 15 powers of two: weights stay in
@@ -136,7 +137,7 @@ struct Shape {
     static constexpr int kWant = D * NT * (kEs / 2) <= 64 ? 4 : D * NT <= 128 && kEs == 2 ? 3 : 2;
     // Halves (a unit's K, or its V) in flight per warp: what those CTAs leave room for, at least 2 and at most 8;
     // with one CTA per SM where two have no room.
-    static constexpr int kRoom = (227 * 1024 / kWant - 3840 - kFixed) / (kWarps * kHalf);
+    static constexpr int kRoom = (227 * 1024 / kWant - 1792 - kFixed) / (kWarps * kHalf);
     static constexpr int kCtas = kRoom < 2 ? 1 : kWant;
     static constexpr int kDepth = kRoom > 8 ? 8 : kRoom < 2 ? 3 : kRoom;
     static constexpr int kSmem = kWarps * kDepth * kHalf + kFixed;
@@ -165,28 +166,20 @@ struct Cursor {
     }
 };
 
-template <typename Q, typename T, int D, int NT>
-__global__ void __launch_bounds__(kThreads, Shape<T, D, NT>::kCtas)
-    kv_attend_kernel(const AttendArgs a) {
-    using S = Shape<T, D, NT>;
-    constexpr bool kF32 = sizeof(T) == 4;
-    constexpr int kKb = S::kPieces / 2;                    // blocks of 64 bytes of a K row
-    constexpr int kDb = S::kPieces / 4;                    // blocks of 128 bytes of a V row
-    constexpr int kAcc = D / 16;                           // 16-row tiles of O^T
-    extern __shared__ __align__(16) char smem[];
-    __shared__ long long s_sum[kWarps];
-    __shared__ long long s_base;
-    __shared__ int s_b, s_last;
-    __shared__ float s_qs[S::kHeads], s_m[kWarps][S::kHeads], s_l[kWarps][S::kHeads];
-    __shared__ float s_M[S::kHeads], s_L[S::kHeads], s_w[kJoin][S::kHeads];
-    char *s_q = smem + kWarps * S::kDepth * S::kHalf;
-    float *s_o = reinterpret_cast<float *>(s_q + 8 * NT * S::kQRow);
-    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, r = lane >> 2, c = lane & 3;
-    const int d = a.kv.head_dim, heads = a.kv.n_head_kv * a.tiles;
-    const uint32_t ring = smem_addr(smem) + warp * S::kDepth * S::kHalf;
+// A CTA's share of the units.
+struct Stretch {
+    long long c0, base, per;  // its first unit; the first unit of the sequence that lies in; units of a CTA
+    int count, b;             // its units; that sequence
+};
 
-    // This CTA's stretch [c0, c1) of the units, and the sequence c0 lies in.
-    const auto units_of = [&](int b) { return b < a.kv.batch ? (kv_length(a.kv, b) + kUnit - 1) / kUnit : 0; };
+// Where the CTA's stretch lies, into shared memory. Not inlined: the kernel's
+// loop gets by with the registers it needs.
+__device__ __noinline__ void find_stretch(const int *lengths, int batch, int slots, int heads, Stretch *out) {
+    __shared__ long long s_sum[kWarps];
+    __shared__ long long s_c0, s_c1, s_base;
+    __shared__ int s_b;
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const auto units_of = [&](int b) { return b < batch ? (min(max(lengths[b], 0), slots) + kUnit - 1) / kUnit : 0; };
     const auto block_scan = [&](long long v, long long *all) {   // inclusive
         for (int k = 1; k < 32; k <<= 1) {
             const long long y = __shfl_up_sync(kFullMask, v, k);
@@ -203,15 +196,84 @@ __global__ void __launch_bounds__(kThreads, Shape<T, D, NT>::kCtas)
         return v;
     };
     long long total = 0, mine = 0, upto = 0, all;
-    for (int b0 = 0; b0 < a.kv.batch; b0 += kThreads) {
-        mine = static_cast<long long>(units_of(b0 + tid)) * heads;
+    int longest = 0;
+    for (int b0 = 0; b0 < batch; b0 += kThreads) {
+        const int units = units_of(b0 + tid);
+        longest = max(longest, units);
+        mine = static_cast<long long>(units) * heads;
         upto = block_scan(mine, &all) + total;
         total += all;
     }
-    // at least one unit per warp: a head of a short sequence is not worth more parts
+    // Even stretches; but a part costs its CTA a fence, a ticket and another CTA the join, about as much time as ten
+    // units of a warp: where no head is longer than that, whole heads, the same number to each CTA.
+    const bool split = __syncthreads_or(longest > kShort);
     long long per = (total + gridDim.x - 1) / gridDim.x;
     if (per < kWarps) per = kWarps;
-    const long long c0 = blockIdx.x * per, c1 = min(c0 + per, total);
+    const int segments = batch * heads, each = (segments + gridDim.x - 1) / gridDim.x;
+    const int from = static_cast<int>(min(static_cast<long long>(blockIdx.x) * each, static_cast<long long>(segments)));
+    const int to = min(from + each, segments);
+    if (tid == 0) {
+        s_c0 = split ? min(blockIdx.x * per, total) : total;
+        s_c1 = split ? min((blockIdx.x + 1) * per, total) : total;
+        s_b = 0;
+        s_base = 0;
+    }
+    __syncthreads();
+    // sequence b's n units come behind `before` others
+    const auto place = [&](int b, long long n, long long before) {
+        if (split) {
+            const long long c0 = blockIdx.x * per;
+            if (before <= c0 && c0 < before + n) s_b = b, s_base = before;
+        } else if (b < batch) {
+            const int k = b * heads;
+            if (k <= from && from < k + heads) s_c0 = before + n / heads * (from - k), s_b = b, s_base = before;
+            if (k <= to && to < k + heads) s_c1 = before + n / heads * (to - k);
+        }
+    };
+    if (batch <= kThreads) {                               // the scan still holds every sequence's place
+        place(tid, mine, upto - mine);
+    } else {
+        long long run = 0;
+        for (int b0 = 0; b0 < batch; b0 += kThreads) {
+            mine = static_cast<long long>(units_of(b0 + tid)) * heads;
+            upto = block_scan(mine, &all) + run;
+            place(b0 + tid, mine, upto - mine);
+            run += all;
+        }
+    }
+    __syncthreads();
+    if (tid == 0) {
+        int b = s_b;
+        if (s_c0 < s_c1)                                   // a sequence without units has none of the stretch
+            while (units_of(b) == 0) ++b;
+        *out = Stretch{s_c0, s_base, per, static_cast<int>(s_c1 - s_c0), b};
+    }
+    __syncthreads();
+}
+
+template <typename Q, typename T, int D, int NT>
+__global__ void __launch_bounds__(kThreads, Shape<T, D, NT>::kCtas)
+    kv_attend_kernel(const AttendArgs a) {
+    using S = Shape<T, D, NT>;
+    constexpr bool kF32 = sizeof(T) == 4;
+    constexpr int kKb = S::kPieces / 2;                    // blocks of 64 bytes of a K row
+    constexpr int kDb = S::kPieces / 4;                    // blocks of 128 bytes of a V row
+    constexpr int kAcc = D / 16;                           // 16-row tiles of O^T
+    extern __shared__ __align__(16) char smem[];
+    __shared__ Stretch s_stretch;
+    __shared__ int s_last;
+    __shared__ float s_qs[S::kHeads], s_m[kWarps][S::kHeads], s_l[kWarps][S::kHeads];
+    __shared__ float s_M[S::kHeads], s_L[S::kHeads];
+    char *s_q = smem + kWarps * S::kDepth * S::kHalf;
+    float *s_o = reinterpret_cast<float *>(s_q + 8 * NT * S::kQRow);
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, r = lane >> 2, c = lane & 3;
+    const int d = a.kv.head_dim, heads = a.kv.n_head_kv * a.tiles;
+    const uint32_t ring = smem_addr(smem) + warp * S::kDepth * S::kHalf;
+
+    const auto units_of = [&](int b) { return (kv_length(a.kv, b) + kUnit - 1) / kUnit; };
+    find_stretch(a.kv.lengths, a.kv.batch, a.kv.cols * a.kv.page_size, heads, &s_stretch);
+    const long long c0 = s_stretch.c0, per = s_stretch.per;
+    const int count = s_stretch.count;
     const auto empty_sequences = [&] {
         for (int b = blockIdx.x; b < a.kv.batch; b += gridDim.x) {
             if (kv_length(a.kv, b) > 0) continue;
@@ -223,33 +285,21 @@ __global__ void __launch_bounds__(kThreads, Shape<T, D, NT>::kCtas)
                 a.lse[static_cast<long long>(b) * a.n_head + h] = -INFINITY;
         }
     };
-    if (c0 >= c1) {
+    if (count <= 0) {
         empty_sequences();
         return;
     }
-    if (a.kv.batch <= kThreads) {                          // the scan above still holds every sequence's place
-        if (upto - mine <= c0 && c0 < upto) s_b = tid, s_base = upto - mine;
-    } else {
-        long long run = 0;
-        for (int b0 = 0; b0 < a.kv.batch && run <= c0; b0 += kThreads) {
-            mine = static_cast<long long>(units_of(b0 + tid)) * heads;
-            upto = block_scan(mine, &all) + run;
-            if (upto - mine <= c0 && c0 < upto) s_b = b0 + tid, s_base = upto - mine;
-            run += all;
-        }
-    }
-    __syncthreads();
 
     Cursor at;                                             // the first unit of the stretch
-    at.b = s_b;
-    at.units = units_of(s_b);
-    at.s = static_cast<int>((c0 - s_base) / at.units);
-    at.u = static_cast<int>((c0 - s_base) - static_cast<long long>(at.s) * at.units);
+    at.b = s_stretch.b;
+    at.units = units_of(at.b);
+    at.s = static_cast<int>((c0 - s_stretch.base) / at.units);
+    at.u = static_cast<int>((c0 - s_stretch.base) - static_cast<long long>(at.s) * at.units);
 
     // The copying side: units c0 + warp, + kWarps, ... of the stretch, each as K then V.
     Cursor in = at;
     in.advance(a, heads, warp);
-    int to_copy = static_cast<int>((c1 - c0 - warp + kWarps - 1) / kWarps);
+    int to_copy = (count - warp + kWarps - 1) / kWarps;
     unsigned long long there = 0;                          // 16 bits per unit in flight: which rows are there
     int flying = 0;
     uint32_t place_in = 0, place_out = 0;                  // ring places, as byte offsets
@@ -341,10 +391,10 @@ __global__ void __launch_bounds__(kThreads, Shape<T, D, NT>::kCtas)
     const uint32_t k_even = r * kRp * 16 + (c ^ swizzle_k(r)) * 16, k_odd = k_even ^ 64;
     const uint32_t v_at = 2 * c * kRp * 16 + (r ^ swizzle_v(2 * c)) * 16;
 
-    long long f = c0;                                      // first unit of the current head's share
-    while (f < c1) {
-        const long long head_start = f - at.u, head_end = head_start + at.units;
-        const long long end = min(head_end, c1);
+    pdl_launch_dependents();                               // the weights' kernel may come: it waits for all of this one
+    int f = 0;                                             // first unit of the current head's share, from c0 on
+    while (f < count) {
+        const int head_start = f - at.u, head_end = head_start + at.units, end = min(head_end, count);
         const int hkv = at.s / a.tiles, tile = at.s - hkv * a.tiles;
         const int h0 = hkv * a.group + tile * S::kHeads;   // the tile's first query head
         const int live = min(S::kHeads, a.group - tile * S::kHeads);
@@ -394,9 +444,8 @@ __global__ void __launch_bounds__(kThreads, Shape<T, D, NT>::kCtas)
             for (int i = 0; i < kAcc; ++i) o[i][t][0] = o[i][t][1] = o[i][t][2] = o[i][t][3] = 0.0f;
         }
         const uint32_t qa = smem_addr(s_q) + r * S::kQRow + c * 16;
-        const int skew = static_cast<int>((f - c0) & (kWarps - 1));
-        for (long long g = f + ((warp - skew) & (kWarps - 1)); g < end; g += kWarps) {
-            const int u = static_cast<int>(g - head_start);
+        for (int g = f + ((warp - f) & (kWarps - 1)); g < end; g += kWarps) {
+            const int u = g - head_start;
             // S^T: 16 slots by the tile's columns
             __syncwarp();                                  // every lane has read what is overwritten now
             if (kEven) copy_v(); else copy_k();
@@ -560,11 +609,11 @@ __global__ void __launch_bounds__(kThreads, Shape<T, D, NT>::kCtas)
             __syncthreads();
         }
 
-        const bool whole = head_start >= c0 && head_end <= c1;
+        const bool whole = head_start >= 0 && head_end <= count;
         bool write = whole;
         if (!whole) {
             // A part: the head's first CTA keeps it in its second place, a later one in its first.
-            const int first = static_cast<int>(head_start / per), last = static_cast<int>((head_end - 1) / per);
+            const int first = static_cast<int>((c0 + head_start) / per), last = static_cast<int>((c0 + head_end - 1) / per);
             float *mine = a.parts + (2ll * blockIdx.x + (static_cast<int>(blockIdx.x) == first)) * S::kPart;
             for (int i = tid; i < S::kHeads * D; i += kThreads) __stcg(mine + i, s_o[i]);
             if (tid < S::kHeads) {
@@ -581,58 +630,43 @@ __global__ void __launch_bounds__(kThreads, Shape<T, D, NT>::kCtas)
             __syncthreads();
             write = s_last;
             if (write) {
-                // m and l of all parts, a few threads to a head; then O, kJoin parts at a time, in order
+                // Each thread joins four elements of a head, kJoin parts on their way at a time, in their order.
                 const auto part = [&](int j) { return a.parts + (2ll * j + (j == first)) * S::kPart; };
-                const int h = tid % S::kHeads;
-                float top = -INFINITY, sum = 0.0f;
-                for (int j = first + tid / S::kHeads; j <= last; j += kThreads / S::kHeads)
-                    top = fmaxf(top, __ldcg(part(j) + S::kHeads * D + h));
-                for (int k = S::kHeads; k < 32; k <<= 1) top = fmaxf(top, __shfl_xor_sync(kFullMask, top, k));
-                if (lane < S::kHeads) s_m[warp][h] = top;
-                __syncthreads();
-                for (int w = 0; w < kWarps; ++w) top = fmaxf(top, s_m[w][h]);
-                for (int j = first + tid / S::kHeads; j <= last; j += kThreads / S::kHeads) {
-                    const float pm = __ldcg(part(j) + S::kHeads * D + h);
-                    if (pm != -INFINITY) sum += __ldcg(part(j) + S::kHeads * (D + 1) + h) * exp2_fast(pm - top);
-                }
-                for (int k = S::kHeads; k < 32; k <<= 1) sum += __shfl_xor_sync(kFullMask, sum, k);
-                if (lane < S::kHeads) s_l[warp][h] = sum;
-                __syncthreads();
-                if (tid < S::kHeads) {
-                    s_M[tid] = top;
-                    s_L[tid] = ((s_l[0][tid] + s_l[1][tid]) + s_l[2][tid]) + s_l[3][tid];
-                }
-                float4 acc[S::kHeads * D / 4 / kThreads > 0 ? S::kHeads * D / 4 / kThreads : 1];
-                constexpr int kItems = sizeof(acc) / sizeof(float4);
+                for (int i = tid; i < S::kHeads * D / 4; i += kThreads) {
+                    const int h = i * 4 / D;
+                    float top = -INFINITY, sum = 0.0f;
+                    float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                    for (int j0 = first; j0 <= last; j0 += kJoin) {
+                        float pm[kJoin], pl[kJoin];
+                        float4 v[kJoin];
 #pragma unroll
-                for (int i = 0; i < kItems; ++i) acc[i] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-                for (int j0 = first; j0 <= last; j0 += kJoin) {
-                    __syncthreads();
-                    for (int i = tid; i < kJoin * S::kHeads; i += kThreads) {
-                        const int j = j0 + i / S::kHeads;
-                        const float pm = j <= last ? __ldcg(part(j) + S::kHeads * D + h) : -INFINITY;
-                        s_w[i / S::kHeads][h] = pm == -INFINITY ? 0.0f : exp2_fast(pm - top);
-                    }
-                    __syncthreads();
-                    const int count = min(kJoin, last + 1 - j0);
+                        for (int j = 0; j < kJoin; ++j) {
+                            const float *p = part(min(j0 + j, last));
+                            pm[j] = j0 + j <= last ? __ldcg(p + S::kHeads * D + h) : -INFINITY;
+                            pl[j] = __ldcg(p + S::kHeads * (D + 1) + h);
+                            v[j] = __ldcg(reinterpret_cast<const float4 *>(p) + i);
+                        }
+                        float next = top;
 #pragma unroll
-                    for (int i = 0; i < kItems; ++i) {
-                        const int at4 = tid + i * kThreads;
-                        if (at4 >= S::kHeads * D / 4) break;
-#pragma unroll 8
-                        for (int j = 0; j < count; ++j) {
-                            const float4 v = __ldcg(reinterpret_cast<const float4 *>(part(j0 + j)) + at4);
-                            const float w = s_w[j][at4 * 4 / D];
-                            acc[i].x = fmaf(v.x, w, acc[i].x);
-                            acc[i].y = fmaf(v.y, w, acc[i].y);
-                            acc[i].z = fmaf(v.z, w, acc[i].z);
-                            acc[i].w = fmaf(v.w, w, acc[i].w);
+                        for (int j = 0; j < kJoin; ++j) next = fmaxf(next, pm[j]);
+                        if (next == -INFINITY) continue;
+                        const float old = exp2_fast(top - next);
+                        top = next;
+                        sum *= old;
+                        acc.x *= old, acc.y *= old, acc.z *= old, acc.w *= old;
+#pragma unroll
+                        for (int j = 0; j < kJoin; ++j) {
+                            const float w = exp2_fast(pm[j] - top);
+                            sum = fmaf(pl[j], w, sum);
+                            acc.x = fmaf(v[j].x, w, acc.x);
+                            acc.y = fmaf(v[j].y, w, acc.y);
+                            acc.z = fmaf(v[j].z, w, acc.z);
+                            acc.w = fmaf(v[j].w, w, acc.w);
                         }
                     }
+                    reinterpret_cast<float4 *>(s_o)[i] = acc;
+                    if (i * 4 % D == 0) s_M[h] = top, s_L[h] = sum;
                 }
-#pragma unroll
-                for (int i = 0; i < kItems; ++i)
-                    if (tid + i * kThreads < S::kHeads * D / 4) reinterpret_cast<float4 *>(s_o)[tid + i * kThreads] = acc[i];
                 __syncthreads();
             }
         }
@@ -649,7 +683,7 @@ __global__ void __launch_bounds__(kThreads, Shape<T, D, NT>::kCtas)
             }
         }
         f = end;
-        if (f < c1) at.advance(a, heads, static_cast<int>(end - head_start) - at.u);
+        if (f < count) at.advance(a, heads, end - head_start - at.u);
     }
     cp_async_wait<0>();
     empty_sequences();
@@ -668,6 +702,7 @@ struct WeightArgs {
 // 2^t), from the scores that the attention left: a thread per slot.
 __global__ void __launch_bounds__(256) kv_weights_kernel(const WeightArgs a) {
     const int h = blockIdx.y, b = blockIdx.z;
+    pdl_wait_prior_grid();                                 // the attention's scores and sums
     const int n = kv_length(a.kv, b);
     for (int slot = blockIdx.x * 256 + threadIdx.x; slot < n; slot += gridDim.x * 256) {
         float w = 0.0f;
@@ -728,6 +763,8 @@ int kv_attend_validate(const b200_kv_t *kv, const b200_kv_attend_t *a, const cha
         return bad("q must be of the cache's type, or float32 with a float16 cache");
     if (a->n_head < 1 || a->n_head % kv->n_head_kv) return bad("n_head must be a multiple of n_head_kv");
     if (a->n_head / kv->n_head_kv > 256) return bad("at most 256 query heads read one cache head");
+    if (static_cast<int64_t>(kv->table_cols) * kv->page_size / kUnit * a->n_head * kv->batch > 1ll << 38)
+        return bad("more than 2^42 slots of query heads in a call");
     if (!a->q || !a->out) return bad("null address");
     if (a->q_batch_stride < 0 || a->q_head_stride < 0 || a->out_batch_stride < 0 || a->out_head_stride < 0)
         return bad("strides must not be negative");
@@ -793,8 +830,16 @@ cudaError_t kv_attend_launch(const b200_kv_t *kv, const b200_kv_attend_t *p, voi
     w.heads = heads_of_tile(a.group);
     w.decay = p->decay;
     const int ctas = static_cast<int>((a.slots + 255) / 256);
-    kv_weights_kernel<<<dim3(ctas < 64 ? ctas : 64, kv->n_head_kv, kv->batch), 256, 0, stream>>>(w);
-    return cudaGetLastError();
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(ctas < 64 ? ctas : 64, kv->n_head_kv, kv->batch);
+    cfg.blockDim = dim3(256);
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, kv_weights_kernel, w);
 }
 
 }  // namespace b200
