@@ -296,6 +296,23 @@ __global__ void __launch_bounds__(kThreads, Shape<T, D, NT>::kCtas)
     at.s = static_cast<int>((c0 - s_stretch.base) / at.units);
     at.u = static_cast<int>((c0 - s_stretch.base) - static_cast<long long>(at.s) * at.units);
 
+    // The queries of a tile: warp w has the heads w, w + kWarps. They are asked for before rows are (behind 100 KB of
+    // those on their way they would come late): the first tile's here, the next one's while a tile is worked on.
+    constexpr int kMine = S::kHeads / kWarps;
+    constexpr bool kAhead = kMine * D / 32 <= 8;           // as registers allow
+    float qx[kMine][D / 32];
+    const auto load_q = [&](const Cursor &at) {
+        const int hkv = at.s / a.tiles, tile = at.s - hkv * a.tiles;
+#pragma unroll
+        for (int i = 0; i < kMine; ++i) {
+            const int h = tile * S::kHeads + warp + i * kWarps;
+            const Q *q = reinterpret_cast<const Q *>(a.q) + at.b * a.q_batch + (hkv * a.group + h) * a.q_head;
+#pragma unroll
+            for (int k = 0; k < D / 32; ++k) qx[i][k] = h < a.group && lane + 32 * k < d ? to_float(q[lane + 32 * k]) : 0.0f;
+        }
+    };
+    load_q(at);
+
     // The copying side: units c0 + warp, + kWarps, ... of the stretch, each as K then V.
     Cursor in = at;
     in.advance(a, heads, warp);
@@ -402,37 +419,40 @@ __global__ void __launch_bounds__(kThreads, Shape<T, D, NT>::kCtas)
 
         // The queries of the tile, split, and the factor that makes t of a product.
         __syncthreads();
-        for (int h = warp; h < S::kHeads; h += kWarps) {
-            float x[D / 32], top = 0.0f;
 #pragma unroll
-            for (int i = 0; i < D / 32; ++i) {
-                const int k = lane + 32 * i;
-                x[i] = h < live && k < d ? to_float(reinterpret_cast<const Q *>(a.q)[at.b * a.q_batch + (h0 + h) * a.q_head + k]) : 0.0f;
-                top = fmaxf(top, fabsf(x[i]));
-            }
+        for (int i = 0; i < kMine; ++i) {
+            const int h = warp + i * kWarps;
             int e = 0;
             if (sizeof(Q) == 4 && !kF32) {                 // float32 into float16: the head's largest to [1, 2)
+                float top = 0.0f;
+#pragma unroll
+                for (int k = 0; k < D / 32; ++k) top = fmaxf(top, fabsf(qx[i][k]));
                 for (int k = 16; k; k >>= 1) top = fmaxf(top, __shfl_xor_sync(kFullMask, top, k));
                 if (top > 0.0f && top < INFINITY) e = ilogbf(top);
             }
             char *row = s_q + 2 * (h & 3) * S::kQRow + (h >> 2) * 8 * S::kQRow;
 #pragma unroll
-            for (int i = 0; i < D / 32; ++i) {
-                const float v = e ? ldexpf(x[i], -e) : x[i];
+            for (int k = 0; k < D / 32; ++k) {
+                const float v = e ? ldexpf(qx[i][k], -e) : qx[i][k];
                 if (kF32) {
                     uint32_t hi, lo;
                     split_tf32(v, &hi, &lo);
-                    reinterpret_cast<uint32_t *>(row)[lane + 32 * i] = hi;
-                    reinterpret_cast<uint32_t *>(row + S::kQRow)[lane + 32 * i] = lo;
+                    reinterpret_cast<uint32_t *>(row)[lane + 32 * k] = hi;
+                    reinterpret_cast<uint32_t *>(row + S::kQRow)[lane + 32 * k] = lo;
                 } else {
                     const uint32_t p = split_pair<T>(v);
-                    reinterpret_cast<unsigned short *>(row)[lane + 32 * i] = static_cast<unsigned short>(p);
-                    reinterpret_cast<unsigned short *>(row + S::kQRow)[lane + 32 * i] = static_cast<unsigned short>(p >> 16);
+                    reinterpret_cast<unsigned short *>(row)[lane + 32 * k] = static_cast<unsigned short>(p);
+                    reinterpret_cast<unsigned short *>(row + S::kQRow)[lane + 32 * k] = static_cast<unsigned short>(p >> 16);
                 }
             }
             if (lane == 0) s_qs[h] = ldexpf(a.scale * kLog2e, e);
         }
         __syncthreads();
+        if (kAhead && head_end < count) {
+            Cursor next = at;
+            next.advance(a, heads, at.units - at.u);
+            load_q(next);
+        }
 
         float m[NT], l[NT], o[kAcc][NT][4], qs[NT];
 #pragma unroll
@@ -683,7 +703,10 @@ __global__ void __launch_bounds__(kThreads, Shape<T, D, NT>::kCtas)
             }
         }
         f = end;
-        if (f < count) at.advance(a, heads, end - head_start - at.u);
+        if (f < count) {
+            at.advance(a, heads, end - head_start - at.u);
+            if (!kAhead) load_q(at);
+        }
     }
     cp_async_wait<0>();
     empty_sequences();
