@@ -157,6 +157,11 @@ B200_API int b200_rope_table_freqs(float *cs, int d, int pos, float base, const 
 B200_API int b200_launch_floor(int device, int launches, int ctas, int threads, int smem, int pdl, int reps,
                                float *us_per_launch);
 
+/* Device address of this rank's logits, float32[n_vocab/nranks], as the last
+ * forward left them (0 for a null decoder): what b200_sample reads in place,
+ * once b200_decoder_forward has returned or on the decoder's stream. */
+B200_API uint64_t b200_decoder_logits(b200_decoder_t *d);
+
 /* The decoder's CUDA stream (cudaStream_t). */
 B200_API void *b200_decoder_stream(b200_decoder_t *d);
 

@@ -184,6 +184,7 @@ SIGNATURES: dict[str, tuple] = {
     "b200_gguf_tensor": (c_int, [c_vp, c_char_p, P(c_vp), P(c_u64), P(c_int), P(ctypes.c_int64)]),
     "b200_decoder_load_gguf": (c_int, [c_vp, c_vp]),
     "b200_decoder_stream": (c_vp, [c_vp]),
+    "b200_decoder_logits": (c_u64, [c_vp]),
     "b200_decoder_destroy": (c_int, [c_vp]),
     "b200_last_error": (c_char_p, []),
 }

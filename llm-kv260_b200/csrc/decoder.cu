@@ -1062,6 +1062,8 @@ extern "C" int b200_launch_floor(int device, int launches, int ctas, int threads
     return rc;
 }
 
+extern "C" uint64_t b200_decoder_logits(b200_decoder_t *d) { return d ? reinterpret_cast<uint64_t>(d->logits) : 0; }
+
 extern "C" void *b200_decoder_stream(b200_decoder_t *d) { return d ? d->stream : nullptr; }
 
 extern "C" int b200_decoder_destroy(b200_decoder_t *d) {

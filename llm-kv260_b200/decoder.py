@@ -29,7 +29,7 @@ class Decoder:
             c.rope_base, c.rms_eps = float(model["rope_base"]), float(model["rms_eps"])
         c.ctx_max, c.kv_f16, c.round_mode, c.exact_norm = ctx_max, int(kv_f16), round_mode, int(exact_norm)
         c.persistent = int(persistent)
-        self.cfg, self.rank, self.nranks, self.ctx_max = c, rank, nranks, ctx_max
+        self.cfg, self.rank, self.nranks, self.ctx_max, self.device = c, rank, nranks, ctx_max, device
         self.h = ctypes.c_void_p()
         check(lib().b200_decoder_create(ctypes.byref(self.h), ctypes.byref(c), device, rank, nranks,
                                         comm.h if comm is not None else None), "b200_decoder_create")
@@ -108,6 +108,49 @@ class Decoder:
 
     def logits(self) -> np.ndarray:
         return self._read(1, self.cfg.n_vocab // self.nranks, np.float32)
+
+    def logits_tensor(self):
+        """The logits in place: a torch view [1, n_vocab / nranks] of the decoder's own device buffer, valid while the
+        decoder lives and overwritten by its next forward."""
+        import torch
+        n = self.cfg.n_vocab // self.nranks
+
+        class View:
+            __cuda_array_interface__ = dict(shape=(1, n), typestr="<f4", version=3, strides=None,
+                                            data=(int(lib().b200_decoder_logits(self.h)), False))
+
+        return torch.as_tensor(View(), device=f"cuda:{self.device}")
+
+    def generate_sampled(self, prompt, n_gen: int, u, temperature: float = 1.0, top_k: int = 0, top_p: float = 1.0,
+                         min_p: float = 0.0, engine=None) -> tuple[np.ndarray, np.ndarray]:
+        """generate with a sampler (Engine.sample) in the greedy pick's place: n_gen tokens and the logs of their
+        probabilities, drawn with the uniform numbers u[n_gen]. One rank: the sampler needs the whole vocabulary."""
+        if self.nranks != 1:
+            raise ValueError("sampling needs the whole vocabulary on one rank")
+        prompt, u = np.asarray(prompt, np.int32), np.asarray(u, np.float32)
+        if u.shape != (n_gen,):
+            raise ValueError(f"u must hold n_gen = {n_gen} numbers")
+        if prompt.size < 1 or prompt.size + n_gen - 1 > self.ctx_max:
+            raise ValueError("the prompt is empty, or prompt and tokens exceed ctx_max")
+        import torch
+        from .engine import Engine
+        dev = f"cuda:{self.device}"
+        eng = engine if engine is not None else Engine(self.device)
+        eng.set_stream(torch.cuda.current_stream(self.device).cuda_stream)
+        logits, du = self.logits_tensor(), torch.from_numpy(u).to(dev)
+        kw = dict(temperature=torch.full((1,), temperature, device=dev), top_p=torch.full((1,), top_p, device=dev),
+                  top_k=torch.full((1,), top_k, dtype=torch.int32, device=dev),
+                  min_p=torch.full((1,), min_p, device=dev))
+        pick, lp = torch.empty(1, dtype=torch.int32, device=dev), torch.empty(1, device=dev)
+        tokens, logprobs = np.empty(n_gen, np.int32), np.empty(n_gen, np.float32)
+        for i, t in enumerate(prompt):
+            self.forward(int(t), i)
+        for i in range(n_gen):
+            eng.sample(logits, du[i:i + 1], pick, lp, **kw)
+            tokens[i], logprobs[i] = int(pick), float(lp)
+            if i + 1 < n_gen:
+                self.forward(int(tokens[i]), prompt.size + i)
+        return tokens, logprobs
 
     def tokens(self) -> np.ndarray:
         return self._read(2, self.ctx_max + 1, np.int32)
