@@ -8,10 +8,14 @@ into libb200gemv.so.
 from __future__ import annotations
 
 import ctypes
+from struct import Struct
 
 from . import capi
 from .capi import check, lib
 from .paged import PagedKV, address, dtype_code, rows
+
+# native struct formats of the C ABI's field types
+_FORMAT = {capi.c_u64: "Q", capi.c_i64: "q", capi.c_int: "i", ctypes.c_float: "f"}
 
 QK = 32
 BLOCK_BYTES = 18
@@ -79,7 +83,7 @@ class Engine:
         h = ctypes.c_void_p()
         check(lib().b200_engine_open(ctypes.byref(h), device), "b200_engine_open")
         self.h = h
-        self._structs, self._ws = {}, None
+        self._structs, self._ws, self._ws_at, self._ws_bytes = {}, None, 0, 0
         self.set_stream(current_stream_handle(device) if stream is None else stream)
 
     def close(self) -> None:
@@ -162,14 +166,14 @@ class Engine:
 
     def _call(self, name: str, struct, values, kv: PagedKV | None = None) -> None:
         """The C call of that name, its argument struct (one per engine, filled anew each time) set to `values`."""
-        L = lib()
         kept = self._structs.get(name)
         if kept is None:
-            c = struct()
-            kept = self._structs[name] = (getattr(L, name), c, ctypes.byref(c), [f for f, _ in struct._fields_])
-        fn, c, ref, fields = kept
-        for f, v in zip(fields, values):
-            setattr(c, f, v)
+            buf = bytearray(ctypes.sizeof(struct))
+            fmt = Struct("".join(_FORMAT[t] for _, t in struct._fields_))
+            c = struct.from_buffer(buf)
+            kept = self._structs[name] = (getattr(lib(), name), ctypes.byref(c), fmt.pack_into, buf)
+        fn, ref, pack, buf = kept
+        pack(buf, 0, *values)
         rc = fn(self.h, ref) if kv is None else fn(self.h, kv.ref, ref)
         if rc < 0:
             check(rc, name)
@@ -210,7 +214,9 @@ class Engine:
         w, stride2 = (0, stride) if weights is None else kv.aux(weights, "float32", "weights")
         if wo and stride != stride2:
             raise ValueError("weights and weights_out must have one shape")
-        ws_bytes = lib().b200_kv_attend_workspace(kv.ref, n_head, 1 if wo else 0)
+        ws_bytes = kv.workspace.get((n_head, wo != 0))
+        if ws_bytes is None:
+            ws_bytes = kv.workspace[n_head, wo != 0] = int(lib().b200_kv_attend_workspace(kv.ref, n_head, int(wo != 0)))
         self._call("b200_kv_attend", capi.b200_kv_attend_t, (
             q.data_ptr(), out.data_ptr(), dtype_code(q, "q"), n_head, qs[0], qs[1], os_[0], os_[1],
             kv.head_dim ** -0.5 if scale is None else scale, address(lse, "float32", "lse", (kv.batch, n_head)), w, wo,
@@ -219,13 +225,13 @@ class Engine:
     def _workspace(self, nbytes: int) -> int:
         """Device memory of this engine's own for calls on its stream, kept and grown; one that is given back stays
         reserved until the work queued on that stream is done."""
-        have = self._ws
-        if have is None or have.numel() < nbytes:
+        if self._ws_bytes < nbytes:
             torch = _torch()
-            if have is not None and self.stream:
-                have.record_stream(torch.cuda.ExternalStream(self.stream, device=self.device))
-            self._ws = have = torch.empty(nbytes, dtype=torch.uint8, device=f"cuda:{self.device}")
-        return have.data_ptr()
+            if self._ws is not None and self.stream:
+                self._ws.record_stream(torch.cuda.ExternalStream(self.stream, device=self.device))
+            self._ws = torch.empty(nbytes, dtype=torch.uint8, device=f"cuda:{self.device}")
+            self._ws_at, self._ws_bytes = self._ws.data_ptr(), nbytes
+        return self._ws_at
 
     def kv_evict(self, kv: PagedKV, weights, positions, seen, budget: int, recent: int = 0, sinks: int = 0,
                  weights_out=None, positions_out=None, lengths_out=None) -> None:

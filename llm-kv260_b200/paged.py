@@ -29,13 +29,14 @@ def address(t, dtype: str, name: str, shape) -> int:
     """Device address of a contiguous CUDA tensor of that type ("int32" or "float32") and shape; 0 for None."""
     if t is None:
         return 0
-    if not t.is_cuda or t.dtype is not (_CODES or codes())[dtype]:
+    want = (_CODES or codes())[dtype]
+    if t.dtype is want and t.is_cuda and t.shape == shape and t.is_contiguous():
+        return t.data_ptr()
+    if not t.is_cuda or t.dtype is not want:
         raise ValueError(f"{name} must be a CUDA {dtype} tensor")
     if t.shape != shape:
         raise ValueError(f"{name} must have shape {shape}, not {tuple(t.shape)}")
-    if not t.is_contiguous():
-        raise ValueError(f"{name} must be contiguous")
-    return t.data_ptr()
+    raise ValueError(f"{name} must be contiguous")
 
 
 def rows(t, name: str, shape) -> tuple[int, int]:
@@ -80,6 +81,7 @@ class PagedKV:
                                 self.n_head_kv, self.head_dim, st[0], st[1], st[2], table.data_ptr(),
                                 max(table.stride(0), cols), cols, at, self.batch)
         self.ref = ctypes.byref(self.c)
+        self.workspace: dict = {}     # bytes that kv_attend needs, by (query heads, with weights)
 
     def aux(self, t, dtype: str, name: str) -> tuple[int, int]:
         """Address and head stride of a [batch, n_head_kv, >= capacity] tensor beside the cache (weights, positions)."""
