@@ -722,28 +722,31 @@ struct WeightArgs {
 };
 
 // weights_out = decay weights + sum over the query heads of 2^(t - log2 sum
-// 2^t), from the scores that the attention left: a thread per slot.
+// 2^t), from the scores that the attention left: a thread per slot. It is on
+// the GPU before the attention ends, and has read by then what that does not
+// write.
 __global__ void __launch_bounds__(256) kv_weights_kernel(const WeightArgs a) {
-    const int h = blockIdx.y, b = blockIdx.z;
+    const int h = blockIdx.y, b = blockIdx.z, slot = blockIdx.x * 256 + threadIdx.x;
+    const long long head = static_cast<long long>(b) * a.kv.n_head_kv + h, aux = head * a.aux_stride + slot;
+    const bool on = slot < kv_length(a.kv, b);
+    float w = on && a.weights ? a.decay * a.weights[aux] : 0.0f;
     pdl_wait_prior_grid();                                 // the attention's scores and sums
-    const int n = kv_length(a.kv, b);
-    for (int slot = blockIdx.x * 256 + threadIdx.x; slot < n; slot += gridDim.x * 256) {
-        float w = 0.0f;
-        for (int tile = 0; tile < a.tiles; ++tile) {
-            const long long s = (static_cast<long long>(b) * a.kv.n_head_kv + h) * a.tiles + tile;
-            const float4 *t4 = reinterpret_cast<const float4 *>(a.scores + (s * a.slots + slot) * a.heads);
-            const int live = min(a.heads, a.group - tile * a.heads);
-            for (int i = 0; i < live; i += 4) {
-                const float4 t = __ldcg(t4 + i / 4);
-                const float v[4] = {t.x, t.y, t.z, t.w};
+    if (!on) return;
+    float sum = 0.0f;
+    for (int tile = 0; tile < a.tiles; ++tile) {
+        const long long s = head * a.tiles + tile;
+        const float4 *t4 = reinterpret_cast<const float4 *>(a.scores + (s * a.slots + slot) * a.heads);
+        const float4 *l4 = reinterpret_cast<const float4 *>(a.lse2 + s * a.heads);
+        const int live = min(a.heads, a.group - tile * a.heads);
+        for (int i = 0; i < live; i += 4) {
+            const float4 t = __ldcg(t4 + i / 4), l = __ldcg(l4 + i / 4);
+            const float v[4] = {t.x, t.y, t.z, t.w}, lse[4] = {l.x, l.y, l.z, l.w};
 #pragma unroll
-                for (int j = 0; j < 4; ++j)
-                    if (i + j < live && v[j] != -INFINITY) w += exp2_fast(v[j] - __ldcg(a.lse2 + s * a.heads + i + j));
-            }
+            for (int j = 0; j < 4; ++j)
+                if (i + j < live && v[j] != -INFINITY) sum += exp2_fast(v[j] - lse[j]);
         }
-        const long long aux = (static_cast<long long>(b) * a.kv.n_head_kv + h) * a.aux_stride + slot;
-        a.weights_out[aux] = (a.weights ? a.decay * a.weights[aux] : 0.0f) + w;
     }
+    a.weights_out[aux] = w + sum;
 }
 
 int heads_of_tile(int group) { return group <= 4 ? 4 : 8; }
@@ -852,9 +855,8 @@ cudaError_t kv_attend_launch(const b200_kv_t *kv, const b200_kv_attend_t *p, voi
     w.tiles = a.tiles;
     w.heads = heads_of_tile(a.group);
     w.decay = p->decay;
-    const int ctas = static_cast<int>((a.slots + 255) / 256);
     cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3(ctas < 64 ? ctas : 64, kv->n_head_kv, kv->batch);
+    cfg.gridDim = dim3(static_cast<unsigned>((a.slots + 255) / 256), kv->n_head_kv, kv->batch);
     cfg.blockDim = dim3(256);
     cfg.stream = stream;
     cudaLaunchAttribute attr[1];
