@@ -68,55 +68,67 @@ __device__ __forceinline__ Eight<Dst> convert(const Eight<Src> &s) {
 }
 
 // The copy is bound by memory: a thread takes eight elements of a row of k and
-// of v, of kTokens tokens at a time, and has asked for all of them before it
-// looks up where they go (sequence, length, page: reads that wait for one
-// another). Consecutive threads write consecutive bytes of a row.
+// of v, of kTokens tokens, and has asked for all of them before the CTA looks
+// up where they go (sequence, length, page: reads that wait for one another,
+// done by one thread per token). Consecutive threads write consecutive bytes of
+// a row.
 template <typename Src, typename Dst>
 __global__ void __launch_bounds__(kThreads) kv_append_kernel(const AppendArgs a) {
     constexpr int kTokens = sizeof(Src) == 4 ? 2 : 4;
+    __shared__ long long s_row[kThreads * kTokens / 8];   // a token's row of head 0, -1: none
+    __shared__ int s_slot[kThreads * kTokens / 8], s_seq[kThreads * kTokens / 8], s_pos[kThreads * kTokens / 8];
     const int per_row = a.kv.head_dim / 8;
     const int units = a.kv.n_head_kv * per_row;      // of a token
     const int lane_units = min(units, kThreads);
-    const int tokens = kThreads / lane_units;        // side by side in a CTA
+    const int tokens = min(kThreads / lane_units, kThreads / 8);   // side by side in a CTA
     const int ty = threadIdx.x / lane_units, tx = threadIdx.x - ty * lane_units;
     const int slots = a.kv.cols * a.kv.page_size;
-    const long long t0 = static_cast<long long>(blockIdx.x) * tokens * kTokens + ty;
-    for (int u = tx; u < units && ty < tokens; u += lane_units) {
-        const int h = u / per_row, c = u - h * per_row;
+    const long long first = static_cast<long long>(blockIdx.x) * tokens * kTokens;
+    const int count = static_cast<int>(min(static_cast<long long>(tokens) * kTokens, a.n_tokens - first));
+    for (int u0 = 0; u0 < units; u0 += lane_units) {
+        const int u = u0 + tx, h = u / per_row, c = u - h * per_row;
+        const bool on = ty < tokens && u < units;
         Eight<Src> k[kTokens], v[kTokens];
 #pragma unroll
         for (int x = 0; x < kTokens; ++x) {
-            const long long t = t0 + x * tokens;
-            if (t >= a.n_tokens) break;
-            const long long src = t * a.token_stride + h * a.head_stride + c * static_cast<int>(sizeof(Eight<Src>));
+            if (!on || ty + x * tokens >= count) break;
+            const long long src = (first + ty + x * tokens) * a.token_stride + h * a.head_stride + c * static_cast<int>(sizeof(Src)) * 8;
             k[x] = load8<Src>(a.k_new + src);
             v[x] = load8<Src>(a.v_new + src);
         }
+        if (u0 == 0) {
+            if (static_cast<int>(threadIdx.x) < count) {
+                const long long t = first + threadIdx.x;
+                int b = static_cast<int>(t), i = 0;
+                if (a.offsets) {
+                    int lo = 0, hi = a.kv.batch;     // offsets[lo] <= t < offsets[hi]
+                    while (hi - lo > 1) {
+                        const int mid = (lo + hi) >> 1;
+                        if (a.offsets[mid] <= t) lo = mid; else hi = mid;
+                    }
+                    b = lo;
+                    i = static_cast<int>(t) - a.offsets[lo];
+                }
+                const int at = kv_length(a.kv, b), slot = i < 0 || at + i >= slots ? -1 : at + i;
+                s_seq[threadIdx.x] = b;
+                s_slot[threadIdx.x] = slot;
+                s_pos[threadIdx.x] = (a.seen ? a.seen[b] : at) + i;
+                s_row[threadIdx.x] = slot < 0 ? -1 : kv_row(a.kv, b, 0, slot);
+            }
+            __syncthreads();
+        }
 #pragma unroll
         for (int x = 0; x < kTokens; ++x) {
-            const long long t = t0 + x * tokens;
-            if (t >= a.n_tokens) break;
-            int b = static_cast<int>(t), i = 0;
-            if (a.offsets) {
-                int lo = 0, hi = a.kv.batch;         // offsets[lo] <= t < offsets[hi]
-                while (hi - lo > 1) {
-                    const int mid = (lo + hi) >> 1;
-                    if (a.offsets[mid] <= t) lo = mid; else hi = mid;
-                }
-                b = lo;
-                i = static_cast<int>(t) - a.offsets[lo];
-            }
-            const int at = kv_length(a.kv, b), slot = at + i;
-            if (i < 0 || slot >= slots) continue;
-            const long long row = kv_row(a.kv, b, h, slot);
-            if (row >= 0) {
-                const long long dst = row + c * static_cast<int>(sizeof(Eight<Dst>));
+            const int j = ty + x * tokens;
+            if (!on || j >= count) break;
+            if (s_row[j] >= 0) {
+                const long long dst = s_row[j] + h * a.kv.head_stride + c * static_cast<int>(sizeof(Dst)) * 8;
                 store8<Dst>(a.kv.k + dst, convert<Src, Dst>(k[x]));
                 store8<Dst>(a.kv.v + dst, convert<Src, Dst>(v[x]));
             }
-            if (c == 0) {
-                const long long aux = (static_cast<long long>(b) * a.kv.n_head_kv + h) * a.aux_stride + slot;
-                if (a.positions) a.positions[aux] = (a.seen ? a.seen[b] : at) + i;
+            if (c == 0 && s_slot[j] >= 0) {
+                const long long aux = (static_cast<long long>(s_seq[j]) * a.kv.n_head_kv + h) * a.aux_stride + s_slot[j];
+                if (a.positions) a.positions[aux] = s_pos[j];
                 if (a.weights) a.weights[aux] = 0.0f;
             }
         }
@@ -137,7 +149,8 @@ __global__ void __launch_bounds__(kThreads) kv_append_kernel(const AppendArgs a)
 template <typename Src, typename Dst>
 cudaError_t launch(const AppendArgs &a, cudaStream_t stream) {
     const int units = a.kv.n_head_kv * a.kv.head_dim / 8;
-    const int tokens = kThreads / (units < kThreads ? units : kThreads) * (sizeof(Src) == 4 ? 2 : 4);
+    const int side = kThreads / (units < kThreads ? units : kThreads);
+    const int tokens = (side < kThreads / 8 ? side : kThreads / 8) * (sizeof(Src) == 4 ? 2 : 4);
     const int grid = a.n_tokens > 0 ? (a.n_tokens + tokens - 1) / tokens : 1;
     kv_append_kernel<Src, Dst><<<grid, kThreads, 0, stream>>>(a);
     return cudaGetLastError();

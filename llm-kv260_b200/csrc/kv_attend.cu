@@ -789,8 +789,9 @@ int kv_attend_validate(const b200_kv_t *kv, const b200_kv_attend_t *a, const cha
         return bad("q must be of the cache's type, or float32 with a float16 cache");
     if (a->n_head < 1 || a->n_head % kv->n_head_kv) return bad("n_head must be a multiple of n_head_kv");
     if (a->n_head / kv->n_head_kv > 256) return bad("at most 256 query heads read one cache head");
-    if (static_cast<int64_t>(kv->table_cols) * kv->page_size / kUnit * a->n_head * kv->batch > 1ll << 38)
-        return bad("more than 2^42 slots of query heads in a call");
+    if (static_cast<int64_t>(a->n_head) * kv->batch > 1 << 24 ||
+        (static_cast<int64_t>(kv->table_cols) * kv->page_size / kUnit + 1) * a->n_head * kv->batch > 1ll << 38)
+        return bad("more than 2^24 query heads, or 2^42 slots of theirs, in a call");
     if (!a->q || !a->out) return bad("null address");
     if (a->q_batch_stride < 0 || a->q_head_stride < 0 || a->out_batch_stride < 0 || a->out_head_stride < 0)
         return bad("strides must not be negative");

@@ -94,6 +94,13 @@ ATTEND = {
     "mha": ([129] * 3, 6, 6, 64, 7, "bf16", "bf16", "head"),
     "one_long": ([20011], 8, 2, 128, 64, "f32", "f16", "head"),
     "many_short": (list(range(1, 70)), 4, 2, 64, 16, "f32", "f16", "head"),
+    "d256_group8": ([300, 77], 16, 2, 256, 16, "bf16", "bf16", "head"),
+    "d256_f32_group6": ([210, 800], 12, 2, 256, 33, "f32", "f32", "head"),
+    "batch_of_300_short": ([(7 * i) % 100 for i in range(300)], 3, 1, 64, 16, "f32", "f16", "head"),
+    "batch_of_200_mixed": ([(37 * i) % 97 * (20 if i % 50 == 3 else 1) for i in range(200)], 2, 1, 64, 32, "bf16", "bf16",
+                           "head"),
+    "heads_of_640_and_641": ([640, 640], 8, 2, 128, 16, "f16", "f16", "head"),
+    "one_head_over": ([641, 3, 640], 8, 2, 128, 16, "f16", "f16", "head"),
 }
 
 
@@ -446,6 +453,7 @@ EVICT = {
     "all_but_one": ([2, 1000], 1, 64, 128, "bf16", 999, 100, 1, "random"),
     "more_moves_than_one_list": ([9000], 1, 64, 64, "f16", 4400, 2500, 0, "random"),
     "long": ([70000], 1, 8, 64, "f16", 30000, 1000, 4, "random"),
+    "longer_than_shared_memory": ([300000, 5000], 1, 8, 64, "f16", 1500, 100, 4, "random"),
 }
 
 
