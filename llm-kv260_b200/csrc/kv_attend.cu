@@ -37,7 +37,6 @@ namespace {
 constexpr int kWarps = 4;
 constexpr int kThreads = kWarps * 32;
 constexpr int kUnit = 16;              // slots
-constexpr int kJoin = 8;               // parts joined at a time
 constexpr int kShort = 40;             // units of a head that are not worth splitting
 constexpr int kMaxCtas = 1024;         // of the grid
 constexpr float kLog2e = 1.44269504088896340736f;
@@ -650,42 +649,56 @@ __global__ void __launch_bounds__(kThreads, Shape<T, D, NT>::kCtas)
             __syncthreads();
             write = s_last;
             if (write) {
-                // Each thread joins four elements of a head, kJoin parts on their way at a time, in their order.
+                // Each thread joins four elements of a head (or of some), kJoin parts on their way at a time, in order.
                 const auto part = [&](int j) { return a.parts + (2ll * j + (j == first)) * S::kPart; };
-                for (int i = tid; i < S::kHeads * D / 4; i += kThreads) {
-                    const int h = i * 4 / D;
-                    float top = -INFINITY, sum = 0.0f;
-                    float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-                    for (int j0 = first; j0 <= last; j0 += kJoin) {
-                        float pm[kJoin], pl[kJoin];
-                        float4 v[kJoin];
+                constexpr int kItems = S::kHeads * D / 4 > kThreads ? S::kHeads * D / 4 / kThreads : 1, kJoin = kItems > 2 ? 4 : 8;
+                float top[kItems], sum[kItems];
+                float4 acc[kItems];
+                int at4[kItems];                           // (a tile of 64 elements has work for half the threads)
 #pragma unroll
-                        for (int j = 0; j < kJoin; ++j) {
-                            const float *p = part(min(j0 + j, last));
-                            pm[j] = j0 + j <= last ? __ldcg(p + S::kHeads * D + h) : -INFINITY;
-                            pl[j] = __ldcg(p + S::kHeads * (D + 1) + h);
-                            v[j] = __ldcg(reinterpret_cast<const float4 *>(p) + i);
-                        }
-                        float next = top;
+                for (int i = 0; i < kItems; ++i) {
+                    top[i] = -INFINITY;
+                    sum[i] = 0.0f;
+                    acc[i] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                    at4[i] = min(tid + i * kThreads, S::kHeads * D / 4 - 1);
+                }
+                for (int j0 = first; j0 <= last; j0 += kJoin) {
+                    float pm[kItems][kJoin], pl[kItems][kJoin];
+                    float4 v[kItems][kJoin];
 #pragma unroll
-                        for (int j = 0; j < kJoin; ++j) next = fmaxf(next, pm[j]);
-                        if (next == -INFINITY) continue;
-                        const float old = exp2_fast(top - next);
-                        top = next;
-                        sum *= old;
-                        acc.x *= old, acc.y *= old, acc.z *= old, acc.w *= old;
+                    for (int j = 0; j < kJoin; ++j) {
+                        const float *p = part(min(j0 + j, last));
 #pragma unroll
-                        for (int j = 0; j < kJoin; ++j) {
-                            const float w = exp2_fast(pm[j] - top);
-                            sum = fmaf(pl[j], w, sum);
-                            acc.x = fmaf(v[j].x, w, acc.x);
-                            acc.y = fmaf(v[j].y, w, acc.y);
-                            acc.z = fmaf(v[j].z, w, acc.z);
-                            acc.w = fmaf(v[j].w, w, acc.w);
+                        for (int i = 0; i < kItems; ++i) {
+                            pm[i][j] = __ldcg(p + S::kHeads * D + at4[i] * 4 / D);
+                            pl[i][j] = __ldcg(p + S::kHeads * (D + 1) + at4[i] * 4 / D);
+                            v[i][j] = __ldcg(reinterpret_cast<const float4 *>(p) + at4[i]);
                         }
                     }
-                    reinterpret_cast<float4 *>(s_o)[i] = acc;
-                    if (i * 4 % D == 0) s_M[h] = top, s_L[h] = sum;
+#pragma unroll
+                    for (int i = 0; i < kItems; ++i) {
+                        float next = top[i];
+#pragma unroll
+                        for (int j = 0; j < kJoin; ++j) next = fmaxf(next, pm[i][j]);
+                        const float old = next == -INFINITY ? 0.0f : exp2_fast(top[i] - next);
+                        top[i] = next;
+                        sum[i] *= old;
+                        acc[i].x *= old, acc[i].y *= old, acc[i].z *= old, acc[i].w *= old;
+#pragma unroll
+                        for (int j = 0; j < kJoin; ++j) {
+                            const float w = j0 + j > last || next == -INFINITY ? 0.0f : exp2_fast(pm[i][j] - next);
+                            sum[i] = fmaf(pl[i][j], w, sum[i]);
+                            acc[i].x = fmaf(v[i][j].x, w, acc[i].x);
+                            acc[i].y = fmaf(v[i][j].y, w, acc[i].y);
+                            acc[i].z = fmaf(v[i][j].z, w, acc[i].z);
+                            acc[i].w = fmaf(v[i][j].w, w, acc[i].w);
+                        }
+                    }
+                }
+#pragma unroll
+                for (int i = 0; i < kItems; ++i) {
+                    reinterpret_cast<float4 *>(s_o)[at4[i]] = acc[i];   // (what more threads than items write is the same)
+                    if (at4[i] * 4 % D == 0) s_M[at4[i] * 4 / D] = top[i], s_L[at4[i] * 4 / D] = sum[i];
                 }
                 __syncthreads();
             }
