@@ -37,7 +37,7 @@ namespace {
 constexpr int kWarps = 4;
 constexpr int kThreads = kWarps * 32;
 constexpr int kUnit = 16;              // slots
-constexpr int kShort = 40;             // units of a head that are not worth splitting
+constexpr int kShort = 96;             // units of a head beyond which heads are split in any case
 constexpr int kMaxCtas = 1024;         // of the grid
 constexpr float kLog2e = 1.44269504088896340736f;
 // The reference m trails the maximum by 7 to 15 powers of two: weights stay in
@@ -203,12 +203,15 @@ __device__ __noinline__ void find_stretch(const int *lengths, int batch, int slo
         upto = block_scan(mine, &all) + total;
         total += all;
     }
-    // Even stretches; but a part costs its CTA a fence, a ticket and another CTA the join, about as much time as ten
-    // units of a warp: where no head is longer than that, whole heads, the same number to each CTA.
-    const bool split = __syncthreads_or(longest > kShort);
+    // Even stretches, or whole heads, the same number to each CTA? A part costs its CTA a fence and a ticket, and
+    // another CTA the join, the more time the more CTAs do so at once; whole heads of different lengths leave CTAs
+    // idle. Measured, split against whole, heads of 128 elements, 8 to a sequence: one sequence of 160, 320, 640
+    // slots 18.4, 14.3, 14.3 against 14.3, 16.4, 20.5 us; 32 of 160, 640, 1280 slots 24.6, 32.8, 45.1 against 16.4,
+    // 27.5, 41.0 us. So heads are split where the longest is well over twice the even share.
     long long per = (total + gridDim.x - 1) / gridDim.x;
     if (per < kWarps) per = kWarps;
     const int segments = batch * heads, each = (segments + gridDim.x - 1) / gridDim.x;
+    const bool split = __syncthreads_or(longest > kShort || static_cast<long long>(longest) * each > 2 * per + 10);
     const int from = static_cast<int>(min(static_cast<long long>(blockIdx.x) * each, static_cast<long long>(segments)));
     const int to = min(from + each, segments);
     if (tid == 0) {
@@ -331,9 +334,9 @@ __global__ void __launch_bounds__(kThreads, Shape<T, D, NT>::kCtas)
     const auto swizzle_k = [](int row) { return (row & 1) << 2; };
     const auto swizzle_v = [](int row) { return (row >> 1 & 3) << 1; };
     const int row_bytes = d * S::kEs;
-    // Rows are read once: they should not push out of the L2 what others will read again. But where several tiles of
-    // query heads read them, they are to be found there.
-    const uint64_t policy = a.tiles == 1 ? l2_policy_evict_first() : l2_policy_evict_normal();
+    // Rows are read once: they should not push out of the L2 what others will read again (100 against 110 us for
+    // 131071 slots of 8 heads; two tiles of query heads that read the same rows: 123 against 131 us).
+    const uint64_t policy = l2_policy_evict_first();
     unsigned row_mask;                                     // which of the unit's rows are in use, their page there
     long long row_off;                                     // byte offset of its first row, or of row `lane & 15`; 0, a
                                                            // row that can be read, in place of one that is not there

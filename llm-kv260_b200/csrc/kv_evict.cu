@@ -339,7 +339,7 @@ cudaError_t kv_evict_launch(const b200_kv_t *kv, const b200_kv_evict_t *p, void 
     // barriers, and where its keys would not fit
     const int slots = kv->table_cols * kv->page_size, heads = kv->n_head_kv * kv->batch;
     int ctas = 1;
-    while (ctas < kMaxCluster && (slots / ctas > kMaxKeys || (heads * ctas < sm_count() && slots / ctas >= 2 * 2048))) ctas *= 2;
+    while (ctas < kMaxCluster && (slots / ctas > kMaxKeys || (heads * ctas <= sm_count() && slots / ctas >= 1536))) ctas *= 2;
     a.max_slice = ((slots + ctas - 1) / ctas + 31) / 32 * 32;
     return a.max_slice <= kMaxKeys ? launch<true>(a, ctas, stream) : launch<false>(a, ctas, stream);
 }

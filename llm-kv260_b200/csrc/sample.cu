@@ -31,8 +31,8 @@ constexpr int kList = 4096;                    // candidates
 constexpr int kBins = 1024;                    // of the threads' maxima
 constexpr int kMaxListK = 2048;                // top_k beyond this goes by the whole row
 constexpr float kNear = -10.0f;                // exponents near the top, tried first for top-p
-enum : int { kTellTop, kTellFirst, kTellAll, kTellNear, kTellSum, kTellTies, kTellKept, kTellCut, kTellAbove = kTellCut + 2, kTellList = kTellAbove + 2, kTold = kTellList + 3 };
-constexpr int kFew = 256;                      // candidates that are ordered each against each
+enum : int { kTellTop, kTellFirst, kTellAll, kTellNear, kTellCount, kTellSum, kTellTies, kTellKept, kTellCut, kTellAbove = kTellCut + 2, kTellList = kTellAbove + 2, kTold = kTellList + 3 };
+constexpr int kFew = 128;                      // candidates that are ordered each against each
 
 using u64 = unsigned long long;
 
@@ -443,6 +443,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleArgs a)
     } else if (k == 0 && by_p) {
         // the weight of all tokens, and of those within 2^-10 of the largest
         u64 all = 0, near = 0;
+        unsigned near_count = 0;
         const auto weigh_all = [&](auto is_plain) {
 #pragma unroll 2
             for (int p = w0 + lane; p < w1; p += 32) {
@@ -457,6 +458,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleArgs a)
                     hi += h, lo += l;
                     const uint32_t is_near = y >= kNear ? kFullMask : 0;
                     near_hi += (h - kBase) & is_near, near_lo += (l - kBase) & is_near;
+                    near_count -= is_near;
                 }
                 all += join_units(hi, lo, kVe);
                 near += join_units(near_hi, near_lo, 0);
@@ -464,14 +466,15 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleArgs a)
         };
         if (plain) weigh_all(Yes()); else weigh_all(No());
         all = warp_sum(all), near = warp_sum(near);
-        if (lane == 0) s.mass[0][warp] = all, s.mass[0][32 + warp] = near;
+        near_count = __reduce_add_sync(kFullMask, near_count);
+        if (lane == 0) s.mass[0][warp] = all, s.mass[0][32 + warp] = near, s.mass[0][64 + warp] = near_count;
         __syncthreads();
         all = warps_total(s.mass[0]), near = warps_total(s.mass[0] + 32);
-        tell(kTellAll, all), tell(kTellNear, near);
+        tell(kTellAll, all), tell(kTellNear, near), tell(kTellCount, warps_total(s.mass[0] + 64));
         cluster_sync_all();
         all = told(kTellAll), near = told(kTellNear);
         s.weight = all;                         // every thread writes the same
-        listed = part_up(static_cast<u64>(p24), all) <= near;
+        listed = part_up(static_cast<u64>(p24), all) <= near && told(kTellCount) <= kList;
     }
     // Tokens that `wanted` names go to this CTA's list, and from there to rank 0's; true where that holds all of them.
     // Call `turn` of a row; s.listed is 0 before it, and rank 0 has the number after it.
