@@ -8,11 +8,21 @@
 // The cut that the filters make is found among few candidates. For top-k, the
 // k-th largest of the threads' own maxima bounds the k-th largest logit from
 // below; for top-p, a sum over the tokens within 2^-10 of the largest shows
-// whether those hold enough weight. The candidates go to one CTA, which
-// orders a few each against each, and selects among more by 8-bit digits. A row that they do not settle (a flat distribution,
-// a large k) is summed by distance from the top over all its tokens first, and
-// the bin that the cut falls in goes to the list; one with too many equal logits
-// for that is cut by digits of all its keys.
+// whether those hold enough weight. The candidates go to one CTA, which orders a
+// few each against each, and selects among more by 8-bit digits. A row that they
+// do not settle (a flat distribution, a large k) is summed by distance from the
+// top over all its tokens first, and the bin that the cut falls in goes to the
+// list; one with too many equal logits for that is cut by digits of all its
+// keys.
+//
+// What bounds it: the chain of barriers within a cluster, about a microsecond
+// each with the CTAs' skew, and for many rows the instructions of the passes
+// (13 a token and pass at least: exponent, power, two halves of the weight). One
+// row of 128256: 8 us on the GPU without filters, 12 with top-k, 34 with top-p
+// alone on a flat distribution. 256 such rows: 47 us greedy, 76 without filters,
+// 106 with top-k 100, 266 with top-p 0.9 alone; a mixture 153 (reading them
+// takes 20). Whole rows by one CTA each, read again through the L2: 150 for the
+// mixture, but slower for greedy rows (63) and for some filters.
 #include <cuda_runtime.h>
 
 #include "common.cuh"
@@ -31,8 +41,20 @@ constexpr int kList = 4096;                    // candidates
 constexpr int kBins = 1024;                    // of the threads' maxima
 constexpr int kMaxListK = 2048;                // top_k beyond this goes by the whole row
 constexpr float kNear = -10.0f;                // exponents near the top, tried first for top-p
-enum : int { kTellTop, kTellFirst, kTellAll, kTellNear, kTellCount, kTellSum, kTellTies, kTellKept, kTellCut, kTellAbove = kTellCut + 2, kTellList = kTellAbove + 2, kTold = kTellList + 3 };
 constexpr int kFew = 128;                      // candidates that are ordered each against each
+// The sides of these, measured on rows of 128256, one and 64 of them. Listed by the maxima against the whole row:
+// k = 1000 24.6 and 51 against 30.7 and 61 us, k = 2000 30.7 and 61 against the same. Near tokens tried first
+// against not: top-p 0.5 at a spread of 3.5, 24 and 50 against 35 and 76 us; where they do not do, no more. Each
+// against each or digits: k = 100 18.4 and 37 against 20.5 and 41 us, k = 200 22.5 and 47 against 20.5 and 41.
+
+// What a CTA tells the others, each thing in a place of its own.
+enum : int {
+    kTellTop, kTellFirst, kTellAll, kTellNear, kTellCount, kTellSum, kTellTies, kTellKept,
+    kTellCut,                                  // of the counts, and of the weights
+    kTellAbove = kTellCut + 2,
+    kTellList = kTellAbove + 2,                // of the first list, and as above
+    kTold = kTellList + 3,
+};
 
 using u64 = unsigned long long;
 
@@ -135,7 +157,7 @@ struct No {
 struct Shared {
     alignas(16) u64 mass[2][256];       // sums by digit, of this pass and the one before
     alignas(16) u64 sums[kBins];        // sums by distance from the top
-    u64 gather[kMaxCluster][kTold];     // what every CTA of the cluster tells the others, each thing in a place of its own
+    u64 gather[kMaxCluster][kTold];     // what every CTA of the cluster tells the others
     u64 warp[kWarps], warp_ties[kWarps];
     u64 left;
     u64 weight;
