@@ -83,7 +83,7 @@ class Engine:
         h = ctypes.c_void_p()
         check(lib().b200_engine_open(ctypes.byref(h), device), "b200_engine_open")
         self.h = h
-        self._structs, self._ws, self._ws_at, self._ws_bytes = {}, None, 0, 0
+        self._structs, self._ws, self._ws_at, self._ws_bytes = {}, [], 0, 0
         self.set_stream(current_stream_handle(device) if stream is None else stream)
 
     def close(self) -> None:
@@ -185,10 +185,10 @@ class Engine:
         where seen is None) and weights of 0 go into `positions` and `weights`. The lengths, and seen, are
         advanced: in lengths_out and seen_out, by default in place."""
         n = k_new.shape[0]
-        shape = (n, kv.n_head_kv, kv.head_dim)
-        st = rows(k_new, "k_new", shape)
-        if rows(v_new, "v_new", shape) != st or v_new.dtype is not k_new.dtype:
-            raise ValueError("k_new and v_new must be alike in type and strides")
+        st = rows(k_new, "k_new", (n, kv.n_head_kv, kv.head_dim))
+        if (v_new.shape != k_new.shape or v_new.stride() != k_new.stride() or v_new.dtype is not k_new.dtype
+                or not v_new.is_cuda):
+            raise ValueError("k_new and v_new must be alike in shape, type and strides")
         pos, stride = (0, 0) if positions is None else kv.aux(positions, "int32", "positions")
         w, stride2 = (0, stride) if weights is None else kv.aux(weights, "float32", "weights")
         if pos and stride != stride2:
@@ -223,14 +223,16 @@ class Engine:
             stride2, decay, self._workspace(ws_bytes), ws_bytes), kv)
 
     def _workspace(self, nbytes: int) -> int:
-        """Device memory of this engine's own for calls on its stream, kept and grown; one that is given back stays
-        reserved until the work queued on that stream is done."""
+        """Device memory of this engine's own for calls on its stream, kept and grown. It comes from that stream's own
+        pool, and a smaller one lives on with the engine: a captured graph may hold its address."""
         if self._ws_bytes < nbytes:
             torch = _torch()
-            if self._ws is not None and self.stream:
-                self._ws.record_stream(torch.cuda.ExternalStream(self.stream, device=self.device))
-            self._ws = torch.empty(nbytes, dtype=torch.uint8, device=f"cuda:{self.device}")
-            self._ws_at, self._ws_bytes = self._ws.data_ptr(), nbytes
+            nbytes = max(nbytes, 2 * self._ws_bytes)
+            dev = torch.device("cuda", self.device)
+            on = torch.cuda.ExternalStream(self.stream, device=dev) if self.stream else torch.cuda.default_stream(dev)
+            with torch.cuda.stream(on):
+                self._ws.append(torch.empty(nbytes, dtype=torch.uint8, device=dev))
+            self._ws_at, self._ws_bytes = self._ws[-1].data_ptr(), nbytes
         return self._ws_at
 
     def kv_evict(self, kv: PagedKV, weights, positions, seen, budget: int, recent: int = 0, sinks: int = 0,

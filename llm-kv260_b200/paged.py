@@ -85,7 +85,7 @@ class PagedKV:
 
     def aux(self, t, dtype: str, name: str) -> tuple[int, int]:
         """Address and head stride of a [batch, n_head_kv, >= capacity] tensor beside the cache (weights, positions)."""
-        if t.dim() != 3 or t.shape[2] < self.capacity:
+        shape = t.shape
+        if len(shape) != 3 or shape[2] < self.capacity:
             raise ValueError(f"{name} must be [{self.batch}, {self.n_head_kv}, >= {self.capacity}]")
-        n = t.shape[2]
-        return address(t, dtype, name, (self.batch, self.n_head_kv, n)), n
+        return address(t, dtype, name, (self.batch, self.n_head_kv, shape[2])), shape[2]

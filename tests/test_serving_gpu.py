@@ -326,6 +326,37 @@ def test_attend_repeats_to_the_bit_and_in_a_graph(torch_mod, pkg):
     e.close()
 
 
+def test_attend_graph_outlives_a_larger_call(torch_mod, pkg):
+    """A captured call keeps its workspace when a later call needs a larger one."""
+    torch = torch_mod
+    stream = torch.cuda.Stream()
+    e = pkg.Engine(0, stream=stream.cuda_stream)
+    cache, _ = make_cache(torch, pkg, [700, 90], 2, 64, 16, "f16", seed=21)
+    q = torch.randn(2, 8, 64, device="cuda")
+    out, w = torch.zeros_like(q), torch.zeros(2, 2, cache.capacity, device="cuda")
+    torch.cuda.synchronize()
+    e.kv_attend(cache, q, out, weights_out=w)
+    e.sync()
+    first = [out.clone(), w.clone()]
+    e.capture_begin()
+    e.kv_attend(cache, q, out, weights_out=w)
+    g = e.capture_end()
+    big, _ = make_cache(torch, pkg, [3000] * 40, 2, 128, 16, "f16", seed=22)
+    q2 = torch.randn(40, 16, 128, device="cuda")
+    out2, w2 = torch.empty_like(q2), torch.empty(40, 2, big.capacity, device="cuda")
+    torch.cuda.synchronize()
+    e.kv_attend(big, q2, out2, weights_out=w2)
+    filler = [torch.full((1 << 20,), 7.0, device="cuda") for _ in range(16)]      # what would take a freed workspace
+    out.zero_(), w.zero_()
+    torch.cuda.synchronize()
+    g.launch()
+    e.sync()
+    assert torch.equal(first[0], out) and torch.equal(first[1], w)
+    assert all(bool((f == 7.0).all()) for f in filler)
+    g.close()
+    e.close()
+
+
 # ------------------------------------------------------------------ append
 
 @pytest.mark.parametrize("src,kv", [("f32", "f16"), ("f32", "bf16"), ("f32", "f32"), ("f16", "f16"), ("bf16", "bf16")])
