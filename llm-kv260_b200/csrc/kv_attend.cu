@@ -507,10 +507,13 @@ __global__ void __launch_bounds__(kThreads, Shape<T, D, NT>::kCtas)
                         uint32_t hi[8], lo[8];
 #pragma unroll
                         for (int i = 0; i < 8; ++i) split_tf32(x[i], &hi[i], &lo[i]);
-                        mma<T>(sc[t][1], lo, q4.x, q4.y);
-                        mma<T>(sc[t][0], hi, q4.x, q4.y);
-                        mma<T>(sc[t][1], lo + 4, q4.z, q4.w);
-                        mma<T>(sc[t][0], hi + 4, q4.z, q4.w);
+                        float block[4] = {0.0f, 0.0f, 0.0f, 0.0f};   // (added up by ordinary additions: see below)
+                        mma<T>(block, lo, q4.x, q4.y);
+                        mma<T>(block, lo + 4, q4.z, q4.w);
+                        mma<T>(block, hi, q4.x, q4.y);
+                        mma<T>(block, hi + 4, q4.z, q4.w);
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) sc[t][k & 1][i] += block[i];
                     } else {
                         const uint32_t a0[4] = {k0.x, k1.x, k0.y, k1.y}, a1[4] = {k0.z, k1.z, k0.w, k1.w};
                         mma<T>(sc[t][0], a0, q4.x, q4.y);
@@ -560,7 +563,9 @@ __global__ void __launch_bounds__(kThreads, Shape<T, D, NT>::kCtas)
                     b1[t] = transpose8x8(split_pair<T>(p1));
                 }
             }
-            // O^T += V^T P^T
+            // O^T += V^T P^T. For float32 outputs a unit's product is added by an ordinary addition: the tensor cores
+            // cut their sums off instead of rounding them, which over many units pulls O (not l) towards 0, by up to
+            // 2e-6 of itself in 60 units; float16 and bfloat16 round a hundred times as coarsely.
             __syncwarp();
             if (kEven) copy_k(); else copy_v();
             cp_async_wait<S::kDepth - 1>();
@@ -593,10 +598,13 @@ __global__ void __launch_bounds__(kThreads, Shape<T, D, NT>::kCtas)
                         }
 #pragma unroll
                         for (int t = 0; t < NT; ++t) {
-                            mma<T>(o[2 * k + j][t], lo, b0[t], b1[t]);
-                            mma<T>(o[2 * k + j][t], lo2, b2[t], b3[t]);
-                            mma<T>(o[2 * k + j][t], hi, b0[t], b1[t]);
-                            mma<T>(o[2 * k + j][t], hi2, b2[t], b3[t]);
+                            float unit[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+                            mma<T>(unit, lo, b0[t], b1[t]);
+                            mma<T>(unit, lo2, b2[t], b3[t]);
+                            mma<T>(unit, hi, b0[t], b1[t]);
+                            mma<T>(unit, hi2, b2[t], b3[t]);
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) o[2 * k + j][t][i] += unit[i];
                         }
                     }
                 } else {
@@ -605,7 +613,16 @@ __global__ void __launch_bounds__(kThreads, Shape<T, D, NT>::kCtas)
                         const uint32_t va[4] = {__byte_perm(w0[j], w1[j], 0x5410), __byte_perm(w0[j], w1[j], 0x7632),
                                                 __byte_perm(w2[j], w3[j], 0x5410), __byte_perm(w2[j], w3[j], 0x7632)};
 #pragma unroll
-                        for (int t = 0; t < NT; ++t) mma<T>(o[4 * k + j][t], va, b0[t], b1[t]);
+                        for (int t = 0; t < NT; ++t) {
+                            if constexpr (sizeof(Q) == 4) {
+                                float unit[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+                                mma<T>(unit, va, b0[t], b1[t]);
+#pragma unroll
+                                for (int i = 0; i < 4; ++i) o[4 * k + j][t][i] += unit[i];
+                            } else {
+                                mma<T>(o[4 * k + j][t], va, b0[t], b1[t]);
+                            }
+                        }
                     }
                 }
             }
