@@ -26,9 +26,10 @@
 // (movmatrix).
 //
 // What bounds it: memory, for long caches. Read once by the kernel, the rows
-// come at 5.4 TB/s (one sequence of 131071 slots, 8 heads of 128 float16: 100
-// us; DRAM traffic 1.00 of the rows') and 6.0 TB/s (32 sequences of up to 16384
-// slots in bfloat16: 190 us), of 6.46 measured for a copy; a kernel that only
+// come at 5.1-5.4 TB/s (one sequence of 131071 slots, 8 heads of 128 float16:
+// 100-105 us on different GPUs; DRAM traffic 1.00 of the rows') and 5.7-6.0 TB/s
+// (32 sequences of up to 16384 slots in bfloat16: 190-200 us), of 6.46 measured
+// for a copy; a kernel that only
 // copies the same pages takes 90 us for the first. The rest is the start (4 us:
 // lengths, then table, then rows, each waiting for the one before), the join (5
 // us) and SMs that get their rows later than others, always the same ones, by
