@@ -318,6 +318,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleArgs a)
         for (int j = 0; j < kVe; ++j) x[j] = to_float(u.t[j]);
     };
 
+    cluster_arrive();                           // every CTA of the cluster runs before any store into its shared memory
     if (kCached) {                              // a warp's whole pieces by one bulk copy, those at the row's ends apart
         const int whole = (n + skew) / kVe, b0 = max(w0, skew ? 1 : 0), b1 = min(w1, whole);
         if (lane == 0) {
@@ -356,6 +357,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(const SampleArgs a)
     const auto tell = [&](int slot, u64 v) {
         if (tid < static_cast<int>(ctas)) cluster_store(cluster_map(&s.gather[rank][slot], tid), v);
     };
+    cluster_wait();
     {
         u64 v = s.warp[lane % kWarps];
         top = __uint_as_float(static_cast<unsigned>(v >> 32));
