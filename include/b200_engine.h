@@ -176,7 +176,9 @@ typedef struct {
     int n_tokens;
     int64_t token_stride, head_stride; /* both and the addresses multiples of 16 bytes */
     uint64_t offsets;                  /* int32 [batch + 1]: sequence b has rows offsets[b] up to offsets[b + 1],
-                                          from 0 to n_tokens in all, not falling; 0: row b is sequence b's */
+                                          from 0 to n_tokens in all, not falling (an offset outside [0, n_tokens]
+                                          counts as the nearer of these, a row that no sequence has is dropped);
+                                          0: row b is sequence b's */
     uint64_t seen;                     /* int32 [batch]: tokens each sequence has had; 0: as lengths */
     uint64_t positions;                /* int32 [batch][n_head_kv][aux_stride], or 0 */
     uint64_t weights;                  /* float [batch][n_head_kv][aux_stride], or 0 */

@@ -67,6 +67,9 @@ __device__ __forceinline__ Eight<Dst> convert(const Eight<Src> &s) {
     }
 }
 
+// Sequence b's first row, of those that there are.
+__device__ __forceinline__ int row_from(const AppendArgs &a, int b) { return min(max(a.offsets[b], 0), a.n_tokens); }
+
 // The copy is bound by memory: a thread takes eight elements of a row of k and
 // of v, of kTokens tokens, and has asked for all of them before the CTA looks
 // up where they go (sequence, length, page: reads that wait for one another,
@@ -100,8 +103,8 @@ __global__ void __launch_bounds__(kThreads) kv_append_kernel(const AppendArgs a)
         }
         if (u0 == 0) {
             if (static_cast<int>(threadIdx.x) < count) {
-                const long long t = first + threadIdx.x;
-                int b = static_cast<int>(t), i = 0;
+                const int t = static_cast<int>(first) + static_cast<int>(threadIdx.x);
+                int b = t, i = 0;
                 if (a.offsets) {
                     int lo = 0, hi = a.kv.batch;     // offsets[lo] <= t < offsets[hi]
                     while (hi - lo > 1) {
@@ -109,9 +112,10 @@ __global__ void __launch_bounds__(kThreads) kv_append_kernel(const AppendArgs a)
                         if (a.offsets[mid] <= t) lo = mid; else hi = mid;
                     }
                     b = lo;
-                    i = static_cast<int>(t) - a.offsets[lo];
+                    const int from = row_from(a, lo);
+                    i = t < from || t >= row_from(a, lo + 1) ? -1 : t - from;   // -1: no sequence has this row
                 }
-                const int at = kv_length(a.kv, b), slot = i < 0 || at + i >= slots ? -1 : at + i;
+                const int at = kv_length(a.kv, b), slot = i < 0 || i >= slots - at ? -1 : at + i;
                 s_seq[threadIdx.x] = b;
                 s_slot[threadIdx.x] = slot;
                 s_pos[threadIdx.x] = (a.seen ? a.seen[b] : at) + i;
@@ -140,10 +144,10 @@ __global__ void __launch_bounds__(kThreads) kv_append_kernel(const AppendArgs a)
     if (!a.lengths_out && !a.seen_out) return;
     if (a.in_place ? !last_cta(a.ticket, gridDim.x) : blockIdx.x != 0) return;
     for (int b = threadIdx.x; b < a.kv.batch; b += kThreads) {
-        const int n = a.offsets ? max(a.offsets[b + 1] - a.offsets[b], 0) : 1;
+        const int n = a.offsets ? max(row_from(a, b + 1) - row_from(a, b), 0) : 1;
         const int at = kv_length(a.kv, b);
         const int seen = a.seen ? a.seen[b] : at;
-        if (a.lengths_out) a.lengths_out[b] = min(at + n, a.kv.cols * a.kv.page_size);
+        if (a.lengths_out) a.lengths_out[b] = at + min(n, slots - at);
         if (a.seen_out) a.seen_out[b] = seen + n;
     }
 }

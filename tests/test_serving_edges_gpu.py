@@ -24,6 +24,50 @@ def eng(pkg, torch_mod):
     e.close()
 
 
+# ------------------------------------------------------------------ append
+
+LOW, HIGH = -2 ** 31, 2 ** 31 - 1
+
+
+@pytest.mark.parametrize("offsets", [[LOW, 2, 4, HIGH, 10], [HIGH] * 5, [LOW] * 5, [5, 5, 6, 6, 6], [-HIGH, -7, 3, 3, 4],
+                                     [LOW, LOW, LOW, LOW, HIGH], [0, 9, 9, 9, 7], [0, 3, 3, 7, 8]])
+@pytest.mark.parametrize("in_place", [False, True])
+def test_append_offsets_out_of_range(torch_mod, pkg, eng, offsets, in_place):
+    """Offsets below 0 or past the rows: what there is of each sequence's rows is appended, nothing else written."""
+    torch = torch_mod
+    n, b, page, hkv, d = 8, 4, 16, 2, 64
+    lens = [0, 31, 40, 2]                       # of 32 slots: the second sequence has one free, the third none
+    table = torch.arange(2 * b, dtype=torch.int32, device="cuda").view(b, 2)
+    k = torch.randn(2 * b, hkv, page, d, device="cuda").half()
+    v = torch.randn_like(k)
+    cache = pkg.PagedKV(k, v, table, torch.tensor(lens, dtype=torch.int32, device="cuda"))
+    kn, vn = torch.randn(n, hkv, d, device="cuda").half(), torch.randn(n, hkv, d, device="cuda").half()
+    seen = torch.tensor([7, 8, 9, 10], dtype=torch.int32, device="cuda")
+    pos = torch.full((b, hkv, 32), -9, dtype=torch.int32, device="cuda")
+    w = torch.full((b, hkv, 32), -9.0, device="cuda")
+    off = [min(max(x, 0), n) for x in offsets]
+    want_k, want_v, want_pos, want_w = k.clone(), v.clone(), pos.clone(), w.clone()
+    want_len, want_seen = [], []
+    for i in range(b):
+        at, m = min(lens[i], 32), max(off[i + 1] - off[i], 0)
+        want_len.append(min(at + m, 32))
+        want_seen.append(7 + i + m)
+        for j in range(m):
+            if at + j < 32:
+                pg, s = 2 * i + (at + j) // page, (at + j) % page
+                want_k[pg, :, s], want_v[pg, :, s] = kn[off[i] + j], vn[off[i] + j]
+                want_pos[i, :, at + j], want_w[i, :, at + j] = 7 + i + j, 0.0
+    out = {} if in_place else dict(lengths_out=torch.zeros_like(seen), seen_out=torch.zeros_like(seen))
+    torch.cuda.synchronize()
+    eng.kv_append(cache, kn, vn, offsets=torch.tensor(offsets, dtype=torch.int32, device="cuda"), seen=seen,
+                  positions=pos, weights=w, **out)
+    eng.sync()
+    assert torch.equal(k, want_k) and torch.equal(v, want_v)
+    assert torch.equal(pos, want_pos) and torch.equal(w, want_w)
+    assert out.get("lengths_out", cache.lengths).tolist() == want_len
+    assert out.get("seen_out", seen).tolist() == want_seen
+
+
 # ------------------------------------------------------------------ sampling
 
 @pytest.mark.parametrize("n", [20000, 50257, 128256])
