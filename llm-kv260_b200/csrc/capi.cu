@@ -478,7 +478,7 @@ struct b200_engine {
     uint8_t *xscratch;  // quantised x for the two-kernel f32 path
     void *sel_scratch;  // argmax candidates
     void *fsel_scratch; // fused greedy pick: per-CTA candidates + ticket
-    void *serve_scratch; // serving ops: tickets and the parts of split sequences
+    void *serve_scratch; // serving ops: tickets
     b200_engine_config_t cfg;
 };
 
@@ -588,9 +588,12 @@ extern "C" int b200_engine_open(b200_engine_t **out, int device) {
     if (err == cudaSuccess) err = cudaMalloc(reinterpret_cast<void **>(&e->xscratch), kXScratchBytes);
     if (err == cudaSuccess) err = cudaMalloc(&e->sel_scratch, static_cast<size_t>(argmax_scratch_bytes()));
     if (err == cudaSuccess) err = cudaMalloc(&e->fsel_scratch, static_cast<size_t>(tile_select_scratch_bytes()));
-    if (err == cudaSuccess) err = cudaMemset(e->fsel_scratch, 0, static_cast<size_t>(tile_select_scratch_bytes()));
+    if (err == cudaSuccess)
+        err = cudaMemsetAsync(e->fsel_scratch, 0, static_cast<size_t>(tile_select_scratch_bytes()), e->own);
     if (err == cudaSuccess) err = cudaMalloc(&e->serve_scratch, serve_scratch_bytes());
-    if (err == cudaSuccess) err = cudaMemset(e->serve_scratch, 0, serve_scratch_bytes());
+    if (err == cudaSuccess) err = cudaMemsetAsync(e->serve_scratch, 0, serve_scratch_bytes(), e->own);
+    // the first call may be on any stream, which need not wait for this one or for the legacy default stream
+    if (err == cudaSuccess) err = cudaStreamSynchronize(e->own);
     if (err != cudaSuccess) {
         b200_engine_close(e);
         return cuda_fail(err, "engine set-up");

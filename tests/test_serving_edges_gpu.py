@@ -24,6 +24,61 @@ def eng(pkg, torch_mod):
     e.close()
 
 
+def make_cache(torch, pkg, lens, hkv, d, page, dtype, seed):
+    """A pool of random rows, every sequence's pages in random order."""
+    gen = torch.Generator(device="cuda").manual_seed(seed)
+    cols = max(1, max(-(-n // page) for n in lens))
+    n_pages = len(lens) * cols
+    k = torch.randn(n_pages, hkv, page, d, generator=gen, device="cuda").to(dtype)
+    v = torch.randn(n_pages, hkv, page, d, generator=gen, device="cuda").to(dtype)
+    table = torch.randperm(n_pages, generator=gen, device="cuda").to(torch.int32).view(len(lens), cols)
+    return pkg.PagedKV(k, v, table, torch.tensor(lens, dtype=torch.int32, device="cuda"))
+
+
+def cache_rows(cache, b, n):
+    """k and v of the first n slots of sequence b in 64 bits, [n_head_kv, n, head_dim]."""
+    page = cache.page_size
+    pages = cache.table[b, :-(-n // page)].long()
+    return tuple(x[pages].double().transpose(0, 1).reshape(cache.n_head_kv, -1, cache.head_dim)[:, :n]
+                 for x in (cache.k, cache.v))
+
+
+def attend_ref(torch, cache, lens, q, scale=None):
+    """softmax(scale q K^T) V and the log-sums in 64 bits."""
+    b, h, d = q.shape
+    out = torch.zeros(b, h, d, dtype=torch.float64, device="cuda")
+    lse = torch.full((b, h), -np.inf, dtype=torch.float64, device="cuda")
+    for i, n in enumerate(lens):
+        if n == 0:
+            continue
+        k, v = cache_rows(cache, i, n)
+        s = (scale or d ** -0.5) * (q[i].double().view(cache.n_head_kv, -1, d) @ k.transpose(1, 2))
+        out[i] = (torch.softmax(s, 2) @ v).view(h, d)
+        lse[i] = torch.logsumexp(s, 2).view(h)
+    return out, lse
+
+
+# ------------------------------------------------------------------ streams
+
+def test_engine_opened_beside_a_busy_default_stream(torch_mod, pkg):
+    """The first call does not wait for the legacy default stream, and the scratch it needs is ready."""
+    torch = torch_mod
+    lens = [5000, 3000]
+    cache = make_cache(torch, pkg, lens, 2, 64, 16, torch.float16, seed=1)
+    q = torch.randn(2, 8, 64, device="cuda")
+    want, _ = attend_ref(torch, cache, lens, q)
+    out, stream = torch.zeros_like(q), torch.cuda.Stream()
+    torch.cuda.synchronize()
+    torch.cuda._sleep(100_000_000)              # of clock cycles: some 50 ms
+    e = pkg.Engine(0, stream=stream.cuda_stream)
+    for _ in range(3):
+        e.kv_attend(cache, q, out)
+    e.sync()
+    torch.cuda.synchronize()
+    assert (out.double() - want).abs().max() < 1e-5
+    e.close()
+
+
 # ------------------------------------------------------------------ append
 
 LOW, HIGH = -2 ** 31, 2 ** 31 - 1
