@@ -475,6 +475,9 @@ struct b200_engine {
     cudaStream_t side;
     cudaEvent_t fork;
     cudaEvent_t done;
+    cudaEvent_t handover;
+    bool serving;       // serving calls were queued on `stream`,
+    bool behind;        // and on an earlier one, up to `handover`, which the next of them has to wait for
     uint8_t *xscratch;  // quantised x for the two-kernel f32 path
     void *sel_scratch;  // argmax candidates
     void *fsel_scratch; // fused greedy pick: per-CTA candidates + ticket
@@ -483,6 +486,25 @@ struct b200_engine {
 };
 
 namespace {
+
+// Also where it cannot be told: the legacy default stream beside another stream's capture.
+bool capturing(cudaStream_t s) {
+    cudaStreamCaptureStatus status = cudaStreamCaptureStatusNone;
+    if (cudaStreamIsCapturing(s, &status) == cudaSuccess) return status != cudaStreamCaptureStatusNone;
+    cudaGetLastError();
+    return true;
+}
+
+// Before a call that shares the serving scratch.
+int serve_begin(b200_engine_t *e) {
+    if (e->behind && !capturing(e->stream)) {
+        const cudaError_t err = cudaStreamWaitEvent(e->stream, e->handover, 0);
+        if (err != cudaSuccess) return cuda_fail(err, "cudaStreamWaitEvent");
+        e->behind = false;
+    }
+    e->serving = true;
+    return 0;
+}
 
 constexpr size_t kXScratchBytes = kMaxK + 4 * (kMaxK / kQK);
 
@@ -585,6 +607,7 @@ extern "C" int b200_engine_open(b200_engine_t **out, int device) {
     if (err == cudaSuccess) err = cudaStreamCreateWithFlags(&e->side, cudaStreamNonBlocking);
     if (err == cudaSuccess) err = cudaEventCreateWithFlags(&e->fork, cudaEventDisableTiming);
     if (err == cudaSuccess) err = cudaEventCreateWithFlags(&e->done, cudaEventDisableTiming);
+    if (err == cudaSuccess) err = cudaEventCreateWithFlags(&e->handover, cudaEventDisableTiming);
     if (err == cudaSuccess) err = cudaMalloc(reinterpret_cast<void **>(&e->xscratch), kXScratchBytes);
     if (err == cudaSuccess) err = cudaMalloc(&e->sel_scratch, static_cast<size_t>(argmax_scratch_bytes()));
     if (err == cudaSuccess) err = cudaMalloc(&e->fsel_scratch, static_cast<size_t>(tile_select_scratch_bytes()));
@@ -618,12 +641,14 @@ extern "C" int b200_engine_close(b200_engine_t *e) {
     use_device(e->device);
     if (e->stream) cudaStreamSynchronize(e->stream);
     if (e->side) cudaStreamSynchronize(e->side);
+    if (e->behind) cudaEventSynchronize(e->handover);
     if (e->xscratch) cudaFree(e->xscratch);
     if (e->sel_scratch) cudaFree(e->sel_scratch);
     if (e->fsel_scratch) cudaFree(e->fsel_scratch);
     if (e->serve_scratch) cudaFree(e->serve_scratch);
     if (e->fork) cudaEventDestroy(e->fork);
     if (e->done) cudaEventDestroy(e->done);
+    if (e->handover) cudaEventDestroy(e->handover);
     if (e->side) cudaStreamDestroy(e->side);
     if (e->own) cudaStreamDestroy(e->own);
     free(e);
@@ -649,7 +674,19 @@ extern "C" int b200_engine_set_config(b200_engine_t *e, const b200_engine_config
 
 extern "C" int b200_engine_set_stream(b200_engine_t *e, void *stream) {
     if (!e) return fail(kErrInval, "engine not open");
-    e->stream = static_cast<cudaStream_t>(stream);  // NULL is the legacy default stream
+    const cudaStream_t next = static_cast<cudaStream_t>(stream);  // NULL is the legacy default stream
+    if (next == e->stream) return 0;
+    // The serving calls share tickets and workspaces, so the new stream's first one waits for those queued on the old
+    // stream. A recorded call runs when its graph is launched, which is not known here.
+    if (e->serving && !capturing(e->stream)) {
+        if (int rc = use_device(e->device)) return rc;
+        cudaError_t err = e->behind ? cudaStreamWaitEvent(e->stream, e->handover, 0) : cudaSuccess;
+        if (err == cudaSuccess) err = cudaEventRecord(e->handover, e->stream);
+        if (err != cudaSuccess) return cuda_fail(err, "set_stream");
+        e->behind = true;
+    }
+    e->serving = false;
+    e->stream = next;
     return 0;
 }
 
@@ -824,6 +861,7 @@ extern "C" int b200_graph_launch(b200_engine_t *e, b200_graph_t *g) {
     if (!e || !g) return fail(kErrInval, "bad arguments");
     if (g->device != e->device) return fail(kErrInval, "graph and engine are on different devices");
     if (int rc = use_device(e->device)) return rc;
+    if (int rc = serve_begin(e)) return rc;  // the graph may hold serving calls
     const cudaError_t err = cudaGraphLaunch(g->exec, e->stream);
     return err == cudaSuccess ? 0 : cuda_fail(err, "cudaGraphLaunch");
 }
@@ -852,6 +890,7 @@ extern "C" int b200_kv_append(b200_engine_t *e, const b200_kv_t *kv, const b200_
     const char *why = nullptr;
     if (kv_append_validate(kv, a, &why)) return fail(kErrInval, "kv_append: %s", why);
     if (int rc = use_device(e->device)) return rc;
+    if (int rc = serve_begin(e)) return rc;
     const cudaError_t err = kv_append_launch(kv, a, e->serve_scratch, e->stream);
     return err == cudaSuccess ? 0 : cuda_fail(err, "kv_append launch");
 }
@@ -861,6 +900,7 @@ extern "C" int b200_kv_attend(b200_engine_t *e, const b200_kv_t *kv, const b200_
     const char *why = nullptr;
     if (kv_attend_validate(kv, a, &why)) return fail(kErrInval, "kv_attend: %s", why);
     if (int rc = use_device(e->device)) return rc;
+    if (int rc = serve_begin(e)) return rc;
     const cudaError_t err = kv_attend_launch(kv, a, e->serve_scratch, e->stream);
     return err == cudaSuccess ? 0 : cuda_fail(err, "kv_attend launch");
 }
@@ -870,6 +910,7 @@ extern "C" int b200_kv_evict(b200_engine_t *e, const b200_kv_t *kv, const b200_k
     const char *why = nullptr;
     if (kv_evict_validate(kv, a, &why)) return fail(kErrInval, "kv_evict: %s", why);
     if (int rc = use_device(e->device)) return rc;
+    if (int rc = serve_begin(e)) return rc;
     const cudaError_t err = kv_evict_launch(kv, a, e->serve_scratch, e->stream);
     return err == cudaSuccess ? 0 : cuda_fail(err, "kv_evict launch");
 }

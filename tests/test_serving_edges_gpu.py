@@ -79,6 +79,64 @@ def test_engine_opened_beside_a_busy_default_stream(torch_mod, pkg):
     e.close()
 
 
+def test_calls_on_two_streams_follow_one_another(torch_mod, pkg):
+    """One engine, two caches, a stream each: the second stream's call waits for the first one's, whose scratch it
+    shares; the same with the first call in a graph."""
+    torch = torch_mod
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    e = pkg.Engine(0, stream=streams[0].cuda_stream)
+    lens = [[9000, 70], [20000, 12, 5000]]      # heads that are split over CTAs
+    caches = [make_cache(torch, pkg, n, 2, 64, 16, torch.float16, seed=i) for i, n in enumerate(lens)]
+    qs = [torch.randn(len(n), 8, 64, device="cuda") for n in lens]
+    want = [attend_ref(torch, c, n, q)[0] for c, n, q in zip(caches, lens, qs)]
+    outs = [torch.zeros_like(q) for q in qs]
+    ws = [torch.zeros(c.batch, 2, c.capacity, device="cuda") for c in caches]
+
+    def call(i):
+        e.kv_attend(caches[i], qs[i], outs[i], weights_out=ws[i])
+
+    torch.cuda.synchronize()
+    call(1), call(0)
+    e.sync()
+    e.capture_begin()
+    call(0)
+    g = e.capture_end()
+    for first in (lambda: call(0), g.launch):
+        for turn in range(5):
+            for t in outs:
+                t.zero_()
+            torch.cuda.synchronize()
+            with torch.cuda.stream(streams[0]):
+                torch.cuda._sleep(20_000_000)   # of clock cycles: some 10 ms
+            e.set_stream(streams[0].cuda_stream)
+            first()
+            e.set_stream(streams[1].cuda_stream)
+            call(1)
+            ended = torch.cuda.Event()
+            ended.record(streams[1])
+            assert not ended.query()            # it waits for the sleeping stream's call
+            torch.cuda.synchronize()
+            for o, w in zip(outs, want):
+                assert (o.double() - w).abs().max() < 1e-5
+    # recording on a stream that the engine comes to in the middle
+    e.set_stream(streams[0].cuda_stream)
+    call(0)
+    graph = torch.cuda.CUDAGraph()
+    outs[1].zero_()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph, stream=streams[1]):
+        e.set_stream(streams[1].cuda_stream)
+        call(1)
+    e.set_stream(streams[0].cuda_stream)
+    call(0)
+    e.sync()
+    graph.replay()
+    torch.cuda.synchronize()
+    assert (outs[1].double() - want[1]).abs().max() < 1e-5
+    g.close()
+    e.close()
+
+
 # ------------------------------------------------------------------ append
 
 LOW, HIGH = -2 ** 31, 2 ** 31 - 1
