@@ -9,6 +9,7 @@ from __future__ import annotations
 
 import ctypes
 from struct import Struct
+from threading import Lock
 
 from . import capi
 from .capi import check, lib
@@ -76,14 +77,15 @@ class QMat:
 
 
 class Engine:
-    """b200_engine.h: the engine_t-level call (tp_llama.cpp:289-375)."""
+    """b200_engine.h: the engine_t-level call (tp_llama.cpp:289-375). One thread at a time, as there; only the serving
+    calls (kv_append, kv_attend, kv_evict, sample) may come from several, on a stream that stays the same."""
 
     def __init__(self, device: int = 0, stream: int | None = None):
         self.device = device
         h = ctypes.c_void_p()
         check(lib().b200_engine_open(ctypes.byref(h), device), "b200_engine_open")
         self.h = h
-        self._structs, self._ws, self._ws_at, self._ws_bytes = {}, [], 0, 0
+        self._lock, self._structs, self._ws, self._ws_at, self._ws_bytes = Lock(), {}, [], 0, 0
         self.set_stream(current_stream_handle(device) if stream is None else stream)
 
     def close(self) -> None:
@@ -165,16 +167,18 @@ class Engine:
         check(lib().b200_prefetch(self.h, ctypes.byref(W.c)), "b200_prefetch")
 
     def _call(self, name: str, struct, values, kv: PagedKV | None = None) -> None:
-        """The C call of that name, its argument struct (one per engine, filled anew each time) set to `values`."""
-        kept = self._structs.get(name)
-        if kept is None:
-            buf = bytearray(ctypes.sizeof(struct))
-            fmt = Struct("".join(_FORMAT[t] for _, t in struct._fields_))
-            c = struct.from_buffer(buf)
-            kept = self._structs[name] = (getattr(lib(), name), ctypes.byref(c), fmt.pack_into, buf)
-        fn, ref, pack, buf = kept
-        pack(buf, 0, *values)
-        rc = fn(self.h, ref) if kv is None else fn(self.h, kv.ref, ref)
+        """The C call of that name, its argument struct (one per engine, filled anew each time) set to `values`. Another
+        thread's call waits: the interpreter's lock is given up while C reads the struct."""
+        with self._lock:
+            kept = self._structs.get(name)
+            if kept is None:
+                buf = bytearray(ctypes.sizeof(struct))
+                fmt = Struct("".join(_FORMAT[t] for _, t in struct._fields_))
+                c = struct.from_buffer(buf)
+                kept = self._structs[name] = (getattr(lib(), name), ctypes.byref(c), fmt.pack_into, buf)
+            fn, ref, pack, buf = kept
+            pack(buf, 0, *values)
+            rc = fn(self.h, ref) if kv is None else fn(self.h, kv.ref, ref)
         if rc < 0:
             check(rc, name)
 
