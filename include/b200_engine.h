@@ -215,6 +215,10 @@ typedef struct {
 /* Bytes a call with these sizes needs, the more of them with weights_out (0 for unusable sizes). */
 B200_API uint64_t b200_kv_attend_workspace(const b200_kv_t *kv, int n_head, int with_weights);
 B200_API int b200_kv_attend(b200_engine_t *e, const b200_kv_t *kv, const b200_kv_attend_t *a);
+/* 1 if a b200_kv_attend call of this engine was recorded into a graph since
+ * this was asked last, else 0: the graph holds the call's workspace, which
+ * then has to outlive it. */
+B200_API int b200_engine_recorded(b200_engine_t *e);
 
 /* Eviction: each head of a sequence with more than `budget` slots in use keeps
  * the tokens at positions >= seen[b] - recent or < sinks, then those of the

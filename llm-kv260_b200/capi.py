@@ -150,6 +150,7 @@ SIGNATURES: dict[str, tuple] = {
     "b200_kv_append": (c_int, [c_vp, P(b200_kv_t), P(b200_kv_append_t)]),
     "b200_kv_attend_workspace": (c_u64, [P(b200_kv_t), c_int, c_int]),
     "b200_kv_attend": (c_int, [c_vp, P(b200_kv_t), P(b200_kv_attend_t)]),
+    "b200_engine_recorded": (c_int, [c_vp]),
     "b200_kv_evict": (c_int, [c_vp, P(b200_kv_t), P(b200_kv_evict_t)]),
     "b200_sample": (c_int, [c_vp, P(b200_sample_t)]),
     # b200_comm.h

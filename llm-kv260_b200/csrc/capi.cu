@@ -478,6 +478,7 @@ struct b200_engine {
     cudaEvent_t handover;
     bool serving;       // serving calls were queued on `stream`,
     bool behind;        // and on an earlier one, up to `handover`, which the next of them has to wait for
+    bool recorded;      // an attention call went into a graph, with its workspace's address
     uint8_t *xscratch;  // quantised x for the two-kernel f32 path
     void *sel_scratch;  // argmax candidates
     void *fsel_scratch; // fused greedy pick: per-CTA candidates + ticket
@@ -901,8 +902,16 @@ extern "C" int b200_kv_attend(b200_engine_t *e, const b200_kv_t *kv, const b200_
     if (kv_attend_validate(kv, a, &why)) return fail(kErrInval, "kv_attend: %s", why);
     if (int rc = use_device(e->device)) return rc;
     if (int rc = serve_begin(e)) return rc;
+    if (capturing(e->stream)) e->recorded = true;
     const cudaError_t err = kv_attend_launch(kv, a, e->serve_scratch, e->stream);
     return err == cudaSuccess ? 0 : cuda_fail(err, "kv_attend launch");
+}
+
+extern "C" int b200_engine_recorded(b200_engine_t *e) {
+    if (!e) return fail(kErrInval, "engine not open");
+    const int was = e->recorded;
+    e->recorded = false;
+    return was;
 }
 
 extern "C" int b200_kv_evict(b200_engine_t *e, const b200_kv_t *kv, const b200_kv_evict_t *a) {

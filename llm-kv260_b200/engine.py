@@ -85,7 +85,8 @@ class Engine:
         h = ctypes.c_void_p()
         check(lib().b200_engine_open(ctypes.byref(h), device), "b200_engine_open")
         self.h = h
-        self._lock, self._structs, self._ws, self._ws_at, self._ws_bytes = Lock(), {}, [], 0, 0
+        self._lock, self._structs = Lock(), {}
+        self._ws, self._ws_at, self._ws_bytes, self._ws_old, self._ws_recorded = None, 0, 0, [], []
         self.set_stream(current_stream_handle(device) if stream is None else stream)
 
     def close(self) -> None:
@@ -167,18 +168,21 @@ class Engine:
         check(lib().b200_prefetch(self.h, ctypes.byref(W.c)), "b200_prefetch")
 
     def _call(self, name: str, struct, values, kv: PagedKV | None = None) -> None:
-        """The C call of that name, its argument struct (one per engine, filled anew each time) set to `values`. Another
-        thread's call waits: the interpreter's lock is given up while C reads the struct."""
+        """The C call of that name with an argument struct of `values`. Another thread's call waits: the interpreter's
+        lock is given up while C reads the struct."""
         with self._lock:
-            kept = self._structs.get(name)
-            if kept is None:
-                buf = bytearray(ctypes.sizeof(struct))
-                fmt = Struct("".join(_FORMAT[t] for _, t in struct._fields_))
-                c = struct.from_buffer(buf)
-                kept = self._structs[name] = (getattr(lib(), name), ctypes.byref(c), fmt.pack_into, buf)
-            fn, ref, pack, buf = kept
-            pack(buf, 0, *values)
-            rc = fn(self.h, ref) if kv is None else fn(self.h, kv.ref, ref)
+            self._queue(name, struct, values, kv)
+
+    def _queue(self, name: str, struct, values, kv: PagedKV | None) -> None:
+        kept = self._structs.get(name)
+        if kept is None:               # the struct is one per engine, filled anew each time
+            buf = bytearray(ctypes.sizeof(struct))
+            fmt = Struct("".join(_FORMAT[t] for _, t in struct._fields_))
+            c = struct.from_buffer(buf)
+            kept = self._structs[name] = (getattr(lib(), name), ctypes.byref(c), fmt.pack_into, buf)
+        fn, ref, pack, buf = kept
+        pack(buf, 0, *values)
+        rc = fn(self.h, ref) if kv is None else fn(self.h, kv.ref, ref)
         if rc < 0:
             check(rc, name)
 
@@ -221,23 +225,36 @@ class Engine:
         ws_bytes = kv.workspace.get((n_head, wo != 0))
         if ws_bytes is None:
             ws_bytes = kv.workspace[n_head, wo != 0] = int(lib().b200_kv_attend_workspace(kv.ref, n_head, int(wo != 0)))
-        self._call("b200_kv_attend", capi.b200_kv_attend_t, (
-            q.data_ptr(), out.data_ptr(), dtype_code(q, "q"), n_head, qs[0], qs[1], os_[0], os_[1],
-            kv.head_dim ** -0.5 if scale is None else scale, address(lse, "float32", "lse", (kv.batch, n_head)), w, wo,
-            stride2, decay, self._workspace(ws_bytes), ws_bytes), kv)
+        with self._lock:
+            if self._ws_bytes < ws_bytes:
+                self._grow(ws_bytes)
+            self._queue("b200_kv_attend", capi.b200_kv_attend_t, (
+                q.data_ptr(), out.data_ptr(), dtype_code(q, "q"), n_head, qs[0], qs[1], os_[0], os_[1],
+                kv.head_dim ** -0.5 if scale is None else scale, address(lse, "float32", "lse", (kv.batch, n_head)),
+                w, wo, stride2, decay, self._ws_at, ws_bytes), kv)
+            if self._ws_old:           # this call waits for all that used them
+                on = self._torch_stream()
+                for ws in self._ws_old:
+                    ws.record_stream(on)
+                self._ws_old.clear()
 
-    def _workspace(self, nbytes: int) -> int:
-        """Device memory of this engine's own for calls on its stream, kept and grown. It comes from that stream's own
-        pool, and a smaller one lives on with the engine: a captured graph may hold its address."""
-        if self._ws_bytes < nbytes:
-            torch = _torch()
-            nbytes = max(nbytes, 2 * self._ws_bytes)
-            dev = torch.device("cuda", self.device)
-            on = torch.cuda.ExternalStream(self.stream, device=dev) if self.stream else torch.cuda.default_stream(dev)
-            with torch.cuda.stream(on):
-                self._ws.append(torch.empty(nbytes, dtype=torch.uint8, device=dev))
-            self._ws_at, self._ws_bytes = self._ws[-1].data_ptr(), nbytes
-        return self._ws_at
+    def _torch_stream(self):
+        torch = _torch()
+        dev = torch.device("cuda", self.device)
+        return torch.cuda.ExternalStream(self.stream, device=dev) if self.stream else torch.cuda.default_stream(dev)
+
+    def _grow(self, nbytes: int) -> None:
+        """A larger workspace, device memory of this engine's own for calls on its stream, with an eighth to spare. The
+        smaller one is given up after the next call, or lives on with the engine where a graph holds its address."""
+        torch, on = _torch(), self._torch_stream()
+        with torch.cuda.stream(on):
+            if torch.cuda.is_current_stream_capturing():
+                raise RuntimeError(f"kv_attend needs a workspace of {nbytes} bytes, which cannot be allocated in a capture: "
+                                   "make the call once before it is captured")
+            ws = torch.empty(nbytes + nbytes // 8, dtype=torch.uint8, device=on.device)
+        if self._ws is not None:
+            (self._ws_recorded if lib().b200_engine_recorded(self.h) else self._ws_old).append(self._ws)
+        self._ws, self._ws_at, self._ws_bytes = ws, ws.data_ptr(), ws.numel()
 
     def kv_evict(self, kv: PagedKV, weights, positions, seen, budget: int, recent: int = 0, sinks: int = 0,
                  weights_out=None, positions_out=None, lengths_out=None) -> None:

@@ -137,6 +137,73 @@ def test_calls_on_two_streams_follow_one_another(torch_mod, pkg):
     e.close()
 
 
+# ------------------------------------------------------------------ workspace
+
+def wide_cache(torch, pkg, batch, columns, hkv=8):
+    """Sequences of one page each under tables of many columns: little memory, a large workspace with weights."""
+    k = torch.randn(batch, hkv, 16, 64, device="cuda").half()
+    table = torch.full((batch, columns), -1, dtype=torch.int32, device="cuda")
+    table[:, 0] = torch.arange(batch, device="cuda")
+    cache = pkg.PagedKV(k, torch.randn_like(k), table, torch.full((batch,), 16, dtype=torch.int32, device="cuda"))
+    return cache, torch.zeros(batch, hkv, cache.capacity, device="cuda")
+
+
+def test_a_grown_workspace_replaces_the_smaller_one(torch_mod, pkg):
+    """Without graphs an engine holds little more than its largest call needs."""
+    import ctypes
+    torch = torch_mod
+    e = pkg.Engine(0, stream=torch.cuda.Stream().cuda_stream)
+    batch, h = 16, 32
+    q = torch.randn(batch, h, 64, device="cuda")
+    outs = [torch.zeros_like(q) for _ in range(3)]
+    calls = [wide_cache(torch, pkg, batch, columns) for columns in (1000, 1010, 1100)]
+    for cache, _ in calls:
+        cache.k.copy_(calls[0][0].k), cache.v.copy_(calls[0][0].v)
+    need = pkg.lib().b200_kv_attend_workspace(ctypes.byref(calls[2][0].c), h, 1)
+    assert need > 32 << 20
+    torch.cuda.synchronize()
+    before = torch.cuda.memory_allocated()
+    for out, (cache, w) in zip(outs, calls):
+        e.kv_attend(cache, q, out, weights_out=w)
+    e.sync()
+    assert torch.cuda.memory_allocated() - before <= 1.25 * need
+    want, _ = attend_ref(torch, calls[0][0], [16] * batch, q)
+    for out in outs:
+        assert (out.double() - want).abs().max() < 1e-5
+    e.close()
+
+
+def test_a_workspace_does_not_grow_in_a_capture(torch_mod, pkg):
+    """A recorded call that needs more than the engine has is refused, and the recording goes on."""
+    torch = torch_mod
+    stream = torch.cuda.Stream()
+    e = pkg.Engine(0, stream=stream.cuda_stream)
+    (small, w0), (large, w1) = wide_cache(torch, pkg, 2, 10), wide_cache(torch, pkg, 64, 3000)
+    q0, q1 = torch.randn(2, 32, 64, device="cuda"), torch.randn(64, 32, 64, device="cuda")
+    out0, out1 = torch.zeros_like(q0), torch.zeros_like(q1)
+    torch.cuda.synchronize()
+    e.kv_attend(small, q0, out0, weights_out=w0)
+    e.sync()
+    want = out0.clone()
+    out0.zero_()
+    torch.cuda.synchronize()
+    e.capture_begin()
+    e.kv_attend(small, q0, out0, weights_out=w0)
+    with pytest.raises(RuntimeError, match="captur"):
+        e.kv_attend(large, q1, out1, weights_out=w1)
+    g = e.capture_end()
+    e.kv_attend(large, q1, out1, weights_out=w1)
+    filler = [torch.full((1 << 20,), 7.0, device="cuda") for _ in range(16)]      # what would take a freed workspace
+    torch.cuda.synchronize()
+    g.launch()
+    e.sync()
+    assert torch.equal(out0, want)
+    assert all(bool((f == 7.0).all()) for f in filler)
+    assert (out1.double() - attend_ref(torch, large, [16] * 64, q1)[0]).abs().max() < 1e-5
+    g.close()
+    e.close()
+
+
 # ------------------------------------------------------------------ append
 
 LOW, HIGH = -2 ** 31, 2 ** 31 - 1
