@@ -248,6 +248,34 @@ def test_append_offsets_out_of_range(torch_mod, pkg, eng, offsets, in_place):
     assert out.get("seen_out", seen).tolist() == want_seen
 
 
+# ------------------------------------------------------------------ attention
+
+@pytest.mark.parametrize("ratio", [1.0, 128.0, 4096.0, 30000.0])
+def test_attend_with_outliers_among_the_query(torch_mod, pkg, eng, ratio):
+    """A float32 query whose largest element, in a channel where all keys are 0, is `ratio` times the others: the
+    others keep their bits. A score is a float32 dot product: off by (d + 16) half units of sum |q k| at most, of the
+    channels that are not 0."""
+    torch = torch_mod
+    lens, d = [400, 1000], 128
+    cache = make_cache(torch, pkg, lens, 2, d, 16, torch.float16, seed=11)
+    cache.k[..., 17] = 0.0
+    gen = torch.Generator(device="cuda").manual_seed(3)
+    q = 1.5 * torch.randn(2, 8, d, generator=gen, device="cuda")
+    q[..., 17] = 3.0 * ratio * torch.where(torch.arange(8, device="cuda") % 2 == 0, 1.0, -1.0)
+    out, lse = torch.empty_like(q), torch.empty(2, 8, device="cuda")
+    torch.cuda.synchronize()
+    eng.kv_attend(cache, q, out, lse, scale=1.0)
+    eng.sync()
+    want, want_lse = attend_ref(torch, cache, lens, q, scale=1.0)
+    for i, n in enumerate(lens):
+        k, v = cache_rows(cache, i, n)
+        sabs = (q[i].double().abs().view(2, 4, d) @ k.abs().transpose(1, 2)).amax(2).view(8)
+        eps = (d + 16) * 2.0 ** -24 * sabs
+        assert bool(((lse[i].double() - want_lse[i]).abs() <= eps + 2.0 ** -22 * want_lse[i].abs()).all())
+        tol = v.abs().max() * (2 * eps + (64 + n / 16) * 2.0 ** -24 + 2.0 ** -20)
+        assert bool(((out[i].double() - want[i]).abs() <= tol[:, None] + 2.0 ** -23 * want[i].abs()).all())
+
+
 # ------------------------------------------------------------------ sampling
 
 @pytest.mark.parametrize("n", [20000, 50257, 128256])
