@@ -538,8 +538,11 @@ __global__ void __launch_bounds__(kThreads, Shape<T, D, NT>::kCtas)
                     if (u * kUnit + r < n) dst[r * S::kHeads] = t0;
                     if (u * kUnit + r + 8 < n) dst[(r + 8) * S::kHeads] = t1;
                 }
-                float top = fmaxf(t0, t1);
-                if (__any_sync(kFullMask, top > m[t] + kSlack)) {
+                // (A score that is not a number makes the reference infinite, and with it all that the head's weights
+                // enter: m must not stay at -infinity, which stands for no slot at all.)
+                const float most = m[t] + kSlack;
+                if (__any_sync(kFullMask, !(t0 <= most && t1 <= most))) {
+                    float top = t0 == t0 && t1 == t1 ? fmaxf(t0, t1) : INFINITY;
                     for (int k = 4; k < 32; k <<= 1) top = fmaxf(top, __shfl_xor_sync(kFullMask, top, k));
                     const float m1 = fmaxf(m[t], top - kLead), old = m1 == -INFINITY ? 1.0f : exp2_fast(m[t] - m1);
                     m[t] = m1;

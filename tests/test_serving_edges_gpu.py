@@ -276,6 +276,39 @@ def test_attend_with_outliers_among_the_query(torch_mod, pkg, eng, ratio):
         assert bool(((out[i].double() - want[i]).abs() <= tol[:, None] + 2.0 ** -23 * want[i].abs()).all())
 
 
+TYPES = {"f32_f16": ("float32", "float16"), "f16": ("float16", "float16"), "bf16": ("bfloat16", "bfloat16"),
+         "f32": ("float32", "float32")}
+
+
+@pytest.mark.parametrize("types", list(TYPES))
+@pytest.mark.parametrize("value", [float("nan"), float("inf")])
+@pytest.mark.parametrize("lens", [[1, 40], [9, 5000]])
+def test_attend_with_a_query_that_is_not_a_number(torch_mod, pkg, eng, types, value, lens):
+    """Scores that are NaN make the head NaN, and only that head: it does not look like an empty cache. (An infinite
+    query element meets positive keys: scores of +infinity.)"""
+    torch = torch_mod
+    qt, kt = (getattr(torch, t) for t in TYPES[types])
+    cache = make_cache(torch, pkg, lens, 2, 64, 16, kt, seed=12)
+    q = torch.randn(2, 8, 64, device="cuda").to(qt)
+    want, want_lse = attend_ref(torch, cache, lens, q)
+    q[0, 1, 5] = q[1, 7, 63] = value
+    if value == float("inf"):
+        cache.k[..., 5] = cache.k[..., 63] = 1.0
+        want, want_lse = attend_ref(torch, cache, lens, q)
+    out, lse = torch.zeros_like(q), torch.zeros(2, 8, device="cuda")
+    w = torch.zeros(2, 2, cache.capacity, device="cuda")
+    torch.cuda.synchronize()
+    eng.kv_attend(cache, q, out, lse, weights_out=w)
+    eng.sync()
+    bad = torch.zeros(2, 8, dtype=torch.bool, device="cuda")
+    bad[0, 1] = bad[1, 7] = True
+    assert bool(out[bad].isnan().all()) and bool(lse[bad].isnan().all())
+    assert bool(((out.double() - want)[~bad].abs() <= 0.02).all()) and bool(((lse.double() - want_lse)[~bad].abs() <= 0.02).all())
+    # the weights of the cache heads that the two query heads read are NaN, the others are not
+    for i, n in enumerate(lens):
+        assert bool(w[i, i, :n].isnan().all()) and bool(w[i, 1 - i, :n].isfinite().all())
+
+
 # ------------------------------------------------------------------ sampling
 
 @pytest.mark.parametrize("n", [20000, 50257, 128256])
