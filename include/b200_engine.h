@@ -192,8 +192,9 @@ B200_API int b200_kv_append(b200_engine_t *e, const b200_kv_t *kv, const b200_kv
 
 /* Attention of one new token per sequence over its slots in use:
  * s = scale * q . k, out = sum exp(s) v / sum exp(s), lse = log sum exp(s);
- * with no slot left, out = 0 and lse = -infinity; with a score that is NaN or
- * +infinity, out, lse and the head's weights are NaN. n_head / n_head_kv query
+ * with no slot left (a score of -infinity leaves none), out = 0 and lse =
+ * -infinity; with a score that is NaN or +infinity, out, lse and the head's
+ * weights are NaN. n_head / n_head_kv query
  * heads read each cache head. Dot products, the running maximum and sum and
  * the output are held in float32; the rounding to the output's type is the
  * last step. With weights_out the weights of the softmax, summed over the

@@ -158,6 +158,22 @@ struct Shape {
     static constexpr int kPart = kHeads * (D + 2);         // floats of a part: O, then m, then l
 };
 
+// Row x of a unit keeps its 16-byte piece y at y ^ swizzle(x).
+__device__ __forceinline__ int swizzle_k(int row) { return (row & 1) << 2; }
+__device__ __forceinline__ int swizzle_v(int row) { return (row >> 1 & 3) << 1; }
+
+// q . k of the unit's row `row`, an element after the other.
+template <typename T, typename S>
+__device__ __noinline__ float whole_score(const char *k_tile, int row, const char *q_row, int d) {
+    constexpr int kPer = 16 / S::kEs;                      // elements of a piece
+    const T *k = reinterpret_cast<const T *>(k_tile + row * S::kRowPieces * 16);
+    const T *hi = reinterpret_cast<const T *>(q_row), *lo = reinterpret_cast<const T *>(q_row + S::kQRow);
+    float sum = 0.0f;
+#pragma unroll 1
+    for (int i = 0; i < d; ++i) sum = fmaf(to_float(k[i ^ swizzle_k(row) * kPer]), to_float(hi[i]) + to_float(lo[i]), sum);
+    return sum;
+}
+
 // A place in the order of units.
 struct Cursor {
     int b, s, u, units;     // sequence, head and tile, unit of it, units of the sequence's heads
@@ -346,8 +362,6 @@ __global__ void __launch_bounds__(kThreads, Shape<T, D, NT>::kCtas)
     const int my_row = kRp <= 32 ? lane / kRp : 0, my_piece = kRp <= 32 ? lane % kRp : lane;
     const auto piece_row = [&](int i) { return kRp <= 32 ? i * kRows + my_row : i / 2; };
     const auto piece_col = [&](int i) { return kRp <= 32 ? my_piece : (i & 1) * 32 + my_piece; };
-    const auto swizzle_k = [](int row) { return (row & 1) << 2; };
-    const auto swizzle_v = [](int row) { return (row >> 1 & 3) << 1; };
     const int row_bytes = d * S::kEs;
     // Rows are read once: they should not push out of the L2 what others will read again (100 against 110 us for
     // 131071 slots of 8 heads; two tiles of query heads that read the same rows: 123 against 131 us).
@@ -394,14 +408,14 @@ __global__ void __launch_bounds__(kThreads, Shape<T, D, NT>::kCtas)
         if (to_copy > 0) {
             const unsigned rows = a.whole_units ? row_mask : __ballot_sync(kFullMask, row_mask) & 0xffffu;
             there |= static_cast<unsigned long long>(rows) << (16 * flying++);
-            copy(a.kv.k, swizzle_k);
+            copy(a.kv.k, [](int row) { return swizzle_k(row); });
         }
         cp_async_commit();
         place_in = place_in == (S::kDepth - 1) * S::kHalf ? 0 : place_in + S::kHalf;
     };
     const auto copy_v = [&] {
         if (to_copy > 0) {
-            copy(a.kv.v, swizzle_v);
+            copy(a.kv.v, [](int row) { return swizzle_v(row); });
             --to_copy;
             in.advance(a, heads, kWarps);
             lookup();
@@ -531,17 +545,17 @@ __global__ void __launch_bounds__(kThreads, Shape<T, D, NT>::kCtas)
             uint32_t b0[NT], b1[NT], b2[NT], b3[NT];       // P^T as the second product's columns
 #pragma unroll
             for (int t = 0; t < NT; ++t) {
-                const float t0 = rows >> r & 1 ? ((sc[t][0][0] + sc[t][1][0]) + (sc[t][0][1] + sc[t][1][1])) * qs[t] : -INFINITY;
-                const float t1 = rows >> (r + 8) & 1 ? ((sc[t][0][2] + sc[t][1][2]) + (sc[t][0][3] + sc[t][1][3])) * qs[t] : -INFINITY;
-                if (a.scores) {
-                    float *dst = a.scores + ((static_cast<long long>(at.b) * heads + at.s) * a.slots + u * kUnit) * S::kHeads + 4 * t + c;
-                    if (u * kUnit + r < n) dst[r * S::kHeads] = t0;
-                    if (u * kUnit + r + 8 < n) dst[(r + 8) * S::kHeads] = t1;
-                }
-                // (A score that is not a number makes the reference infinite, and with it all that the head's weights
-                // enter: m must not stay at -infinity, which stands for no slot at all.)
+                float t0 = rows >> r & 1 ? ((sc[t][0][0] + sc[t][1][0]) + (sc[t][0][1] + sc[t][1][1])) * qs[t] : -INFINITY;
+                float t1 = rows >> (r + 8) & 1 ? ((sc[t][0][2] + sc[t][1][2]) + (sc[t][0][3] + sc[t][1][3])) * qs[t] : -INFINITY;
                 const float most = m[t] + kSlack;
                 if (__any_sync(kFullMask, !(t0 <= most && t1 <= most))) {
+                    // An infinite key element times a low part of 0, or parts of both signs, is NaN where the score is
+                    // infinite: such a score is taken again from whole operands. One that stays NaN makes the reference
+                    // infinite, and with it all that the head's weights enter: m must not stay at -infinity, which stands
+                    // for no slot at all.
+                    const char *q_row = s_q + (8 * t + 2 * c) * S::kQRow, *k_tile = smem + (half - smem_addr(smem));
+                    if (t0 != t0) t0 = whole_score<T, S>(k_tile, r, q_row, d) * qs[t];
+                    if (t1 != t1) t1 = whole_score<T, S>(k_tile, r + 8, q_row, d) * qs[t];
                     float top = t0 == t0 && t1 == t1 ? fmaxf(t0, t1) : INFINITY;
                     for (int k = 4; k < 32; k <<= 1) top = fmaxf(top, __shfl_xor_sync(kFullMask, top, k));
                     const float m1 = fmaxf(m[t], top - kLead), old = m1 == -INFINITY ? 1.0f : exp2_fast(m[t] - m1);
@@ -549,6 +563,11 @@ __global__ void __launch_bounds__(kThreads, Shape<T, D, NT>::kCtas)
                     l[t] *= old;
 #pragma unroll
                     for (int i = 0; i < kAcc; ++i) o[i][t][0] *= old, o[i][t][1] *= old, o[i][t][2] *= old, o[i][t][3] *= old;
+                }
+                if (a.scores) {
+                    float *dst = a.scores + ((static_cast<long long>(at.b) * heads + at.s) * a.slots + u * kUnit) * S::kHeads + 4 * t + c;
+                    if (u * kUnit + r < n) dst[r * S::kHeads] = t0;
+                    if (u * kUnit + r + 8 < n) dst[(r + 8) * S::kHeads] = t1;
                 }
                 const float p0 = t0 == -INFINITY ? 0.0f : exp2_fast(t0 - m[t]);
                 const float p1 = t1 == -INFINITY ? 0.0f : exp2_fast(t1 - m[t]);

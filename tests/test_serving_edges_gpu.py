@@ -309,6 +309,50 @@ def test_attend_with_a_query_that_is_not_a_number(torch_mod, pkg, eng, types, va
         assert bool(w[i, i, :n].isnan().all()) and bool(w[i, 1 - i, :n].isfinite().all())
 
 
+@pytest.mark.parametrize("types", list(TYPES))
+@pytest.mark.parametrize("lens", [[17, 64], [3000, 77]])
+def test_attend_with_infinite_keys(torch_mod, pkg, eng, types, lens):
+    """A key row with an infinite element (a value that float16 does not hold) has a score of -infinity where the
+    query's element is of the other sign: it weighs nothing and the head is that of the other rows. Where it is of the
+    same sign the head is not a number; where a row's infinities cancel, too."""
+    torch = torch_mod
+    qt, kt = (getattr(torch, t) for t in TYPES[types])
+    cache = make_cache(torch, pkg, lens, 1, 64, 16, kt, seed=13)
+    q = torch.randn(2, 4, 64, device="cuda").to(qt)
+    q[..., 7] = 1.0
+    q[..., 9] = -0.5
+    rows = {0: [3, lens[0] - 1], 1: [0, 15, 40]}
+
+    def place(i, s):
+        return cache.table[i, s // 16].item(), 0, s % 16
+
+    for i, slots in rows.items():
+        for s in slots:
+            cache.k[place(i, s)][7] = -float("inf")
+            cache.k[place(i, s)][9] = float("inf")
+    out, lse = torch.zeros_like(q), torch.zeros(2, 4, device="cuda")
+    w = torch.zeros(2, 1, cache.capacity, device="cuda")
+    torch.cuda.synchronize()
+    eng.kv_attend(cache, q, out, lse, weights_out=w)
+    eng.sync()
+    tol = 2e-5 if types == "f32_f16" or types == "f32" else 2e-3 if types == "f16" else 1.6e-2
+    for i, n in enumerate(lens):
+        k, v = cache_rows(cache, i, n)
+        live = torch.ones(n, dtype=torch.bool, device="cuda")
+        live[rows[i]] = False
+        s = 0.125 * (q[i].double().view(1, 4, 64) @ k[:, live].transpose(1, 2))
+        want = (torch.softmax(s, 2) @ v[:, live])[0]
+        assert bool(((out[i].double() - want).abs() <= tol).all())
+        assert bool(((lse[i].double() - torch.logsumexp(s, 2)[0]).abs() <= 2e-5).all())
+        assert bool((w[i, 0, :n][~live] == 0).all()) and bool((w[i, 0, :n][live] > 0).all())
+    cache.k[place(0, 5)][7] = float("inf")      # a score of +infinity
+    cache.k[place(1, 15)][9] = -float("inf")    # -infinity and infinity
+    torch.cuda.synchronize()
+    eng.kv_attend(cache, q, out, lse)
+    eng.sync()
+    assert bool(out.isnan().all()) and bool(lse.isnan().all())
+
+
 # ------------------------------------------------------------------ sampling
 
 @pytest.mark.parametrize("n", [20000, 50257, 128256])
