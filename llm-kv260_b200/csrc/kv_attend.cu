@@ -588,9 +588,9 @@ __global__ void __launch_bounds__(kThreads, Shape<T, D, NT>::kCtas)
                     b1[t] = transpose8x8(split_pair<T>(p1));
                 }
             }
-            // O^T += V^T P^T. For float32 outputs a unit's product is added by an ordinary addition: the tensor cores
-            // cut their sums off instead of rounding them, which over many units pulls O (not l) towards 0, by up to
-            // 2e-6 of itself in 60 units; float16 and bfloat16 round a hundred times as coarsely.
+            // O^T += V^T P^T. A unit's product is added by an ordinary addition: the tensor cores cut their sums off
+            // instead of rounding them, which pulls O (not l) towards 0 with every unit, by 2e-6 of itself in 60 units
+            // and by 1.3e-4 in 1800 (131072 slots in one CTA), a fifth of a float16 unit.
             __syncwarp();
             if (kEven) copy_k(); else copy_v();
             cp_async_wait<S::kDepth - 1>();
@@ -639,14 +639,10 @@ __global__ void __launch_bounds__(kThreads, Shape<T, D, NT>::kCtas)
                                                 __byte_perm(w2[j], w3[j], 0x5410), __byte_perm(w2[j], w3[j], 0x7632)};
 #pragma unroll
                         for (int t = 0; t < NT; ++t) {
-                            if constexpr (sizeof(Q) == 4) {
-                                float unit[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-                                mma<T>(unit, va, b0[t], b1[t]);
+                            float unit[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+                            mma<T>(unit, va, b0[t], b1[t]);
 #pragma unroll
-                                for (int i = 0; i < 4; ++i) o[4 * k + j][t][i] += unit[i];
-                            } else {
-                                mma<T>(o[4 * k + j][t], va, b0[t], b1[t]);
-                            }
+                            for (int i = 0; i < 4; ++i) o[4 * k + j][t][i] += unit[i];
                         }
                     }
                 }

@@ -353,6 +353,32 @@ def test_attend_with_infinite_keys(torch_mod, pkg, eng, types, lens):
     assert bool(out.isnan().all()) and bool(lse.isnan().all())
 
 
+def test_attend_16_bit_outputs_of_long_heads_lean_to_neither_side(torch_mod, pkg, eng):
+    """131072 slots of positive values and so many heads that few are split: over some thousand units added up by a warp
+    float16 outputs are as often above the exact ones as below. (Sums that are cut off at each unit pull all of them down,
+    by a fifth of a unit.) Scores spread by 2 leave some 2400 slots that count, so outputs differ by several units
+    between heads and round independently: the mean error of 32768 of them is below 2^-17 of the values, over five times
+    what the rounding leaves (a unit / sqrt(12 * 32768)); the weights' 22 bits and the 32-bit sums are far below."""
+    torch = torch_mod
+    b, hkv, n, d, page = 64, 8, 131072, 64, 1024
+    k = torch.randn(n // page, hkv, page, d, device="cuda").half()
+    v = (1.2 + 0.3 * torch.rand(hkv, 1, d, device="cuda") + 0.5 * torch.rand(n // page, hkv, page, d, device="cuda")).half()
+    table = torch.arange(n // page, dtype=torch.int32, device="cuda").repeat(b, 1)
+    cache = pkg.PagedKV(k, v, table, torch.full((b,), n, dtype=torch.int32, device="cuda"))
+    q = (2 * torch.randn(b, hkv, d, device="cuda")).half()
+    out = torch.empty_like(q)
+    torch.cuda.synchronize()
+    eng.kv_attend(cache, q, out)
+    eng.sync()
+    kk, vv = (x.double().transpose(0, 1).reshape(hkv, n, d) for x in (k, v))
+    lean = 0.0
+    for i in range(0, b, 8):
+        s = 0.125 * (q[i:i + 8].double().transpose(0, 1) @ kk.transpose(1, 2))      # head, sequence, slot
+        want = (torch.softmax(s, 2) @ vv).transpose(0, 1)
+        lean += float(((out[i:i + 8].double() - want) / want).mean()) * 8 / b
+    assert abs(lean) <= 2.0 ** -17
+
+
 # ------------------------------------------------------------------ sampling
 
 @pytest.mark.parametrize("n", [20000, 50257, 128256])
