@@ -379,6 +379,22 @@ def test_attend_16_bit_outputs_of_long_heads_lean_to_neither_side(torch_mod, pkg
     assert abs(lean) <= 2.0 ** -17
 
 
+def test_attend_float32_error_over_many_units(torch_mod, pkg, eng):
+    """32 heads of 8000 float32 slots: the error's norm against 64 bits is below 1e-6 of the output's, which sums that
+    are cut off instead of rounded miss (2.0e-6)."""
+    torch = torch_mod
+    lens = [8000] * 8
+    cache = make_cache(torch, pkg, lens, 4, 128, 64, torch.float32, seed=14)
+    q = 1.5 * torch.randn(8, 16, 128, device="cuda")
+    out = torch.empty_like(q)
+    torch.cuda.synchronize()
+    eng.kv_attend(cache, q, out)
+    eng.sync()
+    want, _ = attend_ref(torch, cache, lens, q)
+    err = float((out.double() - want).norm() / want.norm())
+    assert err <= 1e-6
+
+
 # ------------------------------------------------------------------ sampling
 
 @pytest.mark.parametrize("n", [20000, 50257, 128256])
