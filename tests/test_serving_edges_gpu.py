@@ -7,6 +7,8 @@ from __future__ import annotations
 import numpy as np
 import pytest
 
+from test_serving_gpu import run_sample, sample_check
+
 pytestmark = pytest.mark.gpu
 
 
@@ -427,3 +429,45 @@ def test_sample_beside_other_kernels(torch_mod, pkg, n):
     torch.cuda.synchronize()
     assert all(torch.equal(t, quiet) for t in token)
     e.close()
+
+
+def equal_logits(kind, n, rng):
+    """Rows in which many logits are equal: more of them than a list of candidates holds."""
+    if kind == "all":
+        return np.full(n, -1.25, np.float32)
+    if kind == "all_but_few":                   # a few above the rest, a few far below
+        x = np.full(n, 0.5, np.float32)
+        x[rng.choice(n, 3, replace=False)] = [2.0, 2.0, 0.75]
+        x[rng.choice(n, 9, replace=False)] = -30.0
+        return x
+    if kind == "three":
+        return rng.choice(np.array([1.0, 0.0, -1.5], np.float32), n)
+    if kind == "five_near":                     # within one bin of distance from the top, and one bit of each other
+        return rng.choice(np.array([3.0, np.nextafter(np.float32(3), np.float32(4)), 2.9999, 2.99, -8.0], np.float32), n)
+    if kind == "infinite":
+        x = rng.standard_normal(n).astype(np.float32)
+        x[rng.random(n) < 0.4] = np.inf
+        x[rng.random(n) < 0.1] = -np.inf
+        return x
+    x = np.where(rng.random(n) < 0.5, -np.inf, 0.0).astype(np.float32)     # "masked"
+    x[rng.random(n) < 0.1] = np.nan
+    return x
+
+
+@pytest.mark.parametrize("kind", ["all", "all_but_few", "three", "five_near", "infinite", "masked"])
+@pytest.mark.parametrize("n,dtype", [(50257, "f32"), (50257, "bf16"), (128256, "f32")])
+@pytest.mark.parametrize("k", [0, 5, 40, 2048, 2049, 30000])
+def test_sample_rows_of_equal_logits(torch_mod, eng, kind, n, dtype, k):
+    """The cut falls among more equal logits than a list of candidates holds: of those, the lowest indexes stay."""
+    rng = np.random.default_rng(n + k)
+    settings = [(p, m, t) for p in (1.0, 0.5, 0.97) for m in (0.0, 0.3) for t in (1.0, 0.6)]
+    b = 2 * len(settings)
+    p, m, t = (np.array([s[j] for s in settings] * 2, np.float32) for j in range(3))
+    x = np.stack([equal_logits(kind, n, rng) for _ in range(b)])
+    u = rng.random(b).astype(np.float32)
+    u[0], u[1] = 0.0, np.float32(1 - 2.0 ** -24)
+    got = run_sample(torch_mod, eng, x, u, t, [k] * b, p, m, dtype, stride=3)
+    for i in range(b):
+        sample_check(got[0][i], t[i], k, p[i], m[i], u[i], int(got[1][i]), got[2][i])
+    again = run_sample(torch_mod, eng, x, u, t, [k] * b, p, m, dtype, stride=3)
+    assert np.array_equal(got[1], again[1]) and np.array_equal(got[2], again[2])
