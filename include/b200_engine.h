@@ -231,7 +231,10 @@ B200_API int b200_engine_recorded(b200_engine_t *e);
  * moves, so slots are not in the order of their positions afterwards
  * (attention does not mind). Slots < the new length of weights_out and
  * positions_out are written, no others. Sequences within budget are left as
- * they are. Pages must not be shared between sequences that are cut. */
+ * they are. Pages must not be shared between sequences that are cut, and those
+ * of their slots in use must all be there: of a kept slot without a page only
+ * weight and position move, and beside them then lies the row of the token
+ * that was given up. */
 typedef struct {
     uint64_t weights, weights_out;     /* float [batch][n_head_kv][aux_stride]; may be the same */
     uint64_t positions, positions_out; /* int32, the same shape; may be the same */

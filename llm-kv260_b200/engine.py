@@ -259,8 +259,8 @@ class Engine:
     def kv_evict(self, kv: PagedKV, weights, positions, seen, budget: int, recent: int = 0, sinks: int = 0,
                  weights_out=None, positions_out=None, lengths_out=None) -> None:
         """Cut every sequence and head to `budget` slots: the `recent` newest of `seen` tokens, the first `sinks` and
-        the largest weights stay. Rows move inside the cache; weights, positions and lengths go to the outputs, by
-        default in place."""
+        the largest weights stay. Rows move inside the cache, whose pages in use must all be there; weights, positions
+        and lengths go to the outputs, by default in place."""
         w, stride = kv.aux(weights, "float32", "weights")
         wo, s1 = (w, stride) if weights_out is None else kv.aux(weights_out, "float32", "weights_out")
         p, s2 = kv.aux(positions, "int32", "positions")

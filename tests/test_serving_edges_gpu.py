@@ -397,6 +397,58 @@ def test_attend_float32_error_over_many_units(torch_mod, pkg, eng):
     assert err <= 1e-6
 
 
+# ------------------------------------------------------------------ eviction
+
+@pytest.mark.parametrize("kv,q", [("float16", "float32"), ("bfloat16", "bfloat16"), ("float32", "float32")])
+@pytest.mark.parametrize("page", [16, 7])
+def test_attention_after_evictions_is_that_over_the_kept_tokens(torch_mod, pkg, eng, kv, q, page):
+    """Append, attend with weights and evict in turn, as a server does: each attention is the softmax over the tokens
+    whose positions are left, from rows kept aside as they were appended; and those are the ones the weights name."""
+    torch = torch_mod
+    kt, qt = getattr(torch, kv), getattr(torch, q)
+    b, hkv, h, d, budget, recent, sinks = 3, 2, 8, 64, 40, 9, 3
+    cols = -(-(budget + 60) // page)
+    gen = torch.Generator(device="cuda").manual_seed(page)
+    k = torch.zeros(b * cols, hkv, page, d, dtype=kt, device="cuda")
+    table = torch.randperm(b * cols, generator=gen, device="cuda").to(torch.int32).view(b, cols)
+    cache = pkg.PagedKV(k, torch.zeros_like(k), table, torch.zeros(b, dtype=torch.int32, device="cuda"))
+    seen = torch.zeros(b, dtype=torch.int32, device="cuda")
+    w = torch.zeros(b, hkv, cache.capacity, device="cuda")
+    pos = torch.zeros(b, hkv, cache.capacity, dtype=torch.int32, device="cuda")
+    rows = [[torch.zeros(0, hkv, d, dtype=kt, device="cuda")] * b for _ in "kv"]       # every token's, in order
+    tol = 2e-5 if qt == torch.float32 else 1.6e-2
+    for news in ([60, 3, 41], [1, 1, 1], [0, 50, 1], [7, 1, 30], [1, 1, 1]):
+        off = torch.tensor(np.concatenate([[0], np.cumsum(news)]), dtype=torch.int32, device="cuda")
+        kn, vn = (torch.randn(sum(news), hkv, d, generator=gen, device="cuda").to(kt) for _ in "kv")
+        qq = (1.5 * torch.randn(b, h, d, generator=gen, device="cuda")).to(qt)
+        out, lse = torch.zeros_like(qq), torch.zeros(b, h, device="cuda")
+        torch.cuda.synchronize()
+        eng.kv_append(cache, kn, vn, offsets=off, seen=seen, positions=pos, weights=w)
+        eng.kv_attend(cache, qq, out, lse, weights=w, weights_out=w, decay=0.9)
+        eng.sync()
+        old_pos, old_w, lens = pos.clone(), w.clone(), cache.lengths.tolist()
+        for i in range(b):
+            for side, new in zip(rows, (kn, vn)):
+                side[i] = torch.cat([side[i], new[off[i]:off[i + 1]]])
+            for j in range(hkv):
+                at = pos[i, j, :lens[i]].long()
+                kk, vv = (side[i][at, j].double() for side in rows)
+                s = d ** -0.5 * (qq[i, 4 * j:4 * j + 4].double() @ kk.T)
+                assert bool(((out[i, 4 * j:4 * j + 4].double() - torch.softmax(s, 1) @ vv).abs() <= tol).all())
+                assert bool(((lse[i, 4 * j:4 * j + 4].double() - torch.logsumexp(s, 1)).abs() <= 2e-5).all())
+        eng.kv_evict(cache, w, pos, seen, budget, recent=recent, sinks=sinks)
+        eng.sync()
+        for i in range(b):
+            n, m = lens[i], min(lens[i], budget)
+            assert cache.lengths[i].item() == m and seen[i].item() == rows[0][i].shape[0]
+            for j in range(hkv):
+                at, weight = old_pos[i, j, :n], old_w[i, j, :n]
+                fixed = (at >= seen[i] - recent) | (at < sinks)
+                order = torch.sort(torch.where(fixed, np.inf, weight), descending=True, stable=True).indices[:m]
+                kept = dict(zip(at[order].tolist(), weight[order].tolist()))
+                assert kept == dict(zip(pos[i, j, :m].tolist(), w[i, j, :m].tolist()))
+
+
 # ------------------------------------------------------------------ sampling
 
 @pytest.mark.parametrize("n", [20000, 50257, 128256])
