@@ -136,20 +136,24 @@ class Decoder:
         from .engine import Engine
         dev = f"cuda:{self.device}"
         eng = engine if engine is not None else Engine(self.device)
-        eng.set_stream(torch.cuda.current_stream(self.device).cuda_stream)
         logits, du = self.logits_tensor(), torch.from_numpy(u).to(dev)
         kw = dict(temperature=torch.full((1,), temperature, device=dev), top_p=torch.full((1,), top_p, device=dev),
                   top_k=torch.full((1,), top_k, dtype=torch.int32, device=dev),
                   min_p=torch.full((1,), min_p, device=dev))
         pick, lp = torch.empty(1, dtype=torch.int32, device=dev), torch.empty(1, device=dev)
         tokens, logprobs = np.empty(n_gen, np.int32), np.empty(n_gen, np.float32)
-        for i, t in enumerate(prompt):
-            self.forward(int(t), i)
-        for i in range(n_gen):
-            eng.sample(logits, du[i:i + 1], pick, lp, **kw)
-            tokens[i], logprobs[i] = int(pick), float(lp)
-            if i + 1 < n_gen:
-                self.forward(int(tokens[i]), prompt.size + i)
+        callers = eng.stream
+        eng.set_stream(torch.cuda.current_stream(self.device).cuda_stream)
+        try:
+            for i, t in enumerate(prompt):
+                self.forward(int(t), i)
+            for i in range(n_gen):
+                eng.sample(logits, du[i:i + 1], pick, lp, **kw)
+                tokens[i], logprobs[i] = int(pick), float(lp)
+                if i + 1 < n_gen:
+                    self.forward(int(tokens[i]), prompt.size + i)
+        finally:
+            eng.set_stream(callers)
         return tokens, logprobs
 
     def tokens(self) -> np.ndarray:

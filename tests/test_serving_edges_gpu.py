@@ -139,6 +139,27 @@ def test_calls_on_two_streams_follow_one_another(torch_mod, pkg):
     e.close()
 
 
+def test_generate_sampled_leaves_the_engine_on_its_stream(torch_mod, pkg):
+    """Also where it ends with an error."""
+    from llm_kv260_b200 import model
+    torch = torch_mod
+    m = model.synth_model(dict(n_layer=1, n_embd=512, n_ff=1024, n_head=8, n_head_kv=2, head_dim=64, n_vocab=1024,
+                               rope_base=500000.0, rms_eps=1e-5), seed=5)
+    dec = pkg.Decoder(m, device=0, ctx_max=16)
+    e = pkg.Engine(0, stream=torch.cuda.Stream().cuda_stream)
+    at = e.stream
+    u = np.full(3, 0.5, np.float32)
+    a, _ = dec.generate_sampled([1, 2], 3, u, engine=e)
+    assert e.stream == at != torch.cuda.current_stream().cuda_stream
+    with pytest.raises(pkg.B200Error):
+        dec.generate_sampled([1, 1 << 30], 3, u, engine=e)     # no such token
+    assert e.stream == at
+    b, _ = dec.generate_sampled([1, 2], 3, u)
+    assert np.array_equal(a, b)
+    e.close()
+    dec.close()
+
+
 # ------------------------------------------------------------------ workspace
 
 def wide_cache(torch, pkg, batch, columns, hkv=8):
