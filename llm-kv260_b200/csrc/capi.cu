@@ -476,7 +476,8 @@ struct b200_engine {
     cudaEvent_t fork;
     cudaEvent_t done;
     cudaEvent_t handover;
-    bool serving;       // serving calls were queued on `stream`,
+    bool served;        // serving calls were made at all,
+    bool serving;       // were queued on `stream`,
     bool behind;        // and on an earlier one, up to `handover`, which the next of them has to wait for
     bool recorded;      // an attention call went into a graph, with its workspace's address
     uint8_t *xscratch;  // quantised x for the two-kernel f32 path
@@ -503,7 +504,7 @@ int serve_begin(b200_engine_t *e) {
         if (err != cudaSuccess) return cuda_fail(err, "cudaStreamWaitEvent");
         e->behind = false;
     }
-    e->serving = true;
+    e->served = e->serving = true;
     return 0;
 }
 
@@ -862,7 +863,8 @@ extern "C" int b200_graph_launch(b200_engine_t *e, b200_graph_t *g) {
     if (!e || !g) return fail(kErrInval, "bad arguments");
     if (g->device != e->device) return fail(kErrInval, "graph and engine are on different devices");
     if (int rc = use_device(e->device)) return rc;
-    if (int rc = serve_begin(e)) return rc;  // the graph may hold serving calls
+    if (e->served)  // the graph may hold serving calls
+        if (int rc = serve_begin(e)) return rc;
     const cudaError_t err = cudaGraphLaunch(g->exec, e->stream);
     return err == cudaSuccess ? 0 : cuda_fail(err, "cudaGraphLaunch");
 }
