@@ -37,7 +37,8 @@
 // no swizzle, took 123 us in that copy where whole rows take 97; the depth of
 // the ring (2 to 8 halves) and 2 to 4 CTAs per SM made no difference. For short
 // caches the chain of dependent reads is all there is: 10 us with the call
-// (200 slots). The tensor pipe is 10 % busy (18 % with float32 rows).
+// (200 slots). The tensor pipe is 10 % busy (17 % with float32 rows, whose kernel
+// is short of warps: 255 registers, 12 % of the SM's).
 #include <cuda_runtime.h>
 
 #include "common.cuh"
@@ -790,9 +791,11 @@ struct WeightArgs {
 };
 
 // weights_out = decay weights + sum over the query heads of 2^(t - log2 sum
-// 2^t), from the scores that the attention left: a thread per slot. It is on
-// the GPU before the attention ends, and has read by then what that does not
-// write.
+// 2^t), from the scores that the attention left: a thread per slot that the
+// table can hold, since the host does not know the lengths (8 sequences of 4300
+// slots, attention and weights: 48 us with a table of 4352 slots, 62 with one of
+// 131072). It is on the GPU before the attention ends, and has read by then what
+// that does not write.
 __global__ void __launch_bounds__(256) kv_weights_kernel(const WeightArgs a) {
     const int h = blockIdx.y, b = blockIdx.z, slot = blockIdx.x * 256 + threadIdx.x;
     const long long head = static_cast<long long>(b) * a.kv.n_head_kv + h, aux = head * a.aux_stride + slot;
@@ -818,7 +821,9 @@ __global__ void __launch_bounds__(256) kv_weights_kernel(const WeightArgs a) {
 }
 
 // Query heads of a tile: eight in one pass over the rows, or four where there are no more. (Groups of eight as two
-// tiles of four, 16 x 8192 slots: 199 against 121 us; 4 x 1024 slots, from the L2: 22.6 against 26.5 us.)
+// tiles of four, 16 x 8192 slots: 199 against 121 us; 4 x 1024 slots, from the L2: 22.6 against 26.5 us.) More query
+// heads than eight read the rows again for each tile: 8 x 65536 bfloat16 slots of 128 take 76 us for 8 heads on one
+// cache head, 117 for 16 and 250 for 40.
 int heads_of_tile(int group) { return group <= 4 ? 4 : 8; }
 int tiles_of(int group) { return (group + heads_of_tile(group) - 1) / heads_of_tile(group); }
 

@@ -18,9 +18,9 @@
 // What bounds it: the chain of barriers within a cluster, about a microsecond
 // each with the CTAs' skew, and for many rows the instructions of the passes
 // (13 a token and pass at least: exponent, power, two halves of the weight). One
-// row of 128256: 8 us on the GPU without filters, 12 with top-k, 34 with top-p
-// alone on a flat distribution. 256 such rows: 47 us greedy, 76 without filters,
-// 106 with top-k 100, 266 with top-p 0.9 alone; a mixture 153 (reading them
+// row of 128256, calls behind one another: 10 us without filters, 14 with top-k,
+// 27 with top-p alone. 256 such rows: 46 us greedy, 76 without filters, 104 with
+// top-k 100, 270 with top-p 0.9 alone (five passes); a mixture 158 (reading them
 // takes 20). Whole rows by one CTA each, read again through the L2: 150 for the
 // mixture, but slower for greedy rows (63) and for some filters.
 #include <cuda_runtime.h>

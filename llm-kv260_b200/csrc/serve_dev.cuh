@@ -12,8 +12,6 @@
 
 namespace b200 {
 
-constexpr unsigned kAllLanes = 0xffffffffu;
-
 __device__ __forceinline__ float to_float(float v) { return v; }
 __device__ __forceinline__ float to_float(__half v) { return __half2float(v); }
 __device__ __forceinline__ float to_float(__nv_bfloat16 v) { return __bfloat162float(v); }
