@@ -194,11 +194,12 @@ B200_API int b200_kv_append(b200_engine_t *e, const b200_kv_t *kv, const b200_kv
  * s = scale * q . k, out = sum exp(s) v / sum exp(s), lse = log sum exp(s);
  * with no slot left (a score of -infinity leaves none), out = 0 and lse =
  * -infinity; with a score that is NaN or +infinity, out, lse and the head's
- * weights are NaN. n_head / n_head_kv query
- * heads read each cache head. Dot products, the running maximum and sum and
- * the output are held in float32; the rounding to the output's type is the
- * last step. With weights_out the weights of the softmax, summed over the
- * query heads of a cache head, are added up: weights_out = decay * weights +
+ * weights are NaN; an element of out that values which are not finite enter is
+ * infinite or NaN. n_head / n_head_kv query heads read each cache head. Dot
+ * products, the running maximum and sum and the output are held in float32;
+ * the rounding to the output's type is the last step. With weights_out the
+ * weights of the softmax, summed over the query heads of a cache head, are
+ * added up: weights_out = decay * weights +
  * sum, for slots in use (others are not written). */
 typedef struct {
     uint64_t q, out;                   /* [batch][n_head][head_dim], strides in elements, rows contiguous */
