@@ -218,7 +218,7 @@ typedef struct {
 /* Bytes a call with these sizes needs, the more of them with weights_out (0 for unusable sizes). */
 B200_API uint64_t b200_kv_attend_workspace(const b200_kv_t *kv, int n_head, int with_weights);
 B200_API int b200_kv_attend(b200_engine_t *e, const b200_kv_t *kv, const b200_kv_attend_t *a);
-/* 1 if a b200_kv_attend call of this engine was recorded into a graph since
+/* 1 if a b200_kv_attend or b200_kv_attend_chunk call of this engine was recorded into a graph since
  * this was asked last, else 0: the graph holds the call's workspace, which
  * then has to outlive it. */
 B200_API int b200_engine_recorded(b200_engine_t *e);
@@ -273,6 +273,150 @@ typedef struct {
     uint64_t logprob;                  /* float [batch]: log of the token's share of the kept weight, or 0 */
 } b200_sample_t;
 B200_API int b200_sample(b200_engine_t *e, const b200_sample_t *s);
+
+/* --------------------------------------------------- prompts in chunks
+ * What new tokens pass through on their way into the caches of several
+ * sequences, prompts in chunks and single tokens mixed: pages and slots, the
+ * norm in front of a matrix, rotary positions with the store into the cache,
+ * and attention of all new tokens. As the calls above, they queue on the
+ * engine's stream, allocate nothing, can be recorded, and read on the device
+ * what the host need not know. */
+
+/* Pages and slots for new tokens. A pool's free pages are a stack, free[0] up
+ * to free[count - 1]; sequence b holds the pages in the first held[b] columns
+ * of its table row and asks for new_tokens[b] slots behind its lengths[b], or,
+ * with a negative number, is done (its length becomes 0). It wants
+ * ceil((length + new) / page_size) pages. First, all pages beyond what a
+ * sequence wants go onto the stack, in the order of sequences and columns
+ * (those that it has no room for are lost). Then, in the same order, sequences
+ * take what they lack from its top. A sequence gets all or nothing: nothing
+ * where the table has no slots for its tokens, or where it lacks pages and all
+ * lacks up to its own exceed the stack (so later ones that lack pages get none
+ * either). Its pages, length and seen then stay as they were.
+ *
+ * Tokens are numbered by sequence: b's are offsets[b] up to offsets[b + 1],
+ * whether it got its slots or not. For token t of sequence b, its i-th:
+ * sequences[t] = b, positions[t] = seen[b] + i, and slots[t] = page *
+ * page_size + row, or -1 where it got none or the page is not in the pool. For
+ * t behind the last sequence's tokens all three are -1. Table entries that
+ * were given up keep their value, and free entries behind the count stay: with
+ * held_out, free_count_out and lengths_out elsewhere a call can be repeated.
+ * Only page_size, table, lengths and n_pages of the cache are used. */
+typedef struct {
+    uint64_t new_tokens;               /* int32 [batch] */
+    uint64_t held, held_out;           /* int32 [batch], may be the same */
+    uint64_t free_pages;               /* int32 [free_capacity] */
+    int free_capacity;
+    uint64_t free_count, free_count_out; /* int32 [1], may be the same */
+    uint64_t offsets;                  /* int32 [batch + 1], written; n_tokens where they would be more */
+    int n_tokens;                      /* of slots, positions and sequences */
+    uint64_t slots;                    /* int64 [n_tokens], or 0 */
+    uint64_t positions, sequences;     /* int32 [n_tokens], or 0 */
+    uint64_t granted;                  /* int32 [batch]: tokens that got slots, or 0 */
+    uint64_t seen, seen_out;           /* int32 [batch], or 0; seen 0: as lengths */
+    uint64_t lengths_out;              /* int32 [batch], may be the cache's lengths */
+} b200_kv_plan_t;
+B200_API int b200_kv_plan(b200_engine_t *e, const b200_kv_t *kv, const b200_kv_plan_t *a);
+
+/* Rotary positions. The first rot_dim elements of a head are pairs (x, y): i
+ * and i + rot_dim / 2, or, interleaved, 2 i and 2 i + 1. Pair i of a token at
+ * position p becomes mscale * (x cos a - y sin a, y cos a + x sin a) with the
+ * angle a = p * freqs[i], held in units of 2^-64 turns, so that the angle of
+ * any position is good to 2^-28 turns; the other elements are copied. With a
+ * cache, k's rotated rows go to its rows slots[t], and v's rows beside them,
+ * both in the cache's type (a slot outside the pool, as -1, is dropped; k_out
+ * is not used). q, k and v in float32 may go to any type, others to their own.
+ * A row may go where it comes from; otherwise inputs and outputs do not
+ * overlap. */
+typedef struct {
+    uint64_t q, q_out;                 /* [n_tokens][n_head][head_dim], strides in elements; 0: no q */
+    int n_head;
+    int64_t q_token_stride, q_head_stride, q_out_token_stride, q_out_head_stride;
+    uint64_t k, k_out;                 /* [n_tokens][n_head_kv][head_dim]; 0: no k */
+    int n_head_kv;
+    int64_t k_token_stride, k_head_stride, k_out_token_stride, k_out_head_stride;
+    uint64_t v;                        /* as k; only with a cache, where it may be 0 */
+    int64_t v_token_stride, v_head_stride;
+    int dtype;                         /* of q, k, v */
+    int out_dtype;                     /* of q_out, k_out: dtype, or any with B200_F32 */
+    int n_tokens;
+    int head_dim;                      /* a multiple of 8, at most 256 */
+    int rot_dim;                       /* even, 2 up to head_dim */
+    int interleaved;
+    uint64_t positions;                /* int32 [n_tokens] */
+    uint64_t freqs;                    /* uint64 [rot_dim / 2], see b200_rope_freqs */
+    float mscale;
+    uint64_t slots;                    /* int64 [n_tokens], with a cache */
+} b200_rope_t;
+B200_API int b200_rope(b200_engine_t *e, const b200_kv_t *kv, const b200_rope_t *a);
+
+/* The frequencies of b200_rope on the host, base^(-2 i / rot_dim) radians for
+ * pair i, divided by factors[i] (NULL: 1, as a model file's rope_freqs), and for
+ * contexts longer than a model was trained for:
+ *   LINEAR divided by factor;
+ *   BANDS  by the turns n that a pair makes in `context` positions: divided by
+ *          factor where n <= low, as it is where n >= high, the mean of the two
+ *          weighted by (n - low) / (high - low) between;
+ *   YARN   the same over the index i of a pair instead: as it is up to the pair
+ *          with `high` turns (its index rounded down), divided from the one with
+ *          `low` on (rounded up), the mean weighted by i between. */
+#define B200_ROPE_PLAIN 0
+#define B200_ROPE_LINEAR 1
+#define B200_ROPE_BANDS 2
+#define B200_ROPE_YARN 3
+B200_API int b200_rope_freqs(uint64_t *freqs, int rot_dim, double base, const float *factors, int scaling, double factor,
+                             double context, double low, double high);
+
+/* Residual addition and root-mean-square norm: r = residual + x (x alone where
+ * residual is 0), residual_out = r, y = r / sqrt(mean(r^2) + eps) * weight, in
+ * float32 with one rounding per output. y goes to out, and with q8 row by row
+ * to the engine's Q8_0 form, int8[k] then float32[k / 32], as
+ * b200_quantize_q8_0 makes it and b200_gemv_q8 reads it. */
+typedef struct {
+    uint64_t x;                        /* [n_rows][k], strides in elements, rows contiguous */
+    int dtype;
+    uint64_t residual, residual_out;   /* or 0; may be the same */
+    int residual_dtype;                /* dtype, or B200_F32 */
+    uint64_t weight;                   /* float32 [k] */
+    uint64_t out;                      /* or 0; may be x */
+    int out_dtype;                     /* dtype, or any with B200_F32 */
+    uint64_t q8;                       /* or 0 */
+    int n_rows, k;                     /* k: a multiple of 8 (of 32 with q8), at most 32768 */
+    int64_t x_stride, residual_stride, residual_out_stride, out_stride;
+    int64_t q8_stride;                 /* bytes, >= k + k / 8 */
+    float eps;
+} b200_rms_norm_t;                     /* addresses and strides are multiples of 16 bytes, q8's of 4 */
+B200_API int b200_rms_norm(b200_engine_t *e, const b200_rms_norm_t *a);
+
+/* Attention of each sequence's new tokens, which are its last slots in use
+ * (b200_kv_append or b200_rope has put them there): with n = offsets[b + 1] -
+ * offsets[b], its row i stands at slot p = lengths[b] - n + i and sees the slots
+ * up to p, with a window > 0 the last `window` of them. out = sum exp(s) v / sum
+ * exp(s), s = scale * q . k, lse = log sum exp(s), with the conventions of
+ * b200_kv_attend for rows that see nothing (p < 0, pages that are not there,
+ * scores of -infinity), for NaN and for infinities; what a row does not see has
+ * no influence on it, whatever it holds. Rows that no sequence has are left as
+ * they are. Dot products, maximum, sum and output are held in float32. With
+ * 16-bit queries the weights of the softmax are rounded to the cache's type
+ * before they meet the values (as much as the output is), with float32 queries
+ * nothing is rounded. */
+typedef struct {
+    uint64_t q, out;                   /* [n_tokens][n_head][head_dim], strides in elements, rows contiguous;
+                                          addresses and strides are multiples of 16 bytes */
+    int dtype;                         /* of both: the cache's type, or B200_F32 with a B200_F16 cache */
+    int n_tokens, n_head;              /* n_head: a multiple of n_head_kv */
+    int64_t q_token_stride, q_head_stride, out_token_stride, out_head_stride;
+    uint64_t offsets;                  /* int32 [batch + 1], as in b200_kv_append_t */
+    float scale;
+    int window;                        /* 0: none */
+    uint64_t lse;                      /* float [n_tokens][n_head], or 0 */
+    uint64_t workspace;                /* b200_kv_chunk_workspace() bytes, 16-byte aligned; holds nothing between calls */
+    uint64_t workspace_bytes;
+} b200_kv_chunk_t;
+/* Bytes that calls with these sizes need on the current device, whatever the
+ * number of tokens (0 for unusable sizes). */
+B200_API uint64_t b200_kv_chunk_workspace(const b200_kv_t *kv, int dtype, int n_head);
+B200_API int b200_kv_attend_chunk(b200_engine_t *e, const b200_kv_t *kv, const b200_kv_chunk_t *a);
 
 /* Block until the engine's queued work is done (bounded; -ETIMEDOUT). */
 B200_API int b200_engine_sync(b200_engine_t *e, int timeout_ms);

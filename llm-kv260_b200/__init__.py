@@ -13,8 +13,8 @@ from . import capi, gguf, model
 from .capi import B200Error, lib
 from .decoder import Decoder
 from .gguf import GGUFFile
-from .engine import LAYOUT_ROWS, LAYOUT_TILES, Engine, Gemv2Dev, GemvDev, QMat, Udmabuf, dev_ptr, tiled_bytes
+from .engine import LAYOUT_ROWS, LAYOUT_TILES, Engine, Gemv2Dev, GemvDev, QMat, Udmabuf, dev_ptr, rope_freqs, tiled_bytes
 from .paged import PagedKV
 
 __all__ = ["B200Error", "Decoder", "Engine", "GGUFFile", "Gemv2Dev", "GemvDev", "LAYOUT_ROWS", "LAYOUT_TILES", "PagedKV",
-           "QMat", "Udmabuf", "capi", "dev_ptr", "gguf", "lib", "model", "tiled_bytes"]
+           "QMat", "Udmabuf", "capi", "dev_ptr", "gguf", "lib", "model", "rope_freqs", "tiled_bytes"]

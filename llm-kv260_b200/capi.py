@@ -94,6 +94,41 @@ class b200_sample_t(ctypes.Structure):
                 ("token", c_u64), ("logprob", c_u64)]
 
 
+class b200_kv_plan_t(ctypes.Structure):
+    """include/b200_engine.h"""
+    _fields_ = [("new_tokens", c_u64), ("held", c_u64), ("held_out", c_u64), ("free_pages", c_u64),
+                ("free_capacity", c_int), ("free_count", c_u64), ("free_count_out", c_u64), ("offsets", c_u64),
+                ("n_tokens", c_int), ("slots", c_u64), ("positions", c_u64), ("sequences", c_u64), ("granted", c_u64),
+                ("seen", c_u64), ("seen_out", c_u64), ("lengths_out", c_u64)]
+
+
+class b200_rope_t(ctypes.Structure):
+    """include/b200_engine.h"""
+    _fields_ = [("q", c_u64), ("q_out", c_u64), ("n_head", c_int), ("q_token_stride", c_i64), ("q_head_stride", c_i64),
+                ("q_out_token_stride", c_i64), ("q_out_head_stride", c_i64), ("k", c_u64), ("k_out", c_u64),
+                ("n_head_kv", c_int), ("k_token_stride", c_i64), ("k_head_stride", c_i64),
+                ("k_out_token_stride", c_i64), ("k_out_head_stride", c_i64), ("v", c_u64), ("v_token_stride", c_i64),
+                ("v_head_stride", c_i64), ("dtype", c_int), ("out_dtype", c_int), ("n_tokens", c_int),
+                ("head_dim", c_int), ("rot_dim", c_int), ("interleaved", c_int), ("positions", c_u64), ("freqs", c_u64),
+                ("mscale", ctypes.c_float), ("slots", c_u64)]
+
+
+class b200_rms_norm_t(ctypes.Structure):
+    """include/b200_engine.h"""
+    _fields_ = [("x", c_u64), ("dtype", c_int), ("residual", c_u64), ("residual_out", c_u64), ("residual_dtype", c_int),
+                ("weight", c_u64), ("out", c_u64), ("out_dtype", c_int), ("q8", c_u64), ("n_rows", c_int), ("k", c_int),
+                ("x_stride", c_i64), ("residual_stride", c_i64), ("residual_out_stride", c_i64), ("out_stride", c_i64),
+                ("q8_stride", c_i64), ("eps", ctypes.c_float)]
+
+
+class b200_kv_chunk_t(ctypes.Structure):
+    """include/b200_engine.h"""
+    _fields_ = [("q", c_u64), ("out", c_u64), ("dtype", c_int), ("n_tokens", c_int), ("n_head", c_int),
+                ("q_token_stride", c_i64), ("q_head_stride", c_i64), ("out_token_stride", c_i64),
+                ("out_head_stride", c_i64), ("offsets", c_u64), ("scale", ctypes.c_float), ("window", c_int),
+                ("lse", c_u64), ("workspace", c_u64), ("workspace_bytes", c_u64)]
+
+
 SIGNATURES: dict[str, tuple] = {
     # gemv_dev.h
     "gemv_dev_open": (c_int, [P(gemv_dev_t)]),
@@ -153,6 +188,12 @@ SIGNATURES: dict[str, tuple] = {
     "b200_engine_recorded": (c_int, [c_vp]),
     "b200_kv_evict": (c_int, [c_vp, P(b200_kv_t), P(b200_kv_evict_t)]),
     "b200_sample": (c_int, [c_vp, P(b200_sample_t)]),
+    "b200_kv_plan": (c_int, [c_vp, P(b200_kv_t), P(b200_kv_plan_t)]),
+    "b200_rope": (c_int, [c_vp, P(b200_kv_t), P(b200_rope_t)]),
+    "b200_rope_freqs": (c_int, [c_vp, c_int, ctypes.c_double, c_vp, c_int] + [ctypes.c_double] * 4),
+    "b200_rms_norm": (c_int, [c_vp, P(b200_rms_norm_t)]),
+    "b200_kv_chunk_workspace": (c_u64, [P(b200_kv_t), c_int, c_int]),
+    "b200_kv_attend_chunk": (c_int, [c_vp, P(b200_kv_t), P(b200_kv_chunk_t)]),
     # b200_comm.h
     "b200_comm_create": (c_int, [P(c_vp), c_int, c_int, c_int, c_int]),
     "b200_comm_handle_bytes": (c_int, []),

@@ -484,6 +484,7 @@ struct b200_engine {
     void *sel_scratch;  // argmax candidates
     void *fsel_scratch; // fused greedy pick: per-CTA candidates + ticket
     void *serve_scratch; // serving ops: tickets
+    void *plan_scratch; // kv_plan: what its second kernel needs of each sequence
     b200_engine_config_t cfg;
 };
 
@@ -617,6 +618,7 @@ extern "C" int b200_engine_open(b200_engine_t **out, int device) {
         err = cudaMemsetAsync(e->fsel_scratch, 0, static_cast<size_t>(tile_select_scratch_bytes()), e->own);
     if (err == cudaSuccess) err = cudaMalloc(&e->serve_scratch, serve_scratch_bytes());
     if (err == cudaSuccess) err = cudaMemsetAsync(e->serve_scratch, 0, serve_scratch_bytes(), e->own);
+    if (err == cudaSuccess) err = cudaMalloc(&e->plan_scratch, kv_plan_scratch_bytes());
     // the first call may be on any stream, which need not wait for this one or for the legacy default stream
     if (err == cudaSuccess) err = cudaStreamSynchronize(e->own);
     if (err != cudaSuccess) {
@@ -648,6 +650,7 @@ extern "C" int b200_engine_close(b200_engine_t *e) {
     if (e->sel_scratch) cudaFree(e->sel_scratch);
     if (e->fsel_scratch) cudaFree(e->fsel_scratch);
     if (e->serve_scratch) cudaFree(e->serve_scratch);
+    if (e->plan_scratch) cudaFree(e->plan_scratch);
     if (e->fork) cudaEventDestroy(e->fork);
     if (e->done) cudaEventDestroy(e->done);
     if (e->handover) cudaEventDestroy(e->handover);
@@ -933,4 +936,51 @@ extern "C" int b200_sample(b200_engine_t *e, const b200_sample_t *s) {
     if (int rc = use_device(e->device)) return rc;
     const cudaError_t err = sample_launch(s, e->stream);
     return err == cudaSuccess ? 0 : cuda_fail(err, "sample launch");
+}
+
+extern "C" int b200_kv_plan(b200_engine_t *e, const b200_kv_t *kv, const b200_kv_plan_t *a) {
+    if (!e) return fail(kErrInval, "engine not open");
+    const char *why = nullptr;
+    if (kv_plan_validate(kv, a, &why)) return fail(kErrInval, "kv_plan: %s", why);
+    if (int rc = use_device(e->device)) return rc;
+    if (int rc = serve_begin(e)) return rc;
+    const cudaError_t err = kv_plan_launch(kv, a, e->plan_scratch, e->stream);
+    return err == cudaSuccess ? 0 : cuda_fail(err, "kv_plan launch");
+}
+
+extern "C" int b200_rope(b200_engine_t *e, const b200_kv_t *kv, const b200_rope_t *a) {
+    if (!e) return fail(kErrInval, "engine not open");
+    const char *why = nullptr;
+    if (rope_validate(kv, a, &why)) return fail(kErrInval, "rope: %s", why);
+    if (int rc = use_device(e->device)) return rc;
+    const cudaError_t err = rope_launch(kv, a, e->stream);
+    return err == cudaSuccess ? 0 : cuda_fail(err, "rope launch");
+}
+
+extern "C" int b200_rope_freqs(uint64_t *freqs, int rot_dim, double base, const float *factors, int scaling,
+                               double factor, double context, double low, double high) {
+    const char *why = nullptr;
+    if (rope_freqs(freqs, rot_dim, base, factors, scaling, factor, context, low, high, &why))
+        return fail(kErrInval, "rope_freqs: %s", why);
+    return 0;
+}
+
+extern "C" int b200_rms_norm(b200_engine_t *e, const b200_rms_norm_t *a) {
+    if (!e) return fail(kErrInval, "engine not open");
+    const char *why = nullptr;
+    if (rms_norm_validate(a, &why)) return fail(kErrInval, "rms_norm: %s", why);
+    if (int rc = use_device(e->device)) return rc;
+    const cudaError_t err = rms_norm_launch(a, e->cfg.round_mode, e->stream);
+    return err == cudaSuccess ? 0 : cuda_fail(err, "rms_norm launch");
+}
+
+extern "C" int b200_kv_attend_chunk(b200_engine_t *e, const b200_kv_t *kv, const b200_kv_chunk_t *a) {
+    if (!e) return fail(kErrInval, "engine not open");
+    const char *why = nullptr;
+    if (int rc = use_device(e->device)) return rc;       // the workspace goes by the device
+    if (kv_chunk_validate(kv, a, &why)) return fail(kErrInval, "kv_attend_chunk: %s", why);
+    if (int rc = serve_begin(e)) return rc;
+    if (capturing(e->stream)) e->recorded = true;
+    const cudaError_t err = kv_chunk_launch(kv, a, e->stream);
+    return err == cudaSuccess ? 0 : cuda_fail(err, "kv_attend_chunk launch");
 }

@@ -1,5 +1,6 @@
 // Launchers of the serving operators (kv_append.cu, kv_attend.cu,
-// kv_evict.cu, sample.cu): the device side of b200_kv_* and b200_sample.
+// kv_evict.cu, sample.cu, kv_plan.cu, rope.cu, rms_norm.cu, kv_chunk.cu): the
+// device side of b200_kv_*, b200_sample, b200_rope and b200_rms_norm.
 #pragma once
 
 #include <cuda_runtime.h>
@@ -32,17 +33,31 @@ int kv_append_validate(const b200_kv_t *kv, const b200_kv_append_t *a, const cha
 int kv_attend_validate(const b200_kv_t *kv, const b200_kv_attend_t *a, const char **why);
 int kv_evict_validate(const b200_kv_t *kv, const b200_kv_evict_t *a, const char **why);
 int sample_validate(const b200_sample_t *s, const char **why);
+int kv_plan_validate(const b200_kv_t *kv, const b200_kv_plan_t *a, const char **why);
+int rope_validate(const b200_kv_t *kv, const b200_rope_t *a, const char **why);
+int rms_norm_validate(const b200_rms_norm_t *a, const char **why);
+int kv_chunk_validate(const b200_kv_t *kv, const b200_kv_chunk_t *a, const char **why);
 
 KvView kv_view(const b200_kv_t *kv);
 
 // `scratch` of each: serve_scratch_bytes() on the device, zeroed once; one
 // call at a time uses it (an engine's calls follow one another on a stream).
+// kv_plan's, kv_plan_scratch_bytes(), needs no zeros.
 size_t serve_scratch_bytes();
+size_t kv_plan_scratch_bytes();
 
 // Each launches on `stream` and returns 0 or a CUDA error.
 cudaError_t kv_append_launch(const b200_kv_t *kv, const b200_kv_append_t *a, void *scratch, cudaStream_t stream);
 cudaError_t kv_attend_launch(const b200_kv_t *kv, const b200_kv_attend_t *a, void *scratch, cudaStream_t stream);
 cudaError_t kv_evict_launch(const b200_kv_t *kv, const b200_kv_evict_t *a, void *scratch, cudaStream_t stream);
 cudaError_t sample_launch(const b200_sample_t *s, cudaStream_t stream);
+cudaError_t kv_plan_launch(const b200_kv_t *kv, const b200_kv_plan_t *a, void *scratch, cudaStream_t stream);
+cudaError_t rope_launch(const b200_kv_t *kv, const b200_rope_t *a, cudaStream_t stream);
+cudaError_t rms_norm_launch(const b200_rms_norm_t *a, int round_mode, cudaStream_t stream);
+cudaError_t kv_chunk_launch(const b200_kv_t *kv, const b200_kv_chunk_t *a, cudaStream_t stream);
+
+// b200_rope_freqs: 0, or kErrInval with *why set.
+int rope_freqs(uint64_t *freqs, int rot_dim, double base, const float *factors, int scaling, double factor,
+               double context, double low, double high, const char **why);
 
 }  // namespace b200

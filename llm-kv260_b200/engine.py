@@ -13,7 +13,7 @@ from threading import Lock
 
 from . import capi
 from .capi import check, lib
-from .paged import PagedKV, address, dtype_code, rows
+from .paged import PagedKV, address, dtype_code, row_stride, rows
 
 # native struct formats of the C ABI's field types
 _FORMAT = {capi.c_u64: "Q", capi.c_i64: "q", capi.c_int: "i", ctypes.c_float: "f"}
@@ -76,9 +76,29 @@ class QMat:
         return self.rows * (self.k // QK) * BLOCK_BYTES
 
 
+ROPE_SCALING = {None: 0, "linear": 1, "bands": 2, "yarn": 3}
+
+
+def rope_freqs(rot_dim: int, base: float = 10000.0, factors=None, scaling: str | None = None, factor: float = 1.0,
+               context: float = 0.0, low: float = 1.0, high: float = 32.0):
+    """Frequencies for Engine.rope, an int64 tensor [rot_dim / 2] on the host in units of 2^-64 turns: base^(-2 i /
+    rot_dim) radians divided by factors[i], and for long contexts "linear", "bands" or "yarn" (b200_rope_freqs)."""
+    torch = _torch()
+    if scaling not in ROPE_SCALING:
+        raise ValueError(f"scaling must be one of {list(ROPE_SCALING)}")
+    out = torch.empty(max(rot_dim // 2, 0), dtype=torch.int64)
+    if factors is not None:
+        factors = torch.as_tensor(factors, dtype=torch.float32, device="cpu").contiguous()
+        if factors.shape != out.shape:
+            raise ValueError(f"factors must hold rot_dim / 2 = {out.numel()} numbers")
+    check(lib().b200_rope_freqs(out.data_ptr(), rot_dim, base, None if factors is None else factors.data_ptr(),
+                                ROPE_SCALING[scaling], factor, context, low, high), "b200_rope_freqs")
+    return out
+
+
 class Engine:
     """b200_engine.h: the engine_t-level call (tp_llama.cpp:289-375). One thread at a time, as there; only the serving
-    calls (kv_append, kv_attend, kv_evict, sample) may come from several, on a stream that stays the same."""
+    calls (kv_*, sample, rope, rms_norm) may come from several, on a stream that stays the same."""
 
     def __init__(self, device: int = 0, stream: int | None = None):
         self.device = device
@@ -167,13 +187,13 @@ class Engine:
     def prefetch(self, W: QMat) -> None:
         check(lib().b200_prefetch(self.h, ctypes.byref(W.c)), "b200_prefetch")
 
-    def _call(self, name: str, struct, values, kv: PagedKV | None = None) -> None:
+    def _call(self, name: str, struct, values, kv: PagedKV | None = None, may_lack_kv: bool = False) -> None:
         """The C call of that name with an argument struct of `values`. Another thread's call waits: the interpreter's
         lock is given up while C reads the struct."""
         with self._lock:
-            self._queue(name, struct, values, kv)
+            self._queue(name, struct, values, kv, may_lack_kv)
 
-    def _queue(self, name: str, struct, values, kv: PagedKV | None) -> None:
+    def _queue(self, name: str, struct, values, kv: PagedKV | None, may_lack_kv: bool = False) -> None:
         kept = self._structs.get(name)
         if kept is None:               # the struct is one per engine, filled anew each time
             buf = bytearray(ctypes.sizeof(struct))
@@ -182,7 +202,7 @@ class Engine:
             kept = self._structs[name] = (getattr(lib(), name), ctypes.byref(c), fmt.pack_into, buf)
         fn, ref, pack, buf = kept
         pack(buf, 0, *values)
-        rc = fn(self.h, ref) if kv is None else fn(self.h, kv.ref, ref)
+        rc = fn(self.h, kv.ref, ref) if kv is not None else fn(self.h, None, ref) if may_lack_kv else fn(self.h, ref)
         if rc < 0:
             check(rc, name)
 
@@ -225,13 +245,35 @@ class Engine:
         ws_bytes = kv.workspace.get((n_head, wo != 0))
         if ws_bytes is None:
             ws_bytes = kv.workspace[n_head, wo != 0] = int(lib().b200_kv_attend_workspace(kv.ref, n_head, int(wo != 0)))
+        self._call_ws("b200_kv_attend", capi.b200_kv_attend_t, ws_bytes, (
+            q.data_ptr(), out.data_ptr(), dtype_code(q, "q"), n_head, qs[0], qs[1], os_[0], os_[1],
+            kv.head_dim ** -0.5 if scale is None else scale, address(lse, "float32", "lse", (kv.batch, n_head)),
+            w, wo, stride2, decay), kv)
+
+    def kv_attend_chunk(self, kv: PagedKV, q, out, offsets, lse=None, scale: float | None = None, window: int = 0) -> None:
+        """out = softmax(scale q K^T) V for new tokens that are in the cache already, rows offsets[b]:offsets[b + 1] for
+        the last slots in use of sequence b: q and out [tokens, n_head, head_dim], lse float32 [tokens, n_head]. Each
+        sees the slots up to its own, with a window the last `window` of them."""
+        if q.dim() != 3 or q.dtype is not out.dtype:
+            raise ValueError("q and out must be [tokens, n_head, head_dim] of one type")
+        n, n_head, _ = q.shape
+        shape = (n, n_head, kv.head_dim)
+        qs, os_ = rows(q, "q", shape), rows(out, "out", shape)
+        code = dtype_code(q, "q")
+        ws_bytes = kv.workspace.get(("chunk", code, n_head))
+        if ws_bytes is None:
+            ws_bytes = kv.workspace["chunk", code, n_head] = int(lib().b200_kv_chunk_workspace(kv.ref, code, n_head))
+        self._call_ws("b200_kv_attend_chunk", capi.b200_kv_chunk_t, ws_bytes, (
+            q.data_ptr(), out.data_ptr(), code, n, n_head, qs[0], qs[1], os_[0], os_[1],
+            address(offsets, "int32", "offsets", (kv.batch + 1,)), kv.head_dim ** -0.5 if scale is None else scale,
+            window, address(lse, "float32", "lse", (n, n_head))), kv)
+
+    def _call_ws(self, name: str, struct, ws_bytes: int, values, kv: PagedKV) -> None:
+        """_call with the engine's workspace, at least ws_bytes of it, behind the values."""
         with self._lock:
             if self._ws_bytes < ws_bytes:
                 self._grow(ws_bytes)
-            self._queue("b200_kv_attend", capi.b200_kv_attend_t, (
-                q.data_ptr(), out.data_ptr(), dtype_code(q, "q"), n_head, qs[0], qs[1], os_[0], os_[1],
-                kv.head_dim ** -0.5 if scale is None else scale, address(lse, "float32", "lse", (kv.batch, n_head)),
-                w, wo, stride2, decay, self._ws_at, ws_bytes), kv)
+            self._queue(name, struct, (*values, self._ws_at, ws_bytes), kv)
             if self._ws_old:           # this call waits for all that used them
                 on = self._torch_stream()
                 for ws in self._ws_old:
@@ -249,7 +291,7 @@ class Engine:
         torch, on = _torch(), self._torch_stream()
         with torch.cuda.stream(on):
             if torch.cuda.is_current_stream_capturing():
-                raise RuntimeError(f"kv_attend needs a workspace of {nbytes} bytes, which cannot be allocated in a capture: "
+                raise RuntimeError(f"attention needs a workspace of {nbytes} bytes, which cannot be allocated in a capture: "
                                    "make the call once before it is captured")
             ws = torch.empty(nbytes + nbytes // 8, dtype=torch.uint8, device=on.device)
         if self._ws is not None:
@@ -272,6 +314,104 @@ class Engine:
             w, wo, p, po, stride, address(seen, "int32", "seen", b),
             address(kv.lengths if lengths_out is None else lengths_out, "int32", "lengths_out", b), budget, recent,
             sinks), kv)
+
+    def kv_plan(self, kv: PagedKV, new, held, free, free_count, offsets, slots=None, positions=None, sequences=None,
+                granted=None, seen=None, lengths_out=None, held_out=None, free_count_out=None, seen_out=None) -> None:
+        """Pages for new[b] tokens (int32 [batch], negative: the sequence is done) behind the slots in use: table rows of
+        which held[b] columns are in use, and a stack of free pages, free[:free_count]. All or nothing for a sequence.
+        Written are offsets [batch + 1], the tokens of each sequence; per token its slot in the pool (int64, -1: none), its
+        position and its sequence (int32 [tokens]); granted, the tokens that got slots; and held, free_count, lengths
+        and seen, by default in place."""
+        n, b = None, (kv.batch,)
+        for t in (slots, positions, sequences):
+            if t is not None:
+                if n is not None and t.shape != n:
+                    raise ValueError("slots, positions and sequences must have one length")
+                n = t.shape
+        if n is not None and len(n) != 1:
+            raise ValueError("slots, positions and sequences must be [tokens]")
+        if free.dim() != 1:
+            raise ValueError("free must be [pages]")
+        self._call("b200_kv_plan", capi.b200_kv_plan_t, (
+            address(new, "int32", "new", b), address(held, "int32", "held", b),
+            address(held if held_out is None else held_out, "int32", "held_out", b),
+            address(free, "int32", "free", free.shape), free.shape[0], address(free_count, "int32", "free_count", (1,)),
+            address(free_count if free_count_out is None else free_count_out, "int32", "free_count_out", (1,)),
+            address(offsets, "int32", "offsets", (kv.batch + 1,)), (0x7fffffff if n is None else n[0]),
+            address(slots, "int64", "slots", n), address(positions, "int32", "positions", n),
+            address(sequences, "int32", "sequences", n), address(granted, "int32", "granted", b),
+            address(seen, "int32", "seen", b), address(seen if seen_out is None else seen_out, "int32", "seen_out", b),
+            address(kv.lengths if lengths_out is None else lengths_out, "int32", "lengths_out", b)), kv)
+
+    def rope(self, positions, freqs, q=None, q_out=None, k=None, k_out=None, interleaved: bool = False, mscale: float = 1.0,
+             kv: PagedKV | None = None, v=None, slots=None) -> None:
+        """Rotary positions (int32 [tokens]) for q [tokens, n_head, head_dim] and k [tokens, n_head_kv, head_dim], with the
+        frequencies of rope_freqs on the device: to q_out and k_out, by default in place. With a cache, k's rows go to
+        its rows slots[t] (int64, -1: nowhere) instead, and v's beside them."""
+        some = k if q is None else q
+        if some is None or some.dim() != 3:
+            raise ValueError("q or k must be [tokens, heads, head_dim]")
+        n, heads, d = some.shape
+        code = dtype_code(some, "q")
+        zero = (0, 0)
+        qp = qo = h = kp = ko = hkv = vp = 0
+        qs = qos = ks = kos = vs = zero
+        out_code = code
+        if q is not None:
+            q_out = q if q_out is None else q_out
+            h, qs, qos = heads, rows(q, "q", q.shape), rows(q_out, "q_out", q.shape)
+            qp, qo, out_code = q.data_ptr(), q_out.data_ptr(), dtype_code(q_out, "q_out")
+        if k is not None:
+            if k.dim() != 3 or dtype_code(k, "k") != code:
+                raise ValueError("k must be [tokens, n_head_kv, head_dim], of q's type")
+            hkv = k.shape[1]
+            kp, ks = k.data_ptr(), rows(k, "k", (n, hkv, d))
+            if kv is None:
+                k_out = k if k_out is None else k_out
+                ko, kos = k_out.data_ptr(), rows(k_out, "k_out", k.shape)
+                if q is not None and dtype_code(k_out, "k_out") != out_code:
+                    raise ValueError("q_out and k_out must be of one type")
+                out_code = dtype_code(k_out, "k_out")
+        if kv is None and (v is not None or slots is not None):
+            raise ValueError("v and slots need a cache")
+        if v is not None:
+            if k is None or v.dtype is not k.dtype:
+                raise ValueError("v must be of k's type")
+            vp, vs = v.data_ptr(), rows(v, "v", k.shape)
+        if freqs.dim() != 1:
+            raise ValueError("freqs must be [rot_dim / 2]")
+        self._call("b200_rope", capi.b200_rope_t, (
+            qp, qo, h, *qs, *qos, kp, ko, hkv, *ks, *kos, vp, *vs, code, out_code, n, d, 2 * freqs.shape[0], int(interleaved),
+            address(positions, "int32", "positions", (n,)), address(freqs, "int64", "freqs", freqs.shape), mscale,
+            address(slots, "int64", "slots", (n,))), kv, True)
+
+    def rms_norm(self, x, weight, out=None, eps: float = 1e-5, residual=None, residual_out=None, q8=None) -> None:
+        """r = residual + x (x alone without one), y = r / sqrt(mean(r^2) + eps) * weight (float32) for rows x [n, k]: r to
+        residual_out, by default in place, y to out and, as Q8_0 rows that gemv_q8 reads, to q8 (uint8 [n, k + k / 8])."""
+        if x.dim() != 2:
+            raise ValueError("x must be [rows, k]")
+        n, k = shape = x.shape
+        code = dtype_code(x, "x")
+        rp = ro = op = qp = rs = ros = os_ = qs = 0
+        r_code = o_code = code
+        xs = row_stride(x, "x", shape)
+        if residual is not None:
+            residual_out = residual if residual_out is None else residual_out
+            if residual_out.dtype is not residual.dtype:
+                raise ValueError("residual and residual_out must be of one type")
+            rp, rs, r_code = residual.data_ptr(), row_stride(residual, "residual", shape), dtype_code(residual, "residual")
+            ro, ros = residual_out.data_ptr(), row_stride(residual_out, "residual_out", shape)
+        elif residual_out is not None:
+            raise ValueError("residual_out without residual")
+        if out is not None:
+            op, os_, o_code = out.data_ptr(), row_stride(out, "out", shape), dtype_code(out, "out")
+        if q8 is not None:
+            if q8.element_size() != 1:
+                raise ValueError("q8 must be bytes")
+            qp, qs = q8.data_ptr(), row_stride(q8, "q8", (n, k + k // 8))
+        self._call("b200_rms_norm", capi.b200_rms_norm_t, (
+            x.data_ptr(), code, rp, ro, r_code, address(weight, "float32", "weight", (k,)), op, o_code, qp, n, k, xs, rs, ros,
+            os_, qs, eps))
 
     def sample(self, logits, u, token, logprob=None, temperature=None, top_k=None, top_p=None, min_p=None) -> None:
         """token int32 [batch] (and the log of its probability) drawn from logits [batch, n_vocab] with the uniform

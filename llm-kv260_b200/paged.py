@@ -14,7 +14,7 @@ def codes() -> dict:
     if not _CODES:
         import torch
         _CODES.update({torch.float32: 0, torch.float16: 1, torch.bfloat16: 2})
-        _CODES["int32"], _CODES["float32"] = torch.int32, torch.float32
+        _CODES["int32"], _CODES["float32"], _CODES["int64"] = torch.int32, torch.float32, torch.int64
     return _CODES
 
 
@@ -26,7 +26,7 @@ def dtype_code(t, name: str) -> int:
 
 
 def address(t, dtype: str, name: str, shape) -> int:
-    """Device address of a contiguous CUDA tensor of that type ("int32" or "float32") and shape; 0 for None."""
+    """Device address of a contiguous CUDA tensor of that type ("int32", "int64" or "float32") and shape; 0 for None."""
     if t is None:
         return 0
     want = (_CODES or codes())[dtype]
@@ -49,6 +49,18 @@ def rows(t, name: str, shape) -> tuple[int, int]:
     if s2 != 1 and shape[2] != 1:
         raise ValueError(f"{name}: a row must be contiguous")
     return s0, s1
+
+
+def row_stride(t, name: str, shape) -> int:
+    """The stride of a [rows, k] tensor's rows, which are contiguous."""
+    if not t.is_cuda:
+        raise ValueError(f"{name} must be a CUDA tensor")
+    if t.shape != shape:
+        raise ValueError(f"{name} must have shape {tuple(shape)}, not {tuple(t.shape)}")
+    s0, s1 = t.stride()
+    if s1 != 1 and shape[1] != 1:
+        raise ValueError(f"{name}: a row must be contiguous")
+    return s0
 
 
 class PagedKV:

@@ -1,0 +1,66 @@
+"""The host side of the operators that a prompt passes through, without a GPU."""
+
+from __future__ import annotations
+
+import math
+
+import numpy as np
+import pytest
+
+TWO64 = 2.0 ** 64
+
+
+def turns(t):
+    """rope_freqs' whole numbers as turns a position."""
+    return t.numpy().view(np.uint64).astype(np.float64) / TWO64
+
+
+@pytest.mark.parametrize("rot,base", [(2, 10000.0), (64, 10000.0), (80, 500000.0), (256, 1.5)])
+def test_frequencies(pkg, rot, base):
+    """To a part in 2^50 of a turn: the double's own rounding."""
+    want = base ** (-2.0 * np.arange(rot // 2) / rot) / (2 * math.pi)
+    assert np.abs(turns(pkg.rope_freqs(rot, base)) - want).max() < 2.0 ** -50
+    assert np.abs(turns(pkg.rope_freqs(rot, base, scaling="linear", factor=4.0)) - want / 4).max() < 2.0 ** -50
+    f = np.linspace(1.0, 8.0, rot // 2).astype(np.float32)
+    assert np.abs(turns(pkg.rope_freqs(rot, base, factors=f)) - want / f).max() < 2.0 ** -50
+
+
+def test_frequencies_for_long_contexts(pkg):
+    rot, base = 64, 500000.0
+    inv = base ** (-2.0 * np.arange(rot // 2) / rot)
+    got = turns(pkg.rope_freqs(rot, base, scaling="bands", factor=8.0, context=8192, low=1.0, high=4.0))
+    n = 8192 * inv / (2 * math.pi)
+    for i in range(rot // 2):
+        keep = min(max((n[i] - 1) / 3, 0), 1)
+        assert abs(got[i] - (inv[i] * keep + inv[i] / 8 * (1 - keep)) / (2 * math.pi)) < 2.0 ** -50
+    assert (n > 4).any() and (n < 1).any()
+    got = turns(pkg.rope_freqs(rot, base, scaling="yarn", factor=16.0, context=4096, low=1.0, high=32.0))
+
+    def index(x):
+        return rot * math.log(4096 / (x * 2 * math.pi)) / (2 * math.log(base))
+
+    lo, hi = math.floor(index(32.0)), math.ceil(index(1.0))
+    assert 0 < lo < hi < rot // 2
+    for i in range(rot // 2):
+        slow = min(max((i - lo) / (hi - lo), 0), 1)
+        assert abs(got[i] - inv[i] * (1 - slow + slow / 16) / (2 * math.pi)) < 2.0 ** -50
+
+
+def test_frequencies_refused(pkg):
+    for kw in (dict(rot_dim=0), dict(rot_dim=7), dict(rot_dim=258), dict(base=0.0), dict(base=-1.0), dict(base=math.nan),
+               dict(scaling="linear", factor=0.0), dict(scaling="bands", factor=2.0), dict(scaling="other"),
+               dict(scaling="bands", factor=2.0, context=100.0, low=4.0, high=4.0), dict(factors=[1.0, 0.0] * 16),
+               dict(scaling="yarn", factor=2.0, context=100.0, base=1.0), dict(factors=[1.0])):
+        with pytest.raises((ValueError, pkg.B200Error)):
+            pkg.rope_freqs(**dict(dict(rot_dim=64), **kw))
+
+
+def test_workspace_of_unusable_sizes(pkg):
+    import ctypes
+    lib, t = pkg.lib(), pkg.capi.b200_kv_t
+    good = dict(k=256, v=256, dtype=1, n_pages=4, page_size=16, n_head_kv=2, head_dim=64, page_stride=2048, head_stride=1024,
+                row_stride=64, table=256, table_stride=2, table_cols=2, lengths=256, batch=1)
+    for change, dtype, n_head in ((dict(head_dim=60), 1, 4), (dict(batch=0), 1, 4), (dict(k=0), 1, 4), ({}, 2, 4), ({}, 1, 3),
+                                  ({}, 1, 1), (dict(dtype=0), 1, 4), (dict(dtype=2), 0, 4), (dict(page_size=0), 1, 4)):
+        kv = t(**dict(good, **change))
+        assert lib.b200_kv_chunk_workspace(ctypes.byref(kv), dtype, n_head) == 0
