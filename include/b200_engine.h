@@ -407,7 +407,7 @@ typedef struct {
     int n_tokens, n_head;              /* n_head: a multiple of n_head_kv */
     int64_t q_token_stride, q_head_stride, out_token_stride, out_head_stride;
     uint64_t offsets;                  /* int32 [batch + 1], as in b200_kv_append_t */
-    float scale;
+    float scale;                       /* positive */
     int window;                        /* 0: none */
     uint64_t lse;                      /* float [n_tokens][n_head], or 0 */
     uint64_t workspace;                /* b200_kv_chunk_workspace() bytes, 16-byte aligned; holds nothing between calls */

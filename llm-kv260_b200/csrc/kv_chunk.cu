@@ -7,7 +7,9 @@ namespace b200 {
 
 namespace {
 
-chunk::Shape shape_of(const b200_kv_t *kv, int) { return chunk::f32_shape(kv->head_dim); }
+chunk::Shape shape_of(const b200_kv_t *kv, int dtype) {
+    return dtype == B200_F32 ? chunk::f32_shape(kv->head_dim) : chunk::mma_shape(kv->head_dim);
+}
 
 uint64_t workspace_bytes(const b200_kv_t *kv, int dtype) {
     const chunk::Shape s = shape_of(kv, dtype);
@@ -26,7 +28,8 @@ int kv_chunk_validate(const b200_kv_t *kv, const b200_kv_chunk_t *a, const char 
     if (a->n_tokens < 0 || static_cast<int64_t>(a->n_tokens) * a->n_head > 1ll << 30)
         return bad("n_tokens must be in [0, 2^30 / n_head]");
     if (a->window < 0) return bad("window must not be negative");
-    if (!(a->scale - a->scale == 0.0f)) return bad("scale must be finite");
+    if (!(a->scale * chunk::kLog2e >= 1e-37f) || !(a->scale * chunk::kLog2e <= 1e37f))
+        return bad("scale must be positive, in [1e-37, 1e37]");
     if (!a->offsets || (a->n_tokens > 0 && (!a->q || !a->out))) return bad("null address");
     const int es = esize(a->dtype);
     if (a->q_token_stride < 0 || a->q_head_stride < 0 || a->out_token_stride < 0 || a->out_head_stride < 0)
@@ -63,7 +66,7 @@ cudaError_t kv_chunk_launch(const b200_kv_t *kv, const b200_kv_chunk_t *p, cudaS
     a.parts = reinterpret_cast<float *>(p->workspace);
     a.joints = reinterpret_cast<chunk::Joint *>(p->workspace + s.grid * 2 * s.part);
     a.status = status_word();
-    return chunk::f32_launch(a, p->dtype, kv->dtype, stream);
+    return p->dtype == B200_F32 ? chunk::f32_launch(a, kv->dtype, stream) : chunk::mma_launch(a, kv->dtype, stream);
 }
 
 }  // namespace b200

@@ -262,14 +262,17 @@ cudaError_t launch_join(const Args &a, int grid, cudaStream_t stream) {
     return cudaLaunchKernelEx(&cfg, join_kernel<T, M, kDim>, a);
 }
 
-// Each launches a call of its types: kv_chunk_f32.cu, any; grid in CTAs and
-// bytes of a part of its tiles for the workspace.
+// Each launches calls of its types: kv_chunk_mma.cu those with 16-bit queries,
+// kv_chunk_f32.cu those with float32 queries; grid in CTAs and bytes of a part
+// of its tiles for the workspace.
 struct Shape {
     int grid;
     long long part;
 };
+Shape mma_shape(int head_dim);
+cudaError_t mma_launch(const Args &a, int kv_dtype, cudaStream_t stream);
 Shape f32_shape(int head_dim);
-cudaError_t f32_launch(const Args &a, int dtype, int kv_dtype, cudaStream_t stream);
+cudaError_t f32_launch(const Args &a, int kv_dtype, cudaStream_t stream);
 
 }  // namespace chunk
 }  // namespace b200

@@ -224,10 +224,8 @@ Shape f32_shape(int head_dim) {
     return Shape{grid_of(dim), part_floats(kM, dim) * 4};
 }
 
-cudaError_t f32_launch(const Args &a, int dtype, int kv_dtype, cudaStream_t stream) {
-    if (kv_dtype == B200_F32) return launch<float, float>(a, stream);
-    if (kv_dtype == B200_BF16) return launch<__nv_bfloat16, __nv_bfloat16>(a, stream);
-    return dtype == B200_F32 ? launch<float, __half>(a, stream) : launch<__half, __half>(a, stream);
+cudaError_t f32_launch(const Args &a, int kv_dtype, cudaStream_t stream) {
+    return kv_dtype == B200_F32 ? launch<float, float>(a, stream) : launch<float, __half>(a, stream);
 }
 
 }  // namespace chunk

@@ -1,0 +1,95 @@
+// Thin inline-PTX wrappers for the fifth-generation tensor cores: tensor memory,
+// its loads and stores, the matrix instruction for 16-bit operands and its
+// completion barriers. One CTA per matrix product (cta_group::1).
+#pragma once
+
+#include <cstdint>
+
+#include "ptx.cuh"
+
+namespace b200 {
+
+// All 32 lanes of one warp; the address of `columns` columns (a power of two,
+// 32 to 512) of 128 lanes of 32 bits goes to shared memory.
+__device__ __forceinline__ void tmem_alloc(uint32_t *at, uint32_t columns) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr(at)), "r"(columns)
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+}
+__device__ __forceinline__ void tmem_free(uint32_t at, uint32_t columns) {
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(at), "r"(columns));
+}
+
+// Order tensor-memory work of this thread before / after a barrier.
+__device__ __forceinline__ void tmem_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void tmem_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void tmem_wait_load() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void tmem_wait_store() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+// Arrives on `bar` when all matrix products that this thread has issued are done.
+__device__ __forceinline__ void mma_commit(uint64_t *bar) {
+    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_addr(bar))
+                 : "memory");
+}
+
+// Writes of this thread to shared memory before reads of the tensor cores.
+__device__ __forceinline__ void fence_async_proxy() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
+
+// A tile in shared memory as the tensor cores see it: rows of 128 bytes, their
+// 16-byte pieces xor-ed with the row's number modulo 8. Where the contraction
+// runs along a row, `stride` is the distance of 8 rows and `lead` is unused;
+// where it runs down the rows, `lead` is the distance of 64 columns.
+__device__ __forceinline__ uint64_t smem_desc(uint32_t at, uint32_t lead, uint32_t stride) {
+    return static_cast<uint64_t>((at >> 4) & 0x3fff) | static_cast<uint64_t>((lead >> 4) & 0x3fff) << 16 |
+           static_cast<uint64_t>((stride >> 4) & 0x3fff) << 32 | 1ull << 46 | 2ull << 61;
+}
+
+// M x N products of f16 or bf16 operands into float32; b_down: the contraction
+// runs down the rows of B.
+__host__ __device__ constexpr uint32_t mma_desc(int m, int n, bool bf16, bool b_down) {
+    return 1u << 4 | (bf16 ? 1u << 7 | 1u << 10 : 0u) | (b_down ? 1u << 16 : 0u) | static_cast<uint32_t>(n >> 3) << 17 |
+           static_cast<uint32_t>(m >> 4) << 24;
+}
+
+// D (tensor memory) = A B, plus D where `add`: A in shared memory, or in tensor memory.
+__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t desc, bool add) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+        "l"(a), "l"(b), "r"(desc), "r"(static_cast<uint32_t>(add))
+        : "memory");
+}
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t desc, bool add) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
+        "r"(a), "l"(b), "r"(desc), "r"(static_cast<uint32_t>(add))
+        : "memory");
+}
+
+// 32 columns of this warp's 32 lanes, a lane's in its registers.
+__device__ __forceinline__ void tmem_load32(uint32_t at, uint32_t (&v)[32]) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
+        "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+        "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+        : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]),
+          "=r"(v[8]), "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15]),
+          "=r"(v[16]), "=r"(v[17]), "=r"(v[18]), "=r"(v[19]), "=r"(v[20]), "=r"(v[21]), "=r"(v[22]), "=r"(v[23]),
+          "=r"(v[24]), "=r"(v[25]), "=r"(v[26]), "=r"(v[27]), "=r"(v[28]), "=r"(v[29]), "=r"(v[30]), "=r"(v[31])
+        : "r"(at));
+}
+__device__ __forceinline__ void tmem_store32(uint32_t at, const uint32_t (&v)[32]) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%32], "
+        "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+        "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31};" ::
+          "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]),
+          "r"(v[8]), "r"(v[9]), "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15]),
+          "r"(v[16]), "r"(v[17]), "r"(v[18]), "r"(v[19]), "r"(v[20]), "r"(v[21]), "r"(v[22]), "r"(v[23]),
+          "r"(v[24]), "r"(v[25]), "r"(v[26]), "r"(v[27]), "r"(v[28]), "r"(v[29]), "r"(v[30]), "r"(v[31]),
+          "r"(at)
+        : "memory");
+}
+
+}  // namespace b200

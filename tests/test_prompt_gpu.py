@@ -618,7 +618,7 @@ def test_refusals(torch_mod, pkg, eng):
     chunk()
     for kw in (dict(q=f(5, 3, 64), out=f(5, 3, 64)), dict(q=f(5, 4, 32), out=f(5, 4, 32)), dict(out=f(5, 4, 64, dt=torch.float32)),
                dict(q=f(5, 4, 64, dt=torch.bfloat16), out=f(5, 4, 64, dt=torch.bfloat16)), dict(offsets=i32(3)),
-               dict(offsets=off.long()), dict(offsets=off.cpu()), dict(window=-1), dict(scale=math.inf), dict(scale=math.nan),
+               dict(offsets=off.long()), dict(offsets=off.cpu()), dict(window=-1), dict(scale=math.inf), dict(scale=math.nan), dict(scale=0.0), dict(scale=-0.1),
                dict(lse=f(5, 4)), dict(lse=f(4, 4, dt=torch.float32)), dict(out=out.cpu()),
                dict(q=f(5, 4, 65)[..., 1:]), dict(q=f(5, 4, 128)[..., ::2]), dict(q=f(5, 4, 68)[..., :64]),
                dict(out=f(5 * 4 * 64 + 8)[4:5 * 4 * 64 + 4].view(5, 4, 64))):
