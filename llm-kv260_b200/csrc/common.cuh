@@ -183,6 +183,8 @@ bool ensure_smem(const void *fn, int bytes);
 int resident_ctas(const void *fn, int threads, int smem);
 // Device address of this device's status word.
 unsigned *status_word();
+// The driver's cuTensorMapEncodeTiled, or NULL.
+void *tensor_map_encoder();
 
 inline int round_up(int v, int a) { return (v + a - 1) / a * a; }
 

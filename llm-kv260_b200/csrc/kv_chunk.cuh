@@ -59,14 +59,14 @@ __device__ __forceinline__ Sequence sequence(const Args &a, int b) {
     return s;
 }
 
-// The units of a tile: first and how many (at least one, so that its rows are written).
+// The units of a tile: first and how many (at least one, so that its rows are
+// written). Packed rows fit 31 bits: there are at most 2^30 query heads in a call.
 template <int M, int N>
 __device__ __forceinline__ int2 units_of(const Args &a, int n, int length, int tile) {
-    const int i0 = static_cast<int>(static_cast<long long>(tile) * M / a.group);
-    const int i1 = static_cast<int>(min(static_cast<long long>(n) - 1, (static_cast<long long>(tile + 1) * M - 1) / a.group));
+    const int i1 = min(n - 1, ((tile + 1) * M - 1) / a.group);
     const int hi = max(length - n + i1 + 1, 0);
-    const long long lo = a.window ? max(0ll, static_cast<long long>(length) - n + i0 - a.window + 1) : 0;
-    const int u0 = static_cast<int>(min(lo, static_cast<long long>(hi)) / N);
+    const int lo = a.window ? max(0, length - n + tile * M / a.group - a.window + 1) : 0;
+    const int u0 = min(lo, hi) / N;
     return make_int2(u0, max((hi + N - 1) / N - u0, 1));
 }
 
@@ -123,7 +123,7 @@ __device__ __forceinline__ Stretch find(const Args &a, Shared<T> *s) {
             int tiles = 0;
             if (base + tid < a.kv.batch) {
                 const Sequence q = sequence(a, base + tid);
-                tiles = static_cast<int>((static_cast<long long>(q.n) * a.group + M - 1) / M);
+                tiles = (q.n * a.group + M - 1) / M;
                 s->n[tid] = q.n;
                 s->length[tid] = q.length;
             }
@@ -183,7 +183,7 @@ __device__ __forceinline__ Stretch find(const Args &a, Shared<T> *s) {
 // The next tile: of the sequence, of the next sequence that has rows, of the next head.
 template <int M>
 __device__ __forceinline__ void next_tile(const Args &a, Sequence &q, int &tile, int &head) {
-    if ((static_cast<long long>(++tile)) * M < static_cast<long long>(q.n) * a.group) return;
+    if (++tile * M < q.n * a.group) return;
     tile = 0;
     int b = q.b;
     do {

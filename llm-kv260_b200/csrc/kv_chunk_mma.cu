@@ -1,4 +1,5 @@
 // b200_kv_attend_chunk for 16-bit queries, on the tensor cores.
+#include <cuda.h>
 #include <cuda_runtime.h>
 
 #include "kv_chunk.cuh"
@@ -9,32 +10,40 @@ namespace chunk {
 
 namespace {
 
-constexpr int kThreads = 384;          // two warpgroups of softmax, one warp of products, three of copies
-constexpr int kCopiers = 96;
-constexpr int kLag = 2;                // copies that a copier leaves in flight behind the newest one
+// A warpgroup of softmax for each tile, a row to a thread, and one with three
+// warps of copies and one that issues the products; and the registers of a
+// thread of each, of the 384 * 168 that a CTA begins with.
+constexpr int kSoftmaxThreads = 256, kCopiers = 96, kThreads = kSoftmaxThreads + kCopiers + 32;
+constexpr int kSoftmaxRegs = 208, kOtherRegs = 88;
+static_assert(kSoftmaxThreads * kSoftmaxRegs + 128 * kOtherRegs <= kThreads * 168);
+constexpr int kLeastBox = 8;           // rows of a page that one tensor copy brings at least
 constexpr int kColumns = 512;          // of tensor memory
 // The reference m trails the maximum by 7 to 15 powers of two: weights stay in
 // 2^15 and below, float16's range, and those of 2^-21 of the largest are still
 // normal numbers there.
 constexpr float kLead = 7.0f, kSlack = 15.0f;
+// Of 8 pairs of weights, how many are computed on the float32 units.
+constexpr int kPolynomial = 0;
 
 template <int kDim>
 struct Plan {
     static constexpr int kTiles = kDim <= 128 ? 2 : 1;     // of 128 rows
     static constexpr int kM = 128 * kTiles, kN = kDim <= 128 ? 128 : 64;
-    static constexpr int kStages = kDim <= 64 ? 6 : 4;
+    static constexpr int kStages = kDim <= 64 ? 8 : 4;     // a power of two
     static constexpr int kQBytes = kM * kDim * 2, kStageBytes = kN * kDim * 2;
     static constexpr int kSmem = 1024 + kQBytes + kStages * kStageBytes;
     // columns of tensor memory: scores (and, over them, weights) per tile, or twice of one, then the outputs
     __device__ static constexpr int scores(int i) { return i * kN; }
+    // the weights of 16 slots, two to a column
+    __device__ static constexpr int weights(int i, int x) { return i * kN + x * 8; }
     __device__ static constexpr int output(int i) { return 256 + i * kDim; }
 };
 
 struct Shared0 {
-    uint64_t full[6], free[6], q_full, q_free, s_full[2], p_full[2], o_done[2], mask_full[2], mask_free[2], last;
+    uint64_t full[8], free[8], q_full, q_free, s_full[2], p_most[2], p_full[2], o_done[2], last;
     uint32_t tmem;
-    uint32_t mask[2][4];               // a unit's slots that are there
-    long long row[2][128];             // byte offsets of their rows
+    int dead;                          // a wait ran out
+    long long row[2][128];             // byte offsets of a unit's rows, -1: not there
     uint32_t bad[256][8];              // a row's columns that a value which is not finite enters
 };
 
@@ -42,6 +51,58 @@ __device__ __forceinline__ float ex2(float x) {
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
+}
+
+// Two float32 numbers side by side, for instructions that take two at once.
+using Pair = unsigned long long;
+__device__ __forceinline__ Pair pair(float lo, float hi) {
+    Pair p;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(p) : "f"(lo), "f"(hi));
+    return p;
+}
+__device__ __forceinline__ void split(Pair p, float &lo, float &hi) { asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(p)); }
+__device__ __forceinline__ Pair fma2(Pair a, Pair b, Pair c) {
+    Pair d;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+    return d;
+}
+__device__ __forceinline__ Pair add2(Pair a, Pair b) {
+    Pair d;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+    return d;
+}
+__device__ __forceinline__ Pair mul2(Pair a, Pair b) {
+    Pair d;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+    return d;
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float d;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+    return d;
+}
+
+// 2^t of two numbers t <= 64 without the special-function unit: t = n + f with n
+// the nearest whole number, 2^f by a polynomial of least relative error on
+// [-1/2, 1/2] (found by Remez' exchange: 2.6e-6, an eightieth of half a step of
+// float16), times 2^n, whose bits are those of t + 1.5 * 2^23 + 127 moved up.
+// Below 2^-126 the result is 0 (n = -127 has no exponent bits), NaN stays NaN.
+__device__ __forceinline__ Pair exp2_of(Pair t) {
+    float t0, t1;
+    split(t, t0, t1);
+    asm("max.NaN.f32 %0, %0, 0fC2FE0000;" : "+f"(t0));     // -127
+    asm("max.NaN.f32 %0, %0, 0fC2FE0000;" : "+f"(t1));
+    t = pair(t0, t1);
+    const float magic = 12582912.0f + 127.0f;
+    const Pair n = add2(t, pair(magic, magic));
+    const Pair f = fma2(add2(n, pair(-magic, -magic)), pair(-1.0f, -1.0f), t);
+    Pair y = fma2(f, pair(0.009570102f, 0.009570102f), pair(0.05591786f, 0.05591786f));
+    y = fma2(f, y, pair(0.24024745f, 0.24024745f));
+    y = fma2(f, y, pair(0.6931218f, 0.6931218f));
+    y = fma2(f, y, pair(0.99999926f, 0.99999926f));
+    float n0, n1;
+    split(n, n0, n1);
+    return mul2(y, pair(__uint_as_float(__float_as_uint(n0) << 23), __uint_as_float(__float_as_uint(n1) << 23)));
 }
 
 __device__ __forceinline__ uint32_t pack(float lo, float hi, __half) {
@@ -76,13 +137,23 @@ __device__ __forceinline__ bool any_of(uint32_t id, uint32_t threads, bool mine)
 }
 
 // A thread's waits. One that runs out says so in the status word and is the
-// last: the thread goes on without waiting, so that it meets every barrier that
-// the others meet and the CTA comes to its end.
+// CTA's last: its threads go on without waiting, so that they meet every barrier
+// that the others meet and come to their end.
 struct Waiter {
     unsigned *status;
-    bool dead = false;
-    __device__ __forceinline__ void operator()(uint64_t *bar, int phase) {
-        if (!dead) dead = !wait_stage(bar, phase & 1, status);
+    volatile int *dead;                // in shared memory
+    __device__ __forceinline__ void operator()(uint64_t *bar, int phase) const {
+        if (mbar_try_wait(bar, phase & 1)) return;
+        uint64_t t0 = 0;
+        for (int n = 1; !mbar_try_wait(bar, phase & 1); ++n) {
+            if (n & 63) continue;
+            if (*dead) return;
+            if (t0 == 0) t0 = globaltimer_ns();
+            if (globaltimer_ns() - t0 > kStageTimeoutNs) {
+                atomicOr(status, kStatusStageTimeout);
+                *dead = 1;
+            }
+        }
     }
 };
 
@@ -99,7 +170,7 @@ __device__ __forceinline__ uint32_t piece(int rows, int r, int c) {
 // A stretch's part of one tile.
 struct Fragment {
     int u0, u1, first;                 // units, the slot of the first new token
-    long long row0, rows;              // first packed row, all of the sequence's
+    int row0, rows;                    // first packed row, all of the sequence's
     bool whole;
     int last_all, first_all;           // slots that every row sees lie between
 };
@@ -111,371 +182,450 @@ __device__ __forceinline__ Fragment fragment(const Args &a, const Sequence &q, i
     f.u0 = all.x + skip;
     f.u1 = all.x + static_cast<int>(min(static_cast<long long>(all.y), skip + left));
     f.first = q.length - q.n;
-    f.rows = static_cast<long long>(q.n) * a.group;
-    f.row0 = static_cast<long long>(tile) * kM;
+    f.rows = q.n * a.group;
+    f.row0 = tile * kM;
     f.whole = f.u1 - f.u0 == all.y;
-    f.last_all = f.first + static_cast<int>(f.row0 / a.group);
-    f.first_all = a.window ? f.first + static_cast<int>(min(f.rows - 1, f.row0 + kM - 1) / a.group) - a.window + 1 : 0;
+    f.last_all = f.first + f.row0 / a.group;
+    f.first_all = a.window ? f.first + min(f.rows - 1, f.row0 + kM - 1) / a.group - a.window + 1 : 0;
     return f;
 }
 
-// The copies of keys, values and queries into shared memory.
-template <typename T, int kDim>
-__device__ __forceinline__ void copier(const Args &a, Shared0 &s, char *smem, Stretch st, unsigned *status) {
+// Arrives on `bar` for this thread when the copies that it has asked for are there.
+__device__ __forceinline__ void arrive_behind_copies(uint64_t *bar) {
+    asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_addr(bar)) : "memory");
+}
+
+// How keys and values come: by tensor copies of `box` rows of a page, or, with
+// box 0, by 16 bytes, whatever the pages' size and strides.
+struct Maps {
+    CUtensorMap k, v;
+};
+
+// The copies of keys, values and queries into shared memory. Nothing waits for
+// a copy here: its arrival is the barrier's, and the reader's fence hands those
+// by 16 bytes to the tensor cores. A tensor copy brings 64 columns of `box` rows;
+// a page that is not there is asked for behind the pool's end, which gives
+// zeros, as copies by 16 bytes of no source do.
+template <typename T, int kDim, bool kBoxes>
+__device__ __forceinline__ void copier(const Args &a, const Maps &maps, int box, Shared0 &s, char *smem, Stretch st,
+                                       unsigned *status) {
     using P = Plan<kDim>;
     constexpr int kPieces = kDim / 8;
-    const int tid = threadIdx.x - (kThreads - kCopiers), lane = tid & 31;
-    const int pieces = (a.kv.head_dim + 15) / 16 * 2, filled = a.kv.head_dim / 8;
+    const int tid = threadIdx.x - kSoftmaxThreads;
+    const int pieces = (a.kv.head_dim + 15) / 16 * 2, filled = a.kv.head_dim / 8, columns = (a.kv.head_dim + 63) / 64;
     const uint32_t q_at = smem_addr(smem), ring = q_at + P::kQBytes;
-    uint64_t *older = nullptr, *newer = nullptr;       // barriers of the copies in flight
-    const auto emit = [&](uint64_t *bar) {
-        cp_async_commit();
-        cp_async_wait<kLag>();
-        if (older) {
-            fence_async_proxy();
-            mbar_arrive(older);
-        }
-        older = newer;
-        newer = bar;
-    };
-    int item = 0, unit = 0, fragments = 0;
+    int stage = 0, use = 0, unit = 0, fragments = 0;
     Sequence q = sequence(a, st.b);
     int tile = st.tile, head = st.head, skip = st.skip;
-    Waiter wait{status};
+    const Waiter wait{status, &s.dead};
     for (;;) {
         const Fragment f = fragment<P::kM, P::kN>(a, q, tile, skip, st.left);
         const char *k_head = a.kv.k + head * a.kv.head_stride, *v_head = a.kv.v + head * a.kv.head_stride;
         const int *table = a.kv.table + q.b * a.kv.table_stride;
-        // a thread looks up two of a unit's slots at most
-        int page[2];
+        int page[2], asked[2], row[2];                 // of two of this unit's and the next one's slots
         const auto ask = [&](int u) {
 #pragma unroll
             for (int x = 0; x < 2; ++x) {
-                const int slot = u * P::kN + tid + x * kCopiers;
-                page[x] = -1;
-                if (tid + x * kCopiers < P::kN && slot < q.length)
-                    page[x] = table[static_cast<int>((slot * a.page_magic) >> 40)];
+                const int n = tid + x * kCopiers, slot = u * P::kN + n;
+                asked[x] = -1;
+                if (n < P::kN && slot < q.length) asked[x] = table[static_cast<int>((slot * a.page_magic) >> 40)];
             }
         };
         const auto place = [&](int u) {
-            const int buf = unit & 1;
-            if (unit >= 2) wait(&s.mask_free[buf], (unit >> 1) - 1);
-            __syncwarp();
 #pragma unroll
             for (int x = 0; x < 2; ++x) {
-                const int r = tid + x * kCopiers, slot = u * P::kN + r;
-                const bool there = static_cast<unsigned>(page[x]) < static_cast<unsigned>(a.kv.n_pages);
-                const uint32_t word = __ballot_sync(kFullMask, there);
-                if (r < P::kN) {
-                    const int col = static_cast<int>((slot * a.page_magic) >> 40);
-                    s.row[buf][r] = there ? page[x] * a.kv.page_stride + (slot - col * a.kv.page_size) * a.kv.row_stride : -1;
-                    if (lane == 0) s.mask[buf][r >> 5] = word;
-                }
+                const int n = tid + x * kCopiers, slot = u * P::kN + n;
+                const bool there = static_cast<unsigned>(asked[x]) < static_cast<unsigned>(a.kv.n_pages);
+                page[x] = there ? asked[x] : a.kv.n_pages;
+                row[x] = slot - static_cast<int>((slot * a.page_magic) >> 40) * a.kv.page_size;
+                if (!kBoxes && n < P::kN) s.row[unit & 1][n] = there ? page[x] * a.kv.page_stride + row[x] * a.kv.row_stride : -1;
             }
-            named_sync(3, kCopiers);
-            if (tid == 0) mbar_arrive(&s.mask_full[buf]);
+            if (!kBoxes) named_sync(3, kCopiers);
         };
         ask(f.u0);
         if (fragments) wait(&s.q_free, fragments - 1);
-        const int rows = static_cast<int>(min(static_cast<long long>(P::kM), f.rows - f.row0));
+        const int rows = min(P::kM, f.rows - f.row0);
+#pragma unroll 1
         for (int i = tid; i < (rows > 128 ? P::kM : 128) * kPieces; i += kCopiers) {
             const int r = i / kPieces, c = i % kPieces;
             if (c >= pieces) continue;
             const bool there = r < rows && c < filled;
             const char *src = a.q;
             if (there) {
-                const int token = static_cast<int>((f.row0 + r) / a.group);
-                const int h = static_cast<int>(f.row0 + r - static_cast<long long>(token) * a.group);
+                const int token = (f.row0 + r) / a.group, h = f.row0 + r - token * a.group;
                 src += (q.from + token) * a.q_token + (head * a.group + h) * a.q_head + c * 16;
             }
             copy16(q_at + (r >> 7) * (128 * kDim * 2) + piece(128, r & 127, c), src, there);
         }
-        emit(&s.q_full);
+        arrive_behind_copies(&s.q_full);
         place(f.u0);
         for (int u = f.u0; u < f.u1; ++u) {
             const int buf = unit & 1;
             if (u + 1 < f.u1) ask(u + 1);
+#pragma unroll 1
             for (int v = 0; v < 2; ++v) {
-                const int stage = item % P::kStages, use = item / P::kStages;
                 if (use) wait(&s.free[stage], use - 1);
-                const char *src = v ? v_head : k_head;
-                const uint32_t dst = ring + stage * P::kStageBytes;
-#pragma unroll 8
-                for (int i = tid; i < P::kN * kPieces; i += kCopiers) {
-                    const int r = i / kPieces, c = i % kPieces;
-                    if (c >= pieces) continue;
-                    const long long at = s.row[buf][r];
-                    const bool there = at >= 0 && c < filled;
-                    copy16(dst + piece(P::kN, r, c), there ? src + at + c * 16 : src, there);
+                if constexpr (kBoxes) {
+                    if (tid == 0) mbar_arrive_expect_tx(&s.full[stage], columns * P::kN * 128);
+#pragma unroll
+                    for (int x = 0; x < 2; ++x) {
+                        const int n = tid + x * kCopiers;
+                        if (n < P::kN && (n & (box - 1)) == 0)
+#pragma unroll 1
+                            for (int c = 0; c < columns; ++c)
+                                tma_load_4d(smem + P::kQBytes + stage * P::kStageBytes + c * (P::kN * 128) + n * 128,
+                                            v ? &maps.v : &maps.k, c * 64, row[x], head, page[x], &s.full[stage],
+                                            l2_policy_evict_normal());
+                    }
+                } else {
+                    const char *src = v ? v_head : k_head;
+                    const uint32_t dst = ring + stage * P::kStageBytes;
+#pragma unroll 4
+                    for (int i = tid; i < P::kN * kPieces; i += kCopiers) {
+                        const int r = i / kPieces, c = i % kPieces;
+                        if (c >= pieces) continue;
+                        const long long at = s.row[buf][r];
+                        const bool there = at >= 0 && c < filled;
+                        copy16(dst + piece(P::kN, r, c), src + (there ? at + c * 16 : 0), there);
+                    }
+                    arrive_behind_copies(&s.full[stage]);
                 }
-                emit(&s.full[stage]);
-                ++item;
+                if (++stage == P::kStages) stage = 0, ++use;
             }
             ++unit;
             if (u + 1 < f.u1) place(u + 1);
         }
-        cp_async_wait<0>();
-        fence_async_proxy();
-        if (older) mbar_arrive(older);
-        if (newer) mbar_arrive(newer);
-        older = newer = nullptr;
         ++fragments;
         st.left -= f.u1 - f.u0;
         if (st.left <= 0) break;
         skip = 0;
         next_tile<P::kM>(a, q, tile, head);
     }
+    cp_async_commit();
+    cp_async_wait<0>();
 }
 
-// The matrix products, issued by one thread. Of a unit j and tile i, in order:
+// The matrix products, issued by one warp's elected lane, always the same, while
+// all of it runs the loop (so that what it computes for them is uniform). Of a unit j and tile i, in order:
 // S_i = Q_i K^T into the columns where the weights of the unit before were, and
 // O_i += P_i V once the softmax has put the weights P_i over S_i. Products of
 // one thread run in the order of issue, so a tile's next scores cannot overtake
 // the use of its weights.
-template <typename T, int kDim>
+template <typename T, int kDim, bool kBoxes>
 __device__ __forceinline__ void products(const Args &a, Shared0 &s, char *smem, Stretch st, unsigned *status) {
     using P = Plan<kDim>;
-    constexpr bool kBf16 = sizeof(T) == 2 && !__is_same(T, __half);
+    constexpr bool kBf16 = !__is_same(T, __half);
+    constexpr int kRing = P::kStages - 1, kSteps = P::kN / 16, kMost = kSteps - 2;
     const int steps = (a.kv.head_dim + 15) / 16;
     const uint32_t score_desc = mma_desc(128, P::kN, kBf16, false), out_desc = mma_desc(128, steps * 16, kBf16, true);
-    const uint32_t q_at = smem_addr(smem), ring = q_at + P::kQBytes, tmem = s.tmem;
+    const uint32_t tmem = __shfl_sync(kFullMask, s.tmem, 0);
+    const uint32_t q_desc = smem_desc(smem_addr(smem), 16);
+    const uint32_t k_desc = smem_desc(smem_addr(smem) + P::kQBytes, 16);
+    const uint32_t v_desc = smem_desc(smem_addr(smem) + P::kQBytes, P::kN * 128);
     int item = 0, fragments = 0;       // copies taken (K, V, K, V ...)
-    int put[2] = {0, 0};               // weights taken per buffer
+    int put = 0;                       // weights taken, a parity per buffer
     Sequence q = sequence(a, st.b);
     int tile = st.tile, head = st.head, skip = st.skip;
-    Waiter wait{status};
+    const Waiter wait{status, &s.dead};
+    // descriptors count in 16 bytes: a step along a row of 128 bytes is 2, the next 64 columns lie a tile's rows further
+    const auto scores = [&](int i, int buf, int k_item, bool frees_k, bool frees_q) {
+        const int stage = k_item & kRing;
+        const uint32_t qa = q_desc + i * (128 * kDim * 2 / 16);
+        const uint32_t kb = __shfl_sync(kFullMask, k_desc + stage * (P::kStageBytes / 16), 0);
+        __syncwarp();
+        if (elect_one()) {
+            const auto step = [&](int x) {
+                mma_ss(tmem + P::scores(buf), qa + (x >> 2) * (128 * 8) + (x & 3) * 2, kb + (x >> 2) * (P::kN * 8) + (x & 3) * 2,
+                       score_desc, x > 0);
+            };
+            if (steps == kDim / 16) {
+#pragma unroll
+                for (int x = 0; x < kDim / 16; ++x) step(x);
+            } else {
+#pragma unroll 1
+                for (int x = 0; x < steps; ++x) step(x);
+            }
+            mma_commit(&s.s_full[buf]);
+            if (frees_k) mma_commit(&s.free[stage]);
+            if (frees_q) mma_commit(&s.q_free);
+        }
+        __syncwarp();
+    };
+    const auto outputs = [&](int i, int buf, int v_item, bool add, bool frees_v) {
+        const int stage = v_item & kRing;
+        const uint32_t vb = __shfl_sync(kFullMask, v_desc + stage * (P::kStageBytes / 16), 0);
+        wait(&s.p_most[buf], put >> buf);
+        tmem_fence_after();
+        __syncwarp();
+        if (elect_one()) {
+#pragma unroll
+            for (int x = 0; x < kMost; ++x)
+                mma_ts(tmem + P::output(i), tmem + P::weights(buf, x), vb + x * 128, out_desc, add || x > 0);
+        }
+        __syncwarp();
+        wait(&s.p_full[buf], put >> buf);
+        put ^= 1 << buf;
+        tmem_fence_after();
+        __syncwarp();
+        if (elect_one()) {
+#pragma unroll
+            for (int x = kMost; x < kSteps; ++x)
+                mma_ts(tmem + P::output(i), tmem + P::weights(buf, x), vb + x * 128, out_desc, true);
+            mma_commit(&s.o_done[i]);
+            if (frees_v) mma_commit(&s.free[stage]);
+        }
+        __syncwarp();
+    };
+    const auto wait_item = [&](int i) {
+        wait(&s.full[i & kRing], i / P::kStages);
+        if (!kBoxes) fence_async_proxy();
+    };
+    // (one place in the code for each kind of product: the loop has to stay in the instruction cache)
     for (;;) {
         const Fragment f = fragment<P::kM, P::kN>(a, q, tile, skip, st.left);
         const int units = f.u1 - f.u0, tiles = P::kTiles == 2 && f.rows - f.row0 > 128 ? 2 : 1;
-        const auto wait_item = [&](int i) { wait(&s.full[i % P::kStages], i / P::kStages); };
-        const auto scores = [&](int i, int buf, int k_item) {
-            const uint32_t qa = q_at + i * (128 * kDim * 2), kb = ring + (k_item % P::kStages) * P::kStageBytes;
-            for (int x = 0; x < steps; ++x)
-                mma_ss(tmem + P::scores(buf), smem_desc(qa + (x >> 2) * (128 * 128) + (x & 3) * 32, 16, 1024),
-                       smem_desc(kb + (x >> 2) * (P::kN * 128) + (x & 3) * 32, 16, 1024), score_desc, x > 0);
-            mma_commit(&s.s_full[buf]);
-        };
-        const auto outputs = [&](int i, int buf, int v_item, bool add) {
-            const uint32_t vb = ring + (v_item % P::kStages) * P::kStageBytes;
-#pragma unroll
-            for (int x = 0; x < P::kN / 16; ++x)
-                mma_ts(tmem + P::output(i), tmem + P::scores(buf) + x * 8, smem_desc(vb + x * 2048, P::kN * 128, 1024), out_desc,
-                       add || x > 0);
-            mma_commit(&s.o_done[i]);
-        };
         wait(&s.q_full, fragments);
-        wait_item(item);
-        tmem_fence_after();
-        for (int i = 0; i < tiles; ++i) scores(i, i, item);
-        mma_commit(&s.free[item % P::kStages]);
-        if (units == 1) mma_commit(&s.q_free);
-        for (int j = 0; j < units; ++j) {
-            const int k_next = item + 2 * j + 2, v_now = item + 2 * j + 1;
+        fence_async_proxy();
+#pragma unroll 1
+        for (int j = -1; j < units; ++j) {             // of unit j the outputs, of the next one the scores
             const bool more = j + 1 < units;
-            if (P::kTiles == 1 && more) {
-                wait_item(k_next);
-                tmem_fence_after();
-                scores(0, (j + 1) & 1, k_next);
-                mma_commit(&s.free[k_next % P::kStages]);
-                if (j + 2 == units) mma_commit(&s.q_free);
-            }
-            wait_item(v_now);
+            if (more) wait_item(item);
+            if (j >= 0) wait_item(item - 1);
+#pragma unroll 1
             for (int i = 0; i < tiles; ++i) {
-                const int buf = P::kTiles == 2 ? i : j & 1;
-                wait(&s.p_full[buf], put[buf]++);
-                tmem_fence_after();
-                outputs(i, buf, v_now, j > 0);
-                if (i == tiles - 1) mma_commit(&s.free[v_now % P::kStages]);
-                if (P::kTiles == 2 && more) {
-                    if (i == 0) {
-                        wait_item(k_next);
-                        tmem_fence_after();
-                    }
-                    scores(i, i, k_next);
-                    if (i == tiles - 1) {
-                        mma_commit(&s.free[k_next % P::kStages]);
-                        if (j + 2 == units) mma_commit(&s.q_free);
-                    }
-                }
+                const bool last = i == tiles - 1;
+                if (P::kTiles == 2 && j >= 0) outputs(i, i, item - 1, j > 0, last);
+                if (more) scores(i, P::kTiles == 2 ? i : (j + 1) & 1, item, last, last && j + 2 == units);
+                if (P::kTiles == 1 && j >= 0) outputs(0, j & 1, item - 1, j > 0, true);
             }
+            item += 2;
         }
-        item += 2 * units;
+        item -= 2;
         ++fragments;
         st.left -= units;
         if (st.left <= 0) break;
         skip = 0;
         next_tile<P::kM>(a, q, tile, head);
     }
-    mma_commit(&s.last);               // before the tensor memory is given back
+    if (elect_one()) mma_commit(&s.last);      // before the tensor memory is given back
+    __syncwarp();
     wait(&s.last, 0);
 }
 
 // The softmax of one tile's scores and its output, a row to a thread.
-template <typename T, int kDim>
+template <typename T, int kDim, bool kBoxes>
 __device__ __forceinline__ void softmax(const Args &a, Shared0 &s, char *smem, Stretch st, unsigned *status) {
     using P = Plan<kDim>;
-    const int wg = threadIdx.x >> 7, r = threadIdx.x & 127, lane = r & 31;
+    constexpr int kRing = P::kStages - 1, kWords = P::kN / 32;
+    const int i = threadIdx.x >> 7, r = threadIdx.x & 127, lane = r & 31;      // i: the tile
     const uint32_t lanes = s.tmem + (static_cast<uint32_t>(r >> 5) << 21);
     char *ring = smem + P::kQBytes;
     const int pieces = (a.kv.head_dim + 15) / 16 * 2;
     int unit = 0, item = 0, got[2] = {0, 0}, done = 0;     // units, copies, scores per buffer, outputs of this tile
     Sequence q = sequence(a, st.b);
     int tile = st.tile, head = st.head, skip = st.skip;
-    Waiter waiter{status};
-    const auto wait = [&](uint64_t *bar, int phase) {
-        waiter(bar, phase);
+    const Waiter wait{status, &s.dead};
+    const auto arrive = [&](uint64_t *bar) {
         __syncwarp();
+        if (lane == 0) mbar_arrive(bar);
     };
     for (;;) {
         const Fragment f = fragment<P::kM, P::kN>(a, q, tile, skip, st.left);
         const int tiles = P::kTiles == 2 && f.rows - f.row0 > 128 ? 2 : 1;
-        const long long row = f.row0 + wg * 128 + r;
-        const bool active = wg < tiles;
-        const int at = row < f.rows ? f.first + static_cast<int>(row / a.group) : -1;
+        const int row = f.row0 + i * 128 + r;
+        const bool active = i < tiles;
+        const int at = row < f.rows ? f.first + row / a.group : -1;
         float ref = -INFINITY, l = 0.0f;
         bool spoilt = false;           // some row has bits in s.bad
+        // Pages of the tile's slots that are not there are rare: looked for once, and only then per unit.
+        const int *table = a.kv.table + q.b * a.kv.table_stride;
+        const auto there_of = [&](int slot) {
+            return static_cast<unsigned>(table[static_cast<int>((slot * a.page_magic) >> 40)]) < static_cast<unsigned>(a.kv.n_pages);
+        };
+        bool gaps = false;
+        if (active) {
+            bool gap = false;
+            const int end = min(f.u1 * P::kN, q.length), last = static_cast<int>(((end - 1) * a.page_magic) >> 40);
+            if (end > 0)
+#pragma unroll 1
+                for (int c = static_cast<int>((f.u0 * P::kN * a.page_magic) >> 40) + r; c <= last; c += 128)
+                    gap |= static_cast<unsigned>(table[c]) >= static_cast<unsigned>(a.kv.n_pages);
+            gaps = any_of(5 + i, 128, gap);
+        }
         for (int u = f.u0; u < f.u1; ++u, ++unit, item += 2) {
-            const int mb = unit & 1;
-            wait(&s.mask_full[mb], unit >> 1);
-            uint32_t there[P::kN / 32];
-            uint32_t all = 0xffffffffu;
-#pragma unroll
-            for (int x = 0; x < P::kN / 32; ++x) all &= there[x] = s.mask[mb][x];
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&s.mask_free[mb]);
             if (!active) continue;
+            uint32_t there[kWords];
+#pragma unroll
+            for (int c = 0; c < kWords; ++c) {
+                there[c] = 0xffffffffu;
+                if (gaps) {
+                    const int slot = u * P::kN + c * 32 + lane;
+                    there[c] = __ballot_sync(kFullMask, slot < q.length && there_of(slot));
+                }
+            }
             const bool edge = (u + 1) * P::kN - 1 > f.last_all || u * P::kN < f.first_all;
             const int lo = a.window ? at - a.window + 1 - u * P::kN : 0, hi = at - u * P::kN;   // columns that this row sees
             if (edge) {
                 // A value that is not finite must not reach rows that do not see it, and 0 times it would: such values
                 // are taken out of the tile, and the rows that see them marked.
-                const int v_item = item + 1;
-                wait(&s.full[v_item % P::kStages], v_item / P::kStages);
-                char *v = ring + (v_item % P::kStages) * P::kStageBytes;
-                const int threads = tiles * 128, me = wg * 128 + r;
+                wait(&s.full[(item + 1) & kRing], (item + 1) / P::kStages);
+                char *v = ring + ((item + 1) & kRing) * P::kStageBytes;
+                // a barrier each for one tile and for two: where a stretch has one tile, the other's warps run ahead
+                const int threads = tiles * 128, scan = tiles == 2 ? 2 : 4, me = threadIdx.x, filled = q.length - u * P::kN;
                 bool bad = false;
-                for (int i = me; i < P::kN * (kDim / 8); i += threads) {
-                    const int n = i / (kDim / 8), c = i % (kDim / 8);
+#pragma unroll 1
+                for (int x = me; x < P::kN * (kDim / 8); x += threads) {
+                    const int n = x / (kDim / 8), c = x % (kDim / 8);
                     if (c >= pieces) continue;
-                    const uint4 w = *reinterpret_cast<const uint4 *>(v + piece(P::kN, n, c));
+                    uint4 *at_v = reinterpret_cast<uint4 *>(v + piece(P::kN, n, c));
+                    if (kBoxes && n >= filled) {       // rows of a page behind the last slot in use
+                        *at_v = make_uint4(0, 0, 0, 0);
+                        continue;
+                    }
+                    const uint4 w = *at_v;
                     bad |= not_finite(w.x, T()) || not_finite(w.y, T()) || not_finite(w.z, T()) || not_finite(w.w, T());
                 }
-                if (any_of(4, threads, bad)) {
+                if (kBoxes) fence_async_proxy();
+                if (any_of(scan, threads, bad)) {
+                    uint32_t *mine = s.bad[me];
                     if (!spoilt)
-                        for (int c = 0; c < 8; ++c) s.bad[me][c] = 0;
+                        for (int c = 0; c < 8; ++c) mine[c] = 0;
                     spoilt = true;
+#pragma unroll 1
                     for (int n = max(lo, 0); n <= min(hi, P::kN - 1); ++n)
+#pragma unroll 1
                         for (int c = 0; c < pieces * 4; ++c) {
                             const uint32_t w = *reinterpret_cast<const uint32_t *>(v + piece(P::kN, n, c >> 2) + (c & 3) * 4);
                             const uint32_t low = not_finite(w & 0xffffu, T()), high = not_finite(w & 0xffff0000u, T());
-                            s.bad[me][c >> 4] |= (low | high << 1) << (2 * (c & 15));
+                            mine[c >> 4] |= (low | high << 1) << (2 * (c & 15));
                         }
                     __syncwarp();
-                    named_sync(4, threads);
-                    for (int i = me; i < P::kN * (kDim / 8); i += threads) {
-                        const int n = i / (kDim / 8), c = i % (kDim / 8);
+                    named_sync(scan, threads);
+#pragma unroll 1
+                    for (int x = me; x < P::kN * (kDim / 8); x += threads) {
+                        const int n = x / (kDim / 8), c = x % (kDim / 8);
                         if (c >= pieces) continue;
                         uint4 *w = reinterpret_cast<uint4 *>(v + piece(P::kN, n, c));
                         *w = make_uint4(only_finite<T>(w->x), only_finite<T>(w->y), only_finite<T>(w->z), only_finite<T>(w->w));
                     }
                     fence_async_proxy();
+                    __syncwarp();
+                    named_sync(scan, threads);            // before either tile's product
                 }
                 __syncwarp();
             }
-            const int buf = P::kTiles == 2 ? wg : (u - f.u0) & 1;
+            const int buf = P::kTiles == 2 ? i : (u - f.u0) & 1;
             wait(&s.s_full[buf], got[buf]++);
+            __syncwarp();
             tmem_fence_after();
-            uint32_t x[P::kN / 32][32];
+            uint32_t x[kWords][32];
 #pragma unroll
-            for (int i = 0; i < P::kN / 32; ++i) tmem_load32(lanes + P::scores(buf) + i * 32, x[i]);
+            for (int c = 0; c < kWords; ++c) tmem_load32(lanes + P::scores(buf) + c * 32, x[c]);
             tmem_wait_load();
-            if (edge || all != 0xffffffffu) {
+            if (edge || gaps) {
 #pragma unroll
-                for (int i = 0; i < P::kN; ++i)
-                    if (i < lo || i > hi || !(there[i >> 5] >> (i & 31) & 1)) x[i >> 5][i & 31] = __float_as_uint(-INFINITY);
+                for (int k = 0; k < P::kN; ++k)
+                    if (k < lo || k > hi || !(there[k >> 5] >> (k & 31) & 1)) x[k >> 5][k & 31] = __float_as_uint(-INFINITY);
             }
             float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-            for (int i = 0; i < P::kN; ++i) top[i & 3] = fmaxf(top[i & 3], __uint_as_float(x[i >> 5][i & 31]));
-            const float m = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * a.scale;
+            for (int k = 0; k < P::kN; k += 2)
+                top[k >> 1 & 3] = max3(top[k >> 1 & 3], __uint_as_float(x[k >> 5][k & 31]), __uint_as_float(x[k >> 5][(k & 31) + 1]));
+            const float m = fmaxf(max3(top[0], top[1], top[2]), top[3]) * a.scale;
             if (__any_sync(kFullMask, m > ref + kSlack)) {
                 const float next = fmaxf(ref, m - kLead);
                 const float keep = next == ref ? 1.0f : ex2(ref - next);
                 ref = next;
                 l *= keep;
                 if (u > f.u0) {
-                    wait(&s.o_done[wg], done - 1);
+                    wait(&s.o_done[i], done - 1);
+                    __syncwarp();
                     tmem_fence_after();
 #pragma unroll 1
                     for (int c = 0; c < kDim; c += 32) {
                         uint32_t o[32];
-                        tmem_load32(lanes + P::output(wg) + c, o);
+                        tmem_load32(lanes + P::output(i) + c, o);
                         tmem_wait_load();
 #pragma unroll
-                        for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * keep);
-                        tmem_store32(lanes + P::output(wg) + c, o);
+                        for (int k = 0; k < 32; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * keep);
+                        tmem_store32(lanes + P::output(i) + c, o);
                     }
                 }
             }
             const float off = ref == -INFINITY ? 0.0f : -ref;
-            float sum[4] = {};
+            const Pair scale2 = pair(a.scale, a.scale), off2 = pair(off, off);
+            Pair sum[2] = {0, 0};
 #pragma unroll
-            for (int i = 0; i < P::kN / 64; ++i) {
-                uint32_t w[32];
+            for (int c = 0; c < kWords; ++c) {
+                uint32_t w[16];
 #pragma unroll
-                for (int k = 0; k < 32; ++k) {
-                    const int c = i * 64 + 2 * k;
-                    const float p0 = ex2(fmaf(__uint_as_float(x[c >> 5][c & 31]), a.scale, off));
-                    const float p1 = ex2(fmaf(__uint_as_float(x[(c + 1) >> 5][(c + 1) & 31]), a.scale, off));
-                    sum[(2 * k) & 3] += p0;
-                    sum[(2 * k + 1) & 3] += p1;
+                for (int k = 0; k < 16; ++k) {
+                    Pair p = fma2(pair(__uint_as_float(x[c][2 * k]), __uint_as_float(x[c][2 * k + 1])), scale2, off2);
+                    float p0, p1;
+                    if (k % 8 < kPolynomial) {
+                        p = exp2_of(p);
+                        split(p, p0, p1);
+                    } else {
+                        split(p, p0, p1);
+                        p0 = ex2(p0);
+                        p1 = ex2(p1);
+                        p = pair(p0, p1);
+                    }
+                    sum[k & 1] = add2(sum[k & 1], p);
                     w[k] = pack(p0, p1, T());
                 }
-                tmem_store32(lanes + P::scores(buf) + i * 32, w);
+                tmem_store16(lanes + P::weights(buf, 2 * c), w);
+                if (c >= kWords - 2) {                 // the products begin before the last weights are there
+                    tmem_wait_store();
+                    tmem_fence_before();
+                    arrive(c == kWords - 2 ? &s.p_most[buf] : &s.p_full[buf]);
+                }
             }
-            l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
-            tmem_wait_store();
-            tmem_fence_before();
-            mbar_arrive(&s.p_full[buf]);
+            float s0, s1;
+            split(add2(sum[0], sum[1]), s0, s1);
+            l += s0 + s1;
             ++done;
         }
         if (active) {
-            wait(&s.o_done[wg], done - 1);
+            // (scores of a single tile do not come behind the output of the unit before: a phase at a time)
+            if (P::kTiles == 1 && f.u1 - f.u0 > 1) wait(&s.o_done[i], done - 2);
+            wait(&s.o_done[i], done - 1);
+            __syncwarp();
             tmem_fence_after();
             const float inv = !f.whole ? 1.0f : l == 0.0f ? 0.0f : 1.0f / l;
-            const int token = static_cast<int>(row / a.group), h = head * a.group + static_cast<int>(row - static_cast<long long>(token) * a.group);
+            const int token = row / a.group, h = head * a.group + row - token * a.group;
             char *out = a.out + (q.from + token) * a.out_token + h * a.out_head;
             float *part = a.parts + (2ll * blockIdx.x + (skip == 0)) * part_floats(P::kM, kDim);
-            const int pr = wg * 128 + r;
+            const int pr = i * 128 + r;
 #pragma unroll 1
             for (int c = 0; c < kDim; c += 32) {
                 uint32_t o[32];
-                tmem_load32(lanes + P::output(wg) + c, o);
+                tmem_load32(lanes + P::output(i) + c, o);
                 tmem_wait_load();
                 if (row < f.rows) {
-    #pragma unroll
-                    for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * inv);
+#pragma unroll
+                    for (int k = 0; k < 32; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * inv);
                     if (spoilt) {
                         const uint32_t b = s.bad[pr][c >> 5];
-    #pragma unroll
-                        for (int i = 0; i < 32; ++i)
-                            if (b >> i & 1) o[i] = 0x7fffffffu;
+#pragma unroll
+                        for (int k = 0; k < 32; ++k)
+                            if (b >> k & 1) o[k] = 0x7fffffffu;
                     }
                     if (f.whole) {
-    #pragma unroll
-                        for (int i = 0; i < 32; i += 8) {
-                            if (c + i >= a.kv.head_dim) break;
+#pragma unroll
+                        for (int k = 0; k < 32; k += 8) {
+                            if (c + k >= a.kv.head_dim) break;
                             uint4 w;
-                            w.x = pack(__uint_as_float(o[i]), __uint_as_float(o[i + 1]), T());
-                            w.y = pack(__uint_as_float(o[i + 2]), __uint_as_float(o[i + 3]), T());
-                            w.z = pack(__uint_as_float(o[i + 4]), __uint_as_float(o[i + 5]), T());
-                            w.w = pack(__uint_as_float(o[i + 6]), __uint_as_float(o[i + 7]), T());
-                            *reinterpret_cast<uint4 *>(out + (c + i) * 2) = w;
+                            w.x = pack(__uint_as_float(o[k]), __uint_as_float(o[k + 1]), T());
+                            w.y = pack(__uint_as_float(o[k + 2]), __uint_as_float(o[k + 3]), T());
+                            w.z = pack(__uint_as_float(o[k + 4]), __uint_as_float(o[k + 5]), T());
+                            w.w = pack(__uint_as_float(o[k + 6]), __uint_as_float(o[k + 7]), T());
+                            *reinterpret_cast<uint4 *>(out + (c + k) * 2) = w;
                         }
                     } else {
-    #pragma unroll
-                        for (int i = 0; i < 32; i += 4)
-                            *reinterpret_cast<uint4 *>(part + pr * kDim + c + i) = make_uint4(o[i], o[i + 1], o[i + 2], o[i + 3]);
+#pragma unroll
+                        for (int k = 0; k < 32; k += 4)
+                            *reinterpret_cast<uint4 *>(part + pr * kDim + c + k) = make_uint4(o[k], o[k + 1], o[k + 2], o[k + 3]);
                     }
                 }
                 __syncwarp();
@@ -489,6 +639,7 @@ __device__ __forceinline__ void softmax(const Args &a, Shared0 &s, char *smem, S
                     a.lse[static_cast<long long>(q.from + token) * a.n_head + h] = (ref + log2f(l)) * kLn2;
                 }
             }
+            __syncwarp();
         }
         st.left -= f.u1 - f.u0;
         if (st.left <= 0) break;
@@ -497,8 +648,8 @@ __device__ __forceinline__ void softmax(const Args &a, Shared0 &s, char *smem, S
     }
 }
 
-template <typename T, int kDim>
-__global__ void __launch_bounds__(kThreads, 1) mma_kernel(const Args a) {
+template <typename T, int kDim, bool kBoxes>
+__global__ void __launch_bounds__(kThreads, 1) mma_kernel(const Args a, const __grid_constant__ Maps maps, int box) {
     using P = Plan<kDim>;
     extern __shared__ char smem_raw[];
     __shared__ Shared0 s;
@@ -506,21 +657,21 @@ __global__ void __launch_bounds__(kThreads, 1) mma_kernel(const Args a) {
     const int tid = threadIdx.x, warp = tid >> 5;
     pdl_launch_dependents();
     if (tid == 0) {
-        for (int i = 0; i < P::kStages; ++i) mbar_init(&s.full[i], kCopiers), mbar_init(&s.free[i], 1);
+        for (int i = 0; i < P::kStages; ++i) mbar_init(&s.full[i], kBoxes ? 1 : kCopiers), mbar_init(&s.free[i], 1);
         mbar_init(&s.q_full, kCopiers);
         mbar_init(&s.q_free, 1);
         mbar_init(&s.last, 1);
+        s.dead = 0;
         for (int i = 0; i < 2; ++i) {
             mbar_init(&s.s_full[i], 1);
-            mbar_init(&s.p_full[i], 128);
+            mbar_init(&s.p_most[i], 4);
+            mbar_init(&s.p_full[i], 4);
             mbar_init(&s.o_done[i], 1);
-            mbar_init(&s.mask_full[i], 1);
-            mbar_init(&s.mask_free[i], 4 * P::kTiles);
         }
         fence_mbar_init();
         a.joints[blockIdx.x].first = -1;
     }
-    if (warp == 8) tmem_alloc(&s.tmem, kColumns);
+    if (warp == kThreads / 32 - 1) tmem_alloc(&s.tmem, kColumns);
     const Stretch st = find<P::kM, P::kN, kThreads>(a, reinterpret_cast<Shared<kThreads> *>(smem));
     tmem_fence_before();
     __syncthreads();
@@ -530,30 +681,68 @@ __global__ void __launch_bounds__(kThreads, 1) mma_kernel(const Args a) {
             const Sequence q = sequence(a, st.b);
             a.joints[blockIdx.x] = Joint{st.first, st.last, q.from, q.n, st.tile, st.head};
         }
-        if (warp < 8) {
-            asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
-            if (warp < 4 * P::kTiles) softmax<T, kDim>(a, s, smem, st, a.status);
+        if (warp < kSoftmaxThreads / 32) {
+            asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftmaxRegs));
+            if (warp < 4 * P::kTiles) softmax<T, kDim, kBoxes>(a, s, smem, st, a.status);
         } else {
-            asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
-            if (warp > 8) copier<T, kDim>(a, s, smem, st, a.status);
-            else if ((tid & 31) == 0) products<T, kDim>(a, s, smem, st, a.status);
+            asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegs));
+            if (warp == kThreads / 32 - 1) products<T, kDim, kBoxes>(a, s, smem, st, a.status);
+            else copier<T, kDim, kBoxes>(a, maps, box, s, smem, st, a.status);
             __syncwarp();
         }
     }
     tmem_fence_before();
     __syncthreads();
     tmem_fence_after();
-    if (warp == 8) tmem_free(s.tmem, kColumns);
+    if (warp == kThreads / 32 - 1) tmem_free(s.tmem, kColumns);
+}
+
+// Rows of a page to a tensor copy: the largest power of two that divides the
+// page and, with it, every place where a tile's slots change the page.
+int box_of(const KvView &kv, int most) {
+    const int n = kv.page_size & -kv.page_size;
+    return n < most ? n : most;
+}
+
+// A cache's rows as the tensor copies see them: [page][head][row][column].
+bool map_rows(CUtensorMap *map, const char *rows, const KvView &kv, bool bf16, int box) {
+    using Encode = CUresult (*)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *, const cuuint64_t *,
+                                const cuuint32_t *, const cuuint32_t *, CUtensorMapInterleave, CUtensorMapSwizzle,
+                                CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+    const Encode encode = reinterpret_cast<Encode>(tensor_map_encoder());
+    if (!encode) return false;
+    const cuuint64_t dims[4] = {static_cast<cuuint64_t>(kv.head_dim), static_cast<cuuint64_t>(kv.page_size),
+                                static_cast<cuuint64_t>(kv.n_head_kv), static_cast<cuuint64_t>(kv.n_pages)};
+    cuuint64_t strides[3] = {static_cast<cuuint64_t>(kv.row_stride), static_cast<cuuint64_t>(kv.head_stride),
+                             static_cast<cuuint64_t>(kv.page_stride)};
+    for (int i = 0; i < 3; ++i) {
+        if (dims[i + 1] == 1) strides[i] = static_cast<cuuint64_t>(kv.head_dim + 7) / 8 * 16;   // not used
+        if (strides[i] == 0 || strides[i] >= 1ull << 40) return false;
+    }
+    const cuuint32_t boxes[4] = {64, static_cast<cuuint32_t>(box), 1, 1}, steps[4] = {1, 1, 1, 1};
+    return encode(map, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4, const_cast<char *>(rows), dims,
+                  strides, boxes, steps, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                  CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+template <typename T, int kDim, bool kBoxes>
+cudaError_t launch(const Args &a, const Maps &maps, int box, cudaStream_t stream) {
+    const auto fn = mma_kernel<T, kDim, kBoxes>;
+    const int grid = sm_count();
+    if (!ensure_smem(reinterpret_cast<const void *>(fn), Plan<kDim>::kSmem)) return cudaGetLastError();
+    fn<<<grid, kThreads, Plan<kDim>::kSmem, stream>>>(a, maps, box);
+    const cudaError_t e = cudaGetLastError();
+    return e != cudaSuccess ? e : launch_join<T, Plan<kDim>::kM, kDim>(a, grid, stream);
 }
 
 template <typename T, int kDim>
 cudaError_t launch(const Args &a, cudaStream_t stream) {
-    const auto fn = mma_kernel<T, kDim>;
-    const int grid = sm_count();
-    if (!ensure_smem(reinterpret_cast<const void *>(fn), Plan<kDim>::kSmem)) return cudaGetLastError();
-    fn<<<grid, kThreads, Plan<kDim>::kSmem, stream>>>(a);
-    const cudaError_t e = cudaGetLastError();
-    return e != cudaSuccess ? e : launch_join<T, Plan<kDim>::kM, kDim>(a, grid, stream);
+    Maps maps{};
+    const int box = box_of(a.kv, Plan<kDim>::kN);
+    const bool bf16 = !__is_same(T, __half);
+    if (box >= kLeastBox && map_rows(&maps.k, a.kv.k, a.kv, bf16, box) && map_rows(&maps.v, a.kv.v, a.kv, bf16, box))
+        return launch<T, kDim, true>(a, maps, box, stream);
+    return launch<T, kDim, false>(a, maps, 0, stream);
 }
 
 template <typename T>

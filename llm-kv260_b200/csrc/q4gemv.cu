@@ -375,6 +375,12 @@ EncodeTiledFn encode_tiled() {
     return fn;
 }
 
+}  // namespace
+
+void *tensor_map_encoder() { return reinterpret_cast<void *>(encode_tiled()); }
+
+namespace {
+
 // The weight view the kernel streams: [chunk][row][byte of chunk] (ROWS), or
 // [chunk][pair][member][byte of chunk] (PAIRS), box = 32 rows x cps chunks,
 // landing in shared memory as [cps][32][144].

@@ -36,13 +36,13 @@ __device__ __forceinline__ void mma_commit(uint64_t *bar) {
 __device__ __forceinline__ void fence_async_proxy() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 
 // A tile in shared memory as the tensor cores see it: rows of 128 bytes, their
-// 16-byte pieces xor-ed with the row's number modulo 8. Where the contraction
-// runs along a row, `stride` is the distance of 8 rows and `lead` is unused;
-// where it runs down the rows, `lead` is the distance of 64 columns.
-__device__ __forceinline__ uint64_t smem_desc(uint32_t at, uint32_t lead, uint32_t stride) {
-    return static_cast<uint64_t>((at >> 4) & 0x3fff) | static_cast<uint64_t>((lead >> 4) & 0x3fff) << 16 |
-           static_cast<uint64_t>((stride >> 4) & 0x3fff) << 32 | 1ull << 46 | 2ull << 61;
-}
+// 16-byte pieces xor-ed with the row's number modulo 8, 1024 bytes from 8 rows
+// to the next. Where the contraction runs along a row, `lead` is unused; where
+// it runs down the rows, it is the distance of 64 columns. This is the lower
+// half of the descriptor, whose addresses count in 16 bytes; the upper half is
+// the same for all.
+__device__ __forceinline__ uint32_t smem_desc(uint32_t at, uint32_t lead) { return (at >> 4 & 0x3fff) | (lead >> 4 & 0x3fff) << 16; }
+constexpr uint32_t kDescHigh = 1024 >> 4 | 1u << 14 | 2u << 29;
 
 // M x N products of f16 or bf16 operands into float32; b_down: the contraction
 // runs down the rows of B.
@@ -52,18 +52,18 @@ __host__ __device__ constexpr uint32_t mma_desc(int m, int n, bool bf16, bool b_
 }
 
 // D (tensor memory) = A B, plus D where `add`: A in shared memory, or in tensor memory.
-__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t desc, bool add) {
+__device__ __forceinline__ void mma_ss(uint32_t d, uint32_t a, uint32_t b, uint32_t desc, bool add) {
     asm volatile(
-        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
-        "l"(a), "l"(b), "r"(desc), "r"(static_cast<uint32_t>(add))
+        "{\n\t.reg .pred p;\n\t.reg .b64 a, b;\n\tsetp.ne.b32 p, %4, 0;\n\tmov.b64 a, {%1, %5};\n\tmov.b64 b, {%2, %5};\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %3, p;\n\t}" ::"r"(d),
+        "r"(a), "r"(b), "r"(desc), "r"(static_cast<uint32_t>(add)), "n"(kDescHigh)
         : "memory");
 }
-__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t desc, bool add) {
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint32_t b, uint32_t desc, bool add) {
     asm volatile(
-        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
-        "r"(a), "l"(b), "r"(desc), "r"(static_cast<uint32_t>(add))
+        "{\n\t.reg .pred p;\n\t.reg .b64 b;\n\tsetp.ne.b32 p, %4, 0;\n\tmov.b64 b, {%2, %5};\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], b, %3, p;\n\t}" ::"r"(d),
+        "r"(a), "r"(b), "r"(desc), "r"(static_cast<uint32_t>(add)), "n"(kDescHigh)
         : "memory");
 }
 
@@ -90,6 +90,31 @@ __device__ __forceinline__ void tmem_store32(uint32_t at, const uint32_t (&v)[32
           "r"(v[24]), "r"(v[25]), "r"(v[26]), "r"(v[27]), "r"(v[28]), "r"(v[29]), "r"(v[30]), "r"(v[31]),
           "r"(at)
         : "memory");
+}
+// The same for 16 columns.
+__device__ __forceinline__ void tmem_store16(uint32_t at, const uint32_t (&v)[16]) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%16], "
+        "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15};" ::
+          "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]),
+          "r"(v[8]), "r"(v[9]), "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15]),
+          "r"(at)
+        : "memory");
+}
+
+// And for 8.
+__device__ __forceinline__ void tmem_store8(uint32_t at, const uint32_t (&v)[8]) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x8.b32 [%8], {%0, %1, %2, %3, %4, %5, %6, %7};" ::"r"(v[0]), "r"(v[1]), "r"(v[2]),
+        "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(at)
+        : "memory");
+}
+
+// True in one lane of a converged warp.
+__device__ __forceinline__ bool elect_one() {
+    uint32_t r;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(r));
+    return r != 0;
 }
 
 }  // namespace b200

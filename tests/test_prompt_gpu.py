@@ -272,6 +272,16 @@ def test_chunk_many_tiles(torch_mod, pkg, eng):
             assert ((c["out"][r].double() - want).abs() <= tol).all(), r
 
 
+@pytest.mark.parametrize("q,kv", TYPES)
+@pytest.mark.parametrize("d,window", [(64, 0), (128, 0), (128, 90), (256, 0)])
+def test_chunk_short_and_long_in_turn(torch_mod, pkg, eng, q, kv, d, window):
+    """Single tokens beside chunks of several tiles, so that a CTA has one after another of both kinds."""
+    new = [1, 150, 3, 70, 1, 1, 260, 2] * 5
+    old = [int(x) for x in np.random.default_rng(14).integers(0, 700, len(new))]
+    c = chunk_case(torch_mod, pkg, new, old, 32, 8, d, 16, q, kv, seed=14, garbage=math.nan)
+    chunk_run(torch_mod, eng, c, window=window)
+
+
 def test_chunk_equals_single_tokens(torch_mod, pkg, eng):
     """Chunks of one token are kv_attend's call."""
     torch = torch_mod
