@@ -2,6 +2,8 @@
 #include <cuda.h>
 #include <cuda_runtime.h>
 
+#include <type_traits>
+
 #include "kv_chunk.cuh"
 #include "tcgen05.cuh"
 
@@ -17,21 +19,19 @@ constexpr int kSoftmaxThreads = 256, kCopiers = 96, kThreads = kSoftmaxThreads +
 constexpr int kSoftmaxRegs = 208, kOtherRegs = 88;
 static_assert(kSoftmaxThreads * kSoftmaxRegs + 128 * kOtherRegs <= kThreads * 168);
 constexpr int kLeastBox = 8;           // rows of a page that one tensor copy brings at least
-constexpr int kColumns = 512;          // of tensor memory
+constexpr int kColumns = 512;          // of tensor memory: all, so that it begins at address 0
 // The reference m trails the maximum by 7 to 15 powers of two: weights stay in
 // 2^15 and below, float16's range, and those of 2^-21 of the largest are still
 // normal numbers there.
 constexpr float kLead = 7.0f, kSlack = 15.0f;
-// Of 8 pairs of weights, how many are computed on the float32 units.
-constexpr int kPolynomial = 0;
 
 template <int kDim>
 struct Plan {
     static constexpr int kTiles = kDim <= 128 ? 2 : 1;     // of 128 rows
     static constexpr int kM = 128 * kTiles, kN = kDim <= 128 ? 128 : 64;
-    static constexpr int kStages = kDim <= 64 ? 8 : 4;     // a power of two
+    static constexpr int kStages = 4;                      // keys and values of two units
     static constexpr int kQBytes = kM * kDim * 2, kStageBytes = kN * kDim * 2;
-    static constexpr int kSmem = 1024 + kQBytes + kStages * kStageBytes;
+    static constexpr int kSmem = kQBytes + kStages * kStageBytes;
     // columns of tensor memory: scores (and, over them, weights) per tile, or twice of one, then the outputs
     __device__ static constexpr int scores(int i) { return i * kN; }
     // the weights of 16 slots, two to a column
@@ -40,7 +40,7 @@ struct Plan {
 };
 
 struct Shared0 {
-    uint64_t full[8], free[8], q_full, q_free, s_full[2], p_most[2], p_full[2], o_done[2], last;
+    uint64_t full[4], free[4], q_full, q_free, s_full[2], p_most[2], p_full[2], o_done[2], last;
     uint32_t tmem;
     int dead;                          // a wait ran out
     long long row[2][128];             // byte offsets of a unit's rows, -1: not there
@@ -80,29 +80,6 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
     float d;
     asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
     return d;
-}
-
-// 2^t of two numbers t <= 64 without the special-function unit: t = n + f with n
-// the nearest whole number, 2^f by a polynomial of least relative error on
-// [-1/2, 1/2] (found by Remez' exchange: 2.6e-6, an eightieth of half a step of
-// float16), times 2^n, whose bits are those of t + 1.5 * 2^23 + 127 moved up.
-// Below 2^-126 the result is 0 (n = -127 has no exponent bits), NaN stays NaN.
-__device__ __forceinline__ Pair exp2_of(Pair t) {
-    float t0, t1;
-    split(t, t0, t1);
-    asm("max.NaN.f32 %0, %0, 0fC2FE0000;" : "+f"(t0));     // -127
-    asm("max.NaN.f32 %0, %0, 0fC2FE0000;" : "+f"(t1));
-    t = pair(t0, t1);
-    const float magic = 12582912.0f + 127.0f;
-    const Pair n = add2(t, pair(magic, magic));
-    const Pair f = fma2(add2(n, pair(-magic, -magic)), pair(-1.0f, -1.0f), t);
-    Pair y = fma2(f, pair(0.009570102f, 0.009570102f), pair(0.05591786f, 0.05591786f));
-    y = fma2(f, y, pair(0.24024745f, 0.24024745f));
-    y = fma2(f, y, pair(0.6931218f, 0.6931218f));
-    y = fma2(f, y, pair(0.99999926f, 0.99999926f));
-    float n0, n1;
-    split(n, n0, n1);
-    return mul2(y, pair(__uint_as_float(__float_as_uint(n0) << 23), __uint_as_float(__float_as_uint(n1) << 23)));
 }
 
 __device__ __forceinline__ uint32_t pack(float lo, float hi, __half) {
@@ -214,6 +191,10 @@ __device__ __forceinline__ void copier(const Args &a, const Maps &maps, int box,
     const int tid = threadIdx.x - kSoftmaxThreads;
     const int pieces = (a.kv.head_dim + 15) / 16 * 2, filled = a.kv.head_dim / 8, columns = (a.kv.head_dim + 63) / 64;
     const uint32_t q_at = smem_addr(smem), ring = q_at + P::kQBytes;
+    // Who waits for a stage has to be who fills it: a barrier tells one phase from the next one only, and comes to the one
+    // after that without a thread that brings nothing.
+    bool issues = !kBoxes || tid == 0;
+    for (int n = tid; n < P::kN; n += kCopiers) issues |= kBoxes && (n & (box - 1)) == 0;
     int stage = 0, use = 0, unit = 0, fragments = 0;
     Sequence q = sequence(a, st.b);
     int tile = st.tile, head = st.head, skip = st.skip;
@@ -264,7 +245,7 @@ __device__ __forceinline__ void copier(const Args &a, const Maps &maps, int box,
             if (u + 1 < f.u1) ask(u + 1);
 #pragma unroll 1
             for (int v = 0; v < 2; ++v) {
-                if (use) wait(&s.free[stage], use - 1);
+                if (use && issues) wait(&s.free[stage], use - 1);
                 if constexpr (kBoxes) {
                     if (tid == 0) mbar_arrive_expect_tx(&s.full[stage], columns * P::kN * 128);
 #pragma unroll
@@ -305,111 +286,136 @@ __device__ __forceinline__ void copier(const Args &a, const Maps &maps, int box,
     cp_async_wait<0>();
 }
 
-// The matrix products, issued by one warp's elected lane, always the same, while
-// all of it runs the loop (so that what it computes for them is uniform). Of a unit j and tile i, in order:
-// S_i = Q_i K^T into the columns where the weights of the unit before were, and
-// O_i += P_i V once the softmax has put the weights P_i over S_i. Products of
-// one thread run in the order of issue, so a tile's next scores cannot overtake
-// the use of its weights.
+// The matrix products, issued by one warp's elected lane while all of it runs
+// the loop. Of a unit j and tile i, in order: O_i += P_i V once the softmax has
+// put the weights P_i over the scores, and S_i = Q_i K^T of the next unit into
+// the same columns. Products of one thread run in the order of issue, so a
+// tile's next scores cannot overtake the use of its weights. (A single tile has
+// two buffers of scores, and its next ones come first.) The loop's body exists
+// for even and odd units, in which all operands are constants: descriptors that
+// have to be computed cost 90 cycles for a product that takes 64.
 template <typename T, int kDim, bool kBoxes>
 __device__ __forceinline__ void products(const Args &a, Shared0 &s, char *smem, Stretch st, unsigned *status) {
     using P = Plan<kDim>;
     constexpr bool kBf16 = !__is_same(T, __half);
-    constexpr int kRing = P::kStages - 1, kSteps = P::kN / 16, kMost = kSteps - 2;
+    constexpr int kSteps = P::kN / 16, kMost = kSteps - 2;
     const int steps = (a.kv.head_dim + 15) / 16;
-    const uint32_t score_desc = mma_desc(128, P::kN, kBf16, false), out_desc = mma_desc(128, steps * 16, kBf16, true);
-    const uint32_t tmem = __shfl_sync(kFullMask, s.tmem, 0);
-    const uint32_t q_desc = smem_desc(smem_addr(smem), 16);
-    const uint32_t k_desc = smem_desc(smem_addr(smem) + P::kQBytes, 16);
-    const uint32_t v_desc = smem_desc(smem_addr(smem) + P::kQBytes, P::kN * 128);
-    int item = 0, fragments = 0;       // copies taken (K, V, K, V ...)
-    int put = 0;                       // weights taken, a parity per buffer
+    const uint32_t out_desc = mma_desc(128, steps * 16, kBf16, true);
+    const bool lead = elect_one();
+    int unit = 0, fragments = 0, used = 0;             // used: weights of a tile taken, a parity each
     Sequence q = sequence(a, st.b);
     int tile = st.tile, head = st.head, skip = st.skip;
     const Waiter wait{status, &s.dead};
-    // descriptors count in 16 bytes: a step along a row of 128 bytes is 2, the next 64 columns lie a tile's rows further
-    const auto scores = [&](int i, int buf, int k_item, bool frees_k, bool frees_q) {
-        const int stage = k_item & kRing;
-        const uint32_t qa = q_desc + i * (128 * kDim * 2 / 16);
-        const uint32_t kb = __shfl_sync(kFullMask, k_desc + stage * (P::kStageBytes / 16), 0);
+    const auto wait_copy = [&](int stage, int phase) {
+        wait(&s.full[stage], phase);
         __syncwarp();
-        if (elect_one()) {
-            const auto step = [&](int x) {
-                mma_ss(tmem + P::scores(buf), qa + (x >> 2) * (128 * 8) + (x & 3) * 2, kb + (x >> 2) * (P::kN * 8) + (x & 3) * 2,
-                       score_desc, x > 0);
-            };
-            if (steps == kDim / 16) {
-#pragma unroll
-                for (int x = 0; x < kDim / 16; ++x) step(x);
-            } else {
-#pragma unroll 1
-                for (int x = 0; x < steps; ++x) step(x);
-            }
-            mma_commit(&s.s_full[buf]);
-            if (frees_k) mma_commit(&s.free[stage]);
-            if (frees_q) mma_commit(&s.q_free);
-        }
-        __syncwarp();
-    };
-    const auto outputs = [&](int i, int buf, int v_item, bool add, bool frees_v) {
-        const int stage = v_item & kRing;
-        const uint32_t vb = __shfl_sync(kFullMask, v_desc + stage * (P::kStageBytes / 16), 0);
-        wait(&s.p_most[buf], put >> buf);
-        tmem_fence_after();
-        __syncwarp();
-        if (elect_one()) {
-#pragma unroll
-            for (int x = 0; x < kMost; ++x)
-                mma_ts(tmem + P::output(i), tmem + P::weights(buf, x), vb + x * 128, out_desc, add || x > 0);
-        }
-        __syncwarp();
-        wait(&s.p_full[buf], put >> buf);
-        put ^= 1 << buf;
-        tmem_fence_after();
-        __syncwarp();
-        if (elect_one()) {
-#pragma unroll
-            for (int x = kMost; x < kSteps; ++x)
-                mma_ts(tmem + P::output(i), tmem + P::weights(buf, x), vb + x * 128, out_desc, true);
-            mma_commit(&s.o_done[i]);
-            if (frees_v) mma_commit(&s.free[stage]);
-        }
-        __syncwarp();
-    };
-    const auto wait_item = [&](int i) {
-        wait(&s.full[i & kRing], i / P::kStages);
         if (!kBoxes) fence_async_proxy();
     };
-    // (one place in the code for each kind of product: the loop has to stay in the instruction cache)
+    // descriptors count in 16 bytes: a step along a row of 128 bytes is 2, the next 64 columns lie a tile's rows further
+    const auto scores = [&](auto parity, auto tile_of) {
+        constexpr int kG = decltype(parity)::value, kI = decltype(tile_of)::value, kBuf = P::kTiles == 2 ? kI : kG;
+        const uint32_t qa = smem_desc(smem_addr(smem) + kI * (128 * kDim * 2), 16);
+        const uint32_t kb = smem_desc(smem_addr(smem) + P::kQBytes + 2 * kG * P::kStageBytes, 16);
+        const auto step = [&](int x) {
+            mma_ss(P::scores(kBuf), qa + (x >> 2) * (128 * 8) + (x & 3) * 2, kb + (x >> 2) * (P::kN * 8) + (x & 3) * 2,
+                   mma_desc(128, P::kN, kBf16, false), x > 0);
+        };
+        if (steps == kDim / 16) {
+#pragma unroll
+            for (int x = 0; x < kDim / 16; ++x) step(x);
+        } else {
+#pragma unroll 1
+            for (int x = 0; x < steps; ++x) step(x);
+        }
+        mma_commit(&s.s_full[kBuf]);
+    };
+    const auto outputs = [&](auto parity, auto tile_of, int from, int to, bool add) {
+        constexpr int kG = decltype(parity)::value, kI = decltype(tile_of)::value, kBuf = P::kTiles == 2 ? kI : kG;
+        const uint32_t vb = smem_desc(smem_addr(smem) + P::kQBytes + (2 * kG + 1) * P::kStageBytes, P::kN * 128);
+#pragma unroll
+        for (int x = 0; x < kSteps; ++x)
+            if (x >= from && x < to) mma_ts(P::output(kI), P::weights(kBuf, x), vb + x * 128, out_desc, add || x > 0);
+    };
+    const auto body = [&](auto parity, int tiles, bool add, bool more, bool last_scores) {
+        constexpr int kG = decltype(parity)::value;
+        using Next = std::integral_constant<int, 1 - kG>;
+        const auto tile_body = [&](auto tile_of) {
+            constexpr int kI = decltype(tile_of)::value, kBuf = P::kTiles == 2 ? kI : kG;
+            const int phase = P::kTiles == 2 ? used >> kI : unit >> 1;
+            const bool ends = kI == tiles - 1;
+            wait(&s.p_most[kBuf], phase);
+            __syncwarp();
+            tmem_fence_after();
+            if (lead) outputs(parity, tile_of, 0, kMost, add);
+            __syncwarp();
+            if (P::kTiles == 2 && kI == 0 && more) wait_copy(2 * Next::value, (unit + 1) >> 1);
+            wait(&s.p_full[kBuf], phase);
+            __syncwarp();
+            tmem_fence_after();
+            if (lead) {
+                outputs(parity, tile_of, kMost, kSteps, true);
+                mma_commit(&s.o_done[kI]);
+                if (P::kTiles == 2 && more) scores(Next{}, tile_of);
+                if (ends) mma_commit(&s.free[2 * kG + 1]);
+                if (P::kTiles == 2 && more && ends) {
+                    mma_commit(&s.free[2 * Next::value]);
+                    if (last_scores) mma_commit(&s.q_free);
+                }
+            }
+            __syncwarp();
+            used ^= 1 << kI;
+        };
+        if (P::kTiles == 1 && more) {
+            wait_copy(2 * Next::value, (unit + 1) >> 1);
+            if (lead) {
+                scores(Next{}, std::integral_constant<int, 0>{});
+                mma_commit(&s.free[2 * Next::value]);
+                if (last_scores) mma_commit(&s.q_free);
+            }
+            __syncwarp();
+        }
+        wait_copy(2 * kG + 1, unit >> 1);
+        tile_body(std::integral_constant<int, 0>{});
+        if constexpr (P::kTiles == 2)
+            if (tiles == 2) tile_body(std::integral_constant<int, 1>{});
+    };
+    const auto begin = [&](auto parity, int tiles, bool last_scores) {
+        constexpr int kG = decltype(parity)::value;
+        wait_copy(2 * kG, unit >> 1);
+        if (lead) {
+            scores(parity, std::integral_constant<int, 0>{});
+            if constexpr (P::kTiles == 2)
+                if (tiles == 2) scores(parity, std::integral_constant<int, 1>{});
+            mma_commit(&s.free[2 * kG]);
+            if (last_scores) mma_commit(&s.q_free);
+        }
+        __syncwarp();
+    };
+    using Even = std::integral_constant<int, 0>;
+    using Odd = std::integral_constant<int, 1>;
     for (;;) {
         const Fragment f = fragment<P::kM, P::kN>(a, q, tile, skip, st.left);
         const int units = f.u1 - f.u0, tiles = P::kTiles == 2 && f.rows - f.row0 > 128 ? 2 : 1;
         wait(&s.q_full, fragments);
+        __syncwarp();
         fence_async_proxy();
+        if (unit & 1) begin(Odd{}, tiles, units == 1);
+        else begin(Even{}, tiles, units == 1);
 #pragma unroll 1
-        for (int j = -1; j < units; ++j) {             // of unit j the outputs, of the next one the scores
-            const bool more = j + 1 < units;
-            if (more) wait_item(item);
-            if (j >= 0) wait_item(item - 1);
-#pragma unroll 1
-            for (int i = 0; i < tiles; ++i) {
-                const bool last = i == tiles - 1;
-                if (P::kTiles == 2 && j >= 0) outputs(i, i, item - 1, j > 0, last);
-                if (more) scores(i, P::kTiles == 2 ? i : (j + 1) & 1, item, last, last && j + 2 == units);
-                if (P::kTiles == 1 && j >= 0) outputs(0, j & 1, item - 1, j > 0, true);
-            }
-            item += 2;
+        for (int j = 0; j < units; ++j, ++unit) {
+            if (unit & 1) body(Odd{}, tiles, j > 0, j + 1 < units, j + 2 == units);
+            else body(Even{}, tiles, j > 0, j + 1 < units, j + 2 == units);
         }
-        item -= 2;
         ++fragments;
         st.left -= units;
         if (st.left <= 0) break;
         skip = 0;
         next_tile<P::kM>(a, q, tile, head);
     }
-    if (elect_one()) mma_commit(&s.last);      // before the tensor memory is given back
+    if (lead) mma_commit(&s.last);     // before the tensor memory is given back
     __syncwarp();
     wait(&s.last, 0);
+    __syncwarp();
 }
 
 // The softmax of one tile's scores and its output, a row to a thread.
@@ -418,10 +424,10 @@ __device__ __forceinline__ void softmax(const Args &a, Shared0 &s, char *smem, S
     using P = Plan<kDim>;
     constexpr int kRing = P::kStages - 1, kWords = P::kN / 32;
     const int i = threadIdx.x >> 7, r = threadIdx.x & 127, lane = r & 31;      // i: the tile
-    const uint32_t lanes = s.tmem + (static_cast<uint32_t>(r >> 5) << 21);
+    const uint32_t lanes = static_cast<uint32_t>(r >> 5) << 21;
     char *ring = smem + P::kQBytes;
     const int pieces = (a.kv.head_dim + 15) / 16 * 2;
-    int unit = 0, item = 0, got[2] = {0, 0}, done = 0;     // units, copies, scores per buffer, outputs of this tile
+    int unit = 0, item = 0, done = 0;  // units, copies, units of this tile
     Sequence q = sequence(a, st.b);
     int tile = st.tile, head = st.head, skip = st.skip;
     const Waiter wait{status, &s.dead};
@@ -465,9 +471,14 @@ __device__ __forceinline__ void softmax(const Args &a, Shared0 &s, char *smem, S
             }
             const bool edge = (u + 1) * P::kN - 1 > f.last_all || u * P::kN < f.first_all;
             const int lo = a.window ? at - a.window + 1 - u * P::kN : 0, hi = at - u * P::kN;   // columns that this row sees
+            const int buf = P::kTiles == 2 ? i : unit & 1;
+            wait(&s.s_full[buf], P::kTiles == 2 ? done : unit >> 1);
+            __syncwarp();
+            tmem_fence_after();
             if (edge) {
                 // A value that is not finite must not reach rows that do not see it, and 0 times it would: such values
-                // are taken out of the tile, and the rows that see them marked.
+                // are taken out of the tile, and the rows that see them marked. (The scores are there, so the values of
+                // two units before were: a phase ahead at most, which is what a barrier can tell.)
                 wait(&s.full[(item + 1) & kRing], (item + 1) / P::kStages);
                 char *v = ring + ((item + 1) & kRing) * P::kStageBytes;
                 // a barrier each for one tile and for two: where a stretch has one tile, the other's warps run ahead
@@ -514,10 +525,6 @@ __device__ __forceinline__ void softmax(const Args &a, Shared0 &s, char *smem, S
                 }
                 __syncwarp();
             }
-            const int buf = P::kTiles == 2 ? i : (u - f.u0) & 1;
-            wait(&s.s_full[buf], got[buf]++);
-            __syncwarp();
-            tmem_fence_after();
             uint32_t x[kWords][32];
 #pragma unroll
             for (int c = 0; c < kWords; ++c) tmem_load32(lanes + P::scores(buf) + c * 32, x[c]);
@@ -527,54 +534,89 @@ __device__ __forceinline__ void softmax(const Args &a, Shared0 &s, char *smem, S
                 for (int k = 0; k < P::kN; ++k)
                     if (k < lo || k > hi || !(there[k >> 5] >> (k & 31) & 1)) x[k >> 5][k & 31] = __float_as_uint(-INFINITY);
             }
+            // The reference moves rarely, so the weights are begun with the one there is while the maximum is found
+            // beside them; only where it has to move, and in the first unit, is the maximum first.
             float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll
-            for (int k = 0; k < P::kN; k += 2)
+            const auto look = [&](int k) {
                 top[k >> 1 & 3] = max3(top[k >> 1 & 3], __uint_as_float(x[k >> 5][k & 31]), __uint_as_float(x[k >> 5][(k & 31) + 1]));
-            const float m = fmaxf(max3(top[0], top[1], top[2]), top[3]) * a.scale;
-            if (__any_sync(kFullMask, m > ref + kSlack)) {
-                const float next = fmaxf(ref, m - kLead);
-                const float keep = next == ref ? 1.0f : ex2(ref - next);
-                ref = next;
-                l *= keep;
-                if (u > f.u0) {
-                    wait(&s.o_done[i], done - 1);
-                    __syncwarp();
-                    tmem_fence_after();
-#pragma unroll 1
-                    for (int c = 0; c < kDim; c += 32) {
-                        uint32_t o[32];
-                        tmem_load32(lanes + P::output(i) + c, o);
-                        tmem_wait_load();
-#pragma unroll
-                        for (int k = 0; k < 32; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * keep);
-                        tmem_store32(lanes + P::output(i) + c, o);
-                    }
-                }
-            }
-            const float off = ref == -INFINITY ? 0.0f : -ref;
-            const Pair scale2 = pair(a.scale, a.scale), off2 = pair(off, off);
-            Pair sum[2] = {0, 0};
-#pragma unroll
-            for (int c = 0; c < kWords; ++c) {
-                uint32_t w[16];
+            };
+            const Pair scale2 = pair(a.scale, a.scale);
+            Pair off2, sum[2];
+            uint32_t w[P::kN / 4];
+            const auto weigh = [&](int c, bool looks) {        // 32 of the weights
 #pragma unroll
                 for (int k = 0; k < 16; ++k) {
                     Pair p = fma2(pair(__uint_as_float(x[c][2 * k]), __uint_as_float(x[c][2 * k + 1])), scale2, off2);
                     float p0, p1;
-                    if (k % 8 < kPolynomial) {
-                        p = exp2_of(p);
-                        split(p, p0, p1);
-                    } else {
-                        split(p, p0, p1);
-                        p0 = ex2(p0);
-                        p1 = ex2(p1);
-                        p = pair(p0, p1);
+                    split(p, p0, p1);
+                    p0 = ex2(p0);
+                    p1 = ex2(p1);
+                    sum[k & 1] = add2(sum[k & 1], pair(p0, p1));
+                    w[(c * 16 + k) % (P::kN / 4)] = pack(p0, p1, T());
+                    if (looks) {
+                        look(c * 32 + 2 * k);
+                        look(P::kN / 2 + c * 32 + 2 * k);
                     }
-                    sum[k & 1] = add2(sum[k & 1], p);
-                    w[k] = pack(p0, p1, T());
                 }
-                tmem_store16(lanes + P::weights(buf, 2 * c), w);
+            };
+            bool moves = u == f.u0;
+            if (moves) {
+#pragma unroll
+                for (int k = 0; k < P::kN; k += 2) look(k);
+            }
+            for (;;) {
+                if (moves) {
+                    const float m = fmaxf(max3(top[0], top[1], top[2]), top[3]) * a.scale;
+                    const float next = fmaxf(ref, m - kLead);
+                    const float keep = next == ref ? 1.0f : ex2(ref - next);
+                    ref = next;
+                    l *= keep;
+                    if (u > f.u0) {
+                        wait(&s.o_done[i], done - 1);
+                        __syncwarp();
+                        tmem_fence_after();
+#pragma unroll 1
+                        for (int c = 0; c < kDim; c += 32) {
+                            uint32_t o[32];
+                            tmem_load32(lanes + P::output(i) + c, o);
+                            tmem_wait_load();
+#pragma unroll
+                            for (int k = 0; k < 32; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * keep);
+                            tmem_store32(lanes + P::output(i) + c, o);
+                        }
+                    }
+                }
+                const float off = ref == -INFINITY ? 0.0f : -ref;
+                off2 = pair(off, off);
+                sum[0] = sum[1] = 0;
+#pragma unroll
+                for (int c = 0; c < kWords / 2; ++c) weigh(c, true);
+                if (moves) break;
+                const float m = fmaxf(max3(top[0], top[1], top[2]), top[3]) * a.scale;
+                moves = __any_sync(kFullMask, m > ref + kSlack);
+                if (!moves) break;
+            }
+            if (P::kTiles == 1 && u > f.u0) {
+                // a single tile's scores do not come behind the output of the unit before, and a barrier tells one phase
+                // from the next one only
+                wait(&s.o_done[i], done - 1);
+                __syncwarp();
+            }
+            if constexpr (P::kN == 128) {
+                tmem_store32(lanes + P::weights(buf, 0), w);
+            } else {
+                tmem_store16(lanes + P::weights(buf, 0), w);
+                tmem_wait_store();
+                tmem_fence_before();
+                arrive(&s.p_most[buf]);
+            }
+#pragma unroll
+            for (int c = kWords / 2; c < kWords; ++c) {
+                weigh(c, false);
+                uint32_t v[16];
+#pragma unroll
+                for (int k = 0; k < 16; ++k) v[k] = w[(c * 16 + k) % (P::kN / 4)];
+                tmem_store16(lanes + P::weights(buf, 2 * c), v);
                 if (c >= kWords - 2) {                 // the products begin before the last weights are there
                     tmem_wait_store();
                     tmem_fence_before();
@@ -587,8 +629,6 @@ __device__ __forceinline__ void softmax(const Args &a, Shared0 &s, char *smem, S
             ++done;
         }
         if (active) {
-            // (scores of a single tile do not come behind the output of the unit before: a phase at a time)
-            if (P::kTiles == 1 && f.u1 - f.u0 > 1) wait(&s.o_done[i], done - 2);
             wait(&s.o_done[i], done - 1);
             __syncwarp();
             tmem_fence_after();
@@ -651,9 +691,8 @@ __device__ __forceinline__ void softmax(const Args &a, Shared0 &s, char *smem, S
 template <typename T, int kDim, bool kBoxes>
 __global__ void __launch_bounds__(kThreads, 1) mma_kernel(const Args a, const __grid_constant__ Maps maps, int box) {
     using P = Plan<kDim>;
-    extern __shared__ char smem_raw[];
+    extern __shared__ __align__(1024) char smem[];
     __shared__ Shared0 s;
-    char *smem = smem_raw + ((1024u - (smem_addr(smem_raw) & 1023u)) & 1023u);
     const int tid = threadIdx.x, warp = tid >> 5;
     pdl_launch_dependents();
     if (tid == 0) {
@@ -676,7 +715,7 @@ __global__ void __launch_bounds__(kThreads, 1) mma_kernel(const Args a, const __
     tmem_fence_before();
     __syncthreads();
     tmem_fence_after();
-    if (st.left > 0) {
+    if (st.left > 0 && s.tmem == 0) {
         if (tid == 0 && st.skip && st.first + 1 == static_cast<int>(blockIdx.x)) {
             const Sequence q = sequence(a, st.b);
             a.joints[blockIdx.x] = Joint{st.first, st.last, q.from, q.n, st.tile, st.head};
@@ -695,6 +734,7 @@ __global__ void __launch_bounds__(kThreads, 1) mma_kernel(const Args a, const __
     __syncthreads();
     tmem_fence_after();
     if (warp == kThreads / 32 - 1) tmem_free(s.tmem, kColumns);
+    if (tid == 0 && (s.tmem != 0 || (smem_addr(smem) & 1023))) atomicOr(a.status, kStatusStageTimeout);   // never
 }
 
 // Rows of a page to a tensor copy: the largest power of two that divides the

@@ -139,6 +139,7 @@ def chunk_run(torch, eng, c, scale=None, window=0, check=True):
     eng.set_stream(torch.cuda.current_stream().cuda_stream)
     n = c["n"]
     eng.kv_attend_chunk(c["cache"], c["q"], c["out"], c["offsets"], lse=c["lse"], scale=scale, window=window)
+    assert eng.status() == 0             # no wait inside the kernel ran out
     if check:
         chunk_check(torch, c, c["d"] ** -0.5 if scale is None else scale, window)
     return c["out"][:n].clone(), c["lse"][:n].clone()
