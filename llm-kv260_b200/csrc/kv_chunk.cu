@@ -25,6 +25,7 @@ int kv_chunk_validate(const b200_kv_t *kv, const b200_kv_chunk_t *a, const char 
     if (a->dtype != kv->dtype && !(a->dtype == B200_F32 && kv->dtype == B200_F16))
         return bad("q must be of the cache's type, or float32 with a float16 cache");
     if (a->n_head < 1 || a->n_head % kv->n_head_kv) return bad("n_head must be a multiple of n_head_kv");
+    if (a->n_head / kv->n_head_kv > 4096) return bad("at most 4096 query heads read one cache head");
     if (a->n_tokens < 0 || static_cast<int64_t>(a->n_tokens) * a->n_head > 1ll << 30)
         return bad("n_tokens must be in [0, 2^30 / n_head]");
     if (a->window < 0) return bad("window must not be negative");
@@ -60,6 +61,7 @@ cudaError_t kv_chunk_launch(const b200_kv_t *kv, const b200_kv_chunk_t *p, cudaS
     a.n_tokens = p->n_tokens;
     a.n_head = p->n_head;
     a.group = p->n_head / kv->n_head_kv;
+    a.group_magic = static_cast<unsigned>((1ull << 32) / static_cast<unsigned>(a.group)) + 1;
     a.window = p->window < kMaxSlots ? p->window : 0;      // one that leaves nothing out
     a.scale = p->scale * chunk::kLog2e;
     const chunk::Shape s = shape_of(kv, p->dtype);

@@ -3,10 +3,11 @@
 //
 // The query heads that read a cache head and a sequence's new tokens are packed
 // into rows, row = token * group + head of the group; M consecutive rows are a
-// tile. A tile sees a range of slots, cut into units of N. All units, in the
-// order cache head, sequence, tile, slot, are dealt out in equal stretches to
-// the CTAs of a grid that fits the GPU at once, whatever the lengths, which only
-// the device knows. A tile that lies in more than one stretch is joined by a
+// tile. A tile sees a range of slots, cut into units of N, and what it takes to
+// begin and end it counts as C more units before them. All units, in the order
+// cache head, sequence, tile, slot, are dealt out in equal stretches to the CTAs
+// of a grid that fits the GPU at once, whatever the lengths, which only the
+// device knows; a stretch that ends among a tile's C leaves all of it to the next. A tile that lies in more than one stretch is joined by a
 // second kernel from the parts (m, l, O) that the CTAs leave in the workspace,
 // in the order of its slots, so that the result does not depend on timing.
 #pragma once
@@ -37,6 +38,7 @@ struct Args {
     const int *offsets;
     long long q_token, q_head, out_token, out_head;  // bytes
     int n_tokens, n_head, group, window;
+    unsigned group_magic;              // x / group = x * group_magic >> 32 for x * group < 2^32, a group of 1 apart
     float scale;                       // times log2(e)
     Joint *joints;                     // [grid]
     float *parts;                      // [grid][2] parts: O [M][dim], m [M], l [M]
@@ -96,9 +98,37 @@ __device__ __forceinline__ int scan(int x, int *s_warp, int *total) {
 // Where a CTA's stretch begins and how long it is.
 struct Stretch {
     long long left;                    // units
-    int head, b, tile, skip;           // its first unit is the skip-th of that tile
-    int first, last;                   // CTAs with units of that tile
+    int head, b, tile, skip;           // its first unit is the skip-th of that tile, its C included
+    int first, last;                   // CTAs with units of that tile, its C not included
 };
+
+// A stretch's part of one tile.
+struct Fragment {
+    int used;                          // units of the stretch
+    int u0, u1;                        // slots by N; none where they are equal
+    int row0, rows;                    // first packed row, all of the sequence's
+    int first;                         // the slot of the first new token
+    bool begins, whole;                // has the tile's first unit, has all of them
+    int last_all, first_all;           // slots that every row sees lie between
+};
+
+template <int M, int N, int C>
+__device__ __forceinline__ Fragment fragment(const Args &a, const Sequence &q, int tile, int skip, long long left) {
+    Fragment f;
+    const int2 all = units_of<M, N>(a, q.n, q.length, tile);
+    const int end = static_cast<int>(min(static_cast<long long>(all.y + C), skip + left)), from = max(skip - C, 0);
+    f.used = end - skip;
+    f.u0 = all.x + from;
+    f.u1 = all.x + max(end - C, from);
+    f.row0 = tile * M;
+    f.rows = q.n * a.group;
+    f.first = q.length - q.n;
+    f.begins = from == 0;
+    f.whole = f.u1 - f.u0 == all.y;
+    f.last_all = f.first + f.row0 / a.group;
+    f.first_all = a.window ? f.first + min(f.rows - 1, f.row0 + M - 1) / a.group - a.window + 1 : 0;
+    return f;
+}
 
 template <int T>
 struct Shared {
@@ -110,7 +140,7 @@ struct Shared {
 // Found by the whole CTA (T threads): sums of the tiles' units, T tiles at a
 // time, first for their total, then up to the stretch's first. A thread has a
 // tile, found by a search in the sums of the tiles of T sequences.
-template <int M, int N, int T>
+template <int M, int N, int C, int T>
 __device__ __forceinline__ Stretch find(const Args &a, Shared<T> *s) {
     const int tid = threadIdx.x;
     long long sum = 0, target = -1, units = 0, begin = 0, end = 0, ctas = 0;
@@ -142,7 +172,7 @@ __device__ __forceinline__ Stretch find(const Args &a, Shared<T> *s) {
                         if (s->tiles[mid] > k) hi = mid; else lo = mid + 1;
                     }
                     tile = k - (lo ? s->tiles[lo - 1] : 0);
-                    count = units_of<M, N>(a, s->n[lo], s->length[lo], tile).y;
+                    count = units_of<M, N>(a, s->n[lo], s->length[lo], tile).y + C;
                 }
                 int all;
                 const int to = scan<T>(count, s->warp, &all);
@@ -174,7 +204,7 @@ __device__ __forceinline__ Stretch find(const Args &a, Shared<T> *s) {
     r.b = s->b;
     r.tile = s->tile;
     r.skip = s->skip;
-    const long long u0 = head * sum + s->before, u1 = u0 + s->count - 1;
+    const long long u0 = head * sum + s->before + C, u1 = u0 + s->count - C - 1;
     r.first = static_cast<int>(((u0 + 1) * ctas - 1) / units);
     r.last = static_cast<int>(((u1 + 1) * ctas - 1) / units);
     return r;

@@ -9,6 +9,7 @@ namespace chunk {
 namespace {
 
 constexpr int kM = 64, kN = 64, kThreads = 256;
+constexpr int kCost = 1;               // units that a tile's begin and end take
 
 template <int kDim>
 struct Smem {
@@ -35,25 +36,23 @@ __global__ void __launch_bounds__(kThreads, 1) f32_kernel(const Args a) {
     extern __shared__ char smem_raw[];
     Smem<kDim> &s = *reinterpret_cast<Smem<kDim> *>(smem_raw);
     const int tid = threadIdx.x, tx = tid & 15, ty = tid >> 4, d = a.kv.head_dim;
-    Stretch st = find<kM, kN, kThreads>(a, &s.find);
+    Stretch st = find<kM, kN, kCost, kThreads>(a, &s.find);
     if (tid == 0) a.joints[blockIdx.x].first = -1;
     if (st.left == 0) return;
     Sequence q = sequence(a, st.b);
     int tile = st.tile, head = st.head, skip = st.skip;
-    if (skip && tid == 0 && st.first + 1 == static_cast<int>(blockIdx.x))
+    if (skip > kCost && tid == 0 && st.first + 1 == static_cast<int>(blockIdx.x))
         a.joints[blockIdx.x] = Joint{st.first, st.last, q.from, q.n, tile, head};
 #pragma unroll 1
     for (;;) {
-        const int2 all = units_of<kM, kN>(a, q.n, q.length, tile);
-        const int u0 = all.x + skip, u1 = all.x + static_cast<int>(min(static_cast<long long>(all.y), skip + st.left));
-        const bool whole = u1 - u0 == all.y;
-        const long long rows = static_cast<long long>(q.n) * a.group, row0 = static_cast<long long>(tile) * kM;
-        const int first = q.length - q.n;              // the slot of the first new token
+        const Fragment f = fragment<kM, kN, kCost>(a, q, tile, skip, st.left);
+        const int row0 = f.row0, rows = f.rows;
+        if (f.u1 > f.u0) {
         for (int i = tid; i < kM * (kDim / 8); i += kThreads) {
             const int r = i / (kDim / 8), c = i % (kDim / 8) * 8;
             float v[8] = {};
             if (row0 + r < rows && c < d) {
-                const int token = static_cast<int>((row0 + r) / a.group), h = static_cast<int>(row0 + r - static_cast<long long>(token) * a.group);
+                const int token = (row0 + r) / a.group, h = row0 + r - token * a.group;
                 load8<TQ>(a.q + (q.from + token) * a.q_token + (head * a.group + h) * a.q_head + c * static_cast<int>(sizeof(TQ)), v);
             }
             *reinterpret_cast<float4 *>(&s.q[r][c]) = make_float4(v[0], v[1], v[2], v[3]);
@@ -63,18 +62,15 @@ __global__ void __launch_bounds__(kThreads, 1) f32_kernel(const Args a) {
         float m[4], l[4], o[4][kDim / 16];
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            const long long r = row0 + ty * 4 + i;
-            at[i] = r < rows ? first + static_cast<int>(r / a.group) : -1;
+            const int r = row0 + ty * 4 + i;
+            at[i] = r < rows ? f.first + r / a.group : -1;
             m[i] = -INFINITY;
             l[i] = 0.0f;
 #pragma unroll
             for (int j = 0; j < kDim / 16; ++j) o[i][j] = 0.0f;
         }
-        // slots that every row of the tile sees
-        const int last_all = first + static_cast<int>(row0 / a.group);
-        const int first_all = a.window ? first + static_cast<int>(min(rows - 1, row0 + kM - 1) / a.group) - a.window + 1 : 0;
 #pragma unroll 1
-        for (int u = u0; u < u1; ++u) {
+        for (int u = f.u0; u < f.u1; ++u) {
             __syncthreads();
             if (tid < kN) {
                 const int slot = u * kN + tid;
@@ -108,7 +104,7 @@ __global__ void __launch_bounds__(kThreads, 1) f32_kernel(const Args a) {
                     for (int j = 0; j < 4; ++j)
                         t[i][j] = fmaf(x[i].w, y[j].w, fmaf(x[i].z, y[j].z, fmaf(x[i].y, y[j].y, fmaf(x[i].x, y[j].x, t[i][j]))));
             }
-            const bool edge = (u + 1) * kN - 1 > last_all || u * kN < first_all;
+            const bool edge = (u + 1) * kN - 1 > f.last_all || u * kN < f.first_all;
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 float top = -INFINITY;
@@ -166,8 +162,8 @@ __global__ void __launch_bounds__(kThreads, 1) f32_kernel(const Args a) {
         for (int i = 0; i < 4; ++i) {
             const int r = ty * 4 + i;
             if (row0 + r >= rows) break;
-            const int token = static_cast<int>((row0 + r) / a.group), h = head * a.group + static_cast<int>(row0 + r - static_cast<long long>(token) * a.group);
-            if (whole) {
+            const int token = (row0 + r) / a.group, h = head * a.group + row0 + r - token * a.group;
+            if (f.whole) {
                 const float inv = l[i] == 0.0f ? 0.0f : 1.0f / l[i];
                 char *out = a.out + (q.from + token) * a.out_token + h * a.out_head;
 #pragma unroll
@@ -178,7 +174,7 @@ __global__ void __launch_bounds__(kThreads, 1) f32_kernel(const Args a) {
                 if (a.lse && tx == 0)
                     a.lse[static_cast<long long>(q.from + token) * a.n_head + h] = (m[i] + log2f(l[i])) * kLn2;
             } else {
-                float *part = a.parts + (2ll * blockIdx.x + (skip == 0)) * part_floats(kM, kDim);
+                float *part = a.parts + (2ll * blockIdx.x + f.begins) * part_floats(kM, kDim);
 #pragma unroll
                 for (int j = 0; j < kDim / 64; ++j)
                     *reinterpret_cast<float4 *>(part + r * kDim + 4 * tx + 64 * j) =
@@ -189,7 +185,8 @@ __global__ void __launch_bounds__(kThreads, 1) f32_kernel(const Args a) {
                 }
             }
         }
-        st.left -= u1 - u0;
+        }
+        st.left -= f.used;
         if (st.left <= 0) break;
         skip = 0;
         next_tile<kM>(a, q, tile, head);

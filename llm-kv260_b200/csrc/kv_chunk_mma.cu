@@ -18,6 +18,7 @@ namespace {
 constexpr int kSoftmaxThreads = 256, kCopiers = 96, kThreads = kSoftmaxThreads + kCopiers + 32;
 constexpr int kSoftmaxRegs = 208, kOtherRegs = 88;
 static_assert(kSoftmaxThreads * kSoftmaxRegs + 128 * kOtherRegs <= kThreads * 168);
+constexpr int kCost = 5;                // units that a tile's begin and end take
 constexpr int kLeastBox = 8;           // rows of a page that one tensor copy brings at least
 constexpr int kColumns = 512;          // of tensor memory: all, so that it begins at address 0
 // The reference m trails the maximum by 7 to 15 powers of two: weights stay in
@@ -144,29 +145,6 @@ __device__ __forceinline__ uint32_t piece(int rows, int r, int c) {
     return static_cast<uint32_t>((c >> 3) * rows * 128 + r * 128 + (((c & 7) ^ (r & 7)) << 4));
 }
 
-// A stretch's part of one tile.
-struct Fragment {
-    int u0, u1, first;                 // units, the slot of the first new token
-    int row0, rows;                    // first packed row, all of the sequence's
-    bool whole;
-    int last_all, first_all;           // slots that every row sees lie between
-};
-
-template <int kM, int kN>
-__device__ __forceinline__ Fragment fragment(const Args &a, const Sequence &q, int tile, int skip, long long left) {
-    Fragment f;
-    const int2 all = units_of<kM, kN>(a, q.n, q.length, tile);
-    f.u0 = all.x + skip;
-    f.u1 = all.x + static_cast<int>(min(static_cast<long long>(all.y), skip + left));
-    f.first = q.length - q.n;
-    f.rows = q.n * a.group;
-    f.row0 = tile * kM;
-    f.whole = f.u1 - f.u0 == all.y;
-    f.last_all = f.first + f.row0 / a.group;
-    f.first_all = a.window ? f.first + min(f.rows - 1, f.row0 + kM - 1) / a.group - a.window + 1 : 0;
-    return f;
-}
-
 // Arrives on `bar` for this thread when the copies that it has asked for are there.
 __device__ __forceinline__ void arrive_behind_copies(uint64_t *bar) {
     asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_addr(bar)) : "memory");
@@ -200,7 +178,8 @@ __device__ __forceinline__ void copier(const Args &a, const Maps &maps, int box,
     int tile = st.tile, head = st.head, skip = st.skip;
     const Waiter wait{status, &s.dead};
     for (;;) {
-        const Fragment f = fragment<P::kM, P::kN>(a, q, tile, skip, st.left);
+        const Fragment f = fragment<P::kM, P::kN, kCost>(a, q, tile, skip, st.left);
+        if (f.u1 > f.u0) {
         const char *k_head = a.kv.k + head * a.kv.head_stride, *v_head = a.kv.v + head * a.kv.head_stride;
         const int *table = a.kv.table + q.b * a.kv.table_stride;
         int page[2], asked[2], row[2];                 // of two of this unit's and the next one's slots
@@ -226,17 +205,16 @@ __device__ __forceinline__ void copier(const Args &a, const Maps &maps, int box,
         ask(f.u0);
         if (fragments) wait(&s.q_free, fragments - 1);
         const int rows = min(P::kM, f.rows - f.row0);
-#pragma unroll 1
+        const int token0 = f.row0 / a.group, rest = f.row0 - token0 * a.group;
+        const char *q_rows = a.q + (q.from + token0) * a.q_token + head * a.group * a.q_head;
+#pragma unroll 4
         for (int i = tid; i < (rows > 128 ? P::kM : 128) * kPieces; i += kCopiers) {
             const int r = i / kPieces, c = i % kPieces;
             if (c >= pieces) continue;
             const bool there = r < rows && c < filled;
-            const char *src = a.q;
-            if (there) {
-                const int token = (f.row0 + r) / a.group, h = f.row0 + r - token * a.group;
-                src += (q.from + token) * a.q_token + (head * a.group + h) * a.q_head + c * 16;
-            }
-            copy16(q_at + (r >> 7) * (128 * kDim * 2) + piece(128, r & 127, c), src, there);
+            const int token = a.group == 1 ? r : static_cast<int>(__umulhi(rest + r, a.group_magic));
+            const char *src = q_rows + token * a.q_token + (rest + r - token * a.group) * a.q_head + c * 16;
+            copy16(q_at + (r >> 7) * (128 * kDim * 2) + piece(128, r & 127, c), there ? src : a.q, there);
         }
         arrive_behind_copies(&s.q_full);
         place(f.u0);
@@ -277,7 +255,8 @@ __device__ __forceinline__ void copier(const Args &a, const Maps &maps, int box,
             if (u + 1 < f.u1) place(u + 1);
         }
         ++fragments;
-        st.left -= f.u1 - f.u0;
+        }
+        st.left -= f.used;
         if (st.left <= 0) break;
         skip = 0;
         next_tile<P::kM>(a, q, tile, head);
@@ -394,7 +373,8 @@ __device__ __forceinline__ void products(const Args &a, Shared0 &s, char *smem, 
     using Even = std::integral_constant<int, 0>;
     using Odd = std::integral_constant<int, 1>;
     for (;;) {
-        const Fragment f = fragment<P::kM, P::kN>(a, q, tile, skip, st.left);
+        const Fragment f = fragment<P::kM, P::kN, kCost>(a, q, tile, skip, st.left);
+        if (f.u1 > f.u0) {
         const int units = f.u1 - f.u0, tiles = P::kTiles == 2 && f.rows - f.row0 > 128 ? 2 : 1;
         wait(&s.q_full, fragments);
         __syncwarp();
@@ -407,7 +387,8 @@ __device__ __forceinline__ void products(const Args &a, Shared0 &s, char *smem, 
             else body(Even{}, tiles, j > 0, j + 1 < units, j + 2 == units);
         }
         ++fragments;
-        st.left -= units;
+        }
+        st.left -= f.used;
         if (st.left <= 0) break;
         skip = 0;
         next_tile<P::kM>(a, q, tile, head);
@@ -436,7 +417,8 @@ __device__ __forceinline__ void softmax(const Args &a, Shared0 &s, char *smem, S
         if (lane == 0) mbar_arrive(bar);
     };
     for (;;) {
-        const Fragment f = fragment<P::kM, P::kN>(a, q, tile, skip, st.left);
+        const Fragment f = fragment<P::kM, P::kN, kCost>(a, q, tile, skip, st.left);
+        if (f.u1 > f.u0) {
         const int tiles = P::kTiles == 2 && f.rows - f.row0 > 128 ? 2 : 1;
         const int row = f.row0 + i * 128 + r;
         const bool active = i < tiles;
@@ -635,7 +617,7 @@ __device__ __forceinline__ void softmax(const Args &a, Shared0 &s, char *smem, S
             const float inv = !f.whole ? 1.0f : l == 0.0f ? 0.0f : 1.0f / l;
             const int token = row / a.group, h = head * a.group + row - token * a.group;
             char *out = a.out + (q.from + token) * a.out_token + h * a.out_head;
-            float *part = a.parts + (2ll * blockIdx.x + (skip == 0)) * part_floats(P::kM, kDim);
+            float *part = a.parts + (2ll * blockIdx.x + f.begins) * part_floats(P::kM, kDim);
             const int pr = i * 128 + r;
 #pragma unroll 1
             for (int c = 0; c < kDim; c += 32) {
@@ -681,7 +663,8 @@ __device__ __forceinline__ void softmax(const Args &a, Shared0 &s, char *smem, S
             }
             __syncwarp();
         }
-        st.left -= f.u1 - f.u0;
+        }
+        st.left -= f.used;
         if (st.left <= 0) break;
         skip = 0;
         next_tile<P::kM>(a, q, tile, head);
@@ -711,12 +694,12 @@ __global__ void __launch_bounds__(kThreads, 1) mma_kernel(const Args a, const __
         a.joints[blockIdx.x].first = -1;
     }
     if (warp == kThreads / 32 - 1) tmem_alloc(&s.tmem, kColumns);
-    const Stretch st = find<P::kM, P::kN, kThreads>(a, reinterpret_cast<Shared<kThreads> *>(smem));
+    const Stretch st = find<P::kM, P::kN, kCost, kThreads>(a, reinterpret_cast<Shared<kThreads> *>(smem));
     tmem_fence_before();
     __syncthreads();
     tmem_fence_after();
     if (st.left > 0 && s.tmem == 0) {
-        if (tid == 0 && st.skip && st.first + 1 == static_cast<int>(blockIdx.x)) {
+        if (tid == 0 && st.skip > kCost && st.first + 1 == static_cast<int>(blockIdx.x)) {
             const Sequence q = sequence(a, st.b);
             a.joints[blockIdx.x] = Joint{st.first, st.last, q.from, q.n, st.tile, st.head};
         }
