@@ -145,6 +145,20 @@ __device__ __forceinline__ Stretch find(const Args &a, Shared<T> *s) {
     const int tid = threadIdx.x;
     long long sum = 0, target = -1, units = 0, begin = 0, end = 0, ctas = 0;
     int head = 0;
+    struct Mine {
+        int b, tile, count;
+        long long before;
+        bool any;
+    } mine{};
+    const auto keep = [&](const Mine &x) {
+        if (!x.any || target < x.before || target >= x.before + x.count) return;
+        s->b = x.b;
+        s->tile = x.tile;
+        s->count = x.count;
+        s->skip = static_cast<int>(target - x.before);
+        s->before = x.before;
+    };
+    int rounds = 0;
 #pragma unroll 1
     for (int pass = 0; pass < 2; ++pass) {
         long long run = 0;
@@ -176,14 +190,10 @@ __device__ __forceinline__ Stretch find(const Args &a, Shared<T> *s) {
                 }
                 int all;
                 const int to = scan<T>(count, s->warp, &all);
-                if (pass && k < total && target >= run + to - count && target < run + to) {
-                    s->b = base + lo;
-                    s->tile = tile;
-                    s->count = count;
-                    s->skip = static_cast<int>(target - (run + to - count));
-                    s->before = run + to - count;
-                }
+                mine = Mine{base + lo, tile, count, run + to - count, k < total};
+                if (pass) keep(mine);
                 run += all;
+                ++rounds;
             }
             __syncthreads();
         }
@@ -196,8 +206,13 @@ __device__ __forceinline__ Stretch find(const Args &a, Shared<T> *s) {
             end = units * (blockIdx.x + 1) / ctas;
             head = static_cast<int>(begin / sum);
             target = begin - head * sum;
+            if (rounds == 1) {             // every thread still has the only tile it saw
+                keep(mine);
+                break;
+            }
         }
     }
+    __syncthreads();
     Stretch r;
     r.left = end - begin;
     r.head = head;
@@ -232,6 +247,8 @@ __device__ __forceinline__ void store4(char *p, float4 v) {
     }
 }
 
+constexpr int kJoinRows = 8;             // CTAs of 8 warps to a tile
+
 // A split tile's rows from their parts, a warp for each: with m the largest of
 // the parts', out = sum 2^(m_i - m) O_i / sum 2^(m_i - m) l_i.
 template <typename T, int M, int kDim>
@@ -239,49 +256,58 @@ __global__ void __launch_bounds__(256) join_kernel(const Args a) {
     pdl_wait_prior_grid();
     const Joint j = a.joints[blockIdx.x];
     if (j.first < 0) return;
-    const int lane = threadIdx.x & 31, r = blockIdx.y * 8 + (threadIdx.x >> 5);
-    const long long row = static_cast<long long>(j.tile) * M + r;
-    if (row >= static_cast<long long>(j.n) * a.group) return;
-    const int i = static_cast<int>(row / a.group), h = j.head * a.group + static_cast<int>(row - static_cast<long long>(i) * a.group);
+    const int lane = threadIdx.x & 31;
     // the first CTA's stretch ends with its part, the others' begin with theirs
     const auto part = [&](int c) { return a.parts + (2ll * c + (c == j.first)) * part_floats(M, kDim); };
-    float m = -INFINITY;
-    for (int c = j.first; c <= j.last; ++c) {
-        const float x = part(c)[M * kDim + r];
-        m = x > m || x != x ? x : m;       // NaN stays
-        if (m != m) break;
-    }
-    const float ref = m == -INFINITY ? 0.0f : m;
-    constexpr int kPer = (kDim + 127) / 128;
-    float l = 0.0f;
-    float4 o[kPer] = {};
-    for (int c = j.first; c <= j.last; ++c) {
-        const float *p = part(c);
-        const float w = exp2f(p[M * kDim + r] - ref);
-        l = fmaf(w, p[M * kDim + M + r], l);
+#pragma unroll 1
+    for (int r = blockIdx.y * 8 + (threadIdx.x >> 5); r < M; r += kJoinRows * 8) {
+        const int row = j.tile * M + r;
+        if (row >= j.n * a.group) return;
+        const int i = row / a.group, h = j.head * a.group + row - i * a.group;
+        // a lane's parts' references, and the largest
+        float m = -INFINITY;
+        for (int c = j.first + lane; c <= j.last; c += 32) {
+            const float x = part(c)[M * kDim + r];
+            m = x > m || x != x ? x : m;   // NaN stays
+        }
+#pragma unroll
+        for (int x = 16; x; x >>= 1) {
+            const float y = __shfl_xor_sync(kFullMask, m, x);
+            m = y > m || y != y ? y : m;
+        }
+        const float ref = m == -INFINITY ? 0.0f : m;
+        constexpr int kPer = (kDim + 127) / 128;
+        float l = 0.0f;
+        float4 o[kPer] = {};
+#pragma unroll 4
+        for (int c = j.first; c <= j.last; ++c) {
+            const float *p = part(c);
+            const float w = exp2f(p[M * kDim + r] - ref);
+            l = fmaf(w, p[M * kDim + M + r], l);
+#pragma unroll
+            for (int k = 0; k < kPer; ++k) {
+                const int at = k * 128 + lane * 4;
+                if (at >= kDim) break;
+                const float4 x = *reinterpret_cast<const float4 *>(p + static_cast<long long>(r) * kDim + at);
+                // a part without weight adds nothing, whatever it holds
+                if (w != 0.0f) o[k] = make_float4(fmaf(w, x.x, o[k].x), fmaf(w, x.y, o[k].y), fmaf(w, x.z, o[k].z), fmaf(w, x.w, o[k].w));
+            }
+        }
+        const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+        char *out = a.out + (j.from + i) * a.out_token + h * a.out_head;
 #pragma unroll
         for (int k = 0; k < kPer; ++k) {
             const int at = k * 128 + lane * 4;
-            if (at >= kDim) break;
-            const float4 x = *reinterpret_cast<const float4 *>(p + static_cast<long long>(r) * kDim + at);
-            // a part without weight adds nothing, whatever it holds
-            if (w != 0.0f) o[k] = make_float4(fmaf(w, x.x, o[k].x), fmaf(w, x.y, o[k].y), fmaf(w, x.z, o[k].z), fmaf(w, x.w, o[k].w));
+            if (at < a.kv.head_dim) store4<T>(out + at * static_cast<int>(sizeof(T)), make_float4(o[k].x * inv, o[k].y * inv, o[k].z * inv, o[k].w * inv));
         }
+        if (a.lse && lane == 0) a.lse[static_cast<long long>(j.from + i) * a.n_head + h] = (m + log2f(l)) * kLn2;
     }
-    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-    char *out = a.out + (j.from + i) * a.out_token + h * a.out_head;
-#pragma unroll
-    for (int k = 0; k < kPer; ++k) {
-        const int at = k * 128 + lane * 4;
-        if (at < a.kv.head_dim) store4<T>(out + at * static_cast<int>(sizeof(T)), make_float4(o[k].x * inv, o[k].y * inv, o[k].z * inv, o[k].w * inv));
-    }
-    if (a.lse && lane == 0) a.lse[static_cast<long long>(j.from + i) * a.n_head + h] = (m + log2f(l)) * kLn2;
 }
 
 template <typename T, int M, int kDim>
 cudaError_t launch_join(const Args &a, int grid, cudaStream_t stream) {
     cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3(grid, M / 8);
+    cfg.gridDim = dim3(grid, kJoinRows);
     cfg.blockDim = dim3(256);
     cfg.stream = stream;
     cudaLaunchAttribute attr[1];

@@ -44,22 +44,27 @@ __device__ __forceinline__ Wish wish_of(const PlanArgs &a, int b) {
 }
 
 // Inclusive sums of two numbers over the CTA; *total is theirs.
-__device__ __forceinline__ void scan2(long long &x, long long &y, long long *total_x, long long *total_y) {
-    __shared__ long long s[2][kThreads / 32];
+__device__ __forceinline__ void scan2(unsigned long long &x, long long &y, unsigned long long *total_x, long long *total_y) {
+    __shared__ unsigned long long sx[kThreads / 32];
+    __shared__ long long sy[kThreads / 32];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
 #pragma unroll
     for (int i = 1; i < 32; i <<= 1) {
-        const long long u = __shfl_up_sync(kFullMask, x, i), v = __shfl_up_sync(kFullMask, y, i);
+        const unsigned long long u = __shfl_up_sync(kFullMask, x, i);
+        const long long v = __shfl_up_sync(kFullMask, y, i);
         if (lane >= i) x += u, y += v;
     }
     __syncthreads();                   // the last scan's sums have been read
-    if (lane == 31) s[0][warp] = x, s[1][warp] = y;
+    if (lane == 31) sx[warp] = x, sy[warp] = y;
     __syncthreads();
-    long long bx = lane < kThreads / 32 ? s[0][lane] : 0, by = lane < kThreads / 32 ? s[1][lane] : 0;
-    const long long ox = bx, oy = by;
+    unsigned long long bx = sx[lane];
+    long long by = sy[lane];
+    const unsigned long long ox = bx;
+    const long long oy = by;
 #pragma unroll
     for (int i = 1; i < 32; i <<= 1) {
-        const long long u = __shfl_up_sync(kFullMask, bx, i), v = __shfl_up_sync(kFullMask, by, i);
+        const unsigned long long u = __shfl_up_sync(kFullMask, bx, i);
+        const long long v = __shfl_up_sync(kFullMask, by, i);
         if (lane >= i) bx += u, by += v;
     }
     *total_x = __shfl_sync(kFullMask, bx, 31);
@@ -79,15 +84,21 @@ __device__ __forceinline__ int first_above(const T *sums, int n, long long i) {
     return lo;
 }
 
-// Token t's slot, from what the first kernel has left.
-__device__ __forceinline__ void slot_of(const PlanArgs &a, int t, int batch, const int *offsets) {
-    const bool any = t < offsets[batch];
+// What the slots' search needs of a sequence, in shared memory as far as it goes.
+struct Ends {
+    int end[kThreads];
+};
+
+// Token t's slot, from what is known of its sequence: `ends` the offsets' tail,
+// `length` its old length or -1 where it got nothing.
+__device__ __forceinline__ void slot_of(const PlanArgs &a, int t, const int *ends) {
+    const int batch = a.kv.batch;
     int b = -1, position = -1;
     long long slot = -1;
-    if (any) {
-        b = first_above(offsets + 1, batch, t);
-        const int i = t - offsets[b], length = a.state[b];
-        position = a.state[a.kv.batch + b] + i;
+    if (t < ends[batch - 1]) {
+        b = first_above(ends, batch, t);
+        const int i = t - (b ? ends[b - 1] : 0), length = a.state[b];
+        position = a.state[batch + b] + i;
         if (length >= 0) {
             const int at = length + i, col = at / a.kv.page_size;
             const int page = a.kv.table[b * a.kv.table_stride + col];
@@ -101,62 +112,73 @@ __device__ __forceinline__ void slot_of(const PlanArgs &a, int t, int batch, con
 }
 
 // One CTA moves the pages: what comes back is on the stack before anything is
-// taken, and a page's place follows from two running sums over the sequences,
-// so any thread can move any page (a search in the sums of up to 1024
-// sequences finds its owner) and the result does not depend on timing. Nothing
-// here is long enough to be bound by anything but the chain of dependent reads.
+// taken, and a page's place follows from running sums over the sequences, so any
+// thread can move any page (a search in the sums of up to 1024 sequences finds
+// its owner) and the result does not depend on timing. Nothing here is long
+// enough to be bound by anything but the chain of dependent reads: the wishes,
+// the pages that move, the slots' pages. Up to 1024 sequences' wishes are read
+// and summed once, more of them twice.
 __global__ void __launch_bounds__(kThreads) kv_plan_kernel(const PlanArgs a) {
-    __shared__ long long s_sum[kThreads];
-    __shared__ int s_from[kThreads], s_given[kThreads];
+    __shared__ int s_sum[kThreads], s_from[kThreads];
+    __shared__ bool s_given[kThreads];
+    __shared__ Ends s_ends;
+    __shared__ int s_most[kThreads / 32];
     const int tid = threadIdx.x, batch = a.kv.batch;
+    const bool once = batch <= kThreads;
     int *table = const_cast<int *>(a.kv.table);
     const long long had = min(max(*a.free_count, 0), a.free_capacity);
-    long long back_all = 0;
-    for (int base = 0; base < batch; base += kThreads) {
-        const int b = base + tid, n = min(kThreads, batch - base);
-        long long back = 0, unused = 0, total, total2;
-        if (b < batch) {
-            const Wish w = wish_of(a, b);
-            back = max(w.held - w.want, 0);
-            s_from[tid] = w.want;
-        }
-        const long long mine = back;
-        scan2(back, unused, &total, &total2);
-        s_sum[tid] = back;
-        s_given[tid] = static_cast<int>(mine);
-        __syncthreads();
-        for (long long p = tid; p < total; p += kThreads) {
-            const int j = first_above(s_sum, n, p);
-            const int col = s_from[j] + static_cast<int>(p - (s_sum[j] - s_given[j]));
-            const long long dst = had + back_all + p;
-            if (dst < a.free_capacity) a.free_pages[dst] = table[(base + j) * a.kv.table_stride + col];
-        }
-        back_all += total;
-        __syncthreads();
-    }
-    const long long count = min(had + back_all, static_cast<long long>(a.free_capacity));
-    long long need_all = 0, tokens_all = 0, taken = 0;
-    for (int base = 0; base < batch; base += kThreads) {
-        const int b = base + tid, n = min(kThreads, batch - base);
-        long long need = 0, upto, tokens, total, total_tokens;
-        Wish w{};
-        int seen = 0;
+    Wish w{};
+    int seen = 0, back = 0, need = 0, back_all = 0, need_all = 0;      // of up to 1024 sequences: below 2^30
+    unsigned long long upto = 0, total = 0;            // pages that come back, and needs above them
+    long long tokens = 0, total_tokens = 0;
+    const auto load = [&](int base) {
+        const int b = base + tid;
+        w = Wish{};
+        seen = 0;
         if (b < batch) {
             w = wish_of(a, b);
-            need = max(w.want - w.held, 0);
             seen = a.seen ? a.seen[b] : w.length;
         }
-        upto = need;
+        back = max(w.held - w.want, 0);
+        need = max(w.want - w.held, 0);
+        upto = static_cast<unsigned>(back) | static_cast<unsigned long long>(need) << 32;
         tokens = w.add;
         scan2(upto, tokens, &total, &total_tokens);
-        const bool given = w.fits && (need == 0 || need_all + upto <= count);
-        s_sum[tid] = upto;
-        s_from[tid] = w.held - static_cast<int>(min(upto - need, 0x7fe00000ll));
+        back_all = static_cast<int>(total & 0xffffffffu);
+        need_all = static_cast<int>(total >> 32);
+    };
+    long long returned = 0;
+    for (int base = 0; base < batch; base += kThreads) {
+        load(base);
+        if (back_all) {
+            s_sum[tid] = static_cast<int>(upto & 0xffffffffu);
+            s_from[tid] = w.want - (static_cast<int>(upto & 0xffffffffu) - back);
+            __syncthreads();
+            for (int p = tid; p < back_all; p += kThreads) {
+                const int j = first_above(s_sum, min(kThreads, batch - base), p);
+                const long long dst = had + returned + p;
+                if (dst < a.free_capacity) a.free_pages[dst] = table[(base + j) * a.kv.table_stride + s_from[j] + p];
+            }
+            returned += back_all;
+            __syncthreads();
+        }
+    }
+    const long long count = min(had + returned, static_cast<long long>(a.free_capacity));
+    long long needed = 0, asked = 0, taken = 0;
+    for (int base = 0; base < batch; base += kThreads) {
+        const int b = base + tid;
+        if (!once) load(base);
+        const int need_upto = static_cast<int>(upto >> 32);
+        const bool given = w.fits && (need == 0 || needed + need_upto <= count);
+        const int got = given ? static_cast<int>(w.add) : 0;
+        const int end = static_cast<int>(min(asked + tokens, static_cast<long long>(a.n_tokens)));
+        s_sum[tid] = need_upto;
+        s_from[tid] = w.held - (need_upto - need);
         s_given[tid] = given;
+        s_ends.end[tid] = end;
         if (b < batch) {
-            const int got = given ? static_cast<int>(w.add) : 0;
             if (b == 0) a.offsets[0] = 0;
-            a.offsets[b + 1] = static_cast<int>(min(tokens_all + tokens, static_cast<long long>(a.n_tokens)));
+            a.offsets[b + 1] = end;
             a.held_out[b] = given ? w.want : w.held;
             if (a.granted) a.granted[b] = got;
             if (a.seen_out) a.seen_out[b] = w.done ? 0 : seen + got;
@@ -164,35 +186,35 @@ __global__ void __launch_bounds__(kThreads) kv_plan_kernel(const PlanArgs a) {
             a.state[b] = given ? w.length : -1;
             a.state[batch + b] = seen;
         }
-        __syncthreads();
-        const long long reach = min(total, count - need_all);
-        for (long long p = tid; p < reach; p += kThreads) {
-            const int j = first_above(s_sum, n, p);
-            if (s_given[j])
-                table[(base + j) * a.kv.table_stride + s_from[j] + static_cast<int>(p)] = a.free_pages[count - 1 - need_all - p];
-        }
         // those that got pages come before those that did not
-        const long long mine = given && need > 0 ? upto : 0;
-        long long most = mine;
-#pragma unroll
-        for (int i = 16; i; i >>= 1) most = max(most, __shfl_xor_sync(kFullMask, most, i));
+        const int most = __reduce_max_sync(kFullMask, given && need ? need_upto : 0);
+        if ((tid & 31) == 0) s_most[tid >> 5] = most;
         __syncthreads();
-        if ((tid & 31) == 0) s_sum[tid >> 5] = most;
-        __syncthreads();
-        for (int i = 0; i < kThreads / 32; ++i) taken = max(taken, s_sum[i] > 0 ? need_all + s_sum[i] : 0ll);
-        need_all += total;
-        tokens_all += total_tokens;
+        const int most_of_all = __reduce_max_sync(kFullMask, s_most[tid & 31]);
+        if (most_of_all) taken = needed + most_of_all;
+        for (int p = tid; p < most_of_all; p += kThreads) {
+            const int j = first_above(s_sum, min(kThreads, batch - base), p);
+            if (s_given[j]) table[(base + j) * a.kv.table_stride + s_from[j] + p] = a.free_pages[count - 1 - needed - p];
+        }
+        needed += need_all;
+        asked += total_tokens;
         __syncthreads();
     }
     if (tid == 0) *a.free_count_out = static_cast<int>(count - taken);
     if (a.n_slots > kAtOnce) return;
-    for (int t = tid; t < a.n_slots; t += kThreads) slot_of(a, t, batch, a.offsets);
+    for (int t = tid; t < a.n_slots; t += kThreads) slot_of(a, t, once ? s_ends.end : a.offsets + 1);
 }
 
 __global__ void __launch_bounds__(kSlotThreads) kv_slots_kernel(const PlanArgs a) {
+    __shared__ Ends s_ends;
     pdl_wait_prior_grid();
+    const bool once = a.kv.batch <= kThreads;
+    if (once) {
+        for (int b = threadIdx.x; b < a.kv.batch; b += kSlotThreads) s_ends.end[b] = a.offsets[b + 1];
+        __syncthreads();
+    }
     const int t = blockIdx.x * kSlotThreads + threadIdx.x;
-    if (t < a.n_slots) slot_of(a, t, a.kv.batch, a.offsets);
+    if (t < a.n_slots) slot_of(a, t, once ? s_ends.end : a.offsets + 1);
 }
 
 }  // namespace

@@ -33,7 +33,12 @@ struct RopeArgs {
     const long long *slots;
     int n_pages, page_size;
     long long page_stride;
+    // items of a row and rows of a token: x / n = x * magic >> 32 for x * n < 2^32 and n > 1
+    int per_row[3];
+    unsigned row_magic[3], head_magic[3];
 };
+
+__device__ __forceinline__ int divide(int x, int n, unsigned magic) { return n == 1 ? x : static_cast<int>(__umulhi(x, magic)); }
 
 // cos and sin of a phase in units of 2^-64 turns. The phase is a whole number,
 // so nothing of a far position's angle is lost; its nearest quarter turn is
@@ -90,7 +95,7 @@ __device__ __forceinline__ void store(char *row, int i, int dtype, const float *
 template <typename T, int V, bool kNext>
 __global__ void __launch_bounds__(kThreads) rope_kernel(const RopeArgs a) {
     extern __shared__ float2 s_cs[];                   // [tokens][rot / 2]
-    __shared__ long long s_row[kMaxTokens];            // a token's row of a pool's head 0, in rows; -1: none
+    __shared__ long long s_row[kMaxTokens];            // byte offset of a token's row of a pool's head 0; -1: none
     const int half = a.rot / 2, first = blockIdx.x * a.tokens, tokens = min(a.tokens, a.n_tokens - first);
     for (int i = threadIdx.x; i < tokens * half; i += kThreads) {
         const int t = i / half, f = i - t * half;
@@ -100,24 +105,26 @@ __global__ void __launch_bounds__(kThreads) rope_kernel(const RopeArgs a) {
     }
     if (a.slots && static_cast<int>(threadIdx.x) < tokens) {
         const long long s = a.slots[first + threadIdx.x];
-        s_row[threadIdx.x] = s >= 0 && s < static_cast<long long>(a.n_pages) * a.page_size ? s : -1;
+        const long long page = s / a.page_size;
+        s_row[threadIdx.x] = s >= 0 && page < a.n_pages ? page * a.page_stride + (s - page * a.page_size) * a.side[1].out_token : -1;
     }
     __syncthreads();
-    const int turned = half / V, copied = (a.head_dim - a.rot) / (V == 8 ? 8 : 1);
+    const int turned = half / V;
 #pragma unroll
     for (int part = 0; part < 3; ++part) {
         const Side &s = a.side[part];
         if (!s.in) continue;
-        const int per_row = part == 2 ? a.head_dim / 8 : turned + copied, per_token = per_row * s.heads;
-        for (int i = threadIdx.x; i < per_token * tokens; i += kThreads) {
-            const int t = i / per_token, r = i - t * per_token, h = r / per_row, c = r - h * per_row;
+        const int per_row = a.per_row[part], items = per_row * s.heads * tokens;
+#pragma unroll 1
+        for (int i = threadIdx.x; i < items; i += kThreads) {
+            const int r = divide(i, per_row, a.row_magic[part]), c = i - r * per_row;
+            const int t = divide(r, s.heads, a.head_magic[part]), h = r - t * s.heads;
             const char *in = s.in + (first + t) * s.in_token + h * s.in_head;
             char *out;
             if (s.stored) {
                 const long long row = s_row[t];
                 if (row < 0) continue;
-                const long long page = row / a.page_size;
-                out = s.out + page * a.page_stride + h * s.out_head + (row - page * a.page_size) * s.out_token;
+                out = s.out + row + h * s.out_head;
             } else {
                 out = s.out + (first + t) * s.out_token + h * s.out_head;
             }
@@ -167,11 +174,16 @@ __global__ void __launch_bounds__(kThreads) rope_kernel(const RopeArgs a) {
 }
 
 template <typename T>
-cudaError_t launch(const RopeArgs &a, bool interleaved, cudaStream_t stream) {
+cudaError_t launch(RopeArgs &a, bool interleaved, cudaStream_t stream) {
     const int smem = a.tokens * a.rot / 2 * static_cast<int>(sizeof(float2));
     const int grid = (a.n_tokens - 1) / a.tokens + 1;
     // eight pairs of a row at a time need rows cut at multiples of 16 bytes
     const bool wide = a.rot % 16 == 0;
+    for (int i = 0; i < 3; ++i) {
+        a.per_row[i] = i == 2 ? a.head_dim / 8 : wide ? a.rot / 16 + (a.head_dim - a.rot) / 8 : a.rot / 2 + a.head_dim - a.rot;
+        a.row_magic[i] = static_cast<unsigned>((1ull << 32) / static_cast<unsigned>(a.per_row[i])) + 1;
+        a.head_magic[i] = a.side[i].heads ? static_cast<unsigned>((1ull << 32) / static_cast<unsigned>(a.side[i].heads)) + 1 : 0;
+    }
     if (interleaved) {
         if (wide) rope_kernel<T, 8, true><<<grid, kThreads, smem, stream>>>(a);
         else rope_kernel<T, 1, true><<<grid, kThreads, smem, stream>>>(a);
@@ -207,14 +219,14 @@ int rope_validate(const b200_kv_t *kv, const b200_rope_t *a, const char **why) {
     };
     const char *aligned = "rows' addresses and strides must be multiples of 16 bytes and not negative";
     if (a->q) {
-        if (a->n_head < 1 || a->n_head > 65536) return bad("n_head must be in [1, 65536]");
+        if (a->n_head < 1 || a->n_head > 4096) return bad("n_head must be in [1, 4096]");
         if (!a->q_out) return bad("q without q_out");
         if (!rows_ok(a->q, a->q_token_stride, a->q_head_stride, es) ||
             !rows_ok(a->q_out, a->q_out_token_stride, a->q_out_head_stride, eo))
             return bad(aligned);
     }
     if (a->k) {
-        if (a->n_head_kv < 1 || a->n_head_kv > 65536) return bad("n_head_kv must be in [1, 65536]");
+        if (a->n_head_kv < 1 || a->n_head_kv > 4096) return bad("n_head_kv must be in [1, 4096]");
         if (!rows_ok(a->k, a->k_token_stride, a->k_head_stride, es)) return bad(aligned);
         if (!kv) {
             if (!a->k_out) return bad("k without k_out or a cache");
