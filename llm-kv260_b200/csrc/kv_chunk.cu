@@ -8,7 +8,8 @@ namespace b200 {
 namespace {
 
 chunk::Shape shape_of(const b200_kv_t *kv, int dtype) {
-    return dtype == B200_F32 ? chunk::f32_shape(kv->head_dim) : chunk::mma_shape(kv->head_dim);
+    if (dtype != B200_F32) return chunk::mma_shape(kv->head_dim);
+    return kv->dtype == B200_F32 ? chunk::f32_shape(kv->head_dim) : chunk::split_shape(kv->head_dim);
 }
 
 uint64_t workspace_bytes(const b200_kv_t *kv, int dtype) {
@@ -68,7 +69,8 @@ cudaError_t kv_chunk_launch(const b200_kv_t *kv, const b200_kv_chunk_t *p, cudaS
     a.parts = reinterpret_cast<float *>(p->workspace);
     a.joints = reinterpret_cast<chunk::Joint *>(p->workspace + s.grid * 2 * s.part);
     a.status = status_word();
-    return p->dtype == B200_F32 ? chunk::f32_launch(a, kv->dtype, stream) : chunk::mma_launch(a, kv->dtype, stream);
+    if (p->dtype != B200_F32) return chunk::mma_launch(a, kv->dtype, stream);
+    return kv->dtype == B200_F32 ? chunk::f32_launch(a, stream) : chunk::split_launch(a, stream);
 }
 
 }  // namespace b200

@@ -319,16 +319,18 @@ cudaError_t launch_join(const Args &a, int grid, cudaStream_t stream) {
 }
 
 // Each launches calls of its types: kv_chunk_mma.cu those with 16-bit queries,
-// kv_chunk_f32.cu those with float32 queries; grid in CTAs and bytes of a part
-// of its tiles for the workspace.
+// kv_chunk_split.cu float32 queries with a float16 cache, kv_chunk_f32.cu all in
+// float32; grid in CTAs and bytes of a part of its tiles for the workspace.
 struct Shape {
     int grid;
     long long part;
 };
 Shape mma_shape(int head_dim);
 cudaError_t mma_launch(const Args &a, int kv_dtype, cudaStream_t stream);
+Shape split_shape(int head_dim);
+cudaError_t split_launch(const Args &a, cudaStream_t stream);
 Shape f32_shape(int head_dim);
-cudaError_t f32_launch(const Args &a, int kv_dtype, cudaStream_t stream);
+cudaError_t f32_launch(const Args &a, cudaStream_t stream);
 
 }  // namespace chunk
 }  // namespace b200

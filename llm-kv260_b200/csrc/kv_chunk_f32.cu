@@ -31,7 +31,7 @@ __device__ __forceinline__ void load8(const char *p, float *v) {
 // 64 rows by 64 slots at a time, 16 x 16 threads: a thread has the scores of
 // rows 4 ty + i and slots tx + 16 j, and of the output the columns 4 tx + 64 j.
 // One pass over the slots with the running maximum m and sum l of each row.
-template <typename TQ, typename TK, int kDim>
+template <int kDim>
 __global__ void __launch_bounds__(kThreads, 1) f32_kernel(const Args a) {
     extern __shared__ char smem_raw[];
     Smem<kDim> &s = *reinterpret_cast<Smem<kDim> *>(smem_raw);
@@ -53,7 +53,7 @@ __global__ void __launch_bounds__(kThreads, 1) f32_kernel(const Args a) {
             float v[8] = {};
             if (row0 + r < rows && c < d) {
                 const int token = (row0 + r) / a.group, h = row0 + r - token * a.group;
-                load8<TQ>(a.q + (q.from + token) * a.q_token + (head * a.group + h) * a.q_head + c * static_cast<int>(sizeof(TQ)), v);
+                load8<float>(a.q + (q.from + token) * a.q_token + (head * a.group + h) * a.q_head + c * static_cast<int>(sizeof(float)), v);
             }
             *reinterpret_cast<float4 *>(&s.q[r][c]) = make_float4(v[0], v[1], v[2], v[3]);
             *reinterpret_cast<float4 *>(&s.q[r][c + 4]) = make_float4(v[4], v[5], v[6], v[7]);
@@ -81,8 +81,8 @@ __global__ void __launch_bounds__(kThreads, 1) f32_kernel(const Args a) {
                 const int r = i / (kDim / 8), c = i % (kDim / 8) * 8;
                 float x[8] = {}, y[8] = {};
                 if (s.row[r] >= 0 && c < d) {
-                    load8<TK>(a.kv.k + s.row[r] + c * static_cast<int>(sizeof(TK)), x);
-                    load8<TK>(a.kv.v + s.row[r] + c * static_cast<int>(sizeof(TK)), y);
+                    load8<float>(a.kv.k + s.row[r] + c * static_cast<int>(sizeof(float)), x);
+                    load8<float>(a.kv.v + s.row[r] + c * static_cast<int>(sizeof(float)), y);
                 }
                 *reinterpret_cast<float4 *>(&s.k[r][c]) = make_float4(x[0], x[1], x[2], x[3]);
                 *reinterpret_cast<float4 *>(&s.k[r][c + 4]) = make_float4(x[4], x[5], x[6], x[7]);
@@ -169,7 +169,7 @@ __global__ void __launch_bounds__(kThreads, 1) f32_kernel(const Args a) {
 #pragma unroll
                 for (int j = 0; j < kDim / 64; ++j)
                     if (4 * tx + 64 * j < d)
-                        store4<TQ>(out + (4 * tx + 64 * j) * static_cast<int>(sizeof(TQ)),
+                        store4<float>(out + (4 * tx + 64 * j) * static_cast<int>(sizeof(float)),
                                    make_float4(o[i][4 * j] * inv, o[i][4 * j + 1] * inv, o[i][4 * j + 2] * inv, o[i][4 * j + 3] * inv));
                 if (a.lse && tx == 0)
                     a.lse[static_cast<long long>(q.from + token) * a.n_head + h] = (m[i] + log2f(l[i])) * kLn2;
@@ -196,22 +196,14 @@ __global__ void __launch_bounds__(kThreads, 1) f32_kernel(const Args a) {
 
 int grid_of(int) { return sm_count(); }
 
-template <typename TQ, typename TK, int kDim>
+template <int kDim>
 cudaError_t launch(const Args &a, cudaStream_t stream) {
-    const auto fn = f32_kernel<TQ, TK, kDim>;
+    const auto fn = f32_kernel<kDim>;
     const int smem = static_cast<int>(sizeof(Smem<kDim>)), grid = grid_of(kDim);
     if (!ensure_smem(reinterpret_cast<const void *>(fn), smem)) return cudaGetLastError();
     fn<<<grid, kThreads, smem, stream>>>(a);
     const cudaError_t e = cudaGetLastError();
-    return e != cudaSuccess ? e : launch_join<TQ, kM, kDim>(a, grid, stream);
-}
-
-template <typename TQ, typename TK>
-cudaError_t launch(const Args &a, cudaStream_t stream) {
-    if (a.kv.head_dim <= 64) return launch<TQ, TK, 64>(a, stream);
-    if (a.kv.head_dim <= 128) return launch<TQ, TK, 128>(a, stream);
-    if (a.kv.head_dim <= 192) return launch<TQ, TK, 192>(a, stream);
-    return launch<TQ, TK, 256>(a, stream);
+    return e != cudaSuccess ? e : launch_join<float, kM, kDim>(a, grid, stream);
 }
 
 }  // namespace
@@ -221,8 +213,11 @@ Shape f32_shape(int head_dim) {
     return Shape{grid_of(dim), part_floats(kM, dim) * 4};
 }
 
-cudaError_t f32_launch(const Args &a, int kv_dtype, cudaStream_t stream) {
-    return kv_dtype == B200_F32 ? launch<float, float>(a, stream) : launch<float, __half>(a, stream);
+cudaError_t f32_launch(const Args &a, cudaStream_t stream) {
+    if (a.kv.head_dim <= 64) return launch<64>(a, stream);
+    if (a.kv.head_dim <= 128) return launch<128>(a, stream);
+    if (a.kv.head_dim <= 192) return launch<192>(a, stream);
+    return launch<256>(a, stream);
 }
 
 }  // namespace chunk
