@@ -14,18 +14,13 @@ constexpr int kCost = 1;               // units that a tile's begin and end take
 template <int kDim>
 struct Smem {
     float q[kM][kDim + 4], k[kN][kDim + 4], v[kN][kDim + 4], p[kM][kN + 4];
-    long long row[kN];                 // byte offset of a slot's row, -1: not there
+    long long row[2][kN];              // byte offset of a slot's row, -1: not there
     Shared<kThreads> find;
 };
 
-template <typename T>
-__device__ __forceinline__ void load8(const char *p, float *v) {
-    uint4 w[sizeof(T) / 2];
-#pragma unroll
-    for (int i = 0; i < static_cast<int>(sizeof(T) / 2); ++i) w[i] = reinterpret_cast<const uint4 *>(p)[i];
-    const T *e = reinterpret_cast<const T *>(w);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = to_float(e[i]);
+// 16 bytes from global memory, or zeros.
+__device__ __forceinline__ void copy16(float *dst, const void *src, bool there) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_addr(dst)), "l"(src), "r"(there ? 16 : 0) : "memory");
 }
 
 // 64 rows by 64 slots at a time, 16 x 16 threads: a thread has the scores of
@@ -48,15 +43,48 @@ __global__ void __launch_bounds__(kThreads, 1) f32_kernel(const Args a) {
         const Fragment f = fragment<kM, kN, kCost>(a, q, tile, skip, st.left);
         const int row0 = f.row0, rows = f.rows;
         if (f.u1 > f.u0) {
-        for (int i = tid; i < kM * (kDim / 8); i += kThreads) {
-            const int r = i / (kDim / 8), c = i % (kDim / 8) * 8;
-            float v[8] = {};
+        // Keys of the next unit come while this one's weights and outputs are computed, values while the next one's scores
+        // are; the rows are looked up a unit before.
+        const int *table = a.kv.table + q.b * a.kv.table_stride;
+        int page = -1;
+        const auto ask = [&](int u) {
+            const int slot = u * kN + tid;
+            page = -1;
+            if (tid < kN && u < f.u1 && slot < q.length) page = table[static_cast<int>((slot * a.page_magic) >> 40)];
+        };
+        const auto place = [&](int u) {
+            if (tid >= kN) return;
+            const int slot = u * kN + tid, col = static_cast<int>((slot * a.page_magic) >> 40);
+            const bool there = static_cast<unsigned>(page) < static_cast<unsigned>(a.kv.n_pages);
+            s.row[u & 1][tid] = there ? page * a.kv.page_stride + (slot - col * a.kv.page_size) * a.kv.row_stride : -1;
+        };
+        const auto copy = [&](const char *from, float (&to)[kN][kDim + 4], int u) {
+            if (u < f.u1) {
+#pragma unroll 4
+                for (int i = tid; i < kN * (kDim / 4); i += kThreads) {
+                    const int r = i / (kDim / 4), c = i % (kDim / 4) * 4;
+                    const long long at = s.row[u & 1][r];
+                    const bool there = at >= 0 && c < d;
+                    copy16(&to[r][c], from + (there ? at + c * 4 : 0), there);
+                }
+            }
+            cp_async_commit();
+        };
+        const char *k_head = a.kv.k + head * a.kv.head_stride, *v_head = a.kv.v + head * a.kv.head_stride;
+        ask(f.u0);
+        place(f.u0);
+        ask(f.u0 + 1);
+        __syncthreads();
+        copy(k_head, s.k, f.u0);
+        copy(v_head, s.v, f.u0);
+        for (int i = tid; i < kM * (kDim / 4); i += kThreads) {
+            const int r = i / (kDim / 4), c = i % (kDim / 4) * 4;
+            float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
             if (row0 + r < rows && c < d) {
                 const int token = (row0 + r) / a.group, h = row0 + r - token * a.group;
-                load8<float>(a.q + (q.from + token) * a.q_token + (head * a.group + h) * a.q_head + c * static_cast<int>(sizeof(float)), v);
+                v = *reinterpret_cast<const float4 *>(a.q + (q.from + token) * a.q_token + (head * a.group + h) * a.q_head + c * 4);
             }
-            *reinterpret_cast<float4 *>(&s.q[r][c]) = make_float4(v[0], v[1], v[2], v[3]);
-            *reinterpret_cast<float4 *>(&s.q[r][c + 4]) = make_float4(v[4], v[5], v[6], v[7]);
+            *reinterpret_cast<float4 *>(&s.q[r][c]) = v;
         }
         int at[4];                                     // the slots that rows stand at
         float m[4], l[4], o[4][kDim / 16];
@@ -71,25 +99,11 @@ __global__ void __launch_bounds__(kThreads, 1) f32_kernel(const Args a) {
         }
 #pragma unroll 1
         for (int u = f.u0; u < f.u1; ++u) {
+            cp_async_wait<1>();                        // the keys; the values may be on their way
             __syncthreads();
-            if (tid < kN) {
-                const int slot = u * kN + tid;
-                s.row[tid] = slot < q.length ? kv_row(a.kv, q.b, head, slot) : -1;
-            }
-            __syncthreads();
-            for (int i = tid; i < kN * (kDim / 8); i += kThreads) {
-                const int r = i / (kDim / 8), c = i % (kDim / 8) * 8;
-                float x[8] = {}, y[8] = {};
-                if (s.row[r] >= 0 && c < d) {
-                    load8<float>(a.kv.k + s.row[r] + c * static_cast<int>(sizeof(float)), x);
-                    load8<float>(a.kv.v + s.row[r] + c * static_cast<int>(sizeof(float)), y);
-                }
-                *reinterpret_cast<float4 *>(&s.k[r][c]) = make_float4(x[0], x[1], x[2], x[3]);
-                *reinterpret_cast<float4 *>(&s.k[r][c + 4]) = make_float4(x[4], x[5], x[6], x[7]);
-                *reinterpret_cast<float4 *>(&s.v[r][c]) = make_float4(y[0], y[1], y[2], y[3]);
-                *reinterpret_cast<float4 *>(&s.v[r][c + 4]) = make_float4(y[4], y[5], y[6], y[7]);
-            }
-            __syncthreads();
+            const long long *row = s.row[u & 1];
+            place(u + 1);
+            ask(u + 2);
             float t[4][4] = {};
 #pragma unroll 4
             for (int c = 0; c < kDim; c += 4) {
@@ -104,6 +118,8 @@ __global__ void __launch_bounds__(kThreads, 1) f32_kernel(const Args a) {
                     for (int j = 0; j < 4; ++j)
                         t[i][j] = fmaf(x[i].w, y[j].w, fmaf(x[i].z, y[j].z, fmaf(x[i].y, y[j].y, fmaf(x[i].x, y[j].x, t[i][j]))));
             }
+            __syncthreads();                           // the keys have been read
+            copy(k_head, s.k, u + 1);
             const bool edge = (u + 1) * kN - 1 > f.last_all || u * kN < f.first_all;
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
@@ -112,7 +128,7 @@ __global__ void __launch_bounds__(kThreads, 1) f32_kernel(const Args a) {
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
                     const int slot = u * kN + tx + 16 * j;
-                    dead[j] = s.row[tx + 16 * j] < 0 || slot > at[i] || (a.window && slot <= at[i] - a.window);
+                    dead[j] = row[tx + 16 * j] < 0 || slot > at[i] || (a.window && slot <= at[i] - a.window);
                     t[i][j] = dead[j] ? -INFINITY : t[i][j] * a.scale;
                     top = fmaxf(top, t[i][j]);
                 }
@@ -134,7 +150,8 @@ __global__ void __launch_bounds__(kThreads, 1) f32_kernel(const Args a) {
 #pragma unroll
                 for (int j = 0; j < kDim / 16; ++j) o[i][j] *= keep;
             }
-            __syncwarp();                              // a row's 16 threads are in one warp
+            cp_async_wait<1>();                        // the values
+            __syncthreads();
 #pragma unroll 2
             for (int n = 0; n < kN; n += 4) {
                 float4 p[4];
@@ -157,7 +174,10 @@ __global__ void __launch_bounds__(kThreads, 1) f32_kernel(const Args a) {
                     }
                 }
             }
+            __syncthreads();                           // the values have been read
+            copy(v_head, s.v, u + 1);
         }
+        cp_async_wait<0>();
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             const int r = ty * 4 + i;
