@@ -401,13 +401,13 @@ B200_API int b200_rms_norm(b200_engine_t *e, const b200_rms_norm_t *a);
  * before they meet the values (as much as the output is), with float32 queries
  * nothing is rounded. */
 typedef struct {
-    uint64_t q, out;                   /* [n_tokens][n_head][head_dim], strides in elements, rows contiguous;
-                                          addresses and strides are multiples of 16 bytes */
+    uint64_t q, out;                   /* [n_tokens][n_head][head_dim], strides in elements, rows contiguous, without
+                                          overlap; addresses and strides are multiples of 16 bytes */
     int dtype;                         /* of both: the cache's type, or B200_F32 with a B200_F16 cache */
-    int n_tokens, n_head;              /* n_head: a multiple of n_head_kv */
+    int n_tokens, n_head;              /* n_head: a multiple of n_head_kv, at most 4096 times it */
     int64_t q_token_stride, q_head_stride, out_token_stride, out_head_stride;
     uint64_t offsets;                  /* int32 [batch + 1], as in b200_kv_append_t */
-    float scale;                       /* positive */
+    float scale;                       /* positive, 1e-37 to 1e37 */
     int window;                        /* 0: none */
     uint64_t lse;                      /* float [n_tokens][n_head], or 0 */
     uint64_t workspace;                /* b200_kv_chunk_workspace() bytes, 16-byte aligned; holds nothing between calls */

@@ -1,4 +1,9 @@
-// b200_kv_attend_chunk on the float32 units.
+// b200_kv_attend_chunk in float32 throughout, on the float32 units: every bit of
+// queries and cache counts, and three products of parts at half the tensor
+// cores' 16-bit rate would not be faster. What bounds it: float32 operations and
+// the shared-memory reads that feed them (12 of 128 bytes for 64 operations of a
+// warp), with 8 warps an SM. 2000 tokens, 32 heads of 128: 1080 us, 30 TFLOP/s
+// (41 % of what the units can do); 33 with heads of 256.
 #include <cuda_runtime.h>
 
 #include "kv_chunk.cuh"
@@ -8,11 +13,14 @@ namespace chunk {
 
 namespace {
 
-constexpr int kM = 64, kN = 64, kThreads = 256;
+constexpr int kN = 64, kThreads = 256;
+// Rows of a thread: eight, half as many reads for an operation as four, where a tile of 128 rows fits shared memory.
+__host__ __device__ constexpr int rows_of(int dim) { return dim <= 128 ? 8 : 4; }
 constexpr int kCost = 1;               // units that a tile's begin and end take
 
 template <int kDim>
 struct Smem {
+    static constexpr int kM = 16 * rows_of(kDim);
     float q[kM][kDim + 4], k[kN][kDim + 4], v[kN][kDim + 4], p[kM][kN + 4];
     long long row[2][kN];              // byte offset of a slot's row, -1: not there
     Shared<kThreads> find;
@@ -23,13 +31,15 @@ __device__ __forceinline__ void copy16(float *dst, const void *src, bool there) 
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_addr(dst)), "l"(src), "r"(there ? 16 : 0) : "memory");
 }
 
-// 64 rows by 64 slots at a time, 16 x 16 threads: a thread has the scores of
-// rows 4 ty + i and slots tx + 16 j, and of the output the columns 4 tx + 64 j.
+// 64 slots by 128 rows (64) at a time, 16 x 16 threads: a thread has the scores
+// of rows 8 ty + i (4 ty + i) and slots tx + 16 j, and of the output the columns
+// 4 tx + 64 j.
 // One pass over the slots with the running maximum m and sum l of each row.
 template <int kDim>
 __global__ void __launch_bounds__(kThreads, 1) f32_kernel(const Args a) {
     extern __shared__ char smem_raw[];
     Smem<kDim> &s = *reinterpret_cast<Smem<kDim> *>(smem_raw);
+    constexpr int kRows = rows_of(kDim), kM = 16 * kRows;
     const int tid = threadIdx.x, tx = tid & 15, ty = tid >> 4, d = a.kv.head_dim;
     Stretch st = find<kM, kN, kCost, kThreads>(a, &s.find);
     if (tid == 0) a.joints[blockIdx.x].first = -1;
@@ -86,11 +96,11 @@ __global__ void __launch_bounds__(kThreads, 1) f32_kernel(const Args a) {
             }
             *reinterpret_cast<float4 *>(&s.q[r][c]) = v;
         }
-        int at[4];                                     // the slots that rows stand at
-        float m[4], l[4], o[4][kDim / 16];
+        int at[kRows];                                     // the slots that rows stand at
+        float m[kRows], l[kRows], o[kRows][kDim / 16];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const int r = row0 + ty * 4 + i;
+        for (int i = 0; i < kRows; ++i) {
+            const int r = row0 + ty * kRows + i;
             at[i] = r < rows ? f.first + r / a.group : -1;
             m[i] = -INFINITY;
             l[i] = 0.0f;
@@ -104,16 +114,16 @@ __global__ void __launch_bounds__(kThreads, 1) f32_kernel(const Args a) {
             const long long *row = s.row[u & 1];
             place(u + 1);
             ask(u + 2);
-            float t[4][4] = {};
+            float t[kRows][4] = {};
 #pragma unroll 4
             for (int c = 0; c < kDim; c += 4) {
-                float4 x[4], y[4];
+                float4 x[kRows], y[4];
 #pragma unroll
-                for (int i = 0; i < 4; ++i) x[i] = *reinterpret_cast<const float4 *>(&s.q[ty * 4 + i][c]);
+                for (int i = 0; i < kRows; ++i) x[i] = *reinterpret_cast<const float4 *>(&s.q[ty * kRows + i][c]);
 #pragma unroll
                 for (int j = 0; j < 4; ++j) y[j] = *reinterpret_cast<const float4 *>(&s.k[tx + 16 * j][c]);
 #pragma unroll
-                for (int i = 0; i < 4; ++i)
+                for (int i = 0; i < kRows; ++i)
 #pragma unroll
                     for (int j = 0; j < 4; ++j)
                         t[i][j] = fmaf(x[i].w, y[j].w, fmaf(x[i].z, y[j].z, fmaf(x[i].y, y[j].y, fmaf(x[i].x, y[j].x, t[i][j]))));
@@ -122,7 +132,7 @@ __global__ void __launch_bounds__(kThreads, 1) f32_kernel(const Args a) {
             copy(k_head, s.k, u + 1);
             const bool edge = (u + 1) * kN - 1 > f.last_all || u * kN < f.first_all;
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
+            for (int i = 0; i < kRows; ++i) {
                 float top = -INFINITY;
                 bool dead[4];
 #pragma unroll
@@ -140,7 +150,7 @@ __global__ void __launch_bounds__(kThreads, 1) f32_kernel(const Args a) {
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
                     const float p = exp2f(t[i][j] - ref);
-                    s.p[ty * 4 + i][tx + 16 * j] = p;
+                    s.p[ty * kRows + i][tx + 16 * j] = p;
                     sum += p;
                 }
 #pragma unroll
@@ -154,16 +164,16 @@ __global__ void __launch_bounds__(kThreads, 1) f32_kernel(const Args a) {
             __syncthreads();
 #pragma unroll 2
             for (int n = 0; n < kN; n += 4) {
-                float4 p[4];
+                float4 p[kRows];
 #pragma unroll
-                for (int i = 0; i < 4; ++i) p[i] = *reinterpret_cast<const float4 *>(&s.p[ty * 4 + i][n]);
+                for (int i = 0; i < kRows; ++i) p[i] = *reinterpret_cast<const float4 *>(&s.p[ty * kRows + i][n]);
 #pragma unroll
                 for (int x = 0; x < 4; ++x) {
 #pragma unroll
                     for (int j = 0; j < kDim / 64; ++j) {
                         const float4 v = *reinterpret_cast<const float4 *>(&s.v[n + x][4 * tx + 64 * j]);
 #pragma unroll
-                        for (int i = 0; i < 4; ++i) {
+                        for (int i = 0; i < kRows; ++i) {
                             const float w = x == 0 ? p[i].x : x == 1 ? p[i].y : x == 2 ? p[i].z : p[i].w;
                             if (edge && w == 0.0f) continue;           // not seen: whatever the value is
                             o[i][4 * j] = fmaf(w, v.x, o[i][4 * j]);
@@ -179,8 +189,8 @@ __global__ void __launch_bounds__(kThreads, 1) f32_kernel(const Args a) {
         }
         cp_async_wait<0>();
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const int r = ty * 4 + i;
+        for (int i = 0; i < kRows; ++i) {
+            const int r = ty * kRows + i;
             if (row0 + r >= rows) break;
             const int token = (row0 + r) / a.group, h = head * a.group + row0 + r - token * a.group;
             if (f.whole) {
@@ -223,14 +233,14 @@ cudaError_t launch(const Args &a, cudaStream_t stream) {
     if (!ensure_smem(reinterpret_cast<const void *>(fn), smem)) return cudaGetLastError();
     fn<<<grid, kThreads, smem, stream>>>(a);
     const cudaError_t e = cudaGetLastError();
-    return e != cudaSuccess ? e : launch_join<float, kM, kDim>(a, grid, stream);
+    return e != cudaSuccess ? e : launch_join<float, 16 * rows_of(kDim), kDim>(a, grid, stream);
 }
 
 }  // namespace
 
 Shape f32_shape(int head_dim) {
     const int dim = (head_dim + 63) / 64 * 64;
-    return Shape{grid_of(dim), part_floats(kM, dim) * 4};
+    return Shape{grid_of(dim), part_floats(16 * rows_of(dim), dim) * 4};
 }
 
 cudaError_t f32_launch(const Args &a, cudaStream_t stream) {

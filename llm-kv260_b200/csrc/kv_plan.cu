@@ -116,8 +116,11 @@ __device__ __forceinline__ void slot_of(const PlanArgs &a, int t, const int *end
 // thread can move any page (a search in the sums of up to 1024 sequences finds
 // its owner) and the result does not depend on timing. Nothing here is long
 // enough to be bound by anything but the chain of dependent reads: the wishes,
-// the pages that move, the slots' pages. Up to 1024 sequences' wishes are read
-// and summed once, more of them twice.
+// the pages that move, the slots' pages (256 sequences: 9.5 us from a cold cache,
+// 13 with the wishes read and summed twice and the slots' search in global
+// memory; the call takes 15). Up to 1024 sequences' wishes are read and summed
+// once, more of them twice. Beyond 8192 tokens, eight to a thread, a second
+// kernel finds the slots (61 prompts of up to 4000 tokens: 4.5 us beside 10.5).
 __global__ void __launch_bounds__(kThreads) kv_plan_kernel(const PlanArgs a) {
     __shared__ int s_sum[kThreads], s_from[kThreads];
     __shared__ bool s_given[kThreads];

@@ -53,7 +53,10 @@ __device__ __forceinline__ void store8(char *row, int i, int dtype, const float 
 }
 
 // A CTA per row, J times eight elements in each thread's registers: one pass
-// over memory. Four neighbouring threads hold a Q8_0 block.
+// over memory, which bounds it (16384 rows of 4096 bfloat16 with their residual,
+// 537 MB: 96 us, 5.6 TB/s, with two units a thread; one 99, four 102). One row:
+// 4.5 us on the GPU, less than the call. Four neighbouring threads hold a Q8_0
+// block.
 template <typename T, int J, bool kStream>
 __global__ void rms_norm_kernel(const NormArgs a) {
     __shared__ float s_sum[32];
