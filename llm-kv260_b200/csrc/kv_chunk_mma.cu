@@ -739,6 +739,10 @@ __global__ void __launch_bounds__(kThreads, 1) mma_kernel(const Args a, const __
     tmem_fence_before();
     __syncthreads();
     tmem_fence_after();
+    if (s.dead) {                      // copies that were not waited for land before the memory is another CTA's
+        const uint64_t t0 = globaltimer_ns();
+        while (globaltimer_ns() - t0 < 1000000ull) {}
+    }
     if (warp == kThreads / 32 - 1) tmem_free(s.tmem, kColumns);
     if (tid == 0 && (s.tmem != 0 || (smem_addr(smem) & 1023))) atomicOr(a.status, kStatusStageTimeout);   // never
 }

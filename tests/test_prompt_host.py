@@ -64,3 +64,49 @@ def test_workspace_of_unusable_sizes(pkg):
                                   ({}, 1, 1), (dict(dtype=0), 1, 4), (dict(dtype=2), 0, 4), (dict(page_size=0), 1, 4)):
         kv = t(**dict(good, **change))
         assert lib.b200_kv_chunk_workspace(ctypes.byref(kv), dtype, n_head) == 0
+
+
+def test_arguments_refused_before_any_call(pkg, monkeypatch):
+    """Python's own checks, with a stand-in for the library that must not be reached."""
+    import torch
+    from llm_kv260_b200 import engine
+
+    from test_serving_host import FakeLib, FakeTensor
+
+    calls = []
+    lib = FakeLib()
+    lib.on_call = lambda name, c: calls.append(name)
+    monkeypatch.setattr(engine, "lib", lambda: lib)
+    eng = pkg.Engine(0, stream=0)
+
+    def t(*shape, dt=torch.float16, at=4096):
+        return FakeTensor(at, shape, dt)
+
+    class Cache:
+        batch, n_head_kv, head_dim, n_pages, page_size, capacity = 3, 2, 64, 4, 16, 32
+        lengths, ref, workspace = t(3, dt=torch.int32), None, {}
+
+    kv, i32 = Cache(), torch.int32
+    del calls[:]
+    q, off, pos, slots = t(5, 4, 64), t(4, dt=i32), t(5, dt=i32), t(5, dt=torch.int64)
+    freqs, new, free = t(32, dt=torch.int64), t(3, dt=i32), t(9, dt=i32)
+    x, w = t(3, 64, dt=torch.float32), t(64, dt=torch.float32)
+    for f in (lambda: eng.kv_attend_chunk(kv, t(5, 4), q, off), lambda: eng.kv_attend_chunk(kv, q, t(5, 4, 64, dt=torch.float32), off),
+              lambda: eng.kv_attend_chunk(kv, t(5, 4, 32), t(5, 4, 32), off), lambda: eng.kv_attend_chunk(kv, q, q, t(3, dt=i32)),
+              lambda: eng.kv_attend_chunk(kv, q, q, t(4, dt=torch.int64)), lambda: eng.kv_attend_chunk(kv, q, q, off, lse=t(5, 4)),
+              lambda: eng.rope(pos, freqs), lambda: eng.rope(t(4, dt=i32), freqs, q=q), lambda: eng.rope(pos, t(32, dt=i32), q=q),
+              lambda: eng.rope(pos, freqs, q=q, k=t(4, 2, 64)), lambda: eng.rope(pos, freqs, q=q, v=q),
+              lambda: eng.rope(pos, freqs, q=q, slots=slots), lambda: eng.rope(pos, freqs, q=q, q_out=t(5, 3, 64)),
+              lambda: eng.rope(pos, freqs, k=t(5, 2, 64), kv=kv, v=t(5, 2, 64, dt=torch.float32), slots=slots),
+              lambda: eng.rope(pos, t(4, 8, dt=torch.int64), q=q), lambda: eng.rms_norm(t(64), w, out=x),
+              lambda: eng.rms_norm(x, t(32, dt=torch.float32), out=x), lambda: eng.rms_norm(x, w, out=t(2, 64, dt=torch.float32)),
+              lambda: eng.rms_norm(x, w, residual_out=x), lambda: eng.rms_norm(x, w, residual=t(3, 64), residual_out=x),
+              lambda: eng.kv_plan(kv, t(2, dt=i32), new, free, t(1, dt=i32), off), lambda: eng.kv_plan(kv, new, new, t(3, 3, dt=i32), t(1, dt=i32), off),
+              lambda: eng.kv_plan(kv, new, new, free, t(2, dt=i32), off), lambda: eng.kv_plan(kv, new, new, free, t(1, dt=i32), off, slots=pos),
+              lambda: eng.kv_plan(kv, new, new, free, t(1, dt=i32), off, slots=slots, positions=t(4, dt=i32)),
+              lambda: eng.kv_plan(kv, new, new, free, t(1, dt=i32), off, sequences=t(5, 1, dt=i32))):
+        with pytest.raises(ValueError):
+            f()
+    assert not [c for c in calls if c != "b200_kv_chunk_workspace"]
+    eng.kv_plan(kv, new, new, free, t(1, dt=i32), off, slots=slots, positions=pos)
+    assert calls[-1] == "b200_kv_plan"
