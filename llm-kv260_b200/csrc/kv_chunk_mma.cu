@@ -469,7 +469,7 @@ __device__ __forceinline__ void softmax(const Args &a, Shared0 &s, char *smem, S
 #pragma unroll
             for (int c = 0; c < kWords; ++c) {
                 there[c] = 0xffffffffu;
-                if (gaps) {
+                if (__builtin_expect(gaps, 0)) {
                     const int slot = u * P::kN + c * 32 + lane;
                     there[c] = __ballot_sync(kFullMask, slot < q.length && there_of(slot));
                 }
@@ -480,7 +480,7 @@ __device__ __forceinline__ void softmax(const Args &a, Shared0 &s, char *smem, S
             wait(&s.s_full[buf], P::kTiles == 2 ? done : unit >> 1);
             __syncwarp();
             tmem_fence_after();
-            if (edge) {
+            if (__builtin_expect(edge, 0)) {
                 // A value that is not finite must not reach rows that do not see it, and 0 times it would: such values
                 // are taken out of the tile, and the rows that see them marked. (The scores are there, so the values of
                 // two units before were: a phase ahead at most, which is what a barrier can tell.)
@@ -534,7 +534,7 @@ __device__ __forceinline__ void softmax(const Args &a, Shared0 &s, char *smem, S
 #pragma unroll
             for (int c = 0; c < kWords; ++c) tmem_load32(lanes + P::scores(buf) + c * 32, x[c]);
             tmem_wait_load();
-            if (edge || gaps) {
+            if (__builtin_expect(edge || gaps, 0)) {
 #pragma unroll
                 for (int k = 0; k < P::kN; ++k)
                     if (k < lo || k > hi || !(there[k >> 5] >> (k & 31) & 1)) x[k >> 5][k & 31] = __float_as_uint(-INFINITY);
@@ -565,12 +565,12 @@ __device__ __forceinline__ void softmax(const Args &a, Shared0 &s, char *smem, S
                 }
             };
             bool moves = u == f.u0;
-            if (moves) {
+            if (__builtin_expect(moves, 0)) {
 #pragma unroll
                 for (int k = 0; k < P::kN; k += 2) look(k);
             }
             for (;;) {
-                if (moves) {
+                if (__builtin_expect(moves, 0)) {
                     const float m = fmaxf(max3(top[0], top[1], top[2]), top[3]) * a.scale;
                     const float next = fmaxf(ref, m - kLead);
                     const float keep = next == ref ? 1.0f : ex2(ref - next);
