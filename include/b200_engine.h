@@ -326,8 +326,8 @@ B200_API int b200_kv_plan(b200_engine_t *e, const b200_kv_t *kv, const b200_kv_p
  * cache, k's rotated rows go to its rows slots[t], and v's rows beside them,
  * both in the cache's type (a slot outside the pool, as -1, is dropped; k_out
  * is not used). q, k and v in float32 may go to any type, others to their own.
- * A row may go where it comes from; otherwise inputs and outputs do not
- * overlap. */
+ * A row may go where it comes from, in its own type and with the same strides;
+ * otherwise inputs and outputs do not overlap. */
 typedef struct {
     uint64_t q, q_out;                 /* [n_tokens][n_head][head_dim], strides in elements; 0: no q */
     int n_head;
@@ -375,10 +375,10 @@ B200_API int b200_rope_freqs(uint64_t *freqs, int rot_dim, double base, const fl
 typedef struct {
     uint64_t x;                        /* [n_rows][k], strides in elements, rows contiguous */
     int dtype;
-    uint64_t residual, residual_out;   /* or 0; may be the same */
+    uint64_t residual, residual_out;   /* or 0; may be the same, with the same stride */
     int residual_dtype;                /* dtype, or B200_F32 */
     uint64_t weight;                   /* float32 [k] */
-    uint64_t out;                      /* or 0; may be x */
+    uint64_t out;                      /* or 0; may be x, its rows as many bytes apart */
     int out_dtype;                     /* dtype, or any with B200_F32 */
     uint64_t q8;                       /* or 0 */
     int n_rows, k;                     /* k: a multiple of 8 (of 32 with q8), at most 32768 */

@@ -225,6 +225,11 @@ int rope_validate(const b200_kv_t *kv, const b200_rope_t *a, const char **why) {
     const auto rows_ok = [](uint64_t at, int64_t token, int64_t head, int size) {
         return token >= 0 && head >= 0 && at % 16 == 0 && token * size % 16 == 0 && head * size % 16 == 0;
     };
+    // in place, the thread that reads a pair writes it only where a row's elements stay where they are
+    const auto moved = [&](uint64_t in, int64_t token, int64_t head, uint64_t out, int64_t to_token, int64_t to_head, int heads) {
+        return in == out && (a->dtype != a->out_dtype || (a->n_tokens > 1 && token != to_token) || (heads > 1 && head != to_head));
+    };
+    const char *in_place = "rows in place keep their type and strides";
     const char *aligned = "rows' addresses and strides must be multiples of 16 bytes and not negative";
     if (a->q) {
         if (a->n_head < 1 || a->n_head > 4096) return bad("n_head must be in [1, 4096]");
@@ -232,6 +237,8 @@ int rope_validate(const b200_kv_t *kv, const b200_rope_t *a, const char **why) {
         if (!rows_ok(a->q, a->q_token_stride, a->q_head_stride, es) ||
             !rows_ok(a->q_out, a->q_out_token_stride, a->q_out_head_stride, eo))
             return bad(aligned);
+        if (moved(a->q, a->q_token_stride, a->q_head_stride, a->q_out, a->q_out_token_stride, a->q_out_head_stride, a->n_head))
+            return bad(in_place);
     }
     if (a->k) {
         if (a->n_head_kv < 1 || a->n_head_kv > 4096) return bad("n_head_kv must be in [1, 4096]");
@@ -239,6 +246,9 @@ int rope_validate(const b200_kv_t *kv, const b200_rope_t *a, const char **why) {
         if (!kv) {
             if (!a->k_out) return bad("k without k_out or a cache");
             if (!rows_ok(a->k_out, a->k_out_token_stride, a->k_out_head_stride, eo)) return bad(aligned);
+            if (moved(a->k, a->k_token_stride, a->k_head_stride, a->k_out, a->k_out_token_stride, a->k_out_head_stride,
+                      a->n_head_kv))
+                return bad(in_place);
         }
     }
     if (kv) {

@@ -688,3 +688,36 @@ def test_empty_calls(torch_mod, pkg, eng):
     eng.rms_norm(x, w, out=x, residual=x)
     s = torch.zeros(0, dtype=torch.int64, device="cuda")
     eng.rope(s.int(), pkg.rope_freqs(64).cuda(), q=c["q"][:0], k=c["q"][:0, :2], kv=c["cache"], v=c["q"][:0, :2], slots=s)
+
+
+def test_rows_in_place_that_would_move(torch_mod, pkg, eng):
+    """Rows that would be written over others still to be read are refused; a row's own place in another type is not."""
+    torch = torch_mod
+    eng.set_stream(torch.cuda.current_stream().cuda_stream)
+    g = torch.Generator().manual_seed(5)
+    buf = torch.randn(6, 4, 64, generator=g).cuda()
+    before, pos, freqs = buf.clone(), torch.arange(5, dtype=torch.int32).cuda(), pkg.rope_freqs(64).cuda()
+    half = buf.view(torch.float16)[:5, :, :64]           # as many bytes apart, of another type
+    apart = buf.as_strided((5, 2, 64), (2 * 256 // 2, 128, 1))
+    for q, out in ((buf[:5], half), (buf[:5, :2], buf.as_strided((5, 2, 64), (128, 64, 1))), (buf[:5, :2], apart)):
+        for kw in (dict(q=q, q_out=out), dict(k=q, k_out=out)):
+            with pytest.raises(pkg.B200Error):
+                eng.rope(pos, freqs, **kw)
+    x, w = buf.view(6, 256)[:, :64], torch.ones(64, device="cuda")
+    dense, res = buf.as_strided((6, 64), (64, 1)), torch.zeros(6, 256, device="cuda")
+    for kw in (dict(out=dense), dict(out=buf.view(torch.float16).as_strided((6, 64), (256, 1))),
+               dict(residual=res[:, :64], residual_out=res.as_strided((6, 64), (64, 1)))):
+        with pytest.raises(pkg.B200Error):
+            eng.rms_norm(x, w, **kw)
+    torch.cuda.synchronize()
+    assert torch.equal(buf, before)
+    # one row has no strides to differ by, and a row may change its type where it stands
+    want, got = torch.empty(1, 2, 64, device="cuda"), before[:1, :2].clone()
+    eng.rope(pos[3:4], freqs, q=before[:1, :2], q_out=want)
+    eng.rope(pos[3:4], freqs, q=got, q_out=got.as_strided((1, 2, 64), (256, 64, 1)))
+    assert torch.equal(got, want)
+    y = torch.empty(6, 64, dtype=torch.float16, device="cuda")
+    eng.rms_norm(x, w, out=y)
+    own = buf.view(torch.float16).view(6, 512)[:, :64]
+    eng.rms_norm(x, w, out=own)
+    assert torch.equal(own, y)
