@@ -68,9 +68,10 @@ B200_API int b200_engine_get_config(b200_engine_t *e, b200_engine_config_t *cfg)
 B200_API int b200_engine_set_config(b200_engine_t *e, const b200_engine_config_t *cfg);
 /* Queue work on the caller's cudaStream_t (NULL: the legacy default stream).
  * Until this is called the engine uses a non-blocking stream of its own.
- * Serving calls and graph launches on the new stream wait for those queued on
- * the old one, which must still exist (they share scratch); calls that are
- * being recorded do not. */
+ * Serving calls (b200_kv_*, b200_sample, b200_rope, b200_rms_norm) and graph
+ * launches on the new stream wait for those queued on the old one, which must
+ * still exist (they share scratch, and one reads what another wrote); calls
+ * that are being recorded do not. */
 B200_API int b200_engine_set_stream(b200_engine_t *e, void *stream);
 B200_API void *b200_engine_stream(b200_engine_t *e);
 

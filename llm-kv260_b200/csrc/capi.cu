@@ -498,7 +498,7 @@ bool capturing(cudaStream_t s) {
     return true;
 }
 
-// Before a call that shares the serving scratch.
+// Before a serving call: each shares the scratch with the others, or reads and writes what they write and read.
 int serve_begin(b200_engine_t *e) {
     if (e->behind && !capturing(e->stream)) {
         const cudaError_t err = cudaStreamWaitEvent(e->stream, e->handover, 0);
@@ -681,8 +681,8 @@ extern "C" int b200_engine_set_stream(b200_engine_t *e, void *stream) {
     if (!e) return fail(kErrInval, "engine not open");
     const cudaStream_t next = static_cast<cudaStream_t>(stream);  // NULL is the legacy default stream
     if (next == e->stream) return 0;
-    // The serving calls share tickets and workspaces, so the new stream's first one waits for those queued on the old
-    // stream. A recorded call runs when its graph is launched, which is not known here.
+    // The serving calls share tickets and workspaces and read what others have written, so the new stream's first one
+    // waits for those queued on the old stream. A recorded call runs when its graph is launched, which is not known here.
     if (e->serving && !capturing(e->stream)) {
         if (int rc = use_device(e->device)) return rc;
         cudaError_t err = e->behind ? cudaStreamWaitEvent(e->stream, e->handover, 0) : cudaSuccess;
@@ -934,6 +934,7 @@ extern "C" int b200_sample(b200_engine_t *e, const b200_sample_t *s) {
     const char *why = nullptr;
     if (sample_validate(s, &why)) return fail(kErrInval, "sample: %s", why);
     if (int rc = use_device(e->device)) return rc;
+    if (int rc = serve_begin(e)) return rc;
     const cudaError_t err = sample_launch(s, e->stream);
     return err == cudaSuccess ? 0 : cuda_fail(err, "sample launch");
 }
@@ -953,6 +954,7 @@ extern "C" int b200_rope(b200_engine_t *e, const b200_kv_t *kv, const b200_rope_
     const char *why = nullptr;
     if (rope_validate(kv, a, &why)) return fail(kErrInval, "rope: %s", why);
     if (int rc = use_device(e->device)) return rc;
+    if (int rc = serve_begin(e)) return rc;
     const cudaError_t err = rope_launch(kv, a, e->stream);
     return err == cudaSuccess ? 0 : cuda_fail(err, "rope launch");
 }
@@ -970,6 +972,7 @@ extern "C" int b200_rms_norm(b200_engine_t *e, const b200_rms_norm_t *a) {
     const char *why = nullptr;
     if (rms_norm_validate(a, &why)) return fail(kErrInval, "rms_norm: %s", why);
     if (int rc = use_device(e->device)) return rc;
+    if (int rc = serve_begin(e)) return rc;
     const cudaError_t err = rms_norm_launch(a, e->cfg.round_mode, e->stream);
     return err == cudaSuccess ? 0 : cuda_fail(err, "rms_norm launch");
 }

@@ -1,0 +1,74 @@
+"""The operators that a prompt passes through where neighbouring work, unusual numbers or unusual settings could change
+what they answer."""
+
+from __future__ import annotations
+
+import pytest
+
+from test_prompt_paths_gpu import STATE, step_case
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module")
+def torch_mod(cuda_lib):
+    import torch
+    torch.cuda.set_device(0)
+    return torch
+
+
+@pytest.fixture(scope="module")
+def eng(pkg, torch_mod):
+    e = pkg.Engine(0)
+    yield e
+    e.close()
+
+
+# ------------------------------------------------------------------ streams
+
+def test_calls_of_a_step_on_two_streams_follow_one_another(torch_mod, pkg):
+    """One engine whose stream changes between any two calls of a step: each waits for the one before, whose stream sleeps,
+    and reads what it wrote."""
+    torch = torch_mod
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    e = pkg.Engine(0, stream=streams[0].cuda_stream)
+    s = step_case(torch, pkg, 21)
+    h, hkv = s["h"], s["hkv"]
+    logits = torch.randn(4, 1000, device="cuda")
+    u, token = torch.rand(4, device="cuda"), torch.zeros(4, dtype=torch.int32, device="cuda")
+    s["new"].copy_(torch.tensor([40, 3, 30, 30, 17]))
+    calls = (
+        lambda: e.kv_plan(s["cache"], s["new"], s["held"], s["free"], s["free_count"], s["offsets"], slots=s["slots"],
+                          positions=s["positions"], granted=s["granted"]),
+        lambda: e.rms_norm(s["add"], s["w"], residual=s["x"], q8=s["q8"]),
+        lambda: e.rope(s["positions"], s["freqs"], q=s["qkv"][:, :h], q_out=s["q"], k=s["qkv"][:, h:h + hkv], kv=s["cache"],
+                       v=s["qkv"][:, h + hkv:], slots=s["slots"]),
+        lambda: e.kv_attend_chunk(s["cache"], s["q"], s["out"], s["offsets"], lse=s["lse"]),
+        lambda: e.sample(logits, u, token))
+    live = [s[k] for k in STATE] + [s["cache"].k, s["cache"].v, s["cache"].table, s["cache"].lengths, token]
+    fresh = [t.clone() for t in live]
+    torch.cuda.synchronize()
+    for call in calls:
+        call()
+    e.sync()
+    want = [t.clone() for t in live]
+    for asleep in range(len(calls)):
+        for t, old in zip(live, fresh):
+            t.copy_(old)
+        torch.cuda.synchronize()
+        for i, call in enumerate(calls):
+            stream = streams[i % 2]
+            e.set_stream(stream.cuda_stream)
+            if i == asleep:
+                with torch.cuda.stream(stream):
+                    torch.cuda._sleep(20_000_000)        # of clock cycles: some 10 ms
+            call()
+            if i == asleep + 1:
+                ended = torch.cuda.Event()
+                ended.record(stream)
+                assert not ended.query(), i              # it waits for the sleeping stream's call
+        torch.cuda.synchronize()
+        for name, a, b in zip(STATE + ("k", "v", "table", "lengths", "token"), live, want):
+            assert torch.equal(a, b), (asleep, name)
+    assert e.status() == 0
+    e.close()
