@@ -396,8 +396,9 @@ B200_API int b200_rms_norm(b200_engine_t *e, const b200_rms_norm_t *a);
  * exp(s), s = scale * q . k, lse = log sum exp(s), with the conventions of
  * b200_kv_attend for rows that see nothing (p < 0, pages that are not there,
  * scores of -infinity), for NaN and for infinities; what a row does not see has
- * no influence on it, whatever it holds. Rows that no sequence has are left as
- * they are. Dot products, maximum, sum and output are held in float32. With
+ * no influence on it, whatever it holds, and a value that is not finite makes
+ * its element infinite or NaN in every row that sees it, however small its
+ * weight. Rows that no sequence has are left as they are. Dot products, maximum, sum and output are held in float32. With
  * 16-bit queries the weights of the softmax are rounded to the cache's type
  * before they meet the values (as much as the output is), with float32 queries
  * nothing is rounded. */

@@ -289,8 +289,8 @@ __global__ void __launch_bounds__(256) join_kernel(const Args a) {
                 const int at = k * 128 + lane * 4;
                 if (at >= kDim) break;
                 const float4 x = *reinterpret_cast<const float4 *>(p + static_cast<long long>(r) * kDim + at);
-                // a part without weight adds nothing, whatever it holds
-                if (w != 0.0f) o[k] = make_float4(fmaf(w, x.x, o[k].x), fmaf(w, x.y, o[k].y), fmaf(w, x.z, o[k].z), fmaf(w, x.w, o[k].w));
+                // a value that is not finite and seen counts however small its part's weight is, 0 included
+                o[k] = make_float4(fmaf(w, x.x, o[k].x), fmaf(w, x.y, o[k].y), fmaf(w, x.z, o[k].z), fmaf(w, x.w, o[k].w));
             }
         }
         const float inv = l == 0.0f ? 0.0f : 1.0f / l;

@@ -181,7 +181,11 @@ __global__ void __launch_bounds__(kThreads, 1) f32_kernel(const Args a) {
 #pragma unroll
                             for (int i = 0; i < kRows; ++i) {
                                 const float w = x == 0 ? p[i].x : x == 1 ? p[i].y : x == 2 ? p[i].z : p[i].w;
-                                if (kEdge && w == 0.0f) continue;          // not seen: whatever the value is
+                                // not seen: whatever the value is; a weight that is 0 for its size alone counts
+                                if (kEdge && w == 0.0f) {
+                                    const int slot = u * kN + n + x;
+                                    if (slot > at[i] || (a.window && slot <= at[i] - a.window)) continue;
+                                }
                                 o[i][4 * j] = fmaf(w, v.x, o[i][4 * j]);
                                 o[i][4 * j + 1] = fmaf(w, v.y, o[i][4 * j + 1]);
                                 o[i][4 * j + 2] = fmaf(w, v.z, o[i][4 * j + 2]);

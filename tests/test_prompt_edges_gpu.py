@@ -3,8 +3,11 @@ what they answer."""
 
 from __future__ import annotations
 
+import math
+
 import pytest
 
+from test_prompt_gpu import TYPES, chunk_case, chunk_run
 from test_prompt_paths_gpu import STATE, step_case
 
 pytestmark = pytest.mark.gpu
@@ -72,3 +75,26 @@ def test_calls_of_a_step_on_two_streams_follow_one_another(torch_mod, pkg):
             assert torch.equal(a, b), (asleep, name)
     assert e.status() == 0
     e.close()
+
+
+# ------------------------------------------------------------------ values that are not finite
+
+@pytest.mark.parametrize("q,kv", TYPES)
+@pytest.mark.parametrize("new,old,low,slots", [
+    (200, 100, 0, (20, 150, 299)),       # a unit that all rows see; units that some rows see
+    (9, 20000, 10000, (10, 5000)),       # parts of a split tile in which no slot has a weight beside the others'
+])
+def test_chunk_seen_values_count_however_small_their_weight(torch_mod, pkg, eng, q, kv, new, old, low, slots):
+    """A value that is not finite spoils its element in every row that sees it, with a weight of e^-250 beside 1, which
+    float32 rounds to 0, as with any other: whichever unit, stretch or part of a tile it falls into."""
+    torch = torch_mod
+    c = chunk_case(torch, pkg, [new], [old], 4, 2, 64, 16, q, kv, seed=22)
+    k, v, table = c["cache"].k, c["cache"].v, c["table"][0]
+    c["q"].fill_(1.0)
+    k.zero_()
+    for s in list(slots) + list(range(low)):
+        k[int(table[s // 16]), :, s % 16] = -250.0 / 64      # exact in every type
+    for i, (s, what) in enumerate(zip(slots, (math.nan, math.inf, -math.inf))):
+        v[int(table[s // 16]), i % 2, s % 16, 5 + i] = what
+    chunk_run(torch, eng, c, scale=1.0)
+    assert not torch.isfinite(c["out"][:new, 0, 5]).any() and torch.isfinite(c["out"][:new, 0, 0]).all()
