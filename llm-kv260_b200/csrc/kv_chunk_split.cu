@@ -1,21 +1,26 @@
 // b200_kv_attend_chunk for float32 queries and a float16 cache.
 //
 // Both products run on the tensor cores (mma.sync, warp by warp, 16 rows each)
-// with the float32 operand in two parts of float16, x = high + low, 22 bits:
-// S = Qh K^T + Ql K^T and O = Ph V + Pl V. A row's queries are multiplied by a
-// power of two first, the largest to [2^14, 2^15), so that an element 2^-j of
-// it keeps 22 bits, or 39 - j where that is less; the scale takes it back. The
-// tensor cores cut sums off at 24 bits instead of rounding them, so the small
-// parts are summed first, S in sums of its own for both parts, and a unit's 64
-// slots are added to the output outside of them: eight cuts of S and four of
-// what a unit adds, each below 2^-24 (8000 slots: 6.8e-7 of the output's norm off
-// the exact one, the plain form 1.8e-6; 120000: 7.5e-7 and 6.4e-6).
+// with the float32 operand in two parts of float16, x = high + 2^-11 low, 22
+// bits: S = Qh K^T + 2^-11 Ql K^T and O = Ph V + 2^-11 Pl V. The factor keeps the
+// low part a normal number wherever the high part is one. A row's queries are
+// multiplied by a power of two first, the largest to [2^14, 2^15), so that an
+// element 2^-j of it keeps 22 bits, or 50 - j where that is less; the scale
+// takes it back. A unit's weights are taken relative to its own largest, which
+// becomes 2^15, so those down to 2^-29 of it keep 22 bits; smaller ones, which
+// matter where larger ones meet small values, take products of their own, 2^29
+// times larger, until none is left (one more round for scores that differ by 20
+// to 40 nats within 64 slots, none for most). The tensor cores cut sums off at
+// 24 bits instead of rounding them, so the small parts are summed first, S in
+// sums of its own for both parts, and a unit's 64 slots are added to the output
+// outside of them: eight cuts of S and four of what a unit adds, each below
+// 2^-24 (8000 slots: 6.8e-7 of the output's norm off the exact one, the plain
+// form 1.8e-6; 120000: 7.5e-7 and 6.4e-6).
 //
 // What bounds it: the products, twice as many as in 16 bits and at the rate of
 // mma.sync, 255 registers and with them 8 warps an SM. 4 chunks of 100 to 333
-// tokens behind up to 2000 slots (24 heads, 8 of the cache, 128): 257 us, 89
-// TFLOP/s of the float32 products' (802 us on the float32 units); 2000 tokens
-// from the start, 32 heads: 407 us, 80 TFLOP/s.
+// tokens behind up to 2000 slots (24 heads, 8 of the cache, 128): 307 us, 75
+// TFLOP/s of the float32 products' (802 us on the float32 units).
 #include <cuda_runtime.h>
 
 #include "kv_chunk.cuh"
@@ -27,10 +32,11 @@ namespace {
 
 constexpr int kM = 64, kN = 64, kThreads = 128;
 constexpr int kCost = 2;               // units that a tile's begin and end take
-// The reference m trails the maximum by 7 to 15 powers of two: weights stay in
-// 2^15 and below, float16's range, and those of 2^-21 of the largest are still
-// normal numbers there.
-constexpr float kLead = 7.0f, kSlack = 15.0f;
+constexpr float kTop = 15.0f;          // a unit's largest weight is 2^15, in float16's range with its low part's 2^14
+constexpr float kLeast = 0x1p-14f, kRound = 0x1p29f;   // of a round of products the least weight, and what the next one's grow by
+constexpr float kLow = 0x1p11f;        // factor of the low parts
+// The reference m of l and O is a maximum of some time ago: it moves, and they are multiplied, where it is passed by 2^8.
+constexpr float kSlack = 8.0f;
 
 template <int kDim>
 struct Smem {
@@ -156,7 +162,7 @@ __global__ void __launch_bounds__(kThreads, kDim <= 128 ? 2 : 1) split_kernel(co
                     const float y0 = x[2 * k] * by, y1 = x[2 * k + 1] * by;
                     hi[k] = pack(y0, y1);
                     const float2 z = unpack(hi[k]);
-                    const float l0 = y0 - z.x, l1 = y1 - z.y;
+                    const float l0 = (y0 - z.x) * kLow, l1 = (y1 - z.y) * kLow;
                     lo[k] = pack(l0 - l0 == 0.0f ? l0 : 0.0f, l1 - l1 == 0.0f ? l1 : 0.0f);
                 }
                 const uint32_t at = piece(kM, r, c);
@@ -220,7 +226,7 @@ __global__ void __launch_bounds__(kThreads, kDim <= 128 ? 2 : 1) split_kernel(co
                 for (int n = 0; n < 8; ++n)
 #pragma unroll
                     for (int k = 0; k < 4; ++k) {
-                        hi[n][k] = (hi[n][k] + lo[n][k]) * scale[k >> 1];
+                        hi[n][k] = fmaf(lo[n][k], 1 / kLow, hi[n][k]) * scale[k >> 1];
                         nan |= hi[n][k] != hi[n][k];
                     }
                 if (__any_sync(kFullMask, nan)) {      // an infinite key, perhaps, whose products with both parts differ in sign
@@ -263,7 +269,7 @@ __global__ void __launch_bounds__(kThreads, kDim <= 128 ? 2 : 1) split_kernel(co
                     float keep[2];
 #pragma unroll
                     for (int x = 0; x < 2; ++x) {
-                        const float next = fmaxf(ref[x], top[x] - kLead);
+                        const float next = fmaxf(ref[x], top[x]);
                         keep[x] = next == ref[x] ? 1.0f : exp2f(ref[x] - next);
                         ref[x] = next;
                         l[x] *= keep[x];
@@ -274,52 +280,88 @@ __global__ void __launch_bounds__(kThreads, kDim <= 128 ? 2 : 1) split_kernel(co
                         o[n][2] *= keep[1], o[n][3] *= keep[1];
                     }
                 }
-                uint32_t ph[4][4], pl[4][4];           // the weights as operands of 16 slots each
-                float off[2], sum[2] = {0.0f, 0.0f};
-                off[0] = ref[0] == -INFINITY ? 0.0f : ref[0];
-                off[1] = ref[1] == -INFINITY ? 0.0f : ref[1];
+                // The unit's weights beside its own largest, and what they count in l and O.
+                float off[2], factor[2], sum[2] = {0.0f, 0.0f};
 #pragma unroll
-                for (int n = 0; n < 8; ++n) {
+                for (int x = 0; x < 2; ++x) {
+                    off[x] = top[x] == -INFINITY ? 0.0f : top[x] - kTop;
+                    factor[x] = top[x] == -INFINITY ? 0.0f : exp2f(off[x] - ref[x]);
+                }
+                bool small = false;                    // a weight below a round's least, 0 included
+#pragma unroll
+                for (int n = 0; n < 8; ++n)
 #pragma unroll
                     for (int k = 0; k < 4; ++k) {
                         hi[n][k] = exp2f(hi[n][k] - off[k >> 1]);
                         sum[k >> 1] += hi[n][k];
+                        small |= hi[n][k] < kLeast;
                     }
-#pragma unroll
-                    for (int x = 0; x < 2; ++x) {
-                        const uint32_t w = pack(hi[n][2 * x], hi[n][2 * x + 1]);
-                        const float2 z = unpack(w);
-                        ph[n >> 1][(n & 1) * 2 + x] = w;
-                        pl[n >> 1][(n & 1) * 2 + x] = pack(hi[n][2 * x] - z.x, hi[n][2 * x + 1] - z.y);
-                    }
-                }
-                l[0] += sum[0];
-                l[1] += sum[1];
+                l[0] = fmaf(sum[0], factor[0], l[0]);
+                l[1] = fmaf(sum[1], factor[1], l[1]);
                 if (!bad) {
+                    const auto products = [&](float (&w)[8][4]) {      // O += factor W V
+                        uint32_t ph[4][4], pl[4][4];   // the weights as operands of 16 slots each
 #pragma unroll
-                    for (int n = 0; n < kDim / 8; n += 2) {
-                        float t[2][4] = {};
-                        uint32_t b[4][4];
+                        for (int n = 0; n < 8; ++n)
 #pragma unroll
-                        for (int k = 0; k < 4; ++k) {
-                            load_matrices_turned(b[k], v_at + piece(kN, k * 16 + (lane & 15), n + (lane >> 4)));
-                            multiply(t[0], pl[k], b[k][0], b[k][1]);
-                            multiply(t[1], pl[k], b[k][2], b[k][3]);
+                            for (int x = 0; x < 2; ++x) {
+                                const uint32_t p = pack(w[n][2 * x], w[n][2 * x + 1]);
+                                const float2 z = unpack(p);
+                                ph[n >> 1][(n & 1) * 2 + x] = p;
+                                pl[n >> 1][(n & 1) * 2 + x] = pack((w[n][2 * x] - z.x) * kLow, (w[n][2 * x + 1] - z.y) * kLow);
+                            }
+#pragma unroll
+                        for (int n = 0; n < kDim / 8; n += 2) {
+                            float t[2][4] = {};
+                            uint32_t b[4][4];
+#pragma unroll
+                            for (int k = 0; k < 4; ++k) {
+                                load_matrices_turned(b[k], v_at + piece(kN, k * 16 + (lane & 15), n + (lane >> 4)));
+                                multiply(t[0], pl[k], b[k][0], b[k][1]);
+                                multiply(t[1], pl[k], b[k][2], b[k][3]);
+                            }
+#pragma unroll
+                            for (int k = 0; k < 4; ++k) t[0][k] *= 1 / kLow, t[1][k] *= 1 / kLow;
+#pragma unroll
+                            for (int k = 0; k < 4; ++k) {
+                                multiply(t[0], ph[k], b[k][0], b[k][1]);
+                                multiply(t[1], ph[k], b[k][2], b[k][3]);
+                            }
+#pragma unroll
+                            for (int k = 0; k < 4; ++k) {
+                                o[n][k] = fmaf(t[0][k], factor[k >> 1], o[n][k]);
+                                o[n + 1][k] = fmaf(t[1][k], factor[k >> 1], o[n + 1][k]);
+                            }
                         }
+                    };
+                    // rounds for weights that are too small for this one; none for most
+                    while (__builtin_expect(__any_sync(kFullMask, small), 0)) {
+                        float w[8][4];
+                        bool left = false;
+                        small = false;
 #pragma unroll
-                        for (int k = 0; k < 4; ++k) {
-                            multiply(t[0], ph[k], b[k][0], b[k][1]);
-                            multiply(t[1], ph[k], b[k][2], b[k][3]);
-                        }
+                        for (int n = 0; n < 8; ++n)
 #pragma unroll
-                        for (int k = 0; k < 4; ++k) o[n][k] += t[0][k], o[n + 1][k] += t[1][k];
+                            for (int k = 0; k < 4; ++k) left |= hi[n][k] > 0.0f && hi[n][k] < kLeast;
+                        if (!__any_sync(kFullMask, left)) break;
+#pragma unroll
+                        for (int n = 0; n < 8; ++n)
+#pragma unroll
+                            for (int k = 0; k < 4; ++k) {
+                                w[n][k] = hi[n][k] < kLeast ? 0.0f : hi[n][k];
+                                hi[n][k] = hi[n][k] < kLeast ? hi[n][k] * kRound : 0.0f;
+                                small |= hi[n][k] < kLeast;
+                            }
+                        products(w);
+                        factor[0] *= 1 / kRound, factor[1] *= 1 / kRound;
                     }
+                    products(hi);
                 } else {
                     // 0 times a value that is not finite must not reach a row that does not see it: weight by weight
 #pragma unroll
                     for (int n = 0; n < 8; ++n)
 #pragma unroll
-                        for (int k = 0; k < 4; ++k) s.p[warp][(lane >> 2) + 8 * (k >> 1)][n * 8 + (lane & 3) * 2 + (k & 1)] = hi[n][k];
+                        for (int k = 0; k < 4; ++k) s.p[warp][(lane >> 2) + 8 * (k >> 1)][n * 8 + (lane & 3) * 2 + (k & 1)] = hi[n][k] * factor[k >> 1];
                     __syncwarp();
 #pragma unroll 1
                     for (int c = 0; c < kN; ++c) {

@@ -7,7 +7,7 @@ import math
 
 import pytest
 
-from test_prompt_gpu import TYPES, chunk_case, chunk_run
+from test_prompt_gpu import TYPES, chunk_case, chunk_exact, chunk_run
 from test_prompt_paths_gpu import STATE, step_case
 
 pytestmark = pytest.mark.gpu
@@ -98,3 +98,46 @@ def test_chunk_seen_values_count_however_small_their_weight(torch_mod, pkg, eng,
         v[int(table[s // 16]), i % 2, s % 16, 5 + i] = what
     chunk_run(torch, eng, c, scale=1.0)
     assert not torch.isfinite(c["out"][:new, 0, 5]).any() and torch.isfinite(c["out"][:new, 0, 0]).all()
+
+
+# ------------------------------------------------------------------ small weights, small elements of queries
+
+SINK = [("bf16", "bf16"), ("f32", "f16"), ("f32", "f32")]
+
+
+@pytest.mark.parametrize("q,kv", SINK)
+@pytest.mark.parametrize("below", [15, 18, 20, 22, 24, 30, 60])
+@pytest.mark.parametrize("new,old", [(5, 4000), (700, 0), (60, 0)])
+def test_chunk_beside_a_slot_without_value(torch_mod, pkg, eng, q, kv, below, new, old):
+    """One slot holds nearly all weight and the value 0, so that all of the output comes from weights of e^-15 to e^-60
+    beside 1, in units with that slot and without. With float32 queries they are as exact as any; with float16 ones a
+    weight is within 2^-38 of the row's largest, so the output within 2^-38 of the values' sum."""
+    torch = torch_mod
+    c = chunk_case(torch, pkg, [new], [old], 4, 2, 64, 16, q, kv, seed=23)
+    k, v, table = c["cache"].k, c["cache"].v, c["table"][0]
+    c["q"].fill_(1.0)
+    k.fill_(-below / 64)                     # exact in every type
+    v.copy_(64 * v.abs() + 32)
+    k[int(table[0]), :, 0] = 0.0
+    v[int(table[0]), :, 0] = 0.0
+    chunk_run(torch, eng, c, scale=1.0, check=False)
+    out, lse, tol, ltol = chunk_exact(torch, c, 1.0)
+    if q == "f16":
+        tol = tol + 2.0 ** -38 * (old + new) * v.max().double()
+    got, n = c["out"].double(), new
+    bad = ~((got - out).abs() <= tol)[:n]
+    assert not bad.any(), f"{int(bad.sum())} of {bad.numel()}: worst {float(((got - out).abs() / tol)[:n][bad].max())} at {bad.nonzero()[0].tolist()}"
+    assert ((c["lse"].double() - lse).abs() <= ltol)[:n].all()
+
+
+@pytest.mark.parametrize("kv", ["f16", "f32"])
+@pytest.mark.parametrize("j", [20, 26, 30, 34])
+def test_chunk_small_elements_of_a_query(torch_mod, pkg, eng, kv, j):
+    """A query whose one large element meets keys of 0: the scores come from elements of 2^-j of it."""
+    torch = torch_mod
+    c = chunk_case(torch, pkg, [70], [200], 4, 2, 64, 16, "f32", kv, seed=24)
+    c["cache"].k.mul_(256.0)
+    c["cache"].k[..., 7] = 0.0
+    c["q"].mul_(2.0 ** -8)
+    c["q"][..., 7] = 2.0 ** (j - 8)
+    chunk_run(torch, eng, c)
