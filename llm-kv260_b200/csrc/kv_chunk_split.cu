@@ -18,9 +18,10 @@
 // form 1.8e-6; 120000: 7.5e-7 and 6.4e-6).
 //
 // What bounds it: the products, twice as many as in 16 bits and at the rate of
-// mma.sync, 255 registers and with them 8 warps an SM. 4 chunks of 100 to 333
-// tokens behind up to 2000 slots (24 heads, 8 of the cache, 128): 307 us, 75
-// TFLOP/s of the float32 products' (802 us on the float32 units).
+// mma.sync, 255 registers and with them 8 warps an SM, two CTAs up to head_dim
+// 128. 4 chunks of 100 to 333 tokens behind up to 2000 slots (24 heads, 8 of the
+// cache, 128): 201 us, 114 TFLOP/s of the float32 products' (307 us with one CTA
+// to an SM, 802 on the float32 units).
 #include <cuda_runtime.h>
 
 #include "kv_chunk.cuh"
@@ -44,7 +45,7 @@ struct Smem {
     __half kv[2][2][kN * kDim];        // keys and values of two units
     long long row[2][kN];              // byte offset of a slot's row, -1: not there
     int shift[kM];                     // exponents that the queries were multiplied by
-    float p[4][16][kN + 1];            // a warp's weights, where values are not finite
+    float p[4][8][kN + 1];             // weights of half a warp's rows, where values are not finite
     Shared<kThreads> find;
 };
 
@@ -78,6 +79,9 @@ __device__ __forceinline__ uint32_t pack(float lo, float hi) {
     return *reinterpret_cast<const uint32_t *>(&h);
 }
 __device__ __forceinline__ float2 unpack(uint32_t w) { return __half22float2(*reinterpret_cast<const __half2 *>(&w)); }
+
+// Two CTAs to an SM of 228 KB, of which each takes 1 KB for itself.
+static_assert(2 * (sizeof(Smem<128>) + 1024) <= 228 * 1024);
 
 template <int kDim>
 __global__ void __launch_bounds__(kThreads, kDim <= 128 ? 2 : 1) split_kernel(const Args a) {
@@ -358,28 +362,31 @@ __global__ void __launch_bounds__(kThreads, kDim <= 128 ? 2 : 1) split_kernel(co
                     products(hi);
                 } else {
                     // 0 times a value that is not finite must not reach a row that does not see it: weight by weight
-#pragma unroll
-                    for (int n = 0; n < 8; ++n)
-#pragma unroll
-                        for (int k = 0; k < 4; ++k) s.p[warp][(lane >> 2) + 8 * (k >> 1)][n * 8 + (lane & 3) * 2 + (k & 1)] = hi[n][k] * factor[k >> 1];
-                    __syncwarp();
 #pragma unroll 1
-                    for (int c = 0; c < kN; ++c) {
-                        const int slot = u * kN + c;
-                        const char *v = reinterpret_cast<const char *>(s.kv[u & 1][1]);
+                    for (int x = 0; x < 2; ++x) {
 #pragma unroll
-                        for (int x = 0; x < 2; ++x) {
-                            if (slot > at[x] || (a.window && slot <= at[x] - a.window) || s.row[u & 1][c] < 0) continue;
-                            const float p = s.p[warp][(lane >> 2) + 8 * x][c];
+                        for (int n = 0; n < 8; ++n)
+#pragma unroll
+                            for (int k = 0; k < 2; ++k)
+                                s.p[warp][lane >> 2][n * 8 + (lane & 3) * 2 + k] = (x ? hi[n][2 + k] : hi[n][k]) * (x ? factor[1] : factor[0]);
+                        __syncwarp();
+#pragma unroll 1
+                        for (int c = 0; c < kN; ++c) {
+                            const int slot = u * kN + c, own = x ? at[1] : at[0];
+                            const char *v = reinterpret_cast<const char *>(s.kv[u & 1][1]);
+                            if (slot > own || (a.window && slot <= own - a.window) || s.row[u & 1][c] < 0) continue;
+                            const float p = s.p[warp][lane >> 2][c];
 #pragma unroll
                             for (int n = 0; n < kDim / 8; ++n) {
                                 const float2 z = unpack(*reinterpret_cast<const uint32_t *>(v + piece(kN, c, n) + (lane & 3) * 4));
-                                o[n][2 * x] = fmaf(p, z.x, o[n][2 * x]);
-                                o[n][2 * x + 1] = fmaf(p, z.y, o[n][2 * x + 1]);
+                                const float y0 = x ? o[n][2] : o[n][0], y1 = x ? o[n][3] : o[n][1];
+                                const float z0 = fmaf(p, z.x, y0), z1 = fmaf(p, z.y, y1);
+                                if (x) o[n][2] = z0, o[n][3] = z1;
+                                else o[n][0] = z0, o[n][1] = z1;
                             }
                         }
+                        __syncwarp();
                     }
-                    __syncwarp();
                 }
             }
             __syncthreads();                           // the stage and its rows are free
@@ -428,13 +435,17 @@ __global__ void __launch_bounds__(kThreads, kDim <= 128 ? 2 : 1) split_kernel(co
     }
 }
 
-// Two CTAs of four warps to an SM where two tiles fit it.
-int grid_of(int dim) { return sm_count() * (dim <= 128 ? 2 : 1); }
+// As many CTAs as the GPU holds at once: two of four warps to an SM for head_dim
+// up to 128, one above.
+template <int kDim>
+int grid_of() {
+    return sm_count() * resident_ctas(reinterpret_cast<const void *>(split_kernel<kDim>), kThreads, static_cast<int>(sizeof(Smem<kDim>)));
+}
 
 template <int kDim>
 cudaError_t launch(const Args &a, cudaStream_t stream) {
     const auto fn = split_kernel<kDim>;
-    const int smem = static_cast<int>(sizeof(Smem<kDim>)), grid = grid_of(kDim);
+    const int smem = static_cast<int>(sizeof(Smem<kDim>)), grid = grid_of<kDim>();
     if (!ensure_smem(reinterpret_cast<const void *>(fn), smem)) return cudaGetLastError();
     fn<<<grid, kThreads, smem, stream>>>(a);
     const cudaError_t e = cudaGetLastError();
@@ -445,7 +456,8 @@ cudaError_t launch(const Args &a, cudaStream_t stream) {
 
 Shape split_shape(int head_dim) {
     const int dim = (head_dim + 63) / 64 * 64;
-    return Shape{grid_of(dim), part_floats(kM, dim) * 4};
+    const int grid = dim <= 64 ? grid_of<64>() : dim <= 128 ? grid_of<128>() : dim <= 192 ? grid_of<192>() : grid_of<256>();
+    return Shape{grid, part_floats(kM, dim) * 4};
 }
 
 cudaError_t split_launch(const Args &a, cudaStream_t stream) {
