@@ -316,8 +316,10 @@ bool ensure_smem(const void *fn, int bytes) {
     struct Entry { const void *fn; int dev; int bytes; };
     static Entry cache[256];
     static int used = 0;
+    static std::mutex mu;              // engines may be called from threads of their own
     int dev = 0;
     if (cudaGetDevice(&dev) != cudaSuccess) return false;
+    std::lock_guard<std::mutex> lock(mu);
     for (int i = 0; i < used; ++i)
         if (cache[i].fn == fn && cache[i].dev == dev && cache[i].bytes >= bytes) return true;
     if (cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) != cudaSuccess) return false;
@@ -334,8 +336,10 @@ int resident_ctas(const void *fn, int threads, int smem) {
     struct Entry { const void *fn; int dev; int threads; int smem; int ctas; };
     static Entry cache[512];
     static int used = 0;
+    static std::mutex mu;
     int dev = 0;
     if (cudaGetDevice(&dev) != cudaSuccess) return 1;
+    std::lock_guard<std::mutex> lock(mu);
     for (int i = 0; i < used; ++i)
         if (cache[i].fn == fn && cache[i].dev == dev && cache[i].threads == threads && cache[i].smem == smem)
             return cache[i].ctas;
