@@ -102,7 +102,7 @@ def test_chunk_seen_values_count_however_small_their_weight(torch_mod, pkg, eng,
 
 # ------------------------------------------------------------------ small weights, small elements of queries
 
-SINK = [("bf16", "bf16"), ("f32", "f16"), ("f32", "f32")]
+SINK = [("f16", "f16"), ("bf16", "bf16"), ("f32", "f16"), ("f32", "f32")]
 
 
 @pytest.mark.parametrize("q,kv", SINK)
@@ -111,7 +111,7 @@ SINK = [("bf16", "bf16"), ("f32", "f16"), ("f32", "f32")]
 def test_chunk_beside_a_slot_without_value(torch_mod, pkg, eng, q, kv, below, new, old):
     """One slot holds nearly all weight and the value 0, so that all of the output comes from weights of e^-15 to e^-60
     beside 1, in units with that slot and without. With float32 queries they are as exact as any; with float16 ones a
-    weight is within 2^-38 of the row's largest, so the output within 2^-38 of the values' sum."""
+    weight is within 2^-35 of the row's largest, so the output within 2^-35 of the values' sum."""
     torch = torch_mod
     c = chunk_case(torch, pkg, [new], [old], 4, 2, 64, 16, q, kv, seed=23)
     k, v, table = c["cache"].k, c["cache"].v, c["table"][0]
@@ -123,7 +123,7 @@ def test_chunk_beside_a_slot_without_value(torch_mod, pkg, eng, q, kv, below, ne
     chunk_run(torch, eng, c, scale=1.0, check=False)
     out, lse, tol, ltol = chunk_exact(torch, c, 1.0)
     if q == "f16":
-        tol = tol + 2.0 ** -38 * (old + new) * v.max().double()
+        tol = tol + 2.0 ** -35 * (old + new) * v.max().double()
     got, n = c["out"].double(), new
     bad = ~((got - out).abs() <= tol)[:n]
     assert not bad.any(), f"{int(bad.sum())} of {bad.numel()}: worst {float(((got - out).abs() / tol)[:n][bad].max())} at {bad.nonzero()[0].tolist()}"
