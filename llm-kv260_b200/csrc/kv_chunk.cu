@@ -17,16 +17,22 @@ uint64_t workspace_bytes(const b200_kv_t *kv, int dtype) {
     return static_cast<uint64_t>(s.grid) * (2 * s.part + sizeof(chunk::Joint)) + 16;
 }
 
+// What the kernels can do of types and heads, apart from the call's other arguments.
+const char *unusable(const b200_kv_t *kv, int dtype, int n_head) {
+    if (dtype != kv->dtype && !(dtype == B200_F32 && kv->dtype == B200_F16))
+        return "q must be of the cache's type, or float32 with a float16 cache";
+    if (n_head < 1 || n_head % kv->n_head_kv) return "n_head must be a multiple of n_head_kv";
+    if (n_head / kv->n_head_kv > 4096) return "at most 4096 query heads read one cache head";
+    return nullptr;
+}
+
 }  // namespace
 
 int kv_chunk_validate(const b200_kv_t *kv, const b200_kv_chunk_t *a, const char **why) {
     if (int rc = kv_validate(kv, why)) return rc;
     const auto bad = [why](const char *w) { *why = w; return kErrInval; };
     if (!a) return bad("null arguments");
-    if (a->dtype != kv->dtype && !(a->dtype == B200_F32 && kv->dtype == B200_F16))
-        return bad("q must be of the cache's type, or float32 with a float16 cache");
-    if (a->n_head < 1 || a->n_head % kv->n_head_kv) return bad("n_head must be a multiple of n_head_kv");
-    if (a->n_head / kv->n_head_kv > 4096) return bad("at most 4096 query heads read one cache head");
+    if (const char *w = unusable(kv, a->dtype, a->n_head)) return bad(w);
     if (a->n_tokens < 0 || static_cast<int64_t>(a->n_tokens) * a->n_head > 1ll << 30)
         return bad("n_tokens must be in [0, 2^30 / n_head]");
     if (a->window < 0) return bad("window must not be negative");
@@ -77,8 +83,6 @@ cudaError_t kv_chunk_launch(const b200_kv_t *kv, const b200_kv_chunk_t *p, cudaS
 
 extern "C" uint64_t b200_kv_chunk_workspace(const b200_kv_t *kv, int dtype, int n_head) {
     const char *why = nullptr;
-    if (b200::kv_validate(kv, &why) || n_head < kv->n_head_kv || n_head % kv->n_head_kv ||
-        (dtype != kv->dtype && !(dtype == B200_F32 && kv->dtype == B200_F16)))
-        return 0;
+    if (b200::kv_validate(kv, &why) || b200::unusable(kv, dtype, n_head)) return 0;
     return b200::workspace_bytes(kv, dtype);
 }

@@ -66,6 +66,18 @@ def test_workspace_of_unusable_sizes(pkg):
         assert lib.b200_kv_chunk_workspace(ctypes.byref(kv), dtype, n_head) == 0
 
 
+def test_workspace_of_too_many_heads(pkg):
+    """0 where the call refuses: more than 4096 query heads to a cache head, none, fewer than none."""
+    import ctypes
+    kv = pkg.capi.b200_kv_t(k=256, v=256, dtype=1, n_pages=4, page_size=16, n_head_kv=2, head_dim=64, page_stride=2048,
+                            head_stride=1024, row_stride=64, table=256, table_stride=2, table_cols=2, lengths=256, batch=1)
+    lib = pkg.lib()
+    for dtype in (0, 1):
+        assert lib.b200_kv_chunk_workspace(ctypes.byref(kv), dtype, 2 * 4096) > 0
+        for n_head in (2 * 4097, 1 << 30, 0, -2):
+            assert lib.b200_kv_chunk_workspace(ctypes.byref(kv), dtype, n_head) == 0
+
+
 def test_arguments_refused_before_any_call(pkg, monkeypatch):
     """Python's own checks, with a stand-in for the library that must not be reached."""
     import torch
