@@ -418,8 +418,8 @@ typedef struct {
     uint64_t workspace;                /* b200_kv_chunk_workspace() bytes, 16-byte aligned; holds nothing between calls */
     uint64_t workspace_bytes;
 } b200_kv_chunk_t;
-/* Bytes that calls with these sizes need on the current device, whatever the
- * number of tokens (0 for unusable sizes). */
+/* Bytes that calls with these sizes need on any device of this machine, whatever
+ * the number of tokens (0 for unusable sizes). */
 B200_API uint64_t b200_kv_chunk_workspace(const b200_kv_t *kv, int dtype, int n_head);
 B200_API int b200_kv_attend_chunk(b200_engine_t *e, const b200_kv_t *kv, const b200_kv_chunk_t *a);
 

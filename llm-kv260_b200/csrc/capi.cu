@@ -980,7 +980,7 @@ extern "C" int b200_rms_norm(b200_engine_t *e, const b200_rms_norm_t *a) {
 extern "C" int b200_kv_attend_chunk(b200_engine_t *e, const b200_kv_t *kv, const b200_kv_chunk_t *a) {
     if (!e) return fail(kErrInval, "engine not open");
     const char *why = nullptr;
-    if (int rc = use_device(e->device)) return rc;       // the workspace goes by the device
+    if (int rc = use_device(e->device)) return rc;       // whose kernels the workspace's size asks for
     if (kv_chunk_validate(kv, a, &why)) return fail(kErrInval, "kv_attend_chunk: %s", why);
     if (int rc = serve_begin(e)) return rc;
     if (capturing(e->stream)) e->recorded = true;

@@ -176,6 +176,8 @@ __device__ __forceinline__ bool wait_stage(uint64_t *bar, uint32_t parity, unsig
 // ------------------------------------------------------------- host helpers
 
 int sm_count();
+// SMs of the largest device: what a workspace that any of them may use goes by.
+int most_sms();
 int max_smem_optin();
 // Raise a kernel's dynamic shared-memory limit once per (kernel, device).
 bool ensure_smem(const void *fn, int bytes);

@@ -14,7 +14,7 @@ chunk::Shape shape_of(const b200_kv_t *kv, int dtype) {
 
 uint64_t workspace_bytes(const b200_kv_t *kv, int dtype) {
     const chunk::Shape s = shape_of(kv, dtype);
-    return static_cast<uint64_t>(s.grid) * (2 * s.part + sizeof(chunk::Joint)) + 16;
+    return static_cast<uint64_t>(most_sms()) * s.ctas * (2 * s.part + sizeof(chunk::Joint)) + 16;
 }
 
 // What the kernels can do of types and heads, apart from the call's other arguments.
@@ -73,7 +73,7 @@ cudaError_t kv_chunk_launch(const b200_kv_t *kv, const b200_kv_chunk_t *p, cudaS
     a.scale = p->scale * chunk::kLog2e;
     const chunk::Shape s = shape_of(kv, p->dtype);
     a.parts = reinterpret_cast<float *>(p->workspace);
-    a.joints = reinterpret_cast<chunk::Joint *>(p->workspace + s.grid * 2 * s.part);
+    a.joints = reinterpret_cast<chunk::Joint *>(p->workspace + static_cast<uint64_t>(sm_count()) * s.ctas * 2 * s.part);
     a.status = status_word();
     if (p->dtype != B200_F32) return chunk::mma_launch(a, kv->dtype, stream);
     return kv->dtype == B200_F32 ? chunk::f32_launch(a, stream) : chunk::split_launch(a, stream);

@@ -320,9 +320,9 @@ cudaError_t launch_join(const Args &a, int grid, cudaStream_t stream) {
 
 // Each launches calls of its types: kv_chunk_mma.cu those with 16-bit queries,
 // kv_chunk_split.cu float32 queries with a float16 cache, kv_chunk_f32.cu all in
-// float32; grid in CTAs and bytes of a part of its tiles for the workspace.
+// float32; CTAs to an SM and bytes of a part of its tiles for the workspace.
 struct Shape {
-    int grid;
+    int ctas;
     long long part;
 };
 Shape mma_shape(int head_dim);

@@ -237,12 +237,10 @@ __global__ void __launch_bounds__(kThreads, 1) f32_kernel(const Args a) {
     }
 }
 
-int grid_of(int) { return sm_count(); }
-
 template <int kDim>
 cudaError_t launch(const Args &a, cudaStream_t stream) {
     const auto fn = f32_kernel<kDim>;
-    const int smem = static_cast<int>(sizeof(Smem<kDim>)), grid = grid_of(kDim);
+    const int smem = static_cast<int>(sizeof(Smem<kDim>)), grid = sm_count();
     if (!ensure_smem(reinterpret_cast<const void *>(fn), smem)) return cudaGetLastError();
     fn<<<grid, kThreads, smem, stream>>>(a);
     const cudaError_t e = cudaGetLastError();
@@ -253,7 +251,7 @@ cudaError_t launch(const Args &a, cudaStream_t stream) {
 
 Shape f32_shape(int head_dim) {
     const int dim = (head_dim + 63) / 64 * 64;
-    return Shape{grid_of(dim), part_floats(16 * rows_of(dim), dim) * 4};
+    return Shape{1, part_floats(16 * rows_of(dim), dim) * 4};
 }
 
 cudaError_t f32_launch(const Args &a, cudaStream_t stream) {

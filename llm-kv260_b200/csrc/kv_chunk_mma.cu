@@ -813,7 +813,7 @@ cudaError_t launch(const Args &a, cudaStream_t stream) {
 
 Shape mma_shape(int head_dim) {
     const int dim = (head_dim + 63) / 64 * 64;
-    return Shape{sm_count(), part_floats(dim <= 128 ? 256 : 128, dim) * 4};
+    return Shape{1, part_floats(dim <= 128 ? 256 : 128, dim) * 4};
 }
 
 cudaError_t mma_launch(const Args &a, int kv_dtype, cudaStream_t stream) {

@@ -438,14 +438,14 @@ __global__ void __launch_bounds__(kThreads, kDim <= 128 ? 2 : 1) split_kernel(co
 // As many CTAs as the GPU holds at once: two of four warps to an SM for head_dim
 // up to 128, one above.
 template <int kDim>
-int grid_of() {
-    return sm_count() * resident_ctas(reinterpret_cast<const void *>(split_kernel<kDim>), kThreads, static_cast<int>(sizeof(Smem<kDim>)));
+int ctas_of() {
+    return resident_ctas(reinterpret_cast<const void *>(split_kernel<kDim>), kThreads, static_cast<int>(sizeof(Smem<kDim>)));
 }
 
 template <int kDim>
 cudaError_t launch(const Args &a, cudaStream_t stream) {
     const auto fn = split_kernel<kDim>;
-    const int smem = static_cast<int>(sizeof(Smem<kDim>)), grid = grid_of<kDim>();
+    const int smem = static_cast<int>(sizeof(Smem<kDim>)), grid = sm_count() * ctas_of<kDim>();
     if (!ensure_smem(reinterpret_cast<const void *>(fn), smem)) return cudaGetLastError();
     fn<<<grid, kThreads, smem, stream>>>(a);
     const cudaError_t e = cudaGetLastError();
@@ -456,8 +456,8 @@ cudaError_t launch(const Args &a, cudaStream_t stream) {
 
 Shape split_shape(int head_dim) {
     const int dim = (head_dim + 63) / 64 * 64;
-    const int grid = dim <= 64 ? grid_of<64>() : dim <= 128 ? grid_of<128>() : dim <= 192 ? grid_of<192>() : grid_of<256>();
-    return Shape{grid, part_floats(kM, dim) * 4};
+    const int ctas = dim <= 64 ? ctas_of<64>() : dim <= 128 ? ctas_of<128>() : dim <= 192 ? ctas_of<192>() : ctas_of<256>();
+    return Shape{ctas, part_floats(kM, dim) * 4};
 }
 
 cudaError_t split_launch(const Args &a, cudaStream_t stream) {

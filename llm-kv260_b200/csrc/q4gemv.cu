@@ -302,6 +302,19 @@ int sm_count() {
     return d ? d->sms : 0;
 }
 
+int most_sms() {
+    static std::atomic<int> most{0};
+    int n = most.load(std::memory_order_relaxed), devices = 0;
+    if (n > 0) return n;
+    if (cudaGetDeviceCount(&devices) != cudaSuccess) return 0;
+    for (int dev = 0; dev < devices; ++dev) {
+        int sms = 0;
+        if (cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) == cudaSuccess && sms > n) n = sms;
+    }
+    most.store(n, std::memory_order_relaxed);
+    return n;
+}
+
 int max_smem_optin() {
     const DeviceInfo *d = device_info();
     return d ? d->smem_optin : 0;
