@@ -3,6 +3,7 @@
 #include <cuda_runtime.h>
 
 #include <cmath>
+#include <limits>
 
 #include "common.cuh"
 #include "q4gemv.h"
@@ -328,21 +329,25 @@ int rope_freqs(uint64_t *freqs, int rot_dim, double base, const float *factors, 
         from = std::fmax(std::floor(pair(high)), 0.0);
         to = std::fmin(std::ceil(pair(low)), rot_dim - 1.0);
     }
+    // in 64 bits: times a position of 31 bits, a double's 53 would leave 2^-25 of a turn
+    using Real = long double;
+    static_assert(std::numeric_limits<Real>::digits >= 64);
+    const Real round = 2 * 3.14159265358979323846264338327950288L;
     for (int i = 0; i < rot_dim / 2; ++i) {
-        double f = std::pow(base, -2.0 * i / rot_dim);
+        Real f = std::pow(static_cast<Real>(base), static_cast<Real>(-2 * i) / rot_dim);
         if (factors) {
             if (!positive(factors[i])) return bad("factors must be positive");
             f /= factors[i];
         }
-        double slow = 0;                               // share of the divided frequency
+        Real slow = 0;                                 // share of the divided frequency
         if (scaling == B200_ROPE_LINEAR) slow = 1;
-        if (scaling == B200_ROPE_BANDS) slow = 1 - (context * f / (2 * pi) - low) / (high - low);
-        if (scaling == B200_ROPE_YARN) slow = (i - from) / std::fmax(to - from, 0.001);
-        slow = std::fmin(std::fmax(slow, 0.0), 1.0);
+        if (scaling == B200_ROPE_BANDS) slow = 1 - (context * f / round - low) / (static_cast<Real>(high) - low);
+        if (scaling == B200_ROPE_YARN) slow = (i - from) / std::fmax(static_cast<Real>(to) - from, static_cast<Real>(0.001));
+        slow = std::fmin(std::fmax(slow, static_cast<Real>(0)), static_cast<Real>(1));
         if (scaling != B200_ROPE_PLAIN) f = f / factor * slow + f * (1 - slow);
-        long double turns = static_cast<long double>(f) / (2 * 3.14159265358979323846264338327950288L);
+        Real turns = f / round;
         turns -= std::floor(turns);
-        const long double units = std::round(std::ldexp(turns, 64));
+        const Real units = std::round(std::ldexp(turns, 64));
         freqs[i] = units >= 0x1p64L ? 0 : static_cast<uint64_t>(units);
     }
     return 0;

@@ -3,6 +3,7 @@
 from __future__ import annotations
 
 import math
+from decimal import Decimal, getcontext
 
 import numpy as np
 import pytest
@@ -44,6 +45,43 @@ def test_frequencies_for_long_contexts(pkg):
     for i in range(rot // 2):
         slow = min(max((i - lo) / (hi - lo), 0), 1)
         assert abs(got[i] - inv[i] * (1 - slow + slow / 16) / (2 * math.pi)) < 2.0 ** -50
+
+
+def exact_turns(rot, base, factor=1):
+    """Turns a position of each pair, to 45 digits."""
+    getcontext().prec = 50
+    pi = Decimal("3.14159265358979323846264338327950288419716939937510582097494459")
+    return [(Decimal(base).ln() * (-2 * i) / rot).exp() / (2 * pi * Decimal(factor)) for i in range(rot // 2)]
+
+
+@pytest.mark.parametrize("rot,base,factor", [(64, 10000.0, 1.0), (128, 500000.0, 1.0), (80, 10000.0, 40.0), (256, 1.5, 3.0)])
+def test_frequencies_carry_the_farthest_position(pkg, rot, base, factor):
+    """Times 2^31 - 1, the last position, to 2^-28 of a turn: a frequency to 2^-59, where a double's 53 bits would not do."""
+    got = pkg.rope_freqs(rot, base, scaling=None if factor == 1 else "linear", factor=factor).numpy().view(np.uint64)
+    for i, want in enumerate(exact_turns(rot, base, factor)):
+        off = (Decimal(int(got[i])) / 2 ** 64 - want % 1) * (2 ** 31 - 1)
+        assert abs(off) < Decimal(2) ** -28, (i, float(off))
+
+
+def test_stretched_frequencies_carry_the_farthest_position(pkg):
+    """The same for bands and for the ramp over a pair's index."""
+    rot, base, factor, context = 64, 500000.0, 8.0, 8192
+    plain = exact_turns(rot, base)
+    got = pkg.rope_freqs(rot, base, scaling="bands", factor=factor, context=context, low=1.0, high=4.0).numpy().view(np.uint64)
+    for i, f in enumerate(plain):
+        keep = min(max((context * f - 1) / 3, Decimal(0)), Decimal(1))
+        off = (Decimal(int(got[i])) / 2 ** 64 - f * (keep + (1 - keep) / 8)) * (2 ** 31 - 1)
+        assert abs(off) < Decimal(2) ** -28, (i, float(off))
+    got = pkg.rope_freqs(rot, base, scaling="yarn", factor=factor, context=context, low=1.0, high=32.0).numpy().view(np.uint64)
+
+    def index(x):
+        return rot * math.log(context / (x * 2 * math.pi)) / (2 * math.log(base))
+
+    lo, hi = math.floor(index(32.0)), math.ceil(index(1.0))
+    for i, f in enumerate(plain):
+        slow = min(max(Decimal(i - lo) / (hi - lo), Decimal(0)), Decimal(1))
+        off = (Decimal(int(got[i])) / 2 ** 64 - f * (1 - slow + slow / 8)) * (2 ** 31 - 1)
+        assert abs(off) < Decimal(2) ** -28, (i, float(off))
 
 
 def test_frequencies_refused(pkg):
