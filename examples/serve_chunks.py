@@ -139,11 +139,13 @@ class ChunkServer:
         tokens a step beside the others' single tokens. A request begins when the pool can hold all of it beside those
         that run."""
         torch = self.torch
+        if n < 1 or chunk < 1 or any(len(p) == 0 for p in prompts):
+            raise ValueError("every request needs a prompt and at least one token behind it, every step a token of its prompt")
         gen = torch.Generator(device=self.dev).manual_seed(seed)
         out, waiting, rows = [[] for _ in prompts], list(range(len(prompts))), [None] * self.batch
         pages = [-(-(len(p) + n - 1) // self.page) for p in prompts]
         pool = self.free.numel()
-        if max(pages) > min(pool, self.table.shape[1]):
+        if max(pages, default=0) > min(pool, self.table.shape[1]):
             raise RuntimeError("a request needs more pages than there are")
         pick, lp = self._ints(self.batch), torch.empty(self.batch, device=self.dev)
         kw = dict(temperature=torch.full((self.batch,), temperature, device=self.dev),
