@@ -328,7 +328,7 @@ B200_API int b200_kv_plan(b200_engine_t *e, const b200_kv_t *kv, const b200_kv_p
  * both in the cache's type (a slot outside the pool, as -1, is dropped; k_out
  * is not used). q, k and v in float32 may go to any type, others to their own.
  * A row may go where it comes from, in its own type and with the same strides;
- * otherwise inputs and outputs do not overlap. */
+ * otherwise inputs and outputs do not overlap, nor do an output's rows. */
 typedef struct {
     uint64_t q, q_out;                 /* [n_tokens][n_head][head_dim], strides in elements; 0: no q */
     int n_head;
@@ -372,7 +372,8 @@ B200_API int b200_rope_freqs(uint64_t *freqs, int rot_dim, double base, const fl
  * residual is 0), residual_out = r, y = r / sqrt(mean(r^2) + eps) * weight, in
  * float32 with one rounding per output. y goes to out, and with q8 row by row
  * to the engine's Q8_0 form, int8[k] then float32[k / 32], as
- * b200_quantize_q8_0 makes it and b200_gemv_q8 reads it. */
+ * b200_quantize_q8_0 makes it and b200_gemv_q8 reads it. An output's rows do not
+ * overlap, and nothing else but what is said below. */
 typedef struct {
     uint64_t x;                        /* [n_rows][k], strides in elements, rows contiguous */
     int dtype;

@@ -176,10 +176,18 @@ int rms_norm_validate(const b200_rms_norm_t *a, const char **why) {
         (a->residual_out && !rows_ok(a->residual_out, a->residual_out_stride, er)) ||
         (a->out && !rows_ok(a->out, a->out_stride, esize(a->out_dtype))))
         return bad("addresses and strides must be multiples of 16 bytes and not negative");
-    // a CTA reads its row before it writes it, so a row in place must be its own
-    if (a->n_rows > 1 && ((a->out == a->x && a->out_stride * esize(a->out_dtype) != a->x_stride * es) ||
-                          (a->residual && a->residual_out == a->residual && a->residual_out_stride != a->residual_stride)))
+    if (a->n_rows > 1 && ((a->out && a->out_stride < a->k) || (a->residual_out && a->residual_out_stride < a->k)))
+        return bad("rows of an output must not overlap");
+    // a CTA reads its row before it writes it, so a row in place must be its own; the sum is written element by element
+    // before all of the row has been read
+    const int eo = esize(a->out_dtype);
+    const auto moves = [a](int64_t from, int64_t to) { return a->n_rows > 1 && from != to; };
+    if ((a->out && a->out == a->x && moves(a->x_stride * es, a->out_stride * eo)) ||
+        (a->out && a->out == a->residual && moves(a->residual_stride * er, a->out_stride * eo)) ||
+        (a->residual_out && a->residual_out == a->residual && moves(a->residual_stride, a->residual_out_stride)) ||
+        (a->residual_out && a->residual_out == a->x && (er != es || moves(a->x_stride, a->residual_out_stride))))
         return bad("rows in place must stay where they are");
+    if (a->out && a->out == a->residual_out) return bad("out and residual_out must differ");
     if (a->q8 && (a->q8 % 4 || a->q8_stride % 4 || a->q8_stride < a->k + a->k / 8))
         return bad("q8 rows must be 4-byte aligned and hold k + k / 8 bytes");
     return 0;

@@ -231,6 +231,10 @@ int rope_validate(const b200_kv_t *kv, const b200_rope_t *a, const char **why) {
         return in == out && (a->dtype != a->out_dtype || (a->n_tokens > 1 && token != to_token) || (heads > 1 && head != to_head));
     };
     const char *in_place = "rows in place keep their type and strides";
+    const auto meet = [a](int64_t token, int64_t head, int heads) {
+        return (a->n_tokens > 1 && token < a->head_dim) || (heads > 1 && head < a->head_dim);
+    };
+    const char *apart = "rows of an output must not overlap";
     const char *aligned = "rows' addresses and strides must be multiples of 16 bytes and not negative";
     if (a->q) {
         if (a->n_head < 1 || a->n_head > 4096) return bad("n_head must be in [1, 4096]");
@@ -238,6 +242,7 @@ int rope_validate(const b200_kv_t *kv, const b200_rope_t *a, const char **why) {
         if (!rows_ok(a->q, a->q_token_stride, a->q_head_stride, es) ||
             !rows_ok(a->q_out, a->q_out_token_stride, a->q_out_head_stride, eo))
             return bad(aligned);
+        if (meet(a->q_out_token_stride, a->q_out_head_stride, a->n_head)) return bad(apart);
         if (moved(a->q, a->q_token_stride, a->q_head_stride, a->q_out, a->q_out_token_stride, a->q_out_head_stride, a->n_head))
             return bad(in_place);
     }
@@ -247,6 +252,7 @@ int rope_validate(const b200_kv_t *kv, const b200_rope_t *a, const char **why) {
         if (!kv) {
             if (!a->k_out) return bad("k without k_out or a cache");
             if (!rows_ok(a->k_out, a->k_out_token_stride, a->k_out_head_stride, eo)) return bad(aligned);
+            if (meet(a->k_out_token_stride, a->k_out_head_stride, a->n_head_kv)) return bad(apart);
             if (moved(a->k, a->k_token_stride, a->k_head_stride, a->k_out, a->k_out_token_stride, a->k_out_head_stride,
                       a->n_head_kv))
                 return bad(in_place);

@@ -141,3 +141,40 @@ def test_chunk_small_elements_of_a_query(torch_mod, pkg, eng, kv, j):
     c["q"].mul_(2.0 ** -8)
     c["q"][..., 7] = 2.0 ** (j - 8)
     chunk_run(torch, eng, c)
+
+
+# ------------------------------------------------------------------ rows that share memory
+
+def test_rows_of_an_output_that_meet_are_refused(torch_mod, pkg, eng):
+    """Also in place, where a broadcast row would be turned, or normed, again for each that reads it."""
+    torch = torch_mod
+    eng.set_stream(torch.cuda.current_stream().cuda_stream)
+    one = torch.randn(1, 1, 64, device="cuda")
+    q, pos, freqs = torch.randn(5, 2, 64, device="cuda"), torch.arange(5, dtype=torch.int32, device="cuda"), pkg.rope_freqs(64).cuda()
+    before = one.clone()
+    for out in (one.expand(5, 2, 64), q[:1].expand(5, 2, 64), q[:, :1].expand(5, 2, 64),
+                q.view(-1).as_strided((5, 2, 64), (32, 320, 1))):
+        for kw in (dict(q=out), dict(k=out), dict(q=q.clone(), q_out=out), dict(k=q.clone(), k_out=out)):
+            with pytest.raises(pkg.B200Error):
+                eng.rope(pos, freqs, **kw)
+    x, w = one.view(1, 64), torch.ones(64, device="cuda")
+    y, half = torch.randn(5, 64, device="cuda"), torch.randn(5, 128, device="cuda").half()
+    for kw in (dict(x=x.expand(5, 64), out=x.expand(5, 64)), dict(x=y, out=x.expand(5, 64)),
+               dict(x=y, residual=x.expand(5, 64), out=y), dict(x=y, residual=y.clone(), residual_out=x.expand(5, 64)),
+               dict(x=y, residual=torch.randn(5, 128, device="cuda")[:, :64], residual_out=y.view(-1).as_strided((5, 64), (32, 1))),
+               # the sum of 32 bits over an input of 16, over rows of other strides, and where the norm goes
+               dict(x=half[:, :64], residual=y, residual_out=half.view(torch.float32)),
+               dict(x=y, residual=half.float()[:, :64], residual_out=y, out=y)):
+        with pytest.raises(pkg.B200Error):
+            eng.rms_norm(weight=w, **kw)
+    torch.cuda.synchronize()
+    assert torch.equal(one, before)
+    # inputs may be broadcast, and one row may lie anywhere
+    a, b = torch.empty(5, 2, 64, device="cuda"), torch.empty(5, 2, 64, device="cuda")
+    eng.rope(pos, freqs, q=one.expand(5, 2, 64), q_out=a)
+    eng.rope(pos, freqs, q=one.expand(5, 2, 64).contiguous(), q_out=b)
+    assert torch.equal(a, b)
+    u, v = torch.empty_like(y), torch.empty_like(y)
+    eng.rms_norm(x.expand(5, 64), w, out=u, residual=y, residual_out=v)
+    eng.rms_norm(x.expand(5, 64).contiguous(), w, out=y, residual=y.clone())
+    assert torch.equal(u, y)
