@@ -7,8 +7,8 @@ import math
 
 import pytest
 
-from test_prompt_gpu import TYPES, chunk_case, chunk_exact, chunk_run
-from test_prompt_paths_gpu import STATE, step_case
+from test_prompt_gpu import DT, TYPES, chunk_case, chunk_exact, chunk_run
+from test_prompt_paths_gpu import STATE, step_case, step_run, step_state
 
 pytestmark = pytest.mark.gpu
 
@@ -178,3 +178,60 @@ def test_rows_of_an_output_that_meet_are_refused(torch_mod, pkg, eng):
     eng.rms_norm(x.expand(5, 64), w, out=u, residual=y, residual_out=v)
     eng.rms_norm(x.expand(5, 64).contiguous(), w, out=y, residual=y.clone())
     assert torch.equal(u, y)
+
+
+# ------------------------------------------------------------------ packed rows
+
+@pytest.mark.parametrize("x,res", [("f32", None), ("f32", "f32"), ("bf16", None), ("bf16", "bf16"), ("bf16", "f32"), ("f16", "f16")])
+@pytest.mark.parametrize("n,k", [(1, 2048), (33, 256), (2050, 4096), (2049, 2080), (3, 32736)])
+def test_norm_q8_of_all_types(torch_mod, eng, x, res, n, k):
+    """The packed rows are b200_quantize_q8_0's of the float32 norm, to the bit, from inputs of any type, with a residual
+    and without, with one, two and four units of eight elements a thread."""
+    torch = torch_mod
+    eng.set_stream(torch.cuda.current_stream().cuda_stream)
+    gen = torch.Generator(device="cuda").manual_seed(n + k)
+    a = torch.randn(n, k, generator=gen, device="cuda").to(getattr(torch, DT[x]))
+    r = None if res is None else (3 * torch.randn(n, k, generator=gen, device="cuda")).to(getattr(torch, DT[res]))
+    w = torch.rand(k, generator=gen, device="cuda") + 0.5
+    q8 = torch.full((n, k + k // 8), 99, dtype=torch.uint8, device="cuda")
+    s = a.float() if r is None else r.float() + a.float()
+    y, again = torch.empty(n, k, device="cuda"), torch.empty(n, k, dtype=a.dtype, device="cuda")
+    eng.rms_norm(s, w, out=y)                # the same sums in the same order
+    eng.rms_norm(a, w, residual=r, out=again, q8=q8)
+    assert torch.equal(again, y.to(a.dtype))
+    if r is not None:
+        assert torch.equal(r, s.to(r.dtype))
+    want = torch.zeros(n, (k + k // 8 + 15) // 16 * 16, dtype=torch.uint8, device="cuda")
+    for i in range(n):
+        eng.quantize(y[i], want[i], k)
+    assert torch.equal(q8, want[:, :k + k // 8])
+
+
+# ------------------------------------------------------------------ engines
+
+def test_two_engines_at_once_leave_each_other_alone(torch_mod, pkg):
+    """Two engines on streams of their own, their steps side by side: both to the bit as alone."""
+    torch = torch_mod
+    requests = [[100, 3, 1, 10, 5], [1, 60, 30, 1, 1], [7, 7, 7, 7, 7], [-1, 1, 90, 1, 2]] * 4
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    engines = [pkg.Engine(0, stream=s.cuda_stream) for s in streams]
+    alone, both = ([step_case(torch, pkg, seed) for seed in (7, 8)] for _ in range(2))
+    news = [torch.tensor(r, dtype=torch.int32, device="cuda") for r in requests]
+    torch.cuda.synchronize()
+    for e, st, s in zip(engines, streams, alone):
+        with torch.cuda.stream(st):
+            for new in news:
+                s["new"].copy_(new)
+                step_run(e, s)
+        torch.cuda.synchronize()
+    for new in news:
+        for e, st, s in zip(engines, streams, both):
+            with torch.cuda.stream(st):
+                s["new"].copy_(new)
+                step_run(e, s)
+    torch.cuda.synchronize()
+    for i in range(2):
+        for name, x, y in zip(STATE + ("k", "v", "table", "lengths"), step_state(alone[i]), step_state(both[i])):
+            assert torch.equal(x, y), (i, name)
+        assert engines[i].status() == 0
+        engines[i].close()
