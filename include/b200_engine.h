@@ -198,7 +198,9 @@ B200_API int b200_kv_append(b200_engine_t *e, const b200_kv_t *kv, const b200_kv
  * weights are NaN; an element of out that values which are not finite enter is
  * infinite or NaN. n_head / n_head_kv query heads read each cache head. Dot
  * products, the running maximum and sum and the output are held in float32;
- * the rounding to the output's type is the last step. With weights_out the
+ * the rounding to the output's type is the last step. The weights meet the
+ * values with 22 bits (16 over a bfloat16 cache), over a float16 cache those
+ * below 2^-26 of the row's largest to within 2^-48 of that. With weights_out the
  * weights of the softmax, summed over the query heads of a cache head, are
  * added up: weights_out = decay * weights +
  * sum, for slots in use (others are not written). */

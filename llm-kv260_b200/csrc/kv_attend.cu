@@ -55,10 +55,14 @@ constexpr int kUnit = 16;              // slots
 constexpr int kShort = 96;             // units of a head beyond which heads are split in any case
 constexpr int kMaxCtas = 1024;         // of the grid
 constexpr float kLog2e = 1.44269504088896340736f;
-// The reference m trails the maximum by 7 to 15 powers of two: weights stay in
-// 2^15 and below, float16's range, and those of 2^-21 of the largest are still
-// normal numbers there.
-constexpr float kLead = 7.0f, kSlack = 15.0f;
+// The reference m trails the maximum by lead to slack powers of two, so weights
+// stay in 2^slack and below, and the larger the difference, the more rarely m
+// moves. Low parts are multiplied by `low`. In float16, whose range ends at 2^16,
+// both leave small weights and elements room: low parts are normal numbers
+// wherever high ones are, so a weight keeps 22 bits down to 2^-26 of the largest,
+// and below that is off by 2^-48 of the largest at most.
+template <typename T> struct Range { static constexpr float lead = 7.0f, slack = 15.0f, low = 1.0f; };
+template <> struct Range<__half> { static constexpr float lead = 12.0f, slack = 15.75f, low = 0x1p11f; };
 
 struct AttendArgs {
     KvView kv;
@@ -127,10 +131,10 @@ __device__ __forceinline__ void mma<float>(float c[4], const uint32_t a[4], uint
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
-// x = hi + lo in the operand's type: 22 bits of x in float16 (as far as its range goes) and tf32, 16 in bfloat16.
+// x = hi + lo / low in the operand's type: 22 bits of x in float16 (as far as its range goes) and tf32, 16 in bfloat16.
 template <typename T>
 __device__ __forceinline__ uint32_t split_pair(float x) {   // hi in the low half, lo in the high one
-    const T hi = from_float<T>(x), lo = from_float<T>(x - to_float(hi));
+    const T hi = from_float<T>(x), lo = from_float<T>((x - to_float(hi)) * Range<T>::low);
     return static_cast<uint32_t>(*reinterpret_cast<const unsigned short *>(&hi)) |
            static_cast<uint32_t>(*reinterpret_cast<const unsigned short *>(&lo)) << 16;
 }
@@ -171,7 +175,7 @@ __device__ __noinline__ float whole_score(const char *k_tile, int row, const cha
     const T *hi = reinterpret_cast<const T *>(q_row), *lo = reinterpret_cast<const T *>(q_row + S::kQRow);
     float sum = 0.0f;
 #pragma unroll 1
-    for (int i = 0; i < d; ++i) sum = fmaf(to_float(k[i ^ swizzle_k(row) * kPer]), to_float(hi[i]) + to_float(lo[i]), sum);
+    for (int i = 0; i < d; ++i) sum = fmaf(to_float(k[i ^ swizzle_k(row) * kPer]), to_float(hi[i]) + to_float(lo[i]) * (1 / Range<T>::low), sum);
     return sum;
 }
 
@@ -456,7 +460,7 @@ __global__ void __launch_bounds__(kThreads, Shape<T, D, NT>::kCtas)
             const int h = warp + i * kWarps;
             int e = 0;
             // float32 into float16: the head's largest to [2^14, 2^15), so that an element 2^-j of it keeps 22 bits, or
-            // 39 - j where that is less (scaled to [1, 2), 24 - j: a score off by 4e-4 beside an element 4096 times the rest)
+            // 50 - j where that is less
             if (sizeof(Q) == 4 && !kF32) {
                 float top = 0.0f;
 #pragma unroll
@@ -546,9 +550,10 @@ __global__ void __launch_bounds__(kThreads, Shape<T, D, NT>::kCtas)
             uint32_t b0[NT], b1[NT], b2[NT], b3[NT];       // P^T as the second product's columns
 #pragma unroll
             for (int t = 0; t < NT; ++t) {
-                float t0 = rows >> r & 1 ? ((sc[t][0][0] + sc[t][1][0]) + (sc[t][0][1] + sc[t][1][1])) * qs[t] : -INFINITY;
-                float t1 = rows >> (r + 8) & 1 ? ((sc[t][0][2] + sc[t][1][2]) + (sc[t][0][3] + sc[t][1][3])) * qs[t] : -INFINITY;
-                const float most = m[t] + kSlack;
+                const auto whole = [](float hi, float lo) { return fmaf(lo, 1 / Range<T>::low, hi); };
+                float t0 = rows >> r & 1 ? whole(sc[t][0][0] + sc[t][1][0], sc[t][0][1] + sc[t][1][1]) * qs[t] : -INFINITY;
+                float t1 = rows >> (r + 8) & 1 ? whole(sc[t][0][2] + sc[t][1][2], sc[t][0][3] + sc[t][1][3]) * qs[t] : -INFINITY;
+                const float most = m[t] + Range<T>::slack;
                 if (__any_sync(kFullMask, !(t0 <= most && t1 <= most))) {
                     // An infinite key element times a low part of 0, or parts of both signs, is NaN where the score is
                     // infinite: such a score is taken again from whole operands. One that stays NaN makes the reference
@@ -559,7 +564,7 @@ __global__ void __launch_bounds__(kThreads, Shape<T, D, NT>::kCtas)
                     if (t1 != t1) t1 = whole_score<T, S>(k_tile, r + 8, q_row, d) * qs[t];
                     float top = t0 == t0 && t1 == t1 ? fmaxf(t0, t1) : INFINITY;
                     for (int k = 4; k < 32; k <<= 1) top = fmaxf(top, __shfl_xor_sync(kFullMask, top, k));
-                    const float m1 = fmaxf(m[t], top - kLead), old = m1 == -INFINITY ? 1.0f : exp2_fast(m[t] - m1);
+                    const float m1 = fmaxf(m[t], top - Range<T>::lead), old = m1 == -INFINITY ? 1.0f : exp2_fast(m[t] - m1);
                     m[t] = m1;
                     l[t] *= old;
 #pragma unroll
@@ -676,7 +681,8 @@ __global__ void __launch_bounds__(kThreads, Shape<T, D, NT>::kCtas)
                     for (int i = 0; i < kAcc; ++i) {
                         const int k = i / (kPer / 2), j = i % (kPer / 2);
                         float2 *dst = reinterpret_cast<float2 *>(s_o + (4 * t + c) * D + k * 8 * kPer + r * kPer + 2 * j);
-                        float2 v = make_float2((o[i][t][0] + o[i][t][1]) * keep[t], (o[i][t][2] + o[i][t][3]) * keep[t]);
+                        constexpr float kLow = 1 / Range<T>::low;
+                        float2 v = make_float2(fmaf(o[i][t][1], kLow, o[i][t][0]) * keep[t], fmaf(o[i][t][3], kLow, o[i][t][2]) * keep[t]);
                         if (w) v.x += dst->x, v.y += dst->y;
                         *dst = v;
                     }

@@ -7,7 +7,7 @@ import math
 
 import pytest
 
-from test_prompt_gpu import DT, TYPES, chunk_case, chunk_exact, chunk_run
+from test_prompt_gpu import DT, TYPES, U, chunk_case, chunk_exact, chunk_run
 from test_prompt_paths_gpu import STATE, step_case, step_run, step_state
 
 pytestmark = pytest.mark.gpu
@@ -235,3 +235,48 @@ def test_two_engines_at_once_leave_each_other_alone(torch_mod, pkg):
             assert torch.equal(x, y), (i, name)
         assert engines[i].status() == 0
         engines[i].close()
+
+
+# ------------------------------------------------------------------ single tokens
+
+@pytest.mark.parametrize("q,kv", SINK)
+@pytest.mark.parametrize("below", [15, 18, 20, 22, 24, 30])
+@pytest.mark.parametrize("old", [40, 4000])
+def test_attend_beside_a_slot_without_value(torch_mod, pkg, eng, q, kv, below, old):
+    """kv_attend where one slot holds nearly all weight and the value 0. A float16 cache's weights are within 2^-48 of the
+    row's largest, or to 22 bits."""
+    torch = torch_mod
+    eng.set_stream(torch.cuda.current_stream().cuda_stream)
+    c = chunk_case(torch, pkg, [1], [old], 4, 2, 64, 16, q, kv, seed=25)
+    k, v, table = c["cache"].k, c["cache"].v, c["table"][0]
+    c["q"].fill_(1.0)
+    k.fill_(-below / 64)
+    v.copy_(64 * v.abs() + 32)
+    k[int(table[0]), :, 0] = 0.0
+    v[int(table[0]), :, 0] = 0.0
+    out, lse = torch.empty(1, 4, 64, dtype=c["q"].dtype, device="cuda"), torch.empty(1, 4, device="cuda")
+    eng.kv_attend(c["cache"], c["q"][:1].contiguous(), out, lse=lse, scale=1.0)
+    want, wl, tol, ltol = (t[:1] for t in chunk_exact(torch, c, 1.0))
+    # weights keep 22 bits, not half a step of the cache's type
+    tol = tol - (U[kv] if q != "f32" else 0) * want.abs() + 2.0 ** -16 * want.abs()
+    if kv == "f16":
+        tol = tol + 2.0 ** -48 * (old + 1) * v.max().double()
+    assert ((out.double() - want).abs() <= tol).all(), float(((out.double() - want).abs() / tol).max())
+    assert ((lse.double() - wl).abs() <= ltol).all()
+
+
+@pytest.mark.parametrize("kv", ["f16", "f32"])
+@pytest.mark.parametrize("j", [20, 26, 30, 34])
+def test_attend_small_elements_of_a_query(torch_mod, pkg, eng, kv, j):
+    """A query whose one large element meets keys of 0: the scores come from elements of 2^-j of it."""
+    torch = torch_mod
+    eng.set_stream(torch.cuda.current_stream().cuda_stream)
+    c = chunk_case(torch, pkg, [1], [200], 4, 2, 64, 16, "f32", kv, seed=26)
+    c["cache"].k.mul_(256.0)
+    c["cache"].k[..., 7] = 0.0
+    c["q"].mul_(2.0 ** -8)
+    c["q"][..., 7] = 2.0 ** (j - 8)
+    out = torch.empty(1, 4, 64, device="cuda")
+    eng.kv_attend(c["cache"], c["q"][:1].contiguous(), out)
+    want, _, tol, _ = (t[:1] for t in chunk_exact(torch, c, 0.125))
+    assert ((out.double() - want).abs() <= tol).all(), float(((out.double() - want).abs() / tol).max())
