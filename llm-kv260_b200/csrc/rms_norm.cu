@@ -9,7 +9,7 @@ namespace b200 {
 
 namespace {
 
-constexpr int kMaxNorm = 32768, kMaxThreads = 1024;
+constexpr int kMaxNorm = 32768, kMaxThreads = 1024;   // a block of so many has 64 registers a thread
 // Outputs above half of the 126 MB L2 are written past it (16384 rows of 4096 bfloat16 with their residual, 268 MB
 // written: 96 us, and 104 without), smaller ones are left there for the matrix that reads them.
 constexpr long long kStreamBytes = 64 << 20;
@@ -58,7 +58,7 @@ __device__ __forceinline__ void store8(char *row, int i, int dtype, const float 
 // 4.5 us on the GPU, less than the call. Four neighbouring threads hold a Q8_0
 // block.
 template <typename T, int J, bool kStream>
-__global__ void __launch_bounds__(kMaxThreads) rms_norm_kernel(const NormArgs a) {
+__global__ void __maxnreg__(65536 / kMaxThreads) rms_norm_kernel(const NormArgs a) {
     __shared__ float s_sum[32];
     const int row = blockIdx.x, threads = blockDim.x, tid = threadIdx.x, units = a.k / 8;
     const char *x = a.x + row * a.x_stride;
