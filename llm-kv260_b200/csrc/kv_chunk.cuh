@@ -7,9 +7,10 @@
 // begin and end it counts as C more units before them. All units, in the order
 // cache head, sequence, tile, slot, are dealt out in equal stretches to the CTAs
 // of a grid that fits the GPU at once, whatever the lengths, which only the
-// device knows; a stretch that ends among a tile's C leaves all of it to the next. A tile that lies in more than one stretch is joined by a
-// second kernel from the parts (m, l, O) that the CTAs leave in the workspace,
-// in the order of its slots, so that the result does not depend on timing.
+// device knows; a stretch that ends among a tile's C leaves all of it to the
+// next. A tile that lies in more than one stretch is joined by a second kernel
+// from the parts (m, l, O) that the CTAs leave in the workspace, in the order of
+// its slots, so that the result does not depend on timing.
 #pragma once
 
 #include "common.cuh"
@@ -235,6 +236,16 @@ __device__ __forceinline__ void next_tile(const Args &a, Sequence &q, int &tile,
         if (++b == a.kv.batch) b = 0, ++head;
         q = sequence(a, b);
     } while (q.n == 0);
+}
+
+// 16 bytes from global memory, or zeros.
+__device__ __forceinline__ void copy16(uint32_t dst, const void *src, bool there) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(there ? 16 : 0) : "memory");
+}
+
+// Byte of the 16-byte piece c of row r in a tile of `rows` rows, 64 16-bit columns beside 64.
+__device__ __forceinline__ uint32_t piece(int rows, int r, int c) {
+    return static_cast<uint32_t>((c >> 3) * rows * 128 + r * 128 + (((c & 7) ^ (r & 7)) << 4));
 }
 
 template <typename T>

@@ -1,9 +1,10 @@
 // b200_kv_attend_chunk in float32 throughout, on the float32 units: every bit of
-// queries and cache counts, and three products of parts at half the tensor
-// cores' 16-bit rate would not be faster. What bounds it: float32 operations and
-// the shared-memory reads that feed them (16 of 128 bytes for 128 operations of
-// a warp), with 8 warps an SM. 2000 tokens, 32 heads of 128: 946 us, 35 TFLOP/s,
-// 47 % of what the units can do (990 with the test for values not seen in the
+// queries and cache counts. (Three bfloat16 parts of each operand hold them too,
+// and six products of parts at the fifth-generation tensor cores' 16-bit rate,
+// 273 TFLOP/s, would leave the float32 units' 75 behind; that is not built.) What
+// bounds it: float32 operations and the shared-memory reads that feed them (16
+// of 128 bytes for 128 operations of a warp), with 8 warps an SM. 2000 tokens, 32
+// heads of 128, 8 of the cache: 946 us, 35 TFLOP/s, 47 % of what the units can do (990 with the test for values not seen in the
 // inner loop, 1080 with four rows to a thread, 1230 with two numbers to an
 // instruction); 35 with heads of 256.
 #include <cuda_runtime.h>
@@ -29,11 +30,6 @@ struct Smem {
     long long row[2][kN];              // byte offset of a slot's row, -1: not there
     Shared<kThreads> find;
 };
-
-// 16 bytes from global memory, or zeros.
-__device__ __forceinline__ void copy16(float *dst, const void *src, bool there) {
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_addr(dst)), "l"(src), "r"(there ? 16 : 0) : "memory");
-}
 
 // 64 slots by 128 rows (64) at a time, 16 x 16 threads: a thread has the scores
 // of rows 8 ty + i (4 ty + i) and slots tx + 16 j, and of the output the columns
@@ -79,7 +75,7 @@ __global__ void __launch_bounds__(kThreads, 1) f32_kernel(const Args a) {
                     const int r = i / (kDim / 4), c = i % (kDim / 4) * 4;
                     const long long at = s.row[u & 1][r];
                     const bool there = at >= 0 && c < d;
-                    copy16(&to[r][c], from + (there ? at + c * 4 : 0), there);
+                    copy16(smem_addr(&to[r][c]), from + (there ? at + c * 4 : 0), there);
                 }
             }
             cp_async_commit();

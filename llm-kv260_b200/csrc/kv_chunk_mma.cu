@@ -164,16 +164,6 @@ struct Waiter {
     }
 };
 
-// 16 bytes from global memory, or zeros.
-__device__ __forceinline__ void copy16(uint32_t dst, const void *src, bool there) {
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(there ? 16 : 0) : "memory");
-}
-
-// Byte of the 16-byte piece c of row r in a tile of `rows` rows.
-__device__ __forceinline__ uint32_t piece(int rows, int r, int c) {
-    return static_cast<uint32_t>((c >> 3) * rows * 128 + r * 128 + (((c & 7) ^ (r & 7)) << 4));
-}
-
 // Arrives on `bar` for this thread when the copies that it has asked for are there.
 __device__ __forceinline__ void arrive_behind_copies(uint64_t *bar) {
     asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_addr(bar)) : "memory");

@@ -49,13 +49,6 @@ struct Smem {
     Shared<kThreads> find;
 };
 
-// Byte of the 16-byte piece c of row r in a tile of `rows` rows of 64 columns each.
-__device__ __forceinline__ uint32_t piece(int rows, int r, int c) {
-    return static_cast<uint32_t>((c >> 3) * rows * 128 + r * 128 + (((c & 7) ^ (r & 7)) << 4));
-}
-__device__ __forceinline__ void copy16(uint32_t dst, const void *src, bool there) {
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(there ? 16 : 0) : "memory");
-}
 __device__ __forceinline__ void load_matrices(uint32_t (&v)[4], uint32_t at) {
     asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
                  : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3])

@@ -102,14 +102,6 @@ __device__ __forceinline__ void tmem_store16(uint32_t at, const uint32_t (&v)[16
         : "memory");
 }
 
-// And for 8.
-__device__ __forceinline__ void tmem_store8(uint32_t at, const uint32_t (&v)[8]) {
-    asm volatile(
-        "tcgen05.st.sync.aligned.32x32b.x8.b32 [%8], {%0, %1, %2, %3, %4, %5, %6, %7};" ::"r"(v[0]), "r"(v[1]), "r"(v[2]),
-        "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(at)
-        : "memory");
-}
-
 // True in one lane of a converged warp.
 __device__ __forceinline__ bool elect_one() {
     uint32_t r;
