@@ -22,6 +22,7 @@ constexpr int kN = 64, kThreads = 256;
 // Rows of a thread: eight, half as many reads for an operation as four, where a tile of 128 rows fits shared memory.
 __host__ __device__ constexpr int rows_of(int dim) { return dim <= 128 ? 8 : 4; }
 constexpr int kCost = 1;               // units that a tile's begin and end take
+constexpr uint32_t kHidden = 0x80000000;   // weight of a slot that the row does not see: -0, beside the 0 of one too small to count
 
 template <int kDim>
 struct Smem {
@@ -149,7 +150,7 @@ __global__ void __launch_bounds__(kThreads, 1) f32_kernel(const Args a) {
                 float sum = 0.0f;
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
-                    const float p = exp2f(t[i][j] - ref);
+                    const float p = dead[j] ? __uint_as_float(kHidden) : exp2f(t[i][j] - ref);
                     s.p[ty * kRows + i][tx + 16 * j] = p;
                     sum += p;
                 }
@@ -177,11 +178,7 @@ __global__ void __launch_bounds__(kThreads, 1) f32_kernel(const Args a) {
 #pragma unroll
                             for (int i = 0; i < kRows; ++i) {
                                 const float w = x == 0 ? p[i].x : x == 1 ? p[i].y : x == 2 ? p[i].z : p[i].w;
-                                // not seen: whatever the value is; a weight that is 0 for its size alone counts
-                                if (kEdge && w == 0.0f) {
-                                    const int slot = u * kN + n + x;
-                                    if (slot > at[i] || (a.window && slot <= at[i] - a.window)) continue;
-                                }
+                                if (kEdge && __float_as_uint(w) == kHidden) continue;      // whatever the value is
                                 o[i][4 * j] = fmaf(w, v.x, o[i][4 * j]);
                                 o[i][4 * j + 1] = fmaf(w, v.y, o[i][4 * j + 1]);
                                 o[i][4 * j + 2] = fmaf(w, v.z, o[i][4 * j + 2]);
