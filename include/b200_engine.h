@@ -328,7 +328,7 @@ B200_API int b200_kv_plan(b200_engine_t *e, const b200_kv_t *kv, const b200_kv_p
  * any position is good to 2^-28 turns; the other elements are copied. With a
  * cache, k's rotated rows go to its rows slots[t], and v's rows beside them,
  * both in the cache's type (a slot outside the pool, as -1, is dropped; k_out
- * is not used). q, k and v in float32 may go to any type, others to their own.
+ * is not used; no two tokens have one slot). q, k and v in float32 may go to any type, others to their own.
  * A row may go where it comes from, in its own type and with the same strides;
  * otherwise inputs and outputs do not overlap, nor do an output's rows. */
 typedef struct {

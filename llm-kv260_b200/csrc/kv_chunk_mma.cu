@@ -15,10 +15,12 @@
 // next scores, of which two run side by side: 2250 cycles of softmax and 1000 of
 // products, 3330 in all, where the products of both tiles take 2048 and the
 // special-function unit, 8.8 cycles for a warp's number beside the products,
-// 2250. One prompt of 8192 tokens (32 heads, 8 of the cache, 128 bfloat16): 602
-// us, 913 TFLOP/s of what its rows see, at the 1.6 GHz that the GPU then runs
-// at; 24 users with chunks and single tokens: 1290 us, 835 TFLOP/s; 200 tokens
-// over 120000 slots: 356 us, 830 TFLOP/s (and a fifth of the rows idle).
+// 2250. By GPU and the clock that it then runs at: one prompt of 8192 tokens (32
+// heads, 8 of the cache, 128 bfloat16) 594-661 us, 830-925 TFLOP/s of what its
+// rows see; 24 users with chunks and single tokens 1250-1510 us, 715-860; 200
+// tokens over 120000 slots 348-434 us, 680-850 (and a fifth of the rows idle);
+// the prompt with heads of 64 in float16 537 us, 4096 tokens with heads of 192 in
+// bfloat16 336, of 256 393 us: 512, 614 and 699 TFLOP/s.
 //
 // What was measured on the way (prompt / 120000 slots, us): copies of 16 bytes
 // by threads 1060 / 600 (pages of fewer than 8 rows still come so); operands of
@@ -54,9 +56,9 @@ constexpr int kColumns = 512;          // of tensor memory: all, so that it begi
 // moves. In bfloat16 all other weights are normal numbers whatever the lead. In
 // float16, whose range ends at 2^16, a lead of 10 leaves the small ones room: a
 // weight of 2^-24 of the largest is still a normal number, a smaller one is off
-// by 2^-35 of the largest at most. (A prompt of 8192 tokens of 128 float16 with a
-// lead of 7, 9, 10, 11, 13: 660, 662, 669, 682, 716 us; of 64: 523, 525, 537,
-// 570, 600.)
+// by 2^-35 of the largest at most. (A prompt of 8192 tokens in float16 takes 0.4,
+// 1.4, 3.3, 5.5 % longer with a lead of 9, 10, 11, 12 than with 7, with heads of
+// 64 instead of 128 0.4, 2.7, 9, 15 %.)
 template <typename T> struct Lead { static constexpr float lead = 7.0f, slack = 15.0f; };
 template <> struct Lead<__half> { static constexpr float lead = 10.0f, slack = 15.75f; };
 
