@@ -4,9 +4,10 @@
 // 273 TFLOP/s, would leave the float32 units' 75 behind; that is not built.) What
 // bounds it: float32 operations and the shared-memory reads that feed them (16
 // of 128 bytes for 128 operations of a warp), with 8 warps an SM. 2000 tokens, 32
-// heads of 128, 8 of the cache: 946 us, 35 TFLOP/s, 47 % of what the units can do (990 with the test for values not seen in the
-// inner loop, 1080 with four rows to a thread, 1230 with two numbers to an
-// instruction); 35 with heads of 256.
+// heads of 128, 8 of the cache: 946 us, 35 TFLOP/s, 47 % of what the units can
+// do (990 with the test for values not seen in the inner loop, 1080 with four
+// rows to a thread, 1230 with two numbers to an instruction); 35 TFLOP/s with
+// heads of 256.
 #include <cuda_runtime.h>
 
 #include <type_traits>

@@ -570,7 +570,8 @@ __device__ __forceinline__ void softmax(const Args &a, Shared0 &s, char *smem, S
             for (;;) {
                 if (__builtin_expect(moves, 0)) {
                     const float m = fmaxf(max3(top[0], top[1], top[2]), top[3]) * a.scale;
-                    const float next = fmaxf(ref, m - Lead<T>::lead);
+                    // of the warp's rows only those that need it: a row's bits do not depend on another's scores
+                    const float next = m > ref + Lead<T>::slack ? m - Lead<T>::lead : ref;
                     const float keep = next == ref ? 1.0f : ex2(ref - next);
                     ref = next;
                     l *= keep;

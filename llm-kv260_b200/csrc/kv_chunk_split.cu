@@ -46,7 +46,6 @@ struct Smem {
     __half kv[2][2][kN * kDim];        // keys and values of two units
     long long row[2][kN];              // byte offset of a slot's row, -1: not there
     int shift[kM];                     // exponents that the queries were multiplied by
-    float p[4][8][kN + 1];             // weights of half a warp's rows, where values are not finite
     Shared<kThreads> find;
 };
 
@@ -191,15 +190,41 @@ __global__ void __launch_bounds__(kThreads, kDim <= 128 ? 2 : 1) split_kernel(co
             const uint32_t k_at = kv_at + (u & 1) * (2 * kN * kDim * 2), v_at = k_at + kN * kDim * 2;
             const bool edge = (u + 1) * kN - 1 > f.last_all || u * kN < f.first_all;
             const bool gap = __syncthreads_or(tid < kN && s.row[u & 1][tid] < 0);
-            bool bad = false;                          // a value that is not finite where rows see different slots
             if (edge) {
-                const uint4 *v = reinterpret_cast<const uint4 *>(s.kv[u & 1][1]);
+                // Where rows see different slots, 0 times a value that is not finite must not reach a row that does not see
+                // it: such values make NaN of what they enter in the rows that see them, and become 0.
+                const auto odd = [](uint32_t x) { return (x & 0x7c00u) == 0x7c00u || (x & 0x7c000000u) == 0x7c000000u; };
+                uint4 *v = reinterpret_cast<uint4 *>(s.kv[u & 1][1]);
+                bool bad = false;
                 for (int i = tid; i < kN * kPieces; i += kThreads) {
                     const uint4 w = v[i];
-                    const auto odd = [](uint32_t x) { return (x & 0x7c00u) == 0x7c00u || (x & 0x7c000000u) == 0x7c000000u; };
                     bad |= odd(w.x) || odd(w.y) || odd(w.z) || odd(w.w);
                 }
-                bad = __syncthreads_or(bad);
+                if (__syncthreads_or(bad)) {
+#pragma unroll 1
+                    for (int c = 0; c < kN; ++c) {
+                        const int slot = u * kN + c;
+                        bool sees[2];
+#pragma unroll
+                        for (int x = 0; x < 2; ++x) sees[x] = slot <= at[x] && !(a.window && slot <= at[x] - a.window);
+#pragma unroll
+                        for (int n = 0; n < kDim / 8; ++n) {
+                            const uint32_t w = *reinterpret_cast<const uint32_t *>(reinterpret_cast<const char *>(v) + piece(kN, c, n) + (lane & 3) * 4);
+#pragma unroll
+                            for (int x = 0; x < 2; ++x) {
+                                if (sees[x] && odd(w & 0xffffu)) o[n][2 * x] = NAN;
+                                if (sees[x] && odd(w & 0xffff0000u)) o[n][2 * x + 1] = NAN;
+                            }
+                        }
+                    }
+                    __syncthreads();
+                    const auto finite = [&](uint32_t w) { return (odd(w & 0xffffu) ? 0u : w & 0xffffu) | (odd(w & 0xffff0000u) ? 0u : w & 0xffff0000u); };
+                    for (int i = tid; i < kN * kPieces; i += kThreads) {
+                        const uint4 w = v[i];
+                        v[i] = make_uint4(finite(w.x), finite(w.y), finite(w.z), finite(w.w));
+                    }
+                    __syncthreads();
+                }
             }
             if (busy) {
                 float hi[8][4] = {}, lo[8][4] = {};
@@ -267,7 +292,8 @@ __global__ void __launch_bounds__(kThreads, kDim <= 128 ? 2 : 1) split_kernel(co
                     float keep[2];
 #pragma unroll
                     for (int x = 0; x < 2; ++x) {
-                        const float next = fmaxf(ref[x], top[x]);
+                        // of the warp's rows only those that need it: a row's bits do not depend on another's scores
+                        const float next = top[x] > ref[x] + kSlack ? top[x] : ref[x];
                         keep[x] = next == ref[x] ? 1.0f : exp2f(ref[x] - next);
                         ref[x] = next;
                         l[x] *= keep[x];
@@ -296,92 +322,63 @@ __global__ void __launch_bounds__(kThreads, kDim <= 128 ? 2 : 1) split_kernel(co
                     }
                 l[0] = fmaf(sum[0], factor[0], l[0]);
                 l[1] = fmaf(sum[1], factor[1], l[1]);
-                if (!bad) {
-                    const auto products = [&](float (&w)[8][4]) {      // O += factor W V
-                        uint32_t ph[4][4], pl[4][4];   // the weights as operands of 16 slots each
+                const auto products = [&](float (&w)[8][4]) {      // O += factor W V
+                    uint32_t ph[4][4], pl[4][4];   // the weights as operands of 16 slots each
 #pragma unroll
-                        for (int n = 0; n < 8; ++n)
+                    for (int n = 0; n < 8; ++n)
 #pragma unroll
-                            for (int x = 0; x < 2; ++x) {
-                                const uint32_t p = pack(w[n][2 * x], w[n][2 * x + 1]);
-                                const float2 z = unpack(p);
-                                ph[n >> 1][(n & 1) * 2 + x] = p;
-                                pl[n >> 1][(n & 1) * 2 + x] = pack((w[n][2 * x] - z.x) * kLow, (w[n][2 * x + 1] - z.y) * kLow);
-                            }
-#pragma unroll
-                        for (int n = 0; n < kDim / 8; n += 2) {
-                            float t[2][4] = {};
-                            uint32_t b[4][4];
-#pragma unroll
-                            for (int k = 0; k < 4; ++k) {
-                                load_matrices_turned(b[k], v_at + piece(kN, k * 16 + (lane & 15), n + (lane >> 4)));
-                                multiply(t[0], pl[k], b[k][0], b[k][1]);
-                                multiply(t[1], pl[k], b[k][2], b[k][3]);
-                            }
-#pragma unroll
-                            for (int k = 0; k < 4; ++k) t[0][k] *= 1 / kLow, t[1][k] *= 1 / kLow;
-#pragma unroll
-                            for (int k = 0; k < 4; ++k) {
-                                multiply(t[0], ph[k], b[k][0], b[k][1]);
-                                multiply(t[1], ph[k], b[k][2], b[k][3]);
-                            }
-#pragma unroll
-                            for (int k = 0; k < 4; ++k) {
-                                o[n][k] = fmaf(t[0][k], factor[k >> 1], o[n][k]);
-                                o[n + 1][k] = fmaf(t[1][k], factor[k >> 1], o[n + 1][k]);
-                            }
+                        for (int x = 0; x < 2; ++x) {
+                            const uint32_t p = pack(w[n][2 * x], w[n][2 * x + 1]);
+                            const float2 z = unpack(p);
+                            ph[n >> 1][(n & 1) * 2 + x] = p;
+                            pl[n >> 1][(n & 1) * 2 + x] = pack((w[n][2 * x] - z.x) * kLow, (w[n][2 * x + 1] - z.y) * kLow);
                         }
-                    };
-                    // rounds for weights that are too small for this one; none for most
-                    while (__builtin_expect(__any_sync(kFullMask, small), 0)) {
-                        float w[8][4];
-                        bool left = false;
-                        small = false;
 #pragma unroll
-                        for (int n = 0; n < 8; ++n)
+                    for (int n = 0; n < kDim / 8; n += 2) {
+                        float t[2][4] = {};
+                        uint32_t b[4][4];
 #pragma unroll
-                            for (int k = 0; k < 4; ++k) left |= hi[n][k] > 0.0f && hi[n][k] < kLeast;
-                        if (!__any_sync(kFullMask, left)) break;
-#pragma unroll
-                        for (int n = 0; n < 8; ++n)
-#pragma unroll
-                            for (int k = 0; k < 4; ++k) {
-                                w[n][k] = hi[n][k] < kLeast ? 0.0f : hi[n][k];
-                                hi[n][k] = hi[n][k] < kLeast ? hi[n][k] * kRound : 0.0f;
-                                small |= hi[n][k] < kLeast;
-                            }
-                        products(w);
-                        factor[0] *= 1 / kRound, factor[1] *= 1 / kRound;
-                    }
-                    products(hi);
-                } else {
-                    // 0 times a value that is not finite must not reach a row that does not see it: weight by weight
-#pragma unroll 1
-                    for (int x = 0; x < 2; ++x) {
-#pragma unroll
-                        for (int n = 0; n < 8; ++n)
-#pragma unroll
-                            for (int k = 0; k < 2; ++k)
-                                s.p[warp][lane >> 2][n * 8 + (lane & 3) * 2 + k] = (x ? hi[n][2 + k] : hi[n][k]) * (x ? factor[1] : factor[0]);
-                        __syncwarp();
-#pragma unroll 1
-                        for (int c = 0; c < kN; ++c) {
-                            const int slot = u * kN + c, own = x ? at[1] : at[0];
-                            const char *v = reinterpret_cast<const char *>(s.kv[u & 1][1]);
-                            if (slot > own || (a.window && slot <= own - a.window) || s.row[u & 1][c] < 0) continue;
-                            const float p = s.p[warp][lane >> 2][c];
-#pragma unroll
-                            for (int n = 0; n < kDim / 8; ++n) {
-                                const float2 z = unpack(*reinterpret_cast<const uint32_t *>(v + piece(kN, c, n) + (lane & 3) * 4));
-                                const float y0 = x ? o[n][2] : o[n][0], y1 = x ? o[n][3] : o[n][1];
-                                const float z0 = fmaf(p, z.x, y0), z1 = fmaf(p, z.y, y1);
-                                if (x) o[n][2] = z0, o[n][3] = z1;
-                                else o[n][0] = z0, o[n][1] = z1;
-                            }
+                        for (int k = 0; k < 4; ++k) {
+                            load_matrices_turned(b[k], v_at + piece(kN, k * 16 + (lane & 15), n + (lane >> 4)));
+                            multiply(t[0], pl[k], b[k][0], b[k][1]);
+                            multiply(t[1], pl[k], b[k][2], b[k][3]);
                         }
-                        __syncwarp();
+#pragma unroll
+                        for (int k = 0; k < 4; ++k) t[0][k] *= 1 / kLow, t[1][k] *= 1 / kLow;
+#pragma unroll
+                        for (int k = 0; k < 4; ++k) {
+                            multiply(t[0], ph[k], b[k][0], b[k][1]);
+                            multiply(t[1], ph[k], b[k][2], b[k][3]);
+                        }
+#pragma unroll
+                        for (int k = 0; k < 4; ++k) {
+                            o[n][k] = fmaf(t[0][k], factor[k >> 1], o[n][k]);
+                            o[n + 1][k] = fmaf(t[1][k], factor[k >> 1], o[n + 1][k]);
+                        }
                     }
+                };
+                // rounds for weights that are too small for this one; none for most
+                while (__builtin_expect(__any_sync(kFullMask, small), 0)) {
+                    float w[8][4];
+                    bool left = false;
+                    small = false;
+#pragma unroll
+                    for (int n = 0; n < 8; ++n)
+#pragma unroll
+                        for (int k = 0; k < 4; ++k) left |= hi[n][k] > 0.0f && hi[n][k] < kLeast;
+                    if (!__any_sync(kFullMask, left)) break;
+#pragma unroll
+                    for (int n = 0; n < 8; ++n)
+#pragma unroll
+                        for (int k = 0; k < 4; ++k) {
+                            w[n][k] = hi[n][k] < kLeast ? 0.0f : hi[n][k];
+                            hi[n][k] = hi[n][k] < kLeast ? hi[n][k] * kRound : 0.0f;
+                            small |= hi[n][k] < kLeast;
+                        }
+                    products(w);
+                    factor[0] *= 1 / kRound, factor[1] *= 1 / kRound;
                 }
+                products(hi);
             }
             __syncthreads();                           // the stage and its rows are free
             if (u + 2 < f.u1) {

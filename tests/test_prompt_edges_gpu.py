@@ -100,6 +100,34 @@ def test_chunk_seen_values_count_however_small_their_weight(torch_mod, pkg, eng,
     assert not torch.isfinite(c["out"][:new, 0, 5]).any() and torch.isfinite(c["out"][:new, 0, 0]).all()
 
 
+@pytest.mark.parametrize("q,kv", TYPES)
+@pytest.mark.parametrize("rising", [False, True])
+@pytest.mark.parametrize("d,page", [(64, 16), (128, 7), (256, 64)])
+def test_chunk_rows_are_the_same_whatever_comes_behind_them(torch_mod, pkg, eng, q, kv, d, page, rising):
+    """To the bit: later tokens' keys and values of other sizes, infinite or NaN leave earlier rows as they are, also where
+    a row's largest score grows from unit to unit."""
+    torch = torch_mod
+    # enough heads that a stretch holds a tile's units, not one of them
+    c = chunk_case(torch, pkg, [300, 40], [500, 90], 64, 32, d, page, q, kv, seed=27)
+    k, v, lens = c["cache"].k, c["cache"].v, c["lens"]
+    if rising:
+        for b in range(2):
+            for s in range(lens[b]):
+                k[int(c["table"][b, s // page]), :, s % page] *= 1 + s / 100
+    want, wl = chunk_run(torch, eng, c)
+    cut = {0: 690, 1: 111}                   # first slot that changes
+    rows = torch.cat([torch.arange(300)[:690 - 500], 300 + torch.arange(40)[:111 - 90]]).cuda()
+    for what in (60.0, -3.0, math.nan, math.inf, -math.inf):
+        for b, first in cut.items():
+            for s in range(first, lens[b]):
+                for pool in (k, v):
+                    row = pool[int(c["table"][b, s // page]), :, s % page]
+                    row.copy_(row.nan_to_num(0.5, 1.0, -1.0) * what if math.isfinite(what) else torch.full_like(row, what))
+        got, gl = chunk_run(torch, eng, c, check=False)
+        assert torch.equal(got[rows], want[rows]), what
+        assert torch.equal(gl[rows], wl[rows]), what
+
+
 # ------------------------------------------------------------------ small weights, small elements of queries
 
 SINK = [("f16", "f16"), ("bf16", "bf16"), ("f32", "f16"), ("f32", "f32")]
