@@ -303,8 +303,8 @@ B200_API int b200_sample(b200_engine_t *e, const b200_sample_t *s);
  * page_size + row, or -1 where it got none or the page is not in the pool. For
  * t behind the last sequence's tokens all three are -1. Table entries that
  * were given up keep their value, and free entries behind the count stay: with
- * held_out, free_count_out and lengths_out elsewhere a call can be repeated.
- * Only page_size, table, lengths and n_pages of the cache are used. */
+ * held_out, free_count_out, lengths_out and seen_out elsewhere a call can be
+ * repeated. Only page_size, table, lengths and n_pages of the cache are used. */
 typedef struct {
     uint64_t new_tokens;               /* int32 [batch] */
     uint64_t held, held_out;           /* int32 [batch], may be the same */
@@ -399,15 +399,16 @@ B200_API int b200_rms_norm(b200_engine_t *e, const b200_rms_norm_t *a);
  * exp(s), s = scale * q . k, lse = log sum exp(s), with the conventions of
  * b200_kv_attend for rows that see nothing (p < 0, pages that are not there,
  * scores of -infinity), for NaN and for infinities; what a row does not see has
- * no influence on it, to the bit, whatever it holds, and a value that is not finite makes
- * its element infinite or NaN in every row that sees it, however small its
- * weight. Rows that no sequence has are left as they are. Dot products, maximum,
- * sum and output are held in float32. With 16-bit queries the weights of the
- * softmax are rounded to the cache's type before they meet the values (as much
- * as the output is; in float16 one below 2^-24 of the row's largest to within
- * 2^-35 of that). With float32 queries over a float16 cache the weights keep 22
- * bits however small they are (down to 2^-111), and an element of q, 2^-j of its
- * row's largest, min(22, 50 - j); over a float32 cache nothing is rounded. */
+ * no influence on it, to the bit, whatever it holds, and a value that is not
+ * finite makes its element infinite or NaN in every row that sees it, however
+ * small its weight. Rows that no sequence has are left as they are. Dot
+ * products, maximum, sum and output are held in float32. With 16-bit queries the
+ * weights of the softmax are rounded to the cache's type before they meet the
+ * values (as much as the output is; in float16 one below 2^-24 of the row's
+ * largest to within 2^-35 of that). With float32 queries over a float16 cache
+ * the weights keep 22 bits however small they are (down to 2^-111), and an
+ * element of q, 2^-j of its row's largest, min(22, 50 - j); over a float32 cache
+ * nothing is rounded. */
 typedef struct {
     uint64_t q, out;                   /* [n_tokens][n_head][head_dim], strides in elements, rows contiguous, without
                                           overlap; addresses and strides are multiples of 16 bytes */
