@@ -11,6 +11,13 @@
 // bring keys and values by tensor copies into a ring of two units. While one
 // tile's softmax runs, the other's products do.
 //
+// The weights are rounded to the cache's type, as operands of these products are:
+// half a step each, which makes the output's error 0.0021 of its norm in bfloat16
+// and 2.4e-4 to 2.9e-4 in float16 where float32 weights leave the output's own
+// rounding, 0.0016 and 2.1e-4. Their low parts would be as many products again,
+// 3072 cycles for the 2048 below, and conversions for every pair. Sums of weights
+// are of what is not rounded, in float32.
+//
 // What bounds it: the chain of a tile's unit, scores -> weights -> outputs and
 // next scores, of which two run side by side: 2250 cycles of softmax and 1000 of
 // products, 3330 in all, where the products of both tiles take 2048 and the
